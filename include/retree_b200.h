@@ -458,6 +458,83 @@ int rt_linear_gather(const void* const* x_ranks, int world, int cols_per_rank, i
                      int n_out, int k, void* out, int64_t ld_out, const int64_t* flags_local, const int64_t* epoch_dev,
                      int64_t epoch_add, int* status, rt_stream_t stream);
 
+/* ------------------------------------------------------------------------
+ * Causal attention over whole prompts (bf16 or fp16, GQA, head_dim 128).
+ * Replaces sdpa_attention_forward on a prompt
+ * (transformers/integrations/sdpa_attention.py:40-104) for the prefill of the
+ * decode loops (ddtree.py:797-808), with several sequences packed into one
+ * call.
+ *
+ * Query row (token i, head h) is at q + i*q_tok_stride + h*q_head_stride, key /
+ * value row j of kv head g at k / v + g*kv_head_stride + j*kv_row_stride, out
+ * row (i, h) at out + i*out_tok_stride + h*out_head_stride (128 values each;
+ * dtype 1 = bf16, 2 = fp16 for all four).  Sequence b owns queries
+ * [cu_q[b], cu_q[b+1]) and keys [cu_k[b], cu_k[b+1]) (int32, DEVICE, num_seqs +
+ * 1 entries; cu_k NULL: the same rows as cu_q; cu_q NULL: one sequence of
+ * total_q queries and total_k keys).  With lq queries and lk keys, query i of
+ * the sequence sees key j iff j <= i + lk - lq, i.e. the queries are the last
+ * lq tokens of the sequence; a query that sees no key gets a zero row.  Rows
+ * outside every sequence are neither read into a result nor written.  A
+ * sequence whose bounds decrease or pass total_q / total_k is skipped
+ * (RT_DEV_BAD_INDEX).  What a key or value row holds where it is hidden (NaN
+ * and infinities included) does not reach the result.
+ * Requires scale >= 0 and finite, num_q_heads / num_kv_heads <= 128, all pointers and strides
+ * multiples of 16 bytes, total_q and total_k below 2^31.  workspace must hold
+ * rt_prompt_attn_workspace_size(...) bytes (alignment 256; 0 for most shapes).
+ * ---------------------------------------------------------------------- */
+size_t rt_prompt_attn_workspace_size(int64_t total_q, int64_t total_k, int num_seqs, int num_q_heads,
+                                     int num_kv_heads);
+int rt_prompt_attn(const void* q, int64_t q_tok_stride, int64_t q_head_stride, const void* k, const void* v,
+                   int64_t kv_head_stride, int64_t kv_row_stride, void* out, int64_t out_tok_stride,
+                   int64_t out_head_stride, int dtype, const int32_t* cu_q, const int32_t* cu_k, int num_seqs,
+                   int64_t total_q, int64_t total_k, int num_q_heads, int num_kv_heads, int head_dim, float scale,
+                   void* workspace, size_t workspace_bytes, int* status, rt_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * A KV cache held in 4 bits (no counterpart in the reference, whose cache is
+ * bf16: transformers/cache_utils.py:102-121).
+ *
+ * One head's 128 values of one token are RT_Q4_ROW_BYTES = 72 bytes: 64 bytes
+ * of 4-bit codes u, then four 16-bit words, one per 32 consecutive values,
+ * holding the scale s (bits 4-14: exponent and three mantissa bits, as in
+ * bf16) and the zero point z (bits 0-3).  32-bit code word i holds values
+ * 8i..8i+7: nibbles 0-3 the even, nibbles 4-7 the odd ones.  The value is
+ * (u - z) * s, a bf16 number exactly.  Written as: lo = min(0, min x), hi =
+ * max(0, max x), s = (hi - lo) / 15 rounded up to four significant bits (0
+ * below 2^-126: the group reads as zero), z = rne(-lo / s), u = clamp(rne(x / s)
+ * + z, 0, 15).  A row with a value that is not finite reads as NaN throughout.
+ * Rows of a head are contiguous (row r at r * RT_Q4_ROW_BYTES); the cache is
+ * compacted by rt_kv_compact with row_bytes = RT_Q4_ROW_BYTES.
+ *
+ * rt_kv_append_q4: writes n_new rows per head of k_new / v_new (bf16[128], row
+ *   r of head h at h*new_head_stride + r*new_row_stride, 16-byte aligned) to
+ *   rows [offset, offset + n_new) of k_cache / v_cache (8-byte aligned).  offset
+ *   is read from offset_dev (int64, DEVICE) when non-NULL.  Rows past `capacity`
+ *   are not written (RT_DEV_OVERFLOW).
+ * rt_kv_read_q4: decodes rows [start, start + n) of every head to bf16[128]
+ *   rows of out (16-byte aligned).
+ * rt_tree_attn_q4: rt_tree_attn on the values of such a cache (same masks,
+ *   prefix, splits, output; see there).  k / v and kv_head_stride are multiples
+ *   of 16 bytes, kv_capacity is even, scale >= 0 and finite; a node that sees no
+ *   key gets a zero row; a prefix length outside the cache writes nothing
+ *   (RT_DEV_BAD_INDEX).  workspace must hold
+ *   rt_tree_attn_q4_workspace_size(...) bytes (alignment 256).
+ * ---------------------------------------------------------------------- */
+#define RT_Q4_ROW_BYTES 72
+int rt_kv_append_q4(void* k_cache, void* v_cache, int64_t cache_head_stride, const void* k_new, const void* v_new,
+                    int64_t new_head_stride, int64_t new_row_stride, int n_heads, int n_new, int head_dim,
+                    int64_t capacity, int64_t offset, const int64_t* offset_dev, int* status, rt_stream_t stream);
+int rt_kv_read_q4(const void* cache, int64_t cache_head_stride, void* out, int64_t out_head_stride,
+                  int64_t out_row_stride, int n_heads, int n, int head_dim, int64_t capacity, int64_t start,
+                  rt_stream_t stream);
+size_t rt_tree_attn_q4_workspace_size(int n, int num_q_heads, int num_kv_heads, int head_dim, int64_t prefix_len,
+                                      int num_splits);
+int rt_tree_attn_q4(const void* q, int64_t q_tok_stride, int64_t q_head_stride, const void* k, const void* v,
+                    int64_t kv_head_stride, int64_t kv_capacity, void* out, int64_t out_tok_stride,
+                    int64_t out_head_stride, const uint32_t* mask, int mask_words, int n, int64_t prefix_len,
+                    const int64_t* prefix_len_dev, int num_q_heads, int num_kv_heads, int head_dim, float scale,
+                    int num_splits, void* workspace, size_t workspace_bytes, int* status, rt_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -62,11 +62,20 @@ SIGNATURES = {
     "rt_linear_check": (_I, [_I, _I, _I, _I]),
     "rt_linear_plan": (_I, [_I, _I, _I, _I, _P, _P, _P]),
     "rt_linear": (_I, [_P, _I64, _I, _I, _P, _I, _I, _P, _I64, _P, _P, _P]),
+    "rt_prompt_attn_workspace_size": (_SZ, [_I64, _I64, _I, _I, _I]),
+    "rt_prompt_attn": (_I, [_P, _I64, _I64, _P, _P, _I64, _I64, _P, _I64, _I64, _I, _P, _P, _I, _I64, _I64, _I, _I,
+                            _I, _F, _P, _SZ, _P, _P]),
+    "rt_kv_append_q4": (_I, [_P, _P, _I64, _P, _P, _I64, _I64, _I, _I, _I, _I64, _I64, _P, _P, _P]),
+    "rt_kv_read_q4": (_I, [_P, _I64, _P, _I64, _I64, _I, _I, _I, _I64, _I64, _P]),
+    "rt_tree_attn_q4_workspace_size": (_SZ, [_I, _I, _I, _I, _I64, _I]),
+    "rt_tree_attn_q4": (_I, [_P, _I64, _I64, _P, _P, _I64, _I64, _P, _I64, _I64, _P, _I, _I, _I64, _P, _I, _I, _I,
+                             _F, _I, _P, _SZ, _P, _P]),
 }
 
 RT_EPI_STORE = 0
 RT_EPI_SILU_MUL = 1
 RT_EPI_QKV_ROPE = 2
+RT_Q4_ROW_BYTES = 72
 
 
 class QkvEpilogue(ctypes.Structure):

@@ -610,3 +610,239 @@ def recovery_walk(parents: torch.Tensor, tokens: torch.Tensor, posterior: torch.
     _lib.check(rc, "rt_recovery_walk")
     _count()
     return out
+
+
+# ---------------------------------------------------------------------------
+# Attention over whole prompts
+# ---------------------------------------------------------------------------
+def _same_device(dev, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != dev:
+            raise RuntimeError(f"{name} must be on {dev}")
+
+
+def _no_grad(*tensors) -> None:
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError("retree_b200 attention and cache kernels are inference-only (no gradient)")
+
+
+def _workspace(nbytes: int, dev) -> torch.Tensor | None:
+    """Scratch of one call, from the caching allocator: ordered by the call's stream, the graph's own in a capture."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+
+
+def _cu_seqlens(t: torch.Tensor | None, name: str) -> None:
+    if t is not None and (t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or t.numel() < 2):
+        raise RuntimeError(f"{name} must be a contiguous int32 tensor of at least two offsets")
+
+
+def _query(q: torch.Tensor) -> torch.Tensor:
+    """``[n, Hq, 128]`` view of a query in that layout or HF's ``[1, Hq, n, 128]``."""
+    if q.dim() == 4:
+        if q.shape[0] != 1:
+            raise RuntimeError("batch size 1 only (pack sequences along the token axis)")
+        q = q[0].transpose(0, 1)
+    if q.dim() != 3 or q.shape[-1] != 128 or q.stride(-1) != 1:
+        raise RuntimeError("query must be [tokens, heads, 128] (or [1, heads, tokens, 128]) with contiguous head_dim")
+    return q
+
+
+def _attn_out(out: torch.Tensor | None, q: torch.Tensor) -> torch.Tensor:
+    if out is None:
+        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if out.shape != q.shape or out.dtype != q.dtype or out.stride(-1) != 1 or \
+            any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
+        raise RuntimeError(f"out must be {q.dtype} {list(q.shape)} with contiguous head_dim and rows of its own")
+    return out
+
+
+def _byte_strides(t: torch.Tensor) -> tuple[int, int]:
+    """Byte strides of the two leading axes of ``[a, b, 128]`` (any aligned number for an axis of one)."""
+    es = t.element_size()
+    return tuple(s * es if n > 1 else 256 for n, s in zip(t.shape[:2], t.stride()))
+
+
+def _rows_apart(t: torch.Tensor) -> torch.Tensor:
+    """``t``, copied if it repeats a row (a zero stride, which a tensor map does not describe)."""
+    return t.contiguous() if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())) else t
+
+
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens_q: torch.Tensor | None = None,
+                     cu_seqlens_k: torch.Tensor | None = None, scale: float | None = None,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal GQA attention over whole prompts, several sequences packed along the token axis.
+
+    q: ``[T, Hq, 128]`` or HF's ``[1, Hq, T, 128]``; k, v: ``[Hkv, Tk, 128]`` or
+    ``[1, Hkv, Tk, 128]``, any token and head strides of 16 bytes; bf16 or
+    fp16.  ``cu_seqlens_q`` / ``cu_seqlens_k``: int32 CUDA offsets of the
+    sequences' queries and keys (``cu_seqlens_k=None``: the same offsets; both
+    None: one sequence).  A sequence's queries are its last tokens: with lq
+    queries and lk keys, query i sees keys ``j <= i + lk - lq``, so a chunk of a
+    prompt attends to the keys of the chunks before it.  Queries that see no
+    key give zero rows; rows outside every sequence are not written.
+    Returns ``out`` ``[T, Hq, 128]``.
+    """
+    lib = _lib.load()
+    _require_cuda(q, k, v, cu_seqlens_q, cu_seqlens_k, out)
+    _no_grad(q, k, v)
+    q, k, v = _query(q), _as3(k), _as3(v)
+    if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise RuntimeError("prompt attention runs on bf16 or fp16 q/k/v of one type")
+    q, k, v = _rows_apart(q), _rows_apart(k), _rows_apart(v)
+    if k.shape != v.shape or _byte_strides(k) != _byte_strides(v):
+        raise RuntimeError("K and V must share shape and strides")
+    t, hq, d = q.shape
+    hkv, tk = k.shape[:2]
+    if k.shape[2] != d or hkv == 0 or hq == 0 or hq % hkv:
+        raise RuntimeError("key heads must divide query heads, with head_dim 128")
+    dev = q.device
+    _same_device(dev, k=k, v=v, cu_seqlens_q=cu_seqlens_q, cu_seqlens_k=cu_seqlens_k, out=out)
+    _cu_seqlens(cu_seqlens_q, "cu_seqlens_q")
+    _cu_seqlens(cu_seqlens_k, "cu_seqlens_k")
+    if cu_seqlens_q is None and cu_seqlens_k is not None:
+        raise RuntimeError("cu_seqlens_k needs cu_seqlens_q")
+    if cu_seqlens_k is not None and cu_seqlens_k.numel() != cu_seqlens_q.numel():
+        raise RuntimeError("cu_seqlens_q and cu_seqlens_k must name the same number of sequences")
+    seqs = 1 if cu_seqlens_q is None else cu_seqlens_q.numel() - 1
+    out = _attn_out(out, q)
+    if t == 0:
+        return out
+    with torch.cuda.device(dev):
+        nbytes = lib.rt_prompt_attn_workspace_size(t, tk, seqs, hq, hkv)
+        ws = _workspace(nbytes, dev)
+        rc = lib.rt_prompt_attn(q.data_ptr(), *_byte_strides(q), k.data_ptr(), v.data_ptr(), *_byte_strides(k),
+                                out.data_ptr(), *_byte_strides(out), _DTYPE_CODE[q.dtype], _ptr(cu_seqlens_q),
+                                _ptr(cu_seqlens_k), seqs, t, tk, hq, hkv, d,
+                                d ** -0.5 if scale is None else float(scale), _ptr(ws), nbytes,
+                                _STATE.status(dev).data_ptr(), _stream(dev))
+    _lib.check(rc, "rt_prompt_attn")
+    _count(2 if nbytes else 1)
+    return out
+
+
+# ---------------------------------------------------------------------------
+# 4-bit KV cache
+# ---------------------------------------------------------------------------
+Q4_ROW_BYTES = _lib.RT_Q4_ROW_BYTES
+
+
+def _q4_cache(t: torch.Tensor, name: str) -> torch.Tensor:
+    if t.dtype != torch.uint8 or t.dim() != 3 or t.shape[-1] != Q4_ROW_BYTES or t.stride(-1) != 1 or \
+            t.stride(-2) != Q4_ROW_BYTES:
+        raise RuntimeError(f"{name} must be uint8 [heads, capacity, {Q4_ROW_BYTES}] with contiguous rows")
+    return t
+
+
+def kv_append_q4(k_cache: torch.Tensor, v_cache: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor,
+                 offset: int = 0, offset_dev: torch.Tensor | None = None) -> None:
+    """Quantise ``[heads, n, 128]`` bf16 rows into rows ``offset..`` of 4-bit caches ``[heads, cap, 72]`` (uint8)."""
+    lib = _lib.load()
+    _require_cuda(k_cache, v_cache, k_new, v_new, offset_dev)
+    _no_grad(k_new, v_new)
+    k_cache, v_cache = _q4_cache(k_cache, "k_cache"), _q4_cache(v_cache, "v_cache")
+    k_new, v_new = _as3(k_new), _as3(v_new)
+    if k_new.dtype != torch.bfloat16 or v_new.dtype != torch.bfloat16:
+        raise RuntimeError("kv_append_q4 takes bf16 rows")
+    if k_cache.shape != v_cache.shape or k_cache.stride() != v_cache.stride():
+        raise RuntimeError("K and V caches must share shape and strides")
+    if k_new.shape != v_new.shape or k_new.shape[0] != k_cache.shape[0] or k_new.shape[2] != 128:
+        raise RuntimeError("new rows must be [cache heads, n, 128], the same for K and V")
+    if offset_dev is not None and offset_dev.dtype != torch.int64:
+        raise RuntimeError("offset_dev must be int64")
+    if _byte_strides(k_new) != _byte_strides(v_new):
+        k_new, v_new = k_new.contiguous(), v_new.contiguous()
+    dev = k_cache.device
+    _same_device(dev, v_cache=v_cache, k_new=k_new, v_new=v_new, offset_dev=offset_dev)
+    heads, n, d = k_new.shape
+    with torch.cuda.device(dev):
+        rc = lib.rt_kv_append_q4(k_cache.data_ptr(), v_cache.data_ptr(),
+                                 k_cache.stride(0) if heads > 1 else k_cache.shape[1] * Q4_ROW_BYTES,
+                                 k_new.data_ptr(), v_new.data_ptr(), *_byte_strides(k_new), heads, n, d,
+                                 k_cache.shape[1], int(offset), _ptr(offset_dev), _STATE.status(dev).data_ptr(),
+                                 _stream(dev))
+    _lib.check(rc, "rt_kv_append_q4")
+    _count()
+
+
+def kv_read_q4(cache: torch.Tensor, start: int, n: int, out: torch.Tensor | None = None) -> torch.Tensor:
+    """bf16 values ``[..., n, 128]`` of rows ``[start, start + n)`` of a 4-bit cache ``[..., cap, 72]``."""
+    lib = _lib.load()
+    _require_cuda(cache, out)
+    if cache.dim() < 2:
+        raise RuntimeError(f"cache must be uint8 [..., capacity, {Q4_ROW_BYTES}]")
+    lead = cache.shape[:-2]
+    try:
+        c = _q4_cache(cache.view(-1, *cache.shape[-2:]), "cache")
+    except RuntimeError:
+        raise RuntimeError(f"cache must be uint8 [..., capacity, {Q4_ROW_BYTES}] with contiguous rows and leading "
+                           "dimensions of one stride") from None
+    dev = c.device
+    start, n = int(start), int(n)
+    if start < 0 or n < 0 or start + n > c.shape[1]:
+        raise RuntimeError(f"rows [{start}, {start + n}) are outside the cache's {c.shape[1]}")
+    if out is None:
+        out = torch.empty((*lead, n, 128), dtype=torch.bfloat16, device=dev)
+    if out.shape != (*lead, n, 128) or out.dtype != torch.bfloat16 or not out.is_contiguous():
+        raise RuntimeError(f"out must be contiguous bf16 {[*lead, n, 128]}")
+    _same_device(dev, out=out)
+    if out.numel() == 0:
+        return out
+    with torch.cuda.device(dev):
+        rc = lib.rt_kv_read_q4(c.data_ptr(), c.stride(0), out.data_ptr(), n * 256, 256, c.shape[0], n, 128,
+                               c.shape[1], start, _stream(dev))
+    _lib.check(rc, "rt_kv_read_q4")
+    _count()
+    return out
+
+
+def tree_attention_q4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask_bits: torch.Tensor, prefix_len: int,
+                      scale: float | None = None, out: torch.Tensor | None = None, num_splits: int = 0,
+                      prefix_len_dev: torch.Tensor | None = None) -> torch.Tensor:
+    """``tree_attention`` over a 4-bit cache.
+
+    q: bf16 ``[n, Hq, 128]`` or HF's ``[1, Hq, n, 128]``; k, v: uint8 caches
+    ``[Hkv, capacity, 72]`` of which rows ``[0, prefix_len + n)`` are used;
+    mask_bits: int32 ``[n, W]`` ancestor bits of the tree block (one bit, set,
+    for a single token).  ``prefix_len_dev`` (int64[1]) supplies the prefix
+    length at run time; ``prefix_len`` is then its upper bound.  Returns ``out``
+    ``[n, Hq, 128]`` bf16.
+    """
+    lib = _lib.load()
+    _require_cuda(q, k, v, mask_bits, out, prefix_len_dev)
+    _no_grad(q)
+    q = _query(q)
+    if q.dtype != torch.bfloat16:
+        raise RuntimeError("tree attention runs on bf16 queries")
+    q = _rows_apart(q)
+    k, v = _q4_cache(k, "k"), _q4_cache(v, "v")
+    if k.shape != v.shape or k.stride() != v.stride():
+        raise RuntimeError("K and V caches must share shape and strides")
+    n, hq, d = q.shape
+    hkv, cap = k.shape[:2]
+    if n == 0 or hkv == 0 or hq == 0 or hq % hkv:
+        raise RuntimeError("at least one node, and key heads that divide the query heads")
+    if mask_bits.dtype != torch.int32 or mask_bits.dim() != 2 or mask_bits.shape[0] < n or \
+            mask_bits.shape[1] * 32 < n:
+        raise RuntimeError("mask_bits must be int32 [n, at least ceil(n / 32)]")
+    if prefix_len_dev is not None and prefix_len_dev.dtype != torch.int64:
+        raise RuntimeError("prefix_len_dev must be int64")
+    if mask_bits.stride(-1) != 1 or mask_bits.stride(0) < mask_bits.shape[1]:
+        mask_bits = mask_bits.contiguous()
+    dev = q.device
+    _same_device(dev, k=k, v=v, mask_bits=mask_bits, out=out, prefix_len_dev=prefix_len_dev)
+    out = _attn_out(out, q)
+    prefix_len = int(prefix_len)
+    with torch.cuda.device(dev):
+        nbytes = lib.rt_tree_attn_q4_workspace_size(n, hq, hkv, d, prefix_len, int(num_splits))
+        ws = _workspace(nbytes, dev)
+        rc = lib.rt_tree_attn_q4(q.data_ptr(), *_byte_strides(q), k.data_ptr(), v.data_ptr(),
+                                 k.stride(0) if hkv > 1 else cap * Q4_ROW_BYTES, cap, out.data_ptr(),
+                                 *_byte_strides(out), mask_bits.data_ptr(), mask_bits.stride(0), n, prefix_len,
+                                 _ptr(prefix_len_dev), hq, hkv, d, d ** -0.5 if scale is None else float(scale),
+                                 int(num_splits), _ptr(ws), nbytes, _STATE.status(dev).data_ptr(), _stream(dev))
+    _lib.check(rc, "rt_tree_attn_q4")
+    _count(2 if nbytes else 1)
+    return out
+
+
+__all__ += ["prompt_attention", "kv_append_q4", "kv_read_q4", "tree_attention_q4", "Q4_ROW_BYTES"]
