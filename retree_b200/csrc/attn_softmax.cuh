@@ -1,0 +1,79 @@
+// One 128-key block of the online softmax for one query row held by one thread
+// (S, P and O of the row live in the thread's TMEM lane).
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include <type_traits>
+
+#include "common.cuh"
+
+namespace rt {
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (std::is_same_v<T, __half>) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    return pack_bf16x2(a, b);
+  }
+}
+
+constexpr float kLazyRescale = 8.0f;  // log2 units
+
+// sr: the row's 128 raw scores (-inf where hidden), read from the S tile whose
+// first 64 columns (ts) take the weights P = 2^(s * sl2 - m) as 16-bit pairs.
+// The running maximum m moves only when a score passes it by 2^8, so weights stay
+// below that and O (128 columns at `to`) is rescaled rarely; O must hold every
+// earlier block (`rescale` is false for a row's first block).  l sums the
+// weights in fp32, before they are rounded.  fp16 weights sit 2^6 above the
+// maximum's 1 (2^14 at most), which keeps weights down to 2^-20 of it out of the
+// subnormal range.
+template <typename T>
+__device__ __forceinline__ void softmax_block(const uint32_t (&sr)[4][32], uint32_t ts, uint32_t to, bool rescale,
+                                              float sl2, float& m, float& l) {
+  constexpr float kLift = std::is_same_v<T, __half> ? 6.f : 0.f;
+  float a[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+#pragma unroll
+    for (int i = 0; i < 32; ++i) a[i & 3] = fmaxf(a[i & 3], __uint_as_float(sr[c][i]));
+  const float m_new = fmaxf(m, fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])) * sl2);
+  const bool need = m_new > m + kLazyRescale;  // false while m_new is -inf
+  if (__any_sync(0xFFFFFFFFu, need)) {
+    if (rescale) {
+      const float f = need ? ex2(m - m_new) : 1.f;
+#pragma unroll 1
+      for (int c = 0; c < 8; ++c) {
+        uint32_t o[16];
+        tmem_ld16(to + c * 16, o);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+        tmem_st16(to + c * 16, o);
+      }
+      l *= f;
+    }
+    if (need) m = m_new;
+  }
+  const float mu = (m == -INFINITY ? 0.f : m) - kLift;
+  const float2 sc2 = make_float2(sl2, sl2), sh2 = make_float2(-mu, -mu);
+  float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    uint32_t pk[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float2 x =
+          ffma2(make_float2(__uint_as_float(sr[c][2 * i]), __uint_as_float(sr[c][2 * i + 1])), sc2, sh2);
+      const float p0 = ex2(x.x), p1 = ex2(x.y);
+      acc[i & 1] = fadd2(acc[i & 1], make_float2(p0, p1));
+      pk[i] = pack2<T>(p0, p1);
+    }
+    tmem_st16(ts + c * 16, pk);
+  }
+  l += (acc[0].x + acc[1].x) + (acc[0].y + acc[1].y);
+}
+
+}  // namespace rt

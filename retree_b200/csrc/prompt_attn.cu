@@ -26,8 +26,7 @@
 #include <cuda.h>
 #include <cuda_fp16.h>
 
-#include <type_traits>
-
+#include "attn_softmax.cuh"
 #include "common.cuh"
 #include "host_util.h"
 #include "tmap.h"
@@ -51,7 +50,6 @@ constexpr int kPMaxSeqs = 4096;
 constexpr uint32_t kPOffBar = kPOffTab + (kPMaxSeqs + 1) * 4 + 12;
 constexpr uint32_t kPSmem = kPOffBar + 512 + 1024;
 constexpr uint32_t kPTmemO = 256;              // S0 | S1 | O0 | O1, P_t in S_t's first 64 columns
-constexpr float kPRescale = 8.0f;              // log2 units
 constexpr int kPSms = 148;
 
 struct PromptParams {
@@ -127,15 +125,6 @@ __device__ __forceinline__ bool prompt_item(const PromptParams& p, const int* ta
   return true;
 }
 
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-  if constexpr (std::is_same_v<T, __half>) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  } else {
-    return pack_bf16x2(a, b);
-  }
-}
 template <typename T>
 __device__ __forceinline__ float2 unpack2(uint32_t w) {
   if constexpr (std::is_same_v<T, __half>) {
@@ -422,9 +411,6 @@ __global__ void __launch_bounds__(kPThreads, 1)
     const uint32_t ts = tmem + lane_base + t * kPB, to = tmem + lane_base + kPTmemO + t * kPD;
     const int rt = r / p.group, rh = r - rt * p.group;
     const float sl2 = p.scale_log2;
-    // fp16 weights sit 2^6 above the running maximum's 1 (and at most 2^14),
-    // which keeps weights down to 2^-20 of it out of the subnormal range
-    constexpr float kLift = std::is_same_v<T, __half> ? 6.f : 0.f;
     int ns = 0, no = 0;
     bool ok = true;
     for (int it = 0; ok && prompt_item(p, tab, it, w); ++it) {
@@ -452,50 +438,10 @@ __global__ void __launch_bounds__(kPThreads, 1)
             for (int i = 0; i < 32; ++i)
               if (c * 32 + i >= left) sr[c][i] = __float_as_uint(-INFINITY);
         }
-        float a[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int i = 0; i < 32; ++i) a[i & 3] = fmaxf(a[i & 3], __uint_as_float(sr[c][i]));
-        const float m_new = fmaxf(m, fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])) * sl2);
-        const bool need = m_new > m + kPRescale;  // false while m_new is -inf
-        if (__any_sync(0xFFFFFFFFu, need)) {
-          // (S_j's arrival also says that PV_{j-1} is complete)
-          const float f = need ? ex2(m - m_new) : 1.f;
-          if (j > 0) {
-#pragma unroll 1
-            for (int c = 0; c < 8; ++c) {
-              uint32_t o[16];
-              tmem_ld16(to + c * 16, o);
-              tmem_wait_ld();
-#pragma unroll
-              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-              tmem_st16(to + c * 16, o);
-            }
-            l *= f;
-          }
-          if (need) m = m_new;
-        }
-        const float mu = (m == -INFINITY ? 0.f : m) - kLift;
-        const float2 sc2 = make_float2(sl2, sl2), sh2 = make_float2(-mu, -mu);
-        float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t pk[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float2 x =
-                ffma2(make_float2(__uint_as_float(sr[c][2 * i]), __uint_as_float(sr[c][2 * i + 1])), sc2, sh2);
-            const float p0 = ex2(x.x), p1 = ex2(x.y);
-            acc[i & 1] = fadd2(acc[i & 1], make_float2(p0, p1));
-            pk[i] = pack2<T>(p0, p1);
-          }
-          tmem_st16(ts + c * 16, pk);
-        }
+        softmax_block<T>(sr, ts, to, j > 0, sl2, m, l);
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(&bar.p_full[t]);
-        l += (acc[0].x + acc[1].x) + (acc[0].y + acc[1].y);
       }
       if (!ok) break;
       char* dst = p.out + static_cast<int64_t>(w.q0 + tok) * p.out_tok_stride +

@@ -37,11 +37,10 @@
 #include "common.cuh"
 #include "host_util.h"
 #include "tmap.h"
+#include "tree_attn.cuh"
 
 namespace rt {
 
-constexpr int kHD = 128;
-constexpr int kBM = 128;
 constexpr int kBN = 128;
 constexpr int kSoftmaxThreads = 256;  // warps 0-7: two threads per tile row
 constexpr int kProducerWarp = 8;
@@ -60,7 +59,6 @@ constexpr uint32_t kAttnSmem = kOffBar + 1536 + 1024;  // + barriers/exchange + 
 constexpr uint32_t kOffStage = 0;
 constexpr uint32_t kOffMl = 2 * kTile;
 constexpr uint32_t kOffWeights = 3 * kTile;  // [owned rows][kMaxMerge] fp32 merge weights
-constexpr int kMaxMerge = 16;  // cluster size limit (16 needs the non-portable cluster attribute)
 constexpr uint32_t kTmemCols = 512;                   // S0 | S1 | O | P0 P1
 // P_b (bf16, two keys per 32-bit column, row r in lane r) at TMEM columns
 // kPCol + 64*b: the A operand of the PV product, read by the tensor core
@@ -68,48 +66,12 @@ constexpr uint32_t kTmemCols = 512;                   // S0 | S1 | O | P0 P1
 constexpr uint32_t kPCol = 3 * 128;
 constexpr float kRescaleThreshold = 8.0f;             // log2 units
 
-struct AttnParams {
-  const char* q;
-  int64_t q_tok_stride, q_head_stride;
-  char* out;
-  int64_t out_tok_stride, out_head_stride;
-  const uint32_t* mask;
-  int mask_words;
-  int n;
-  int64_t prefix_len;
-  const int64_t* prefix_len_dev;
-  int group, num_kv_heads, tiles, num_splits;
-  int merge;       // 1: the splits of a (kv head, tile) form one cluster and are merged in the kernel
-  float scale_log2;
-  float* ws_o;     // [split][kv_head][tiles*128][128]
-  float2* ws_ml;   // [split][kv_head][tiles*128]  (m in log2 units, l)
-  int* status;
-  // warp-level path only
-  const char* k;
-  const char* v;
-  int64_t kv_head_stride, kv_row_stride;
-};
-
 struct Barriers {
   uint64_t full_q, full_k[2], full_v[2], empty_k[2], empty_v[2], s_full[2], s_free[2], p_full[2], o_done[2], fin;
   uint32_t tmem_base;
   int abort_flag;
   float xchg[2][kBM];  // per-row partial max / sum of the two column halves
 };
-
-__device__ __forceinline__ int64_t key_count(const AttnParams& p) {
-  const int64_t L = p.prefix_len_dev != nullptr ? *p.prefix_len_dev : p.prefix_len;
-  return L + p.n;
-}
-
-// Block range [b0, b1) of this split: the blocks spread evenly (range sizes
-// differ by at most one, so no split runs two blocks while another idles).
-__device__ __forceinline__ void split_range(int64_t total_keys, int split, int splits, int64_t blk, int64_t& b0,
-                                            int64_t& b1) {
-  const int64_t nblk = (total_keys + blk - 1) / blk;
-  b0 = nblk * split / splits;
-  b1 = nblk * (split + 1) / splits;
-}
 
 __device__ __forceinline__ void write_neutral_partial(const AttnParams& p, int split, int kvh, int row0, int rows) {
   const int64_t rows_ws = static_cast<int64_t>(p.tiles) * kBM;
@@ -126,43 +88,6 @@ __device__ __forceinline__ float max128(const uint32_t (&s)[4][32]) {
 #pragma unroll
     for (int c = 0; c < 32; ++c) a[c & 3] = fmaxf(a[c & 3], __uint_as_float(s[c4][c]));
   return fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3]));
-}
-
-// Visibility of the 32 keys [k0, k0+32) for one node: prefix keys (< L) are
-// visible, tree key t = key - L uses bit t of the node's mask row, keys at or
-// past L + n are hidden.
-__device__ __forceinline__ uint32_t visible_word(int64_t k0, int64_t L, int n, const uint32_t* mrow, int words) {
-  const int64_t pre = L - k0;  // prefix columns at the start of the window
-  if (pre >= 32) return 0xFFFFFFFFu;
-  uint32_t bits = pre > 0 ? ((1u << pre) - 1u) : 0u;
-  const int64_t t0 = k0 - L;  // tree index of column 0 (negative: starts in the prefix)
-  uint32_t tb;
-  if (t0 >= 0) {
-    const int w = static_cast<int>(t0 >> 5), sh = static_cast<int>(t0 & 31);
-    const uint32_t lo = w < words ? mrow[w] : 0u;
-    const uint32_t hi = (sh != 0 && w + 1 < words) ? mrow[w + 1] : 0u;
-    tb = sh ? ((lo >> sh) | (hi << (32 - sh))) : lo;
-  } else {
-    tb = mrow[0] << static_cast<int>(-t0);
-  }
-  // tree columns past the last node are hidden
-  const int64_t lim = static_cast<int64_t>(n) - t0;  // columns c < lim have t < n
-  if (lim < 32) tb &= lim <= 0 ? 0u : ((1u << lim) - 1u);
-  return bits | tb;
-}
-
-__device__ __forceinline__ float2 ld_cluster_f32x2(uint32_t addr) {
-  float2 v;
-  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
-  return v;
-}
-__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(addr)
-               : "memory");
-  return v;
 }
 
 // Byte offset of 16-byte chunk `c` (0..31) of row `r` in the merge's O stage.
@@ -183,37 +108,6 @@ __device__ __forceinline__ uint32_t stage_off(int r, int c) {
 // thread per row forms the weights into a shared table first and the item
 // threads then load only the chunks.  The last barrier keeps every CTA's
 // shared memory until all ranks have read it.
-__device__ __forceinline__ float4 merge_chunk(const float4 (&o)[kMaxMerge], int S, const float* wrow) {
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-  for (int u = 0; u < kMaxMerge; ++u) {
-    const float wu = wrow[u];
-    if (u < S && wu != 0.f) {
-      acc.x = fmaf(wu, o[u].x, acc.x);
-      acc.y = fmaf(wu, o[u].y, acc.y);
-      acc.z = fmaf(wu, o[u].z, acc.z);
-      acc.w = fmaf(wu, o[u].w, acc.w);
-    }
-  }
-  return acc;
-}
-
-// The rank weights of one row from every rank's (m, l).
-__device__ __forceinline__ void merge_weights(const float2 (&ml)[kMaxMerge], float (&w)[kMaxMerge]) {
-  float M = -INFINITY;
-#pragma unroll
-  for (int u = 0; u < kMaxMerge; ++u) M = fmaxf(M, ml[u].x);
-  float lsum = 0.f;
-#pragma unroll
-  for (int u = 0; u < kMaxMerge; ++u) {
-    w[u] = (M == -INFINITY || ml[u].x == -INFINITY) ? 0.f : ex2(ml[u].x - M);
-    lsum = fmaf(w[u], ml[u].y, lsum);
-  }
-  const float inv = lsum > 0.f ? 1.f / lsum : 0.f;
-#pragma unroll
-  for (int u = 0; u < kMaxMerge; ++u) w[u] = w[u] * inv;
-}
-
 __device__ __forceinline__ void merge_splits(const AttnParams& p, unsigned char* smem, int rank, int kvh, int row0,
                                              int rows_total) {
   __syncwarp();
@@ -817,110 +711,6 @@ __global__ void __launch_bounds__(128) tree_attn_simt_kernel(const AttnParams p)
 }
 
 // ---------------------------------------------------------------------------
-// Split merge: one warp per (kv head, tile row); lane owns 4 dims.
-// ---------------------------------------------------------------------------
-constexpr int kFastSplits = 24;  // up to this many splits: every load of a row issued at once
-
-__global__ void __launch_bounds__(128) attn_combine_kernel(const AttnParams p) {
-  pdl_launch_dependents();
-  pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const int rows = p.n * p.group;
-  const int64_t rows_ws = static_cast<int64_t>(p.tiles) * kBM;
-  const int S = p.num_splits;
-  const float2 none = make_float2(-INFINITY, 0.f);
-  if (S <= kFastSplits) {
-    // Two warps per (kv head, row), one per 64-dim half, lane owns 2 dims.
-    // Every load of the row is independent of the others, so all of them --
-    // the splits' partial rows and (max, sum) pairs -- go out at once: one
-    // L2 round trip instead of one for the maxima and one per batch of rows.
-    // A split whose weight is zero (max -inf) is skipped, never multiplied;
-    // the per-element sum runs over the splits in order, as below.
-    const int gw = (blockIdx.x * blockDim.x + threadIdx.x) >> 5;
-    if (gw >= 2 * p.num_kv_heads * rows) return;
-    const int half = gw & 1, pair = gw >> 1;
-    const int kvh = pair / rows, R = pair - kvh * rows;
-    auto slot = [&](int s) { return (static_cast<int64_t>(s) * p.num_kv_heads + kvh) * rows_ws + R; };
-    const int d0 = half * 64 + lane * 2;
-    float2 o[kFastSplits];
-#pragma unroll
-    for (int u = 0; u < kFastSplits; ++u)
-      o[u] = u < S ? *reinterpret_cast<const float2*>(p.ws_o + slot(u) * kHD + d0) : make_float2(0.f, 0.f);
-    const float2 ml = lane < S ? p.ws_ml[slot(lane)] : none;
-    float M = ml.x;
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xFFFFFFFFu, M, off));
-    float2 acc = make_float2(0.f, 0.f);
-    float lsum = 0.f;
-    if (M > -INFINITY) {
-      const float w = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
-      lsum = w * ml.y;
-#pragma unroll
-      for (int u = 0; u < kFastSplits; ++u) {
-        const float wu = __shfl_sync(0xFFFFFFFFu, w, u);
-        if (u < S && wu != 0.f) {
-          acc.x = fmaf(wu, o[u].x, acc.x);
-          acc.y = fmaf(wu, o[u].y, acc.y);
-        }
-      }
-#pragma unroll
-      for (int off = 16; off > 0; off >>= 1) lsum += __shfl_xor_sync(0xFFFFFFFFu, lsum, off);
-    }
-    const float inv = lsum > 0.f ? 1.f / lsum : 0.f;
-    const int node = R / p.group, h = kvh * p.group + (R - node * p.group);
-    *reinterpret_cast<uint32_t*>(p.out + node * p.out_tok_stride + h * p.out_head_stride + d0 * 2) =
-        pack_bf16x2(acc.x * inv, acc.y * inv);
-    return;
-  }
-  const int gw = (blockIdx.x * blockDim.x + threadIdx.x) >> 5;
-  if (gw >= p.num_kv_heads * rows) return;
-  const int kvh = gw / rows, R = gw - kvh * rows;
-  auto slot = [&](int s) { return (static_cast<int64_t>(s) * p.num_kv_heads + kvh) * rows_ws + R; };
-  // lane s holds split s's (max, sum); one load per lane instead of a serial walk
-  const float2 first = lane < S ? p.ws_ml[slot(lane)] : none;
-  float M = first.x;
-  for (int base = 32; base < S; base += 32) M = fmaxf(M, base + lane < S ? p.ws_ml[slot(base + lane)].x : -INFINITY);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xFFFFFFFFu, M, o));
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  float lsum = 0.f;
-  if (M > -INFINITY) {
-    for (int base = 0; base < S; base += 32) {
-      const float2 ml = base == 0 ? first : (base + lane < S ? p.ws_ml[slot(base + lane)] : none);
-      const float w = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
-      lsum += w * ml.y;
-      const int cnt = min(32, S - base);
-      for (int j = 0; j < cnt; j += 8) {
-        float4 o[8];
-        float ww[8];
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          ww[u] = __shfl_sync(0xFFFFFFFFu, w, (j + u) & 31);
-          o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (j + u < cnt && ww[u] != 0.f)
-            o[u] = *reinterpret_cast<const float4*>(p.ws_o + slot(base + j + u) * kHD + lane * 4);
-        }
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          acc.x = fmaf(ww[u], o[u].x, acc.x);
-          acc.y = fmaf(ww[u], o[u].y, acc.y);
-          acc.z = fmaf(ww[u], o[u].z, acc.z);
-          acc.w = fmaf(ww[u], o[u].w, acc.w);
-        }
-      }
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) lsum += __shfl_xor_sync(0xFFFFFFFFu, lsum, o);
-  }
-  const float inv = lsum > 0.f ? 1.f / lsum : 0.f;
-  const int node = R / p.group, h = kvh * p.group + (R - node * p.group);
-  uint2 pk;
-  pk.x = pack_bf16x2(acc.x * inv, acc.y * inv);
-  pk.y = pack_bf16x2(acc.z * inv, acc.w * inv);
-  *reinterpret_cast<uint2*>(p.out + node * p.out_tok_stride + h * p.out_head_stride + lane * 8) = pk;
-}
-
-// ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
 static int make_kv_tmap(CUtensorMap* m, const void* base, int64_t head_stride, int64_t row_stride, int64_t capacity,
@@ -953,8 +743,6 @@ static int make_q_tmap(CUtensorMap* m, const void* q, int64_t tok_stride, int64_
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? RT_OK : RT_ERR_INVALID_ARGUMENT;
 }
-
-static int tiles_for(int n, int G) { return (n * G + kBM - 1) / kBM; }
 
 static int default_splits(int n, int G, int hkv, int64_t prefix_len, bool tc) {
   const int64_t keys = prefix_len + n;

@@ -1,82 +1,756 @@
-// Tree-verify attention over the 4-bit cache: one warp per (node, query head).
+// Tree-verify attention over the 4-bit cache (q4_row.cuh): bf16 queries, GQA,
+// head_dim 128, packed ancestor bits over the tree block.
+//
+// Few query rows (n * group <= 16: single tokens, small trees)
+// ---------------------------------------------------------------------------
+// One CTA per (key split, kv head), sixteen warps that work alone: each streams
+// 32-key tiles (2304 bytes of K, 2304 of V, contiguous) through its own 3-stage
+// ring of bulk copies and keeps its rows' running maximum, sum and output in
+// registers.  The codes go from shared memory to mma.sync fragments in
+// registers, so nothing decoded is stored:
+//   S = Q K^T  m16n8k16, n = keys: lane (g, t) = (lane / 4, lane % 4) decodes key
+//              g's group t (its four code words), and the contraction runs over
+//              values in the order the code words hold them -- Q's fragments are
+//              laid out once in that order;
+//   O += P V   k = keys: lane (g, t) decodes keys 2t, 2t+1, 2t+8, 2t+9 at code
+//              words 2g, 2g+1, pairing two keys' nibbles with one byte permute.
+// The warps' results are merged in shared memory, the splits' in the cluster
+// (distributed shared memory) or through the workspace (attn_combine_kernel).
+//
+// More query rows
+// ---------------------------------------------------------------------------
+// One CTA per (key split, kv head, 256 query rows): two 128-row tiles (row r of
+// a tile is (node r / group, query head r % group)) in ping-pong on tcgen05 as in
+// the prompt attention.  Sixteen warps:
+//   warps 0-3, 4-7  softmax of tile 0 / 1, one thread per row;
+//   warps 8-11      decode: a thread per key turns the 72 bytes of K (then V) of
+//                   a 128-key block into its row of a bf16 SW128 tile;
+//   warp 12         producer: Q by TMA, the blocks' bytes by bulk copies (9216
+//                   contiguous bytes each) into a 3-stage ring;
+//   warp 13         MMA issuer.
+//
+// What hides: the rows behind the tree are stale bytes, so the last tile reads
+// their scales as zero; a tree row that reads as NaN turns the scores of the
+// nodes that see it into NaN and counts as zero otherwise.
+#include <cuda.h>
+
+#include <mutex>
+
+#include "attn_softmax.cuh"
 #include "common.cuh"
 #include "host_util.h"
 #include "q4_row.cuh"
+#include "tmap.h"
+#include "tree_attn.cuh"
 
 namespace rt {
 
-struct Q4AttnParams {
-  const char* q;
-  int64_t q_tok_stride, q_head_stride;
-  const char* k;
-  const char* v;
-  int64_t kv_head_stride;
-  char* out;
-  int64_t out_tok_stride, out_head_stride;
-  const uint32_t* mask;
-  int mask_words, n, hq, group;
-  int64_t prefix_len;
-  const int64_t* prefix_len_dev;
-  float scale_log2;
-  int64_t capacity;
-  int* status;
-};
+constexpr int kQsWarps = 16;
+constexpr int kQsThreads = kQsWarps * 32;
+constexpr int kQsKeys = 32;                               // keys per tile
+constexpr uint32_t kQsHalf = kQsKeys * kQ4Row;            // one tile of K (or V)
+constexpr int kQsStages = 3;
+constexpr uint32_t kQsRing = kQsStages * 2 * kQsHalf;     // of one warp
+constexpr uint32_t kQsOffQ = kQsWarps * kQsRing;          // Q fragments [8 k-steps][32 lanes] x 16 bytes
+constexpr uint32_t kQsOffBar = kQsOffQ + 8 * 32 * 16;
+constexpr uint32_t kQsSmem = kQsOffBar + kQsWarps * kQsStages * 8 + 16 + 128;
+// after the key loop the rings hold the warps' results, then the CTA's
+constexpr int kQsRows = 16;
+constexpr uint32_t kQsOffPart = 0;                                       // [warp][row][128] fp32
+constexpr uint32_t kQsOffPartMl = kQsOffPart + kQsWarps * kQsRows * 512;  // [warp][row] (m, l)
+constexpr uint32_t kQsOffStage = kQsOffPartMl + kQsWarps * kQsRows * 8;   // [row][128] fp32
+constexpr uint32_t kQsOffStageMl = kQsOffStage + kQsRows * 512;           // [row] (m, l)
+static_assert(kQsOffStageMl + kQsRows * 8 <= kQsOffQ, "results fit in the rings");
 
-__global__ void __launch_bounds__(128) tree_attn_q4_simple(const Q4AttnParams p) {
+__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t q4_zero_pair(uint32_t a, uint32_t b) {
+  return 0x43004300u | (a & 15u) | ((b & 15u) << 16);
+}
+__device__ __forceinline__ uint32_t q4_scale_pair(uint32_t a, uint32_t b) { return (a & 0x7FF0u) | ((b & 0x7FF0u) << 16); }
+__device__ __forceinline__ bool q4_is_nan(uint32_t w) { return (w & 0x7F80u) == 0x7F80u; }
+
+__device__ __forceinline__ void store_bf16x4(char* dst, const float4& v) {
+  *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+}
+
+__global__ void __launch_bounds__(kQsThreads, 1) tree_attn_q4_small_kernel(const AttnParams p) {
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem =
+      reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kQsOffBar) + (threadIdx.x >> 5) * kQsStages;
+  int* abort_word = reinterpret_cast<int*>(smem + kQsOffBar + kQsWarps * kQsStages * 8);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int split = blockIdx.x, kvh = blockIdx.y, G = p.group, rows = p.n * G;
+  if (lane == 0) {
+    for (int i = 0; i < kQsStages; ++i) mbar_init(&full[i], 1);
+    if (warp == 0) *abort_word = 0;
+    fence_mbar_init();
+    fence_proxy_async_smem();
+  }
   pdl_launch_dependents();
   pdl_wait();
-  const int gw = (blockIdx.x * blockDim.x + threadIdx.x) >> 5, lane = threadIdx.x & 31;
-  if (gw >= p.n * p.hq) return;
-  const int node = gw / p.hq, h = gw - node * p.hq, g = h / p.group;
-  const int64_t L = p.prefix_len_dev ? *p.prefix_len_dev : p.prefix_len;
-  if (L < 0 || L + p.n > p.capacity) {
-    if (lane == 0) set_status(p.status, RT_DEV_BAD_INDEX);
+  const int64_t total = key_count(p), L = total - p.n;
+  if (L < 0 || total > p.capacity) {  // the same in every CTA of the launch
+    if (tid == 0) set_status(p.status, RT_DEV_BAD_INDEX);
     return;
   }
-  const char* kb = p.k + g * p.kv_head_stride;
-  const char* vb = p.v + g * p.kv_head_stride;
-  const uint2 qr = *reinterpret_cast<const uint2*>(p.q + node * p.q_tok_stride + h * p.q_head_stride + lane * 8);
-  const float q0 = __uint_as_float(qr.x << 16), q1 = __uint_as_float(qr.x & 0xFFFF0000u);
-  const float q2 = __uint_as_float(qr.y << 16), q3 = __uint_as_float(qr.y & 0xFFFF0000u);
-  auto decode4 = [&](const char* row, float (&x)[4]) {
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(row + (lane >> 1) * 4) >> ((lane & 1) * 8);
-    const uint32_t m = *reinterpret_cast<const uint16_t*>(row + kQ4Codes + (lane >> 3) * 2);
-    const uint32_t a = q4_pair(w, q4_zero2(m), q4_scale2(m)), b = q4_pair(w >> 4, q4_zero2(m), q4_scale2(m));
-    x[0] = __uint_as_float(a << 16);
-    x[1] = __uint_as_float(a & 0xFFFF0000u);
-    x[2] = __uint_as_float(b << 16);
-    x[3] = __uint_as_float(b & 0xFFFF0000u);
+  int64_t b0, b1;
+  split_range(total, split, p.num_splits, kQsKeys, b0, b1);
+  const char* kb = p.k + kvh * p.kv_head_stride;
+  const char* vb = p.v + kvh * p.kv_head_stride;
+  unsigned char* ring = smem + warp * kQsRing;
+  const int tiles = static_cast<int>(b1 - b0) > warp ? (static_cast<int>(b1 - b0) - warp + kQsWarps - 1) / kQsWarps : 0;
+  auto issue = [&](int i) {  // tile i of this warp (lane 0)
+    const int s = i % kQsStages;
+    const int64_t key0 = (b0 + warp + static_cast<int64_t>(i) * kQsWarps) * kQsKeys;
+    // an even number of rows: 16-byte pieces that end inside the (even) capacity
+    const uint32_t bytes = static_cast<uint32_t>((min(static_cast<int64_t>(kQsKeys), total - key0) + 1) & ~int64_t(1)) * kQ4Row;
+    mbar_arrive_expect_tx(&full[s], 2 * bytes);
+    bulk_load(ring + s * 2 * kQsHalf, kb + key0 * kQ4Row, bytes, &full[s]);
+    bulk_load(ring + s * 2 * kQsHalf + kQsHalf, vb + key0 * kQ4Row, bytes, &full[s]);
   };
-  float m = -INFINITY, l = 0.f, acc[4] = {};
-  for (int64_t key = 0; key < L + p.n; ++key) {
-    const int64_t t = key - L;
-    if (t >= 0 && !((p.mask[static_cast<int64_t>(node) * p.mask_words + (t >> 5)] >> (t & 31)) & 1u)) continue;
-    float x[4];
-    decode4(kb + key * kQ4Row, x);
-    float s = q0 * x[0] + q1 * x[1] + q2 * x[2] + q3 * x[3];
+  if (lane == 0)
+    for (int i = 0; i < min(tiles, kQsStages); ++i) issue(i);
+  // Q fragments in the code words' order: k-step kk of lane (g, t) holds values 32t + 4kk .. + 3 of rows g and g + 8
+  uint4* qs = reinterpret_cast<uint4*>(smem + kQsOffQ);
+  if (tid < 256) {
+    uint2 x[2];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
-    s *= p.scale_log2;
-    const float mn = fmaxf(m, s);
-    const float f = ex2(m - mn), e = ex2(s - mn);
-    decode4(vb + key * kQ4Row, x);
-    l = l * f + e;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[i] = acc[i] * f + e * x[i];
-    m = mn;
+    for (int i = 0; i < 2; ++i) {
+      const int R = g + 8 * i;
+      x[i] = make_uint2(0, 0);
+      if (R < rows) {
+        const int node = R / G, h = kvh * G + (R - node * G);
+        x[i] = *reinterpret_cast<const uint2*>(p.q + node * p.q_tok_stride + h * p.q_head_stride +
+                                               (32 * t + 4 * warp) * 2);
+      }
+    }
+    qs[tid] = make_uint4(x[0].x, x[1].x, x[0].y, x[1].y);
   }
-  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-  uint2 pk;
-  pk.x = pack_bf16x2(acc[0] * inv, acc[1] * inv);
-  pk.y = pack_bf16x2(acc[2] * inv, acc[3] * inv);
-  *reinterpret_cast<uint2*>(p.out + node * p.out_tok_stride + h * p.out_head_stride + lane * 8) = pk;
+  __syncthreads();
+
+  const float sl2 = p.scale_log2;
+  float O[16][4];
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) O[i][c] = 0.f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  const uint32_t* mrow[2];
+  bool live[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    live[i] = g + 8 * i < rows;
+    mrow[i] = p.mask + static_cast<int64_t>(live[i] ? (g + 8 * i) / G : 0) * p.mask_words;
+  }
+  bool ok = true;
+  int i = 0;
+  for (; i < tiles; ++i) {
+    const int s = i % kQsStages;
+    ok = mbar_wait(&full[s], (i / kQsStages) & 1, abort_word, p.status, RT_DEV_WAIT_TIMEOUT);
+    ok = __all_sync(0xFFFFFFFFu, ok);
+    if (!ok) break;
+    const int64_t key0 = (b0 + warp + static_cast<int64_t>(i) * kQsWarps) * kQsKeys;
+    const unsigned char* kt = ring + s * 2 * kQsHalf;
+    const unsigned char* vt = kt + kQsHalf;
+    // ---- S = Q K^T for 32 keys
+    float S[4][4];
+    {
+      uint32_t kw[4][4], z2[4], s2[4];
+#pragma unroll
+      for (int nt = 0; nt < 4; ++nt) {
+        const unsigned char* row = kt + (nt * 8 + g) * kQ4Row;
+        const uint2 a = *reinterpret_cast<const uint2*>(row + t * 16);
+        const uint2 b = *reinterpret_cast<const uint2*>(row + t * 16 + 8);
+        const uint32_t w = *reinterpret_cast<const uint16_t*>(row + kQ4Codes + t * 2);
+        kw[nt][0] = a.x;
+        kw[nt][1] = a.y;
+        kw[nt][2] = b.x;
+        kw[nt][3] = b.y;
+        z2[nt] = q4_zero2(w);
+        s2[nt] = q4_scale2(w);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) S[nt][c] = 0.f;
+      }
+#pragma unroll
+      for (int wd = 0; wd < 4; ++wd) {
+        const uint4 qa = qs[(2 * wd) * 32 + lane], qb = qs[(2 * wd + 1) * 32 + lane];
+#pragma unroll
+        for (int nt = 0; nt < 4; ++nt) {
+          const uint4 b = q4_decode8(kw[nt][wd], z2[nt], s2[nt]);
+          mma_bf16(S[nt], qa, b.x, b.y);
+          mma_bf16(S[nt], qb, b.z, b.w);
+        }
+      }
+    }
+    // ---- this lane's V codes: keys 16ks + {2t, 2t+1, 2t+8, 2t+9}, code words 2g, 2g+1
+    uint2 vw[2][4];
+    uint32_t vm[2][4];
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const unsigned char* row = vt + (ks * 16 + 2 * t + (c & 1) + 8 * (c >> 1)) * kQ4Row;
+        vw[ks][c] = *reinterpret_cast<const uint2*>(row + g * 8);
+        vm[ks][c] = *reinterpret_cast<const uint16_t*>(row + kQ4Codes + (g >> 1) * 2);
+      }
+    __syncwarp();
+    // ---- hide, online softmax
+    if (key0 + kQsKeys > L) {
+      const uint32_t vis0 = live[0] ? visible_word(key0, L, p.n, mrow[0], p.mask_words) : 0u;
+      const uint32_t vis1 = live[1] ? visible_word(key0, L, p.n, mrow[1], p.mask_words) : 0u;
+#pragma unroll
+      for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int key = nt * 8 + 2 * t + c;
+          uint32_t& w = vm[nt >> 1][(nt & 1) * 2 + c];
+          const bool bad = key0 + key < total && q4_is_nan(w);
+          if (bad || key0 + key >= total) w = 0;  // reads as zero
+          if (bad) S[nt][c] = S[nt][2 + c] = __int_as_float(0x7FC00000);
+          if (!((vis0 >> key) & 1u)) S[nt][c] = -INFINITY;
+          if (!((vis1 >> key) & 1u)) S[nt][2 + c] = -INFINITY;
+        }
+    }
+    float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) mx[c >> 1] = fmaxf(mx[c >> 1], S[nt][c]);
+    // lazy: the maximum moves when a score passes it by 8 in log2, so weights stay below 2^8
+    if (__any_sync(0xFFFFFFFFu, mx[0] * sl2 > m[0] + 8.f || mx[1] * sl2 > m[1] + 8.f)) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float x = mx[h];
+        x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 1));
+        x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 2));
+        const float mn = fmaxf(m[h], x * sl2);
+        const float f = mn == -INFINITY ? 1.f : ex2(m[h] - mn);
+        m[h] = mn;
+        l[h] *= f;
+#pragma unroll
+        for (int n = 0; n < 16; ++n) {
+          O[n][2 * h] *= f;
+          O[n][2 * h + 1] *= f;
+        }
+      }
+    }
+    const float mu0 = m[0] == -INFINITY ? 0.f : m[0], mu1 = m[1] == -INFINITY ? 0.f : m[1];
+    uint4 pf[2];
+    uint32_t pk[4][2];
+#pragma unroll
+    for (int nt = 0; nt < 4; ++nt) {
+      const float p0 = ex2(fmaf(S[nt][0], sl2, -mu0)), p1 = ex2(fmaf(S[nt][1], sl2, -mu0));
+      const float p2 = ex2(fmaf(S[nt][2], sl2, -mu1)), p3 = ex2(fmaf(S[nt][3], sl2, -mu1));
+      l[0] += p0 + p1;
+      l[1] += p2 + p3;
+      pk[nt][0] = pack_bf16x2(p0, p1);
+      pk[nt][1] = pack_bf16x2(p2, p3);
+    }
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) pf[ks] = make_uint4(pk[2 * ks][0], pk[2 * ks][1], pk[2 * ks + 1][0], pk[2 * ks + 1][1]);
+    // the stage is read: refill it
+    if (lane == 0 && i + kQsStages < tiles) issue(i + kQsStages);
+    // ---- O += P V
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      const uint32_t za = q4_zero_pair(vm[ks][0], vm[ks][1]), sa = q4_scale_pair(vm[ks][0], vm[ks][1]);
+      const uint32_t zb = q4_zero_pair(vm[ks][2], vm[ks][3]), sb = q4_scale_pair(vm[ks][2], vm[ks][3]);
+#pragma unroll
+      for (int wd = 0; wd < 2; ++wd) {
+        const uint32_t w0 = wd ? vw[ks][0].y : vw[ks][0].x, w1 = wd ? vw[ks][1].y : vw[ks][1].x;
+        const uint32_t w2 = wd ? vw[ks][2].y : vw[ks][2].x, w3 = wd ? vw[ks][3].y : vw[ks][3].x;
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          // nibble j of two keys: the words' low (or high) halves side by side
+          const uint4 x = q4_decode8(__byte_perm(w0, w1, hf ? 0x7632 : 0x5410), za, sa);
+          const uint4 y = q4_decode8(__byte_perm(w2, w3, hf ? 0x7632 : 0x5410), zb, sb);
+          mma_bf16(O[wd * 8 + hf * 4 + 0], pf[ks], x.x, y.x);
+          mma_bf16(O[wd * 8 + hf * 4 + 1], pf[ks], x.y, y.y);
+          mma_bf16(O[wd * 8 + hf * 4 + 2], pf[ks], x.z, y.z);
+          mma_bf16(O[wd * 8 + hf * 4 + 3], pf[ks], x.w, y.w);
+        }
+      }
+    }
+  }
+  if (!ok && lane == 0)  // copies in flight land before the block leaves
+    for (int j = i; j < min(tiles, i + kQsStages); ++j) mbar_wait_drain(&full[j % kQsStages], (j / kQsStages) & 1);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], 1);
+    l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], 2);
+    if (l[h] != l[h]) m[h] = INFINITY;  // a NaN weight wins every merge
+  }
+  __syncthreads();  // every warp is done with its ring
+  // ---- the warps' results side by side; column c = 2t + e of fragment n is value 16c + 8(n / 8) + order(n % 8)
+  float* part = reinterpret_cast<float*>(smem + kQsOffPart) + warp * kQsRows * 128;
+#pragma unroll
+  for (int n = 0; n < 16; ++n) {
+    const int d = 8 * (n >> 3) + ((n & 3) * 2 + ((n >> 2) & 1));
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int R = g + 8 * (c >> 1);
+      if (R < rows) part[R * 128 + 16 * (2 * t + (c & 1)) + d] = O[n][c];
+    }
+  }
+  if (t == 0) {
+    float2* ml = reinterpret_cast<float2*>(smem + kQsOffPartMl) + warp * kQsRows;
+    ml[g] = make_float2(m[0], l[0]);
+    ml[g + 8] = make_float2(m[1], l[1]);
+  }
+  __syncthreads();
+  const int S = p.num_splits;
+  for (int it = tid; it < rows * 32; it += kQsThreads) {
+    const int R = it >> 5, c = it & 31;
+    float2 ml[kQsWarps];
+    float M = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < kQsWarps; ++u) {
+      ml[u] = reinterpret_cast<const float2*>(smem + kQsOffPartMl)[u * kQsRows + R];
+      M = fmaxf(M, ml[u].x);
+    }
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float lsum = 0.f;
+#pragma unroll
+    for (int u = 0; u < kQsWarps; ++u) {
+      const float wu = ml[u].x == -INFINITY ? 0.f : ex2(ml[u].x - M);
+      if (wu != 0.f) {
+        const float4 o = reinterpret_cast<const float4*>(smem + kQsOffPart)[(u * kQsRows + R) * 32 + c];
+        lsum = fmaf(wu, ml[u].y, lsum);
+        acc.x = fmaf(wu, o.x, acc.x);
+        acc.y = fmaf(wu, o.y, acc.y);
+        acc.z = fmaf(wu, o.z, acc.z);
+        acc.w = fmaf(wu, o.w, acc.w);
+      }
+    }
+    if (p.merge > 1) {
+      reinterpret_cast<float4*>(smem + kQsOffStage)[R * 32 + c] = acc;
+      if (c == 0) reinterpret_cast<float2*>(smem + kQsOffStageMl)[R] = make_float2(M, lsum);
+    } else if (S > 1) {
+      const int64_t slot = (static_cast<int64_t>(split) * p.num_kv_heads + kvh) * kBM + R;
+      *reinterpret_cast<float4*>(p.ws_o + slot * kHD + c * 4) = acc;
+      if (c == 0) p.ws_ml[slot] = make_float2(M, lsum);
+    } else {
+      const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
+      const int node = R / G, h = kvh * G + (R - node * G);
+      store_bf16x4(p.out + node * p.out_tok_stride + h * p.out_head_stride + c * 8,
+                   make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+    }
+  }
+  if (p.merge > 1) {
+    __syncthreads();
+    cluster_sync_all();
+    const uint32_t base = smem_u32(smem);
+    for (int it = tid * S + split; it < rows * 32; it += kQsThreads * S) {
+      const int R = it >> 5, c = it & 31;
+      float2 ml[kMaxMerge];
+      float4 o[kMaxMerge];
+#pragma unroll
+      for (int u = 0; u < kMaxMerge; ++u) {
+        ml[u] = make_float2(-INFINITY, 0.f);
+        o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (u < S) {
+          ml[u] = ld_cluster_f32x2(cluster_map(base + kQsOffStageMl + R * 8, u));
+          o[u] = ld_cluster_f32x4(cluster_map(base + kQsOffStage + (R * 32 + c) * 16, u));
+        }
+      }
+      float w[kMaxMerge];
+      merge_weights(ml, w);
+      const int node = R / G, h = kvh * G + (R - node * G);
+      store_bf16x4(p.out + node * p.out_tok_stride + h * p.out_head_stride + c * 8, merge_chunk(o, S, w));
+    }
+    __syncwarp();
+    cluster_sync_all();
+  }
+}
+
+// ---------------------------------------------------------------------------
+// More query rows: decoded tiles on tcgen05
+// ---------------------------------------------------------------------------
+constexpr int kQtThreads = 512;
+// registers a thread; the block is launched with 128 x 512 (2 x 176 + 88 + 72 = 4 x 128)
+constexpr int kQtRegsSoftmax = 176, kQtRegsDecode = 88, kQtRegsOther = 72;
+constexpr int kQtKeys = 128;
+constexpr uint32_t kQtTile = 128 * 128 * 2, kQtHalf = kQtTile / 2;
+constexpr int kQtStages = 4;                          // decoded tiles
+constexpr int kQtPacked = 3;                          // blocks of bytes
+constexpr uint32_t kQtBlock = kQtKeys * kQ4Row;
+constexpr uint32_t kQtOffQ = 0;
+constexpr uint32_t kQtOffKV = 2 * kQtTile;
+constexpr uint32_t kQtOffPacked = kQtOffKV + kQtStages * kQtTile;
+constexpr uint32_t kQtOffBar = kQtOffPacked + kQtPacked * kQtBlock;
+constexpr uint32_t kQtSmem = kQtOffBar + 512 + 1024;
+constexpr uint32_t kQtTmemO = 256;                    // S0 | S1 | O0 | O1, P_t in S_t's first 64 columns
+
+struct Q4Bars {
+  uint64_t q_full[2], in_full[kQtPacked], in_empty[kQtPacked], kv_full[kQtStages], kv_empty[kQtStages], s_full[2],
+      p_full[2], o_full[2], fin;
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+// A key's row of a decoded tile: 128 bf16 values in two SW128 halves.
+__device__ __forceinline__ void q4_decode_row(const unsigned char* src, unsigned char* tile, int r, bool zero,
+                                              bool nan) {
+  const uint2 mw = *reinterpret_cast<const uint2*>(src + kQ4Codes);
+  const uint32_t meta[4] = {mw.x & 0xFFFFu, mw.x >> 16, mw.y & 0xFFFFu, mw.y >> 16};
+  unsigned char* dst = tile + r * 128;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    // (a row that must read as zero or NaN does so through its scale)
+    const uint32_t z2 = q4_zero2(meta[g]);
+    const uint32_t s2 = nan ? 0x7FC07FC0u : (zero ? 0u : q4_scale2(meta[g]));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint2 w = *reinterpret_cast<const uint2*>(src + g * 16 + i * 8);
+      const int ch = g * 4 + i * 2;
+      unsigned char* half = dst + (ch >> 3) * kQtHalf;
+      *reinterpret_cast<uint4*>(half + (((ch & 7) ^ (r & 7)) << 4)) = q4_decode8(w.x, z2, s2);
+      *reinterpret_cast<uint4*>(half + ((((ch + 1) & 7) ^ (r & 7)) << 4)) = q4_decode8(w.y, z2, s2);
+    }
+  }
+}
+
+__global__ void __launch_bounds__(kQtThreads, 1)
+    tree_attn_q4_tile_kernel(const __grid_constant__ CUtensorMap tmap_q, const AttnParams p, const int tok) {
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem =
+      reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  Q4Bars& bar = *reinterpret_cast<Q4Bars*>(smem + kQtOffBar);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int split = blockIdx.x, kvh = blockIdx.y, G = p.group;
+  const int node0 = blockIdx.z * 2 * tok;               // first node of tile 0
+  const int tiles = node0 + tok < p.n ? 2 : 1;
+  if (warp == 12 && lane == 0) {
+    prefetch_tmap(&tmap_q);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bar.q_full[i], 1);
+      mbar_init(&bar.s_full[i], 1);
+      mbar_init(&bar.p_full[i], 128);
+      mbar_init(&bar.o_full[i], 1);
+    }
+    for (int i = 0; i < kQtPacked; ++i) {
+      mbar_init(&bar.in_full[i], 1);
+      mbar_init(&bar.in_empty[i], 128);
+    }
+    for (int i = 0; i < kQtStages; ++i) {
+      mbar_init(&bar.kv_full[i], 128);
+      mbar_init(&bar.kv_empty[i], 1);
+    }
+    mbar_init(&bar.fin, 1);
+    bar.abort_flag = 0;
+    fence_mbar_init();
+    fence_proxy_async_smem();
+  }
+  if (warp == 13) {
+    tmem_alloc(&bar.tmem_base, 512);
+    tmem_relinquish();
+  }
+  pdl_wait();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_launch_dependents();
+  const uint32_t tmem = bar.tmem_base;
+  volatile int* abort_flag = &bar.abort_flag;
+  const int64_t total = key_count(p), L = total - p.n;
+  const bool inside = L >= 0 && total <= p.capacity;    // the same in every thread of the launch
+  if (!inside && tid == 0) set_status(p.status, RT_DEV_BAD_INDEX);
+  int64_t b0 = 0, b1 = 0;
+  if (inside) split_range(total, split, p.num_splits, kQtKeys, b0, b1);
+  const int nb = static_cast<int>(b1 - b0);
+
+  if (warp >= 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kQtRegsOther));
+    if (warp == 12 && lane == 0 && nb > 0) {
+      // ---------------- producer ----------------
+      bool ok = true;
+      const uint32_t qbytes = static_cast<uint32_t>(tok * G) * 256u;
+      for (int t = 0; t < tiles; ++t) {
+        unsigned char* dst = smem + kQtOffQ + t * kQtTile;
+        mbar_arrive_expect_tx(&bar.q_full[t], qbytes);
+        tma_load_3d(dst, &tmap_q, &bar.q_full[t], 0, kvh * G, node0 + t * tok);
+        tma_load_3d(dst + kQtHalf, &tmap_q, &bar.q_full[t], 64, kvh * G, node0 + t * tok);
+      }
+      const char* kb = p.k + kvh * p.kv_head_stride;
+      const char* vb = p.v + kvh * p.kv_head_stride;
+      int n = 0;
+      for (; n < 2 * nb; ++n) {
+        const int s = n % kQtPacked;
+        ok = mbar_wait(&bar.in_empty[s], ((n / kQtPacked) & 1) ^ 1, abort_flag, p.status, RT_DEV_WAIT_TIMEOUT);
+        if (!ok) break;
+        const int64_t key0 = (b0 + (n >> 1)) * kQtKeys;
+        // an even number of rows: 16-byte pieces that end inside the (even) capacity
+        const uint32_t bytes =
+            static_cast<uint32_t>((min(static_cast<int64_t>(kQtKeys), total - key0) + 1) & ~int64_t(1)) * kQ4Row;
+        mbar_arrive_expect_tx(&bar.in_full[s], bytes);
+        bulk_load(smem + kQtOffPacked + s * kQtBlock, ((n & 1) ? vb : kb) + key0 * kQ4Row, bytes, &bar.in_full[s]);
+      }
+      if (*abort_flag) {
+        for (int t = 0; t < tiles; ++t) mbar_wait_drain(&bar.q_full[t], 0);
+        for (int i = max(0, n - kQtPacked); i < n; ++i)
+          mbar_wait_drain(&bar.in_full[i % kQtPacked], (i / kQtPacked) & 1);
+      }
+    } else if (warp == 13 && lane == 0) {
+      // ---------------- MMA issuer ----------------
+      constexpr uint32_t idesc_qk = idesc_bf16_f32(kBM, kQtKeys, false, false);
+      constexpr uint32_t idesc_pv = idesc_bf16_f32(kBM, kHD, false, true);
+      const uint32_t sq = smem_u32(smem + kQtOffQ), skv = smem_u32(smem + kQtOffKV);
+      bool ok = true;
+      auto wait = [&](uint64_t* b, uint32_t ph) {
+        ok = ok && mbar_wait(b, ph & 1, abort_flag, p.status, RT_DEV_WAIT_TIMEOUT);
+        return ok;
+      };
+      auto qk = [&](int t, int stage) {
+        const uint32_t a = sq + t * kQtTile, b = skv + stage * kQtTile;
+#pragma unroll
+        for (int kk = 0; kk < kHD / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * kQtHalf + (kk & 3) * 32;
+          umma_f16(tmem + t * 128, smem_desc_sw128(a + off, 16, 1024), smem_desc_sw128(b + off, 16, 1024), idesc_qk,
+                   kk > 0);
+        }
+        umma_commit(&bar.s_full[t]);
+      };
+      for (int j = -1; j < nb && ok && nb > 0; ++j) {
+        // loads 2j+1 = V_j and 2j+2 = K_{j+1}
+        const int nv = 2 * j + 1, nk = 2 * j + 2;
+        const int sv = nv & (kQtStages - 1), sk = nk % kQtStages;
+        const bool more = j + 1 < nb;
+        if (j >= 0 && !wait(&bar.kv_full[sv], nv / kQtStages)) break;
+        for (int t = 0; t < tiles; ++t) {
+          if (j >= 0) {
+            if (!wait(&bar.p_full[t], j)) break;
+            tc_fence_after();
+            const uint32_t b = skv + sv * kQtTile;
+#pragma unroll
+            for (int kk = 0; kk < kQtKeys / 16; ++kk)
+              umma_f16_ts(tmem + kQtTmemO + t * kHD, tmem + t * 128 + kk * 8,
+                          smem_desc_sw128(b + kk * 2048, kQtHalf, 1024), idesc_pv, (j > 0 || kk > 0) ? 1u : 0u);
+            if (!more) umma_commit(&bar.o_full[t]);
+            if (t + 1 == tiles) umma_commit(&bar.kv_empty[sv]);
+          }
+          if (more) {
+            if (t == 0 && !wait(&bar.kv_full[sk], nk / kQtStages)) break;
+            if (j < 0 && !wait(&bar.q_full[t], 0)) break;
+            tc_fence_after();
+            qk(t, sk);
+          }
+        }
+        if (ok && more) umma_commit(&bar.kv_empty[sk]);
+      }
+      // all issued MMAs complete before TMEM is released
+      umma_commit(&bar.fin);
+      mbar_wait_drain(&bar.fin, 0);
+    }
+  } else if (warp >= 8) {
+    // ---------------- decode ----------------
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kQtRegsDecode));
+    const int r = tid & 127;
+    const char* vb = p.v + kvh * p.kv_head_stride;
+    for (int n = 0; n < 2 * nb; ++n) {
+      const int si = n % kQtPacked, so = n % kQtStages;
+      const int64_t key = (b0 + (n >> 1)) * kQtKeys + r;
+      bool ok = mbar_wait(&bar.in_full[si], (n / kQtPacked) & 1, abort_flag, p.status, RT_DEV_WAIT_TIMEOUT) &&
+                mbar_wait(&bar.kv_empty[so], ((n / kQtStages) & 1) ^ 1, abort_flag, p.status, RT_DEV_WAIT_TIMEOUT);
+      if (!ok) break;
+      // behind the tree: zero.  A tree row of V that reads as NaN: zero in V, and
+      // NaN in K, so that only the nodes that see the key get it.
+      bool zero = key >= total, nan = false;
+      if (key >= L && !zero && q4_is_nan(*reinterpret_cast<const uint16_t*>(vb + key * kQ4Row + kQ4Codes))) {
+        zero = (n & 1) != 0;
+        nan = !zero;
+      }
+      q4_decode_row(smem + kQtOffPacked + si * kQtBlock + r * kQ4Row, smem + kQtOffKV + so * kQtTile, r, zero, nan);
+      fence_proxy_async_smem();
+      mbar_arrive(&bar.in_empty[si]);
+      mbar_arrive(&bar.kv_full[so]);
+    }
+  } else {
+    // ---------------- softmax and result of tile t ----------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kQtRegsSoftmax));
+    const int t = warp >> 2, r = tid & 127;
+    const int rt = r / G;
+    const int node = node0 + t * tok + rt;
+    const bool valid = t < tiles && rt < tok && node < p.n;
+    const int h = kvh * G + (r - rt * G);
+    const int64_t R = static_cast<int64_t>(node) * G + (r - rt * G);
+    const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t ts = tmem + lane_base + t * 128, to = tmem + lane_base + kQtTmemO + t * kHD;
+    const uint32_t* mrow = p.mask + static_cast<int64_t>(valid ? node : 0) * p.mask_words;
+    // a warp without a query only keeps the barriers' count
+    const bool warp_live = t < tiles && ((warp & 3) * 32) / G < tok && node0 + t * tok + ((warp & 3) * 32) / G < p.n;
+    const float sl2 = p.scale_log2;
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int j = 0; j < nb && t < tiles; ++j) {
+      ok = mbar_wait(&bar.s_full[t], j & 1, abort_flag, p.status, RT_DEV_WAIT_TIMEOUT);
+      ok = __all_sync(0xFFFFFFFFu, ok);
+      if (!ok) break;
+      if (warp_live) {
+        tc_fence_after();
+        uint32_t sr[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32(ts + c * 32, sr[c]);
+        tmem_wait_ld();
+        const int64_t key0 = (b0 + j) * kQtKeys;
+        if (key0 + kQtKeys > L) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const uint32_t vm = valid ? visible_word(key0 + c * 32, L, p.n, mrow, p.mask_words) : 0u;
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (!((vm >> i) & 1u)) sr[c][i] = __float_as_uint(-INFINITY);
+          }
+        }
+        softmax_block<__nv_bfloat16>(sr, ts, to, j > 0, sl2, m, l);
+        tmem_wait_st();
+        tc_fence_before();
+      }
+      mbar_arrive(&bar.p_full[t]);
+    }
+    const int64_t rows_ws = static_cast<int64_t>(p.tiles) * kBM;
+    const int64_t slot = (static_cast<int64_t>(split) * p.num_kv_heads + kvh) * rows_ws + R;
+    if (l != l) m = INFINITY;  // a NaN weight wins the merge
+    if (ok && inside && warp_live && nb > 0) {
+      ok = mbar_wait(&bar.o_full[t], 0, abort_flag, p.status, RT_DEV_WAIT_TIMEOUT);
+      ok = __all_sync(0xFFFFFFFFu, ok);
+      if (ok) {
+        tc_fence_after();
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          uint32_t o[32];
+          tmem_ld32(to + c * 32, o);
+          tmem_wait_ld();
+          if (!valid) continue;
+          if (p.num_splits == 1) {
+            char* dst = p.out + node * p.out_tok_stride + h * p.out_head_stride + c * 64;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              uint32_t w[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                w[i] = l == 0.f ? 0u
+                                : pack_bf16x2(__uint_as_float(o[q * 8 + 2 * i]) * inv,
+                                              __uint_as_float(o[q * 8 + 2 * i + 1]) * inv);
+              *reinterpret_cast<uint4*>(dst + q * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          } else {
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+              *reinterpret_cast<uint4*>(p.ws_o + slot * kHD + c * 32 + q * 4) =
+                  make_uint4(o[q * 4], o[q * 4 + 1], o[q * 4 + 2], o[q * 4 + 3]);
+          }
+        }
+        if (valid && p.num_splits > 1) p.ws_ml[slot] = make_float2(m, l);
+        tc_fence_before();
+      }
+    } else if (inside && valid && nb == 0 && p.num_splits > 1) {
+      p.ws_ml[slot] = make_float2(-INFINITY, 0.f);
+    }
+  }
+  __syncthreads();
+  if (warp == 13) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+// Q viewed as [n nodes][Hq heads][128]: one box is `tok` nodes x G heads x 64 values.
+static int make_q4_query_tmap(CUtensorMap* m, const void* q, int64_t tok_stride, int64_t head_stride, int n, int hq,
+                              int G, int tok) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) return RT_ERR_CUDA;
+  const cuuint64_t dims[3] = {kHD, static_cast<cuuint64_t>(hq), static_cast<cuuint64_t>(n)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(head_stride), static_cast<cuuint64_t>(tok_stride)};
+  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(G), static_cast<cuuint32_t>(tok)};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(q), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? RT_OK : RT_ERR_INVALID_ARGUMENT;
+}
+
+struct Q4Plan {
+  bool small;  // the mma.sync path
+  int splits;
+  bool merge;
+};
+
+static int q4_clusters_fit(int c) {
+  static std::mutex mu;
+  static int cache[kMaxMerge + 1] = {};
+  static bool done[kMaxMerge + 1] = {};
+  std::lock_guard<std::mutex> lock(mu);
+  if (c < 2 || c > kMaxMerge) return 0;
+  if (done[c]) return cache[c];
+  int n = 0;
+  if (cudaFuncSetAttribute(tree_attn_q4_small_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           static_cast<int>(kQsSmem)) == cudaSuccess &&
+      (c <= 8 || cudaFuncSetAttribute(tree_attn_q4_small_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) ==
+                     cudaSuccess)) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(c, 1, 1);
+    cfg.blockDim = dim3(kQsThreads);
+    cfg.dynamicSmemBytes = kQsSmem;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = static_cast<unsigned>(c);
+    attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, tree_attn_q4_small_kernel, &cfg) != cudaSuccess) n = 0;
+  }
+  cudaGetLastError();
+  cache[c] = n;
+  done[c] = true;
+  return n;
+}
+
+static Q4Plan q4_plan(int n, int G, int hkv, int64_t prefix_len, int num_splits) {
+  const bool small = n * G <= kQsRows;
+  if (small) {
+    const int64_t tiles = (prefix_len + n + kQsKeys - 1) / kQsKeys;
+    int64_t want = num_splits;
+    if (want <= 0) want = std::max<int64_t>(1, std::min<int64_t>(148 / hkv, (tiles + 7) / 8));
+    want = std::min<int64_t>(std::min<int64_t>(want, tiles), 256);
+    const int s = static_cast<int>(want);
+    return {true, s, s >= 2 && s <= kMaxMerge && hkv <= q4_clusters_fit(s)};
+  }
+  const int64_t blocks = (prefix_len + n + kQtKeys - 1) / kQtKeys;
+  const int tok = kBM / G;
+  const int64_t ctas = static_cast<int64_t>(hkv) * ((n + 2 * tok - 1) / (2 * tok));
+  int64_t want = num_splits;
+  if (want <= 0) want = std::max<int64_t>(1, 148 / ctas);
+  want = std::min<int64_t>(std::min<int64_t>(want, blocks), 256);
+  return {false, static_cast<int>(want), false};
 }
 
 }  // namespace rt
 
 using namespace rt;
 
-extern "C" size_t rt_tree_attn_q4_workspace_size(int, int, int, int, int64_t, int) { return 0; }
+extern "C" size_t rt_tree_attn_q4_workspace_size(int n, int num_q_heads, int num_kv_heads, int head_dim,
+                                                 int64_t prefix_len, int num_splits) {
+  if (n <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads || head_dim != kHD ||
+      prefix_len < 0)
+    return 0;
+  const Q4Plan pl = q4_plan(n, num_q_heads / num_kv_heads, num_kv_heads, prefix_len, num_splits);
+  if (pl.splits <= 1 || pl.merge) return 0;
+  const size_t slots = static_cast<size_t>(pl.splits) * num_kv_heads * tiles_for(n, num_q_heads / num_kv_heads) * kBM;
+  return align_up(slots * kHD * 4, 256) + align_up(slots * 8, 256);
+}
 
 extern "C" int rt_tree_attn_q4(const void* q, int64_t q_tok_stride, int64_t q_head_stride, const void* k,
                                const void* v, int64_t kv_head_stride, int64_t kv_capacity, void* out,
@@ -88,7 +762,7 @@ extern "C" int rt_tree_attn_q4(const void* q, int64_t q_tok_stride, int64_t q_he
   if (n <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads || prefix_len < 0)
     return RT_ERR_INVALID_ARGUMENT;
   if (!(scale >= 0.f) || scale > 3e38f) return RT_ERR_INVALID_ARGUMENT;
-  if (head_dim != 128) return RT_ERR_UNSUPPORTED;
+  if (head_dim != kHD) return RT_ERR_UNSUPPORTED;
   if (mask_words < (n + 31) / 32) return RT_ERR_INVALID_ARGUMENT;
   if (prefix_len_dev == nullptr && prefix_len + n > kv_capacity) return RT_ERR_INVALID_ARGUMENT;
   const uint64_t align_bits = reinterpret_cast<uint64_t>(q) | reinterpret_cast<uint64_t>(k) |
@@ -97,10 +771,57 @@ extern "C" int rt_tree_attn_q4(const void* q, int64_t q_tok_stride, int64_t q_he
                               static_cast<uint64_t>(kv_head_stride) | static_cast<uint64_t>(out_tok_stride) |
                               static_cast<uint64_t>(out_head_stride);
   if ((align_bits & 15) || (kv_capacity & 1)) return RT_ERR_INVALID_ARGUMENT;
-  Q4AttnParams p{static_cast<const char*>(q), q_tok_stride, q_head_stride, static_cast<const char*>(k),
-                 static_cast<const char*>(v), kv_head_stride, static_cast<char*>(out), out_tok_stride,
-                 out_head_stride, mask, mask_words, n, num_q_heads, num_q_heads / num_kv_heads, prefix_len,
-                 prefix_len_dev, scale * 1.4426950408889634f, kv_capacity, status};
-  return record_cuda(launch_ex(tree_attn_q4_simple, dim3((n * num_q_heads + 3) / 4), dim3(128), 0,
-                               reinterpret_cast<cudaStream_t>(stream), 1, p));
+  const int G = num_q_heads / num_kv_heads;
+  if (n * G > kQsRows && G > kBM) return RT_ERR_UNSUPPORTED;
+  const Q4Plan pl = q4_plan(n, G, num_kv_heads, prefix_len, num_splits);
+  AttnParams p{};
+  p.q = static_cast<const char*>(q);
+  p.q_tok_stride = q_tok_stride;
+  p.q_head_stride = q_head_stride;
+  p.out = static_cast<char*>(out);
+  p.out_tok_stride = out_tok_stride;
+  p.out_head_stride = out_head_stride;
+  p.mask = mask;
+  p.mask_words = mask_words;
+  p.n = n;
+  p.prefix_len = prefix_len;
+  p.prefix_len_dev = prefix_len_dev;
+  p.group = G;
+  p.num_kv_heads = num_kv_heads;
+  p.tiles = tiles_for(n, G);
+  p.num_splits = pl.splits;
+  p.merge = pl.merge ? pl.splits : 1;
+  // (never 0: a hidden score is -inf and stays so; scores times 2^-126 are 0 in the sum)
+  p.scale_log2 = std::max(scale * 1.4426950408889634f, 1.17549435e-38f);
+  p.status = status;
+  p.k = static_cast<const char*>(k);
+  p.v = static_cast<const char*>(v);
+  p.kv_head_stride = kv_head_stride;
+  p.capacity = kv_capacity;
+  if (pl.splits > 1 && !pl.merge) {
+    const size_t need = rt_tree_attn_q4_workspace_size(n, num_q_heads, num_kv_heads, head_dim, prefix_len, num_splits);
+    if (workspace == nullptr || workspace_bytes < need) return RT_ERR_WORKSPACE;
+    const size_t slots = static_cast<size_t>(pl.splits) * num_kv_heads * p.tiles * kBM;
+    p.ws_o = static_cast<float*>(workspace);
+    p.ws_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + align_up(slots * kHD * 4, 256));
+  }
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  int rc;
+  if (pl.small) {
+    set_smem_limit(tree_attn_q4_small_kernel, kQsSmem);
+    rc = record_cuda(launch_ex_cluster(tree_attn_q4_small_kernel, dim3(pl.splits, num_kv_heads), dim3(kQsThreads),
+                                       kQsSmem, s, dim3(pl.merge ? pl.splits : 1, 1, 1), p));
+  } else {
+    if (q_tok_stride <= 0 || q_head_stride <= 0) return RT_ERR_UNSUPPORTED;
+    const int tok = kBM / G;
+    CUtensorMap tq;
+    rc = make_q4_query_tmap(&tq, q, q_tok_stride, q_head_stride, n, num_q_heads, G, tok);
+    if (rc != RT_OK) return rc;
+    set_smem_limit(tree_attn_q4_tile_kernel, kQtSmem);
+    const dim3 grid(pl.splits, num_kv_heads, (n + 2 * tok - 1) / (2 * tok));
+    rc = record_cuda(launch_ex(tree_attn_q4_tile_kernel, grid, dim3(kQtThreads), kQtSmem, s, 1, tq, p, tok));
+  }
+  if (rc != RT_OK || pl.merge || pl.splits == 1) return rc;
+  const int warps = num_kv_heads * n * G * (pl.splits <= kFastSplits ? 2 : 1);
+  return record_cuda(launch_ex(attn_combine_kernel, dim3((warps + 3) / 4), dim3(128), 0, s, 1, p));
 }
