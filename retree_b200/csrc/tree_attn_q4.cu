@@ -8,12 +8,16 @@
 // ring of bulk copies and keeps its rows' running maximum, sum and output in
 // registers.  The codes go from shared memory to mma.sync fragments in
 // registers, so nothing decoded is stored:
-//   S = Q K^T  m16n8k16, n = keys: lane (g, t) = (lane / 4, lane % 4) decodes key
-//              g's group t (its four code words), and the contraction runs over
-//              values in the order the code words hold them -- Q's fragments are
-//              laid out once in that order;
-//   O += P V   k = keys: lane (g, t) decodes keys 2t, 2t+1, 2t+8, 2t+9 at code
-//              words 2g, 2g+1, pairing two keys' nibbles with one byte permute.
+//   S^T = K Q^T      m16n8k16, m = keys, n = query rows: lane (g, t) = (lane / 4,
+//                    lane % 4) decodes group t of keys g and g + 8, and the
+//                    contraction runs over values in the order the code words
+//                    hold them -- Q's fragments are laid out once in that order;
+//   O^T += V^T P^T   m = values, k = keys: lane (g, t) decodes code words 2g,
+//                    2g+1 of keys 2t, 2t+1, 2t+8, 2t+9, pairing two keys' nibbles
+//                    with one byte permute; P^T comes from S^T by 8 x 8
+//                    transposes between the lanes.
+// With the queries on the n side a single token of a group of four to eight
+// heads costs one 8-wide tile, not a 16-wide one.
 // The warps' results are merged in shared memory, the splits' in the cluster
 // (distributed shared memory) or through the workspace (attn_combine_kernel).
 //
@@ -51,22 +55,32 @@ constexpr int kQsKeys = 32;                               // keys per tile
 constexpr uint32_t kQsHalf = kQsKeys * kQ4Row;            // one tile of K (or V)
 constexpr int kQsStages = 3;
 constexpr uint32_t kQsRing = kQsStages * 2 * kQsHalf;     // of one warp
-constexpr uint32_t kQsOffQ = kQsWarps * kQsRing;          // Q fragments [8 k-steps][32 lanes] x 16 bytes
-constexpr uint32_t kQsOffBar = kQsOffQ + 8 * 32 * 16;
+constexpr uint32_t kQsOffQ = kQsWarps * kQsRing;          // Q fragments [8-row tile][code word][32 lanes] x 16 bytes
+constexpr uint32_t kQsOffBar = kQsOffQ + 2 * 4 * 32 * 16;
 constexpr uint32_t kQsSmem = kQsOffBar + kQsWarps * kQsStages * 8 + 16 + 128;
 // after the key loop the rings hold the warps' results, then the CTA's
 constexpr int kQsRows = 16;
-constexpr uint32_t kQsOffPart = 0;                                       // [warp][row][128] fp32
+constexpr uint32_t kQsOffPart = 0;                                        // [warp][fragment][lane] x 16 bytes
 constexpr uint32_t kQsOffPartMl = kQsOffPart + kQsWarps * kQsRows * 512;  // [warp][row] (m, l)
-constexpr uint32_t kQsOffStage = kQsOffPartMl + kQsWarps * kQsRows * 8;   // [row][128] fp32
-constexpr uint32_t kQsOffStageMl = kQsOffStage + kQsRows * 512;           // [row] (m, l)
+constexpr uint32_t kQsOffW = kQsOffPartMl + kQsWarps * kQsRows * 8;       // [warp][row] merge weights
+constexpr uint32_t kQsStageRow = 132 * 4;                                 // (padded against bank conflicts)
+constexpr uint32_t kQsOffStage = kQsOffW + kQsWarps * kQsRows * 4;        // [row][128] fp32
+constexpr uint32_t kQsOffStageMl = kQsOffStage + kQsRows * kQsStageRow;   // [row] (m, l)
 static_assert(kQsOffStageMl + kQsRows * 8 <= kQsOffQ, "results fit in the rings");
 
-__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Transpose of an 8 x 8 tile of 16-bit values, two of a row in each lane.
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
 }
 
 __device__ __forceinline__ uint32_t q4_zero_pair(uint32_t a, uint32_t b) {
@@ -79,6 +93,8 @@ __device__ __forceinline__ void store_bf16x4(char* dst, const float4& v) {
   *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
 }
 
+// NT: 8-row tiles of queries (rows <= 8 * NT).
+template <int NT>
 __global__ void __launch_bounds__(kQsThreads, 1) tree_attn_q4_small_kernel(const AttnParams p) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem =
@@ -117,40 +133,40 @@ __global__ void __launch_bounds__(kQsThreads, 1) tree_attn_q4_small_kernel(const
   };
   if (lane == 0)
     for (int i = 0; i < min(tiles, kQsStages); ++i) issue(i);
-  // Q fragments in the code words' order: k-step kk of lane (g, t) holds values 32t + 4kk .. + 3 of rows g and g + 8
+  // Q fragments in the code words' order: word wd of lane (g, t) is values 32t + 8wd .. + 7 of row g
   uint4* qs = reinterpret_cast<uint4*>(smem + kQsOffQ);
-  if (tid < 256) {
-    uint2 x[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int R = g + 8 * i;
-      x[i] = make_uint2(0, 0);
-      if (R < rows) {
-        const int node = R / G, h = kvh * G + (R - node * G);
-        x[i] = *reinterpret_cast<const uint2*>(p.q + node * p.q_tok_stride + h * p.q_head_stride +
-                                               (32 * t + 4 * warp) * 2);
-      }
+  if (warp < 4 * NT) {
+    const int R = g + 8 * (warp >> 2);
+    uint4 x = make_uint4(0, 0, 0, 0);
+    if (R < rows) {
+      const int node = R / G, h = kvh * G + (R - node * G);
+      x = *reinterpret_cast<const uint4*>(p.q + node * p.q_tok_stride + h * p.q_head_stride +
+                                          (32 * t + 8 * (warp & 3)) * 2);
     }
-    qs[tid] = make_uint4(x[0].x, x[1].x, x[0].y, x[1].y);
+    qs[tid] = x;
   }
   __syncthreads();
 
   const float sl2 = p.scale_log2;
-  float O[16][4];
+  uint4 qr[NT == 1 ? 4 : 1];  // one tile of queries stays in registers
+  if constexpr (NT == 1) {
 #pragma unroll
-  for (int i = 0; i < 16; ++i)
+    for (int wd = 0; wd < 4; ++wd) qr[wd] = qs[wd * 32 + lane];
+  }
+  float O[8][NT][4];
+  float m[NT][2], l[NT][2];  // rows 8nt + 2t, + 1
 #pragma unroll
-    for (int c = 0; c < 4; ++c) O[i][c] = 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-  const uint32_t* mrow[2];
-  bool live[2];
+  for (int nt = 0; nt < NT; ++nt) {
+    m[nt][0] = m[nt][1] = -INFINITY;
+    l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    live[i] = g + 8 * i < rows;
-    mrow[i] = p.mask + static_cast<int64_t>(live[i] ? (g + 8 * i) / G : 0) * p.mask_words;
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) O[i][nt][c] = 0.f;
   }
   bool ok = true;
   int i = 0;
+#pragma unroll 1
   for (; i < tiles; ++i) {
     const int s = i % kQsStages;
     ok = mbar_wait(&full[s], (i / kQsStages) & 1, abort_word, p.status, RT_DEV_WAIT_TIMEOUT);
@@ -159,33 +175,36 @@ __global__ void __launch_bounds__(kQsThreads, 1) tree_attn_q4_small_kernel(const
     const int64_t key0 = (b0 + warp + static_cast<int64_t>(i) * kQsWarps) * kQsKeys;
     const unsigned char* kt = ring + s * 2 * kQsHalf;
     const unsigned char* vt = kt + kQsHalf;
-    // ---- S = Q K^T for 32 keys
-    float S[4][4];
-    {
-      uint32_t kw[4][4], z2[4], s2[4];
+    // ---- S^T = K Q^T: 16 keys (rows g, g + 8) a step
+    float S[2][NT][4];
 #pragma unroll
-      for (int nt = 0; nt < 4; ++nt) {
-        const unsigned char* row = kt + (nt * 8 + g) * kQ4Row;
+    for (int mt = 0; mt < 2; ++mt) {
+      uint32_t kw[2][4], z2[2], s2[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const unsigned char* row = kt + (mt * 16 + e * 8 + g) * kQ4Row;
         const uint2 a = *reinterpret_cast<const uint2*>(row + t * 16);
         const uint2 b = *reinterpret_cast<const uint2*>(row + t * 16 + 8);
         const uint32_t w = *reinterpret_cast<const uint16_t*>(row + kQ4Codes + t * 2);
-        kw[nt][0] = a.x;
-        kw[nt][1] = a.y;
-        kw[nt][2] = b.x;
-        kw[nt][3] = b.y;
-        z2[nt] = q4_zero2(w);
-        s2[nt] = q4_scale2(w);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) S[nt][c] = 0.f;
+        kw[e][0] = a.x;
+        kw[e][1] = a.y;
+        kw[e][2] = b.x;
+        kw[e][3] = b.y;
+        z2[e] = q4_zero2(w);
+        s2[e] = q4_scale2(w);
       }
 #pragma unroll
-      for (int wd = 0; wd < 4; ++wd) {
-        const uint4 qa = qs[(2 * wd) * 32 + lane], qb = qs[(2 * wd + 1) * 32 + lane];
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int nt = 0; nt < 4; ++nt) {
-          const uint4 b = q4_decode8(kw[nt][wd], z2[nt], s2[nt]);
-          mma_bf16(S[nt], qa, b.x, b.y);
-          mma_bf16(S[nt], qb, b.z, b.w);
+        for (int c = 0; c < 4; ++c) S[mt][nt][c] = 0.f;
+#pragma unroll
+      for (int wd = 0; wd < 4; ++wd) {
+        const uint4 a = q4_decode8(kw[0][wd], z2[0], s2[0]), b = q4_decode8(kw[1][wd], z2[1], s2[1]);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const uint4 q = NT == 1 ? qr[wd] : qs[(nt * 4 + wd) * 32 + lane];
+          mma_bf16(S[mt][nt], a.x, b.x, a.y, b.y, q.x, q.y);
+          mma_bf16(S[mt][nt], a.z, b.z, a.w, b.w, q.z, q.w);
         }
       }
     }
@@ -200,64 +219,85 @@ __global__ void __launch_bounds__(kQsThreads, 1) tree_attn_q4_small_kernel(const
         vw[ks][c] = *reinterpret_cast<const uint2*>(row + g * 8);
         vm[ks][c] = *reinterpret_cast<const uint16_t*>(row + kQ4Codes + (g >> 1) * 2);
       }
-    __syncwarp();
     // ---- hide, online softmax
     if (key0 + kQsKeys > L) {
-      const uint32_t vis0 = live[0] ? visible_word(key0, L, p.n, mrow[0], p.mask_words) : 0u;
-      const uint32_t vis1 = live[1] ? visible_word(key0, L, p.n, mrow[1], p.mask_words) : 0u;
 #pragma unroll
-      for (int nt = 0; nt < 4; ++nt)
+      for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {  // (a tree row of NaN shows up in its key's scores instead)
+          const int64_t key = key0 + ks * 16 + 2 * t + (c & 1) + 8 * (c >> 1);
+          if (key >= total || (key >= L && q4_is_nan(vm[ks][c]))) vm[ks][c] = 0;
+        }
+      uint32_t bad = 0;  // bit 2 mt + e: this lane's key 16mt + 8e + g is such a row
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int key = e * 8 + g;
+        if (key0 + key >= L && key0 + key < total &&
+            q4_is_nan(*reinterpret_cast<const uint16_t*>(vt + key * kQ4Row + kQ4Codes)))
+          bad |= 1u << e;
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          const int key = nt * 8 + 2 * t + c;
-          uint32_t& w = vm[nt >> 1][(nt & 1) * 2 + c];
-          const bool bad = key0 + key < total && q4_is_nan(w);
-          if (bad || key0 + key >= total) w = 0;  // reads as zero
-          if (bad) S[nt][c] = S[nt][2 + c] = __int_as_float(0x7FC00000);
-          if (!((vis0 >> key) & 1u)) S[nt][c] = -INFINITY;
-          if (!((vis1 >> key) & 1u)) S[nt][2 + c] = -INFINITY;
+          const int R = nt * 8 + 2 * t + c;
+          const uint32_t vis =
+              R < rows ? visible_word(key0, L, p.n, p.mask + static_cast<int64_t>(R / G) * p.mask_words, p.mask_words)
+                       : 0u;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float& x = S[e >> 1][nt][2 * (e & 1) + c];
+            if ((bad >> e) & 1u) x = __int_as_float(0x7FC00000);
+            if (!((vis >> (e * 8 + g)) & 1u)) x = -INFINITY;
+          }
         }
     }
-    float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-    for (int nt = 0; nt < 4; ++nt)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) mx[c >> 1] = fmaxf(mx[c >> 1], S[nt][c]);
     // lazy: the maximum moves when a score passes it by 8 in log2, so weights stay below 2^8
-    if (__any_sync(0xFFFFFFFFu, mx[0] * sl2 > m[0] + 8.f || mx[1] * sl2 > m[1] + 8.f)) {
+    bool need = false;
+    float mx[NT][2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float x = mx[h];
-        x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 1));
-        x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 2));
-        const float mn = fmaxf(m[h], x * sl2);
-        const float f = mn == -INFINITY ? 1.f : ex2(m[h] - mn);
-        m[h] = mn;
-        l[h] *= f;
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int n = 0; n < 16; ++n) {
-          O[n][2 * h] *= f;
-          O[n][2 * h + 1] *= f;
+      for (int c = 0; c < 2; ++c) {
+        mx[nt][c] = sl2 * fmaxf(fmaxf(S[0][nt][c], S[0][nt][2 + c]), fmaxf(S[1][nt][c], S[1][nt][2 + c]));
+        need |= mx[nt][c] > m[nt][c] + 8.f;
+      }
+    if (__any_sync(0xFFFFFFFFu, need)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float x = mx[nt][c];
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, o));
+          const float mn = fmaxf(m[nt][c], x);
+          const float f = mn == -INFINITY ? 1.f : ex2(m[nt][c] - mn);
+          m[nt][c] = mn;
+          l[nt][c] *= f;
+#pragma unroll
+          for (int n = 0; n < 8; ++n) {
+            O[n][nt][c] *= f;
+            O[n][nt][2 + c] *= f;
+          }
         }
+    }
+    // weights, transposed into the B fragments of P V: pf[ks][nt] = keys 2t, 2t+1 | + 8 of row g
+    uint2 pf[2][NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const float mu0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], mu1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+        const float p0 = ex2(fmaf(S[mt][nt][0], sl2, -mu0)), p1 = ex2(fmaf(S[mt][nt][1], sl2, -mu1));
+        const float p2 = ex2(fmaf(S[mt][nt][2], sl2, -mu0)), p3 = ex2(fmaf(S[mt][nt][3], sl2, -mu1));
+        l[nt][0] += p0 + p2;
+        l[nt][1] += p1 + p3;
+        pf[mt][nt] = make_uint2(transpose8x8(pack_bf16x2(p0, p1)), transpose8x8(pack_bf16x2(p2, p3)));
       }
     }
-    const float mu0 = m[0] == -INFINITY ? 0.f : m[0], mu1 = m[1] == -INFINITY ? 0.f : m[1];
-    uint4 pf[2];
-    uint32_t pk[4][2];
-#pragma unroll
-    for (int nt = 0; nt < 4; ++nt) {
-      const float p0 = ex2(fmaf(S[nt][0], sl2, -mu0)), p1 = ex2(fmaf(S[nt][1], sl2, -mu0));
-      const float p2 = ex2(fmaf(S[nt][2], sl2, -mu1)), p3 = ex2(fmaf(S[nt][3], sl2, -mu1));
-      l[0] += p0 + p1;
-      l[1] += p2 + p3;
-      pk[nt][0] = pack_bf16x2(p0, p1);
-      pk[nt][1] = pack_bf16x2(p2, p3);
-    }
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks) pf[ks] = make_uint4(pk[2 * ks][0], pk[2 * ks][1], pk[2 * ks + 1][0], pk[2 * ks + 1][1]);
-    // the stage is read: refill it
+    // the stage is read (every lane has taken part in the votes above): refill it
     if (lane == 0 && i + kQsStages < tiles) issue(i + kQsStages);
-    // ---- O += P V
+    // ---- O^T += V^T P^T: a step is 16 keys; an m-tile two values of every lane g's sixteen
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       const uint32_t za = q4_zero_pair(vm[ks][0], vm[ks][1]), sa = q4_scale_pair(vm[ks][0], vm[ks][1]);
@@ -268,13 +308,15 @@ __global__ void __launch_bounds__(kQsThreads, 1) tree_attn_q4_small_kernel(const
         const uint32_t w2 = wd ? vw[ks][2].y : vw[ks][2].x, w3 = wd ? vw[ks][3].y : vw[ks][3].x;
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
-          // nibble j of two keys: the words' low (or high) halves side by side
+          // nibbles of two keys: the words' low (or high) halves side by side
           const uint4 x = q4_decode8(__byte_perm(w0, w1, hf ? 0x7632 : 0x5410), za, sa);
           const uint4 y = q4_decode8(__byte_perm(w2, w3, hf ? 0x7632 : 0x5410), zb, sb);
-          mma_bf16(O[wd * 8 + hf * 4 + 0], pf[ks], x.x, y.x);
-          mma_bf16(O[wd * 8 + hf * 4 + 1], pf[ks], x.y, y.y);
-          mma_bf16(O[wd * 8 + hf * 4 + 2], pf[ks], x.z, y.z);
-          mma_bf16(O[wd * 8 + hf * 4 + 3], pf[ks], x.w, y.w);
+          const int o = wd * 4 + hf * 2;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            mma_bf16(O[o][nt], x.x, x.y, y.x, y.y, pf[ks][nt].x, pf[ks][nt].y);
+            mma_bf16(O[o + 1][nt], x.z, x.w, y.z, y.w, pf[ks][nt].x, pf[ks][nt].y);
+          }
         }
       }
     }
@@ -282,69 +324,74 @@ __global__ void __launch_bounds__(kQsThreads, 1) tree_attn_q4_small_kernel(const
   if (!ok && lane == 0)  // copies in flight land before the block leaves
     for (int j = i; j < min(tiles, i + kQsStages); ++j) mbar_wait_drain(&full[j % kQsStages], (j / kQsStages) & 1);
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], 1);
-    l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], 2);
-    if (l[h] != l[h]) m[h] = INFINITY;  // a NaN weight wins every merge
-  }
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) l[nt][c] += __shfl_xor_sync(0xFFFFFFFFu, l[nt][c], o);
+      if (l[nt][c] != l[nt][c]) m[nt][c] = INFINITY;  // a NaN weight wins every merge
+    }
   __syncthreads();  // every warp is done with its ring
-  // ---- the warps' results side by side; column c = 2t + e of fragment n is value 16c + 8(n / 8) + order(n % 8)
-  float* part = reinterpret_cast<float*>(smem + kQsOffPart) + warp * kQsRows * 128;
+  float4* part = reinterpret_cast<float4*>(smem + kQsOffPart);
 #pragma unroll
-  for (int n = 0; n < 16; ++n) {
-    const int d = 8 * (n >> 3) + ((n & 3) * 2 + ((n >> 2) & 1));
+  for (int n = 0; n < 8; ++n)
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const int R = g + 8 * (c >> 1);
-      if (R < rows) part[R * 128 + 16 * (2 * t + (c & 1)) + d] = O[n][c];
+    for (int nt = 0; nt < NT; ++nt)
+      part[((warp * 8 + n) * NT + nt) * 32 + lane] = make_float4(O[n][nt][0], O[n][nt][1], O[n][nt][2], O[n][nt][3]);
+  if (g == 0) {
+    float2* ml = reinterpret_cast<float2*>(smem + kQsOffPartMl) + warp * kQsRows;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) ml[nt * 8 + 2 * t + c] = make_float2(m[nt][c], l[nt][c]);
+  }
+  __syncthreads();
+  // ---- the warps' merge weights 2^(m_u - M), and the rows' (M, sum)
+  float* wtab = reinterpret_cast<float*>(smem + kQsOffW);
+  if (tid < kQsWarps * 8 * NT) {
+    const float2* ml = reinterpret_cast<const float2*>(smem + kQsOffPartMl);
+    const int R = tid % (8 * NT), u = tid / (8 * NT);
+    float M = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < kQsWarps; ++x) M = fmaxf(M, ml[x * kQsRows + R].x);
+    auto weight = [&](int x) { return ml[x * kQsRows + R].x == -INFINITY ? 0.f : ex2(ml[x * kQsRows + R].x - M); };
+    wtab[u * kQsRows + R] = weight(u);
+    if (u == 0) {
+      float lsum = 0.f;
+#pragma unroll
+      for (int x = 0; x < kQsWarps; ++x) lsum = fmaf(weight(x), ml[x * kQsRows + R].y, lsum);
+      reinterpret_cast<float2*>(smem + kQsOffStageMl)[R] = make_float2(M, lsum);
     }
   }
-  if (t == 0) {
-    float2* ml = reinterpret_cast<float2*>(smem + kQsOffPartMl) + warp * kQsRows;
-    ml[g] = make_float2(m[0], l[0]);
-    ml[g + 8] = make_float2(m[1], l[1]);
+  __syncthreads();
+  // ---- their sum, into rows: lane (g, t) of fragment n = 4wd + 2hf + q holds values 16g + 8wd + (nibble order)
+  for (int it = tid; it < 8 * NT * 32; it += kQsThreads) {
+    const int nt = (it >> 5) % NT, n = (it >> 5) / NT, it_g = (it & 31) >> 2, R = nt * 8 + 2 * (it & 3);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int u = 0; u < kQsWarps; ++u) {
+      const float2 w = *reinterpret_cast<const float2*>(wtab + u * kQsRows + R);
+      const float4 o = part[((u * 8 + n) * NT + nt) * 32 + (it & 31)];
+      acc.x = fmaf(w.x, o.x, acc.x);
+      acc.y = fmaf(w.y, o.y, acc.y);
+      acc.z = fmaf(w.x, o.z, acc.z);
+      acc.w = fmaf(w.y, o.w, acc.w);
+    }
+    const int d = 16 * it_g + 8 * (n >> 2) + ((n >> 1) & 1) + 4 * (n & 1);
+    float* row = reinterpret_cast<float*>(smem + kQsOffStage + R * kQsStageRow) + d;
+    float* next = reinterpret_cast<float*>(smem + kQsOffStage + (R + 1) * kQsStageRow) + d;
+    row[0] = acc.x;
+    next[0] = acc.y;
+    row[2] = acc.z;
+    next[2] = acc.w;
   }
   __syncthreads();
   const int S = p.num_splits;
-  for (int it = tid; it < rows * 32; it += kQsThreads) {
-    const int R = it >> 5, c = it & 31;
-    float2 ml[kQsWarps];
-    float M = -INFINITY;
-#pragma unroll
-    for (int u = 0; u < kQsWarps; ++u) {
-      ml[u] = reinterpret_cast<const float2*>(smem + kQsOffPartMl)[u * kQsRows + R];
-      M = fmaxf(M, ml[u].x);
-    }
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    float lsum = 0.f;
-#pragma unroll
-    for (int u = 0; u < kQsWarps; ++u) {
-      const float wu = ml[u].x == -INFINITY ? 0.f : ex2(ml[u].x - M);
-      if (wu != 0.f) {
-        const float4 o = reinterpret_cast<const float4*>(smem + kQsOffPart)[(u * kQsRows + R) * 32 + c];
-        lsum = fmaf(wu, ml[u].y, lsum);
-        acc.x = fmaf(wu, o.x, acc.x);
-        acc.y = fmaf(wu, o.y, acc.y);
-        acc.z = fmaf(wu, o.z, acc.z);
-        acc.w = fmaf(wu, o.w, acc.w);
-      }
-    }
-    if (p.merge > 1) {
-      reinterpret_cast<float4*>(smem + kQsOffStage)[R * 32 + c] = acc;
-      if (c == 0) reinterpret_cast<float2*>(smem + kQsOffStageMl)[R] = make_float2(M, lsum);
-    } else if (S > 1) {
-      const int64_t slot = (static_cast<int64_t>(split) * p.num_kv_heads + kvh) * kBM + R;
-      *reinterpret_cast<float4*>(p.ws_o + slot * kHD + c * 4) = acc;
-      if (c == 0) p.ws_ml[slot] = make_float2(M, lsum);
-    } else {
-      const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
-      const int node = R / G, h = kvh * G + (R - node * G);
-      store_bf16x4(p.out + node * p.out_tok_stride + h * p.out_head_stride + c * 8,
-                   make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
-    }
-  }
+  auto out_at = [&](int R, int c) {
+    const int node = R / G, h = kvh * G + (R - node * G);
+    return p.out + node * p.out_tok_stride + h * p.out_head_stride + c * 8;
+  };
   if (p.merge > 1) {
-    __syncthreads();
     cluster_sync_all();
     const uint32_t base = smem_u32(smem);
     for (int it = tid * S + split; it < rows * 32; it += kQsThreads * S) {
@@ -357,16 +404,29 @@ __global__ void __launch_bounds__(kQsThreads, 1) tree_attn_q4_small_kernel(const
         o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (u < S) {
           ml[u] = ld_cluster_f32x2(cluster_map(base + kQsOffStageMl + R * 8, u));
-          o[u] = ld_cluster_f32x4(cluster_map(base + kQsOffStage + (R * 32 + c) * 16, u));
+          o[u] = ld_cluster_f32x4(cluster_map(base + kQsOffStage + R * kQsStageRow + c * 16, u));
         }
       }
       float w[kMaxMerge];
       merge_weights(ml, w);
-      const int node = R / G, h = kvh * G + (R - node * G);
-      store_bf16x4(p.out + node * p.out_tok_stride + h * p.out_head_stride + c * 8, merge_chunk(o, S, w));
+      store_bf16x4(out_at(R, c), merge_chunk(o, S, w));
     }
     __syncwarp();
     cluster_sync_all();
+    return;
+  }
+  for (int it = tid; it < rows * 32; it += kQsThreads) {
+    const int R = it >> 5, c = it & 31;
+    float4 acc = *reinterpret_cast<const float4*>(smem + kQsOffStage + R * kQsStageRow + c * 16);
+    const float2 ml = reinterpret_cast<const float2*>(smem + kQsOffStageMl)[R];
+    if (S > 1) {
+      const int64_t slot = (static_cast<int64_t>(split) * p.num_kv_heads + kvh) * kBM + R;
+      *reinterpret_cast<float4*>(p.ws_o + slot * kHD + c * 4) = acc;
+      if (c == 0) p.ws_ml[slot] = ml;
+    } else {
+      const float inv = ml.y == 0.f ? 0.f : 1.f / ml.y;
+      store_bf16x4(out_at(R, c), make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+    }
   }
 }
 
@@ -695,9 +755,9 @@ static int q4_clusters_fit(int c) {
   if (c < 2 || c > kMaxMerge) return 0;
   if (done[c]) return cache[c];
   int n = 0;
-  if (cudaFuncSetAttribute(tree_attn_q4_small_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  if (cudaFuncSetAttribute(tree_attn_q4_small_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            static_cast<int>(kQsSmem)) == cudaSuccess &&
-      (c <= 8 || cudaFuncSetAttribute(tree_attn_q4_small_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) ==
+      (c <= 8 || cudaFuncSetAttribute(tree_attn_q4_small_kernel<2>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) ==
                      cudaSuccess)) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(c, 1, 1);
@@ -710,12 +770,20 @@ static int q4_clusters_fit(int c) {
     attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    if (cudaOccupancyMaxActiveClusters(&n, tree_attn_q4_small_kernel, &cfg) != cudaSuccess) n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, tree_attn_q4_small_kernel<2>, &cfg) != cudaSuccess) n = 0;
   }
   cudaGetLastError();
   cache[c] = n;
   done[c] = true;
   return n;
+}
+
+template <int NT>
+static int launch_q4_small(dim3 grid, dim3 cluster, cudaStream_t s, const AttnParams& p) {
+  set_smem_limit(tree_attn_q4_small_kernel<NT>, kQsSmem);
+  if (cluster.x > 8) cudaFuncSetAttribute(tree_attn_q4_small_kernel<NT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  return record_cuda(
+      launch_ex_cluster(tree_attn_q4_small_kernel<NT>, grid, dim3(kQsThreads), kQsSmem, s, cluster, p));
 }
 
 static Q4Plan q4_plan(int n, int G, int hkv, int64_t prefix_len, int num_splits) {
@@ -808,9 +876,8 @@ extern "C" int rt_tree_attn_q4(const void* q, int64_t q_tok_stride, int64_t q_he
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   int rc;
   if (pl.small) {
-    set_smem_limit(tree_attn_q4_small_kernel, kQsSmem);
-    rc = record_cuda(launch_ex_cluster(tree_attn_q4_small_kernel, dim3(pl.splits, num_kv_heads), dim3(kQsThreads),
-                                       kQsSmem, s, dim3(pl.merge ? pl.splits : 1, 1, 1), p));
+    const dim3 grid(pl.splits, num_kv_heads), cluster(pl.merge ? pl.splits : 1, 1, 1);
+    rc = n * G <= 8 ? launch_q4_small<1>(grid, cluster, s, p) : launch_q4_small<2>(grid, cluster, s, p);
   } else {
     if (q_tok_stride <= 0 || q_head_stride <= 0) return RT_ERR_UNSUPPORTED;
     const int tok = kBM / G;

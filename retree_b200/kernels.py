@@ -613,17 +613,32 @@ def recovery_walk(parents: torch.Tensor, tokens: torch.Tensor, posterior: torch.
 
 
 # ---------------------------------------------------------------------------
-# Attention over whole prompts
+# Attention over whole prompts, 4-bit KV cache
+#
+# A call of these takes a few microseconds on the GPU, so the wrappers test one
+# condition on the common layout and look for the reason only when it fails.
 # ---------------------------------------------------------------------------
-def _same_device(dev, **tensors) -> None:
-    for name, t in tensors.items():
-        if t is not None and t.device != dev:
-            raise RuntimeError(f"{name} must be on {dev}")
+Q4_ROW_BYTES = _lib.RT_Q4_ROW_BYTES
 
 
-def _no_grad(*tensors) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise RuntimeError("retree_b200 attention and cache kernels are inference-only (no gradient)")
+def _raw_stream(dev) -> int:
+    return torch._C._cuda_getCurrentRawStream(dev.index)
+
+
+def _elsewhere(dev) -> bool:
+    return torch.cuda.current_device() != dev.index
+
+
+def _refuse(what: str, *conditions) -> None:
+    """Raise for the first of ``(ok, reason)`` that does not hold."""
+    for ok, reason in conditions:
+        if not ok:
+            raise RuntimeError(f"{what}: {reason}")
+    raise RuntimeError(f"{what}: tensors must be on one device")
+
+
+def _needs_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
 
 
 def _workspace(nbytes: int, dev) -> torch.Tensor | None:
@@ -631,40 +646,46 @@ def _workspace(nbytes: int, dev) -> torch.Tensor | None:
     return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
 
 
-def _cu_seqlens(t: torch.Tensor | None, name: str) -> None:
-    if t is not None and (t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or t.numel() < 2):
-        raise RuntimeError(f"{name} must be a contiguous int32 tensor of at least two offsets")
+def _offsets(t) -> bool:
+    return t.dtype is torch.int32 and t.dim() == 1 and t.numel() >= 2 and t.is_contiguous()
 
 
-def _query(q: torch.Tensor) -> torch.Tensor:
+def _one_batch(t: torch.Tensor, what: str) -> torch.Tensor:
+    if t.dim() == 4 and t.shape[0] == 1:
+        return t[0]
+    if t.dim() != 3:
+        raise RuntimeError(f"{what}: expected three dimensions, or four with a batch of 1 (pack sequences along the "
+                           "token axis)")
+    return t
+
+
+def _query(q: torch.Tensor, what: str) -> torch.Tensor:
     """``[n, Hq, 128]`` view of a query in that layout or HF's ``[1, Hq, n, 128]``."""
-    if q.dim() == 4:
-        if q.shape[0] != 1:
-            raise RuntimeError("batch size 1 only (pack sequences along the token axis)")
-        q = q[0].transpose(0, 1)
-    if q.dim() != 3 or q.shape[-1] != 128 or q.stride(-1) != 1:
-        raise RuntimeError("query must be [tokens, heads, 128] (or [1, heads, tokens, 128]) with contiguous head_dim")
-    return q
+    return q if q.dim() == 3 else _one_batch(q, what).transpose(0, 1)
 
 
-def _attn_out(out: torch.Tensor | None, q: torch.Tensor) -> torch.Tensor:
+def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int, int]:
+    """``t`` and the byte strides of its two leading axes (any aligned number for an axis of one).
+
+    A tensor that repeats a row (a zero stride, which a tensor map does not describe) is copied.
+    """
+    a, b, _ = t.stride()
+    if a > 0 and b > 0 and t.shape[0] > 1 and t.shape[1] > 1:
+        return t, 2 * a, 2 * b
+    if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
+        t = t.contiguous()
+        a, b, _ = t.stride()
+    return t, 2 * a if t.shape[0] > 1 else 256, 2 * b if t.shape[1] > 1 else 256
+
+
+def _attn_out(out: torch.Tensor | None, q: torch.Tensor, what: str) -> torch.Tensor:
     if out is None:
-        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    if out.shape != q.shape or out.dtype != q.dtype or out.stride(-1) != 1 or \
+        return q.new_empty(q.shape)
+    if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(-1) != 1 or \
             any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
-        raise RuntimeError(f"out must be {q.dtype} {list(q.shape)} with contiguous head_dim and rows of its own")
+        raise RuntimeError(f"{what}: out must be {q.dtype} {list(q.shape)} on {q.device} with contiguous head_dim and "
+                           "rows of its own")
     return out
-
-
-def _byte_strides(t: torch.Tensor) -> tuple[int, int]:
-    """Byte strides of the two leading axes of ``[a, b, 128]`` (any aligned number for an axis of one)."""
-    es = t.element_size()
-    return tuple(s * es if n > 1 else 256 for n, s in zip(t.shape[:2], t.stride()))
-
-
-def _rows_apart(t: torch.Tensor) -> torch.Tensor:
-    """``t``, copied if it repeats a row (a zero stride, which a tensor map does not describe)."""
-    return t.contiguous() if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())) else t
 
 
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens_q: torch.Tensor | None = None,
@@ -682,115 +703,148 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     key give zero rows; rows outside every sequence are not written.
     Returns ``out`` ``[T, Hq, 128]``.
     """
-    lib = _lib.load()
-    _require_cuda(q, k, v, cu_seqlens_q, cu_seqlens_k, out)
-    _no_grad(q, k, v)
-    q, k, v = _query(q), _as3(k), _as3(v)
-    if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
-        raise RuntimeError("prompt attention runs on bf16 or fp16 q/k/v of one type")
-    q, k, v = _rows_apart(q), _rows_apart(k), _rows_apart(v)
-    if k.shape != v.shape or _byte_strides(k) != _byte_strides(v):
-        raise RuntimeError("K and V must share shape and strides")
-    t, hq, d = q.shape
-    hkv, tk = k.shape[:2]
-    if k.shape[2] != d or hkv == 0 or hq == 0 or hq % hkv:
-        raise RuntimeError("key heads must divide query heads, with head_dim 128")
+    what = "prompt_attention"
+    q = _query(q, what)
+    if k.dim() != 3 or v.dim() != 3:
+        k, v = _one_batch(k, what), _one_batch(v, what)
     dev = q.device
-    _same_device(dev, k=k, v=v, cu_seqlens_q=cu_seqlens_q, cu_seqlens_k=cu_seqlens_k, out=out)
-    _cu_seqlens(cu_seqlens_q, "cu_seqlens_q")
-    _cu_seqlens(cu_seqlens_k, "cu_seqlens_k")
-    if cu_seqlens_q is None and cu_seqlens_k is not None:
-        raise RuntimeError("cu_seqlens_k needs cu_seqlens_q")
-    if cu_seqlens_k is not None and cu_seqlens_k.numel() != cu_seqlens_q.numel():
-        raise RuntimeError("cu_seqlens_q and cu_seqlens_k must name the same number of sequences")
-    seqs = 1 if cu_seqlens_q is None else cu_seqlens_q.numel() - 1
-    out = _attn_out(out, q)
+    t, hq, d = q.shape
+    hkv, tk, dk = k.shape
+    dt = q.dtype
+    cq, ck = cu_seqlens_q, cu_seqlens_k
+    if not (q.is_cuda and k.device == dev and v.device == dev and (dt is torch.bfloat16 or dt is torch.float16)
+            and k.dtype is dt and v.dtype is dt and d == 128 and dk == 128 and q.stride(2) == 1 and k.stride(2) == 1
+            and k.shape == v.shape and v.stride(2) == 1 and hq and hkv and hq % hkv == 0
+            and (ck is None or (cq is not None and _offsets(ck) and ck.device == dev and ck.numel() == cq.numel()))
+            and (cq is None or (_offsets(cq) and cq.device == dev)) and not _needs_grad(q, k, v)):
+        _refuse(what,
+                (q.is_cuda and k.is_cuda and v.is_cuda, "takes CUDA tensors (no CPU path)"),
+                (not _needs_grad(q, k, v), "inference-only (no gradient)"),
+                (dt in (torch.bfloat16, torch.float16) and k.dtype == dt and v.dtype == dt,
+                 "runs on bf16 or fp16 q/k/v of one type"),
+                (d == 128 and dk == 128 and q.stride(2) == 1 and k.stride(2) == 1 and v.stride(2) == 1,
+                 "head_dim must be 128 and contiguous"),
+                (k.shape == v.shape, "K and V must share their shape"),
+                (hq and hkv and hq % hkv == 0, "key heads must divide query heads"),
+                (cq is not None or ck is None, "cu_seqlens_k needs cu_seqlens_q"),
+                (all(x is None or _offsets(x) for x in (cq, ck)),
+                 "cu_seqlens must be contiguous int32 tensors of at least two offsets"),
+                (ck is None or cq is None or ck.numel() == cq.numel(), "cu_seqlens must name the same number of sequences"))
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return prompt_attention(q, k, v, cq, ck, scale, out)
+    q, q0, q1 = _rows(q)
+    k, k0, k1 = _rows(k)
+    v, v0, v1 = _rows(v)
+    if (k0, k1) != (v0, v1):
+        raise RuntimeError(f"{what}: K and V must share strides")
+    out = _attn_out(out, q, what)
     if t == 0:
         return out
-    with torch.cuda.device(dev):
-        nbytes = lib.rt_prompt_attn_workspace_size(t, tk, seqs, hq, hkv)
-        ws = _workspace(nbytes, dev)
-        rc = lib.rt_prompt_attn(q.data_ptr(), *_byte_strides(q), k.data_ptr(), v.data_ptr(), *_byte_strides(k),
-                                out.data_ptr(), *_byte_strides(out), _DTYPE_CODE[q.dtype], _ptr(cu_seqlens_q),
-                                _ptr(cu_seqlens_k), seqs, t, tk, hq, hkv, d,
-                                d ** -0.5 if scale is None else float(scale), _ptr(ws), nbytes,
-                                _STATE.status(dev).data_ptr(), _stream(dev))
-    _lib.check(rc, "rt_prompt_attn")
+    _, o0, o1 = _rows(out)
+    seqs = 1 if cq is None else cq.numel() - 1
+    lib = _lib.load()
+    nbytes = lib.rt_prompt_attn_workspace_size(t, tk, seqs, hq, hkv)
+    ws = _workspace(nbytes, dev)
+    rc = lib.rt_prompt_attn(q.data_ptr(), q0, q1, k.data_ptr(), v.data_ptr(), k0, k1, out.data_ptr(), o0, o1,
+                            _DTYPE_CODE[dt], None if cq is None else cq.data_ptr(),
+                            None if ck is None else ck.data_ptr(), seqs, t, tk, hq, hkv, d,
+                            128 ** -0.5 if scale is None else float(scale), None if ws is None else ws.data_ptr(), nbytes,
+                            _STATE.status(dev).data_ptr(), _raw_stream(dev))
+    if rc:
+        _lib.check(rc, "rt_prompt_attn")
     _count(2 if nbytes else 1)
     return out
 
 
-# ---------------------------------------------------------------------------
-# 4-bit KV cache
-# ---------------------------------------------------------------------------
-Q4_ROW_BYTES = _lib.RT_Q4_ROW_BYTES
-
-
-def _q4_cache(t: torch.Tensor, name: str) -> torch.Tensor:
-    if t.dtype != torch.uint8 or t.dim() != 3 or t.shape[-1] != Q4_ROW_BYTES or t.stride(-1) != 1 or \
-            t.stride(-2) != Q4_ROW_BYTES:
-        raise RuntimeError(f"{name} must be uint8 [heads, capacity, {Q4_ROW_BYTES}] with contiguous rows")
-    return t
+def _q4_rows(t: torch.Tensor) -> bool:
+    """Whether ``t`` is a 4-bit cache ``[heads, capacity, 72]`` with contiguous rows."""
+    return t.is_cuda and t.dtype is torch.uint8 and t.dim() == 3 and t.shape[2] == Q4_ROW_BYTES and \
+        t.stride()[1:] == (Q4_ROW_BYTES, 1)
 
 
 def kv_append_q4(k_cache: torch.Tensor, v_cache: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor,
                  offset: int = 0, offset_dev: torch.Tensor | None = None) -> None:
-    """Quantise ``[heads, n, 128]`` bf16 rows into rows ``offset..`` of 4-bit caches ``[heads, cap, 72]`` (uint8)."""
-    lib = _lib.load()
-    _require_cuda(k_cache, v_cache, k_new, v_new, offset_dev)
-    _no_grad(k_new, v_new)
-    k_cache, v_cache = _q4_cache(k_cache, "k_cache"), _q4_cache(v_cache, "v_cache")
-    k_new, v_new = _as3(k_new), _as3(v_new)
-    if k_new.dtype != torch.bfloat16 or v_new.dtype != torch.bfloat16:
-        raise RuntimeError("kv_append_q4 takes bf16 rows")
-    if k_cache.shape != v_cache.shape or k_cache.stride() != v_cache.stride():
-        raise RuntimeError("K and V caches must share shape and strides")
-    if k_new.shape != v_new.shape or k_new.shape[0] != k_cache.shape[0] or k_new.shape[2] != 128:
-        raise RuntimeError("new rows must be [cache heads, n, 128], the same for K and V")
-    if offset_dev is not None and offset_dev.dtype != torch.int64:
-        raise RuntimeError("offset_dev must be int64")
-    if _byte_strides(k_new) != _byte_strides(v_new):
-        k_new, v_new = k_new.contiguous(), v_new.contiguous()
+    """Quantise ``[heads, n, 128]`` bf16 rows into rows ``offset..`` of 4-bit caches ``[heads, cap, 72]`` (uint8).
+
+    ``offset_dev`` (int64[1] on the device) supplies the offset at run time;
+    rows that do not fit are then left out and reported by the device status.
+    """
+    what = "kv_append_q4"
+    if k_new.dim() != 3 or v_new.dim() != 3:
+        k_new, v_new = _one_batch(k_new, what), _one_batch(v_new, what)
     dev = k_cache.device
-    _same_device(dev, v_cache=v_cache, k_new=k_new, v_new=v_new, offset_dev=offset_dev)
     heads, n, d = k_new.shape
-    with torch.cuda.device(dev):
-        rc = lib.rt_kv_append_q4(k_cache.data_ptr(), v_cache.data_ptr(),
-                                 k_cache.stride(0) if heads > 1 else k_cache.shape[1] * Q4_ROW_BYTES,
-                                 k_new.data_ptr(), v_new.data_ptr(), *_byte_strides(k_new), heads, n, d,
-                                 k_cache.shape[1], int(offset), _ptr(offset_dev), _STATE.status(dev).data_ptr(),
-                                 _stream(dev))
-    _lib.check(rc, "rt_kv_append_q4")
+    bf16 = torch.bfloat16
+    if not (_q4_rows(k_cache) and _q4_rows(v_cache) and k_cache.shape == v_cache.shape
+            and k_cache.stride() == v_cache.stride() and k_new.dtype is bf16 and v_new.dtype is bf16
+            and k_new.shape == v_new.shape and heads == k_cache.shape[0] and d == 128 and k_new.stride(2) == 1
+            and v_new.stride(2) == 1 and v_cache.device == dev and k_new.device == dev and v_new.device == dev
+            and (offset_dev is None or (offset_dev.dtype is torch.int64 and offset_dev.device == dev))
+            and not _needs_grad(k_new, v_new)):
+        _refuse(what,
+                (all(x.is_cuda for x in (k_cache, v_cache, k_new, v_new)), "takes CUDA tensors (no CPU path)"),
+                (not _needs_grad(k_new, v_new), "inference-only (no gradient)"),
+                (_q4_rows(k_cache) and _q4_rows(v_cache),
+                 f"caches must be uint8 [heads, capacity, {Q4_ROW_BYTES}] with contiguous rows"),
+                (k_cache.shape == v_cache.shape and k_cache.stride() == v_cache.stride(),
+                 "K and V caches must share shape and strides"),
+                (k_new.dtype == bf16 and v_new.dtype == bf16, "takes bf16 rows"),
+                (k_new.shape == v_new.shape and heads == k_cache.shape[0] and d == 128 and k_new.stride(2) == 1
+                 and v_new.stride(2) == 1,
+                 "new rows must be [cache heads, n, 128] with contiguous head_dim, the same for K and V"),
+                (offset_dev is None or offset_dev.dtype == torch.int64, "offset_dev must be int64"))
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return kv_append_q4(k_cache, v_cache, k_new, v_new, offset, offset_dev)
+    k_new, s0, s1 = _rows(k_new)
+    v_new, *sv = _rows(v_new)
+    if sv != [s0, s1]:
+        k_new, v_new, s0, s1 = k_new.contiguous(), v_new.contiguous(), n * 256, 256
+    cap = k_cache.shape[1]
+    rc = _lib.load().rt_kv_append_q4(k_cache.data_ptr(), v_cache.data_ptr(),
+                                     k_cache.stride(0) if heads > 1 else cap * Q4_ROW_BYTES, k_new.data_ptr(),
+                                     v_new.data_ptr(), s0, s1, heads, n, d, cap, int(offset),
+                                     None if offset_dev is None else offset_dev.data_ptr(),
+                                     _STATE.status(dev).data_ptr(), _raw_stream(dev))
+    if rc:
+        _lib.check(rc, "rt_kv_append_q4")
     _count()
 
 
 def kv_read_q4(cache: torch.Tensor, start: int, n: int, out: torch.Tensor | None = None) -> torch.Tensor:
     """bf16 values ``[..., n, 128]`` of rows ``[start, start + n)`` of a 4-bit cache ``[..., cap, 72]``."""
-    lib = _lib.load()
-    _require_cuda(cache, out)
-    if cache.dim() < 2:
-        raise RuntimeError(f"cache must be uint8 [..., capacity, {Q4_ROW_BYTES}]")
-    lead = cache.shape[:-2]
-    try:
-        c = _q4_cache(cache.view(-1, *cache.shape[-2:]), "cache")
-    except RuntimeError:
-        raise RuntimeError(f"cache must be uint8 [..., capacity, {Q4_ROW_BYTES}] with contiguous rows and leading "
-                           "dimensions of one stride") from None
-    dev = c.device
+    what = "kv_read_q4"
+    if not cache.is_cuda:
+        raise RuntimeError(f"{what}: takes CUDA tensors (no CPU path)")
+    dev = cache.device
+    c = cache
+    if c.dim() != 3:
+        try:
+            c = cache.view(-1, *cache.shape[-2:]) if cache.dim() > 1 else None
+        except RuntimeError:
+            c = None
+    if c is None or not _q4_rows(c):
+        raise RuntimeError(f"{what}: the cache must be uint8 [..., capacity, {Q4_ROW_BYTES}] with contiguous rows and "
+                           "leading dimensions of one stride")
+    heads, cap, _ = c.shape
     start, n = int(start), int(n)
-    if start < 0 or n < 0 or start + n > c.shape[1]:
-        raise RuntimeError(f"rows [{start}, {start + n}) are outside the cache's {c.shape[1]}")
+    if start < 0 or n < 0 or start + n > cap:
+        raise RuntimeError(f"{what}: rows [{start}, {start + n}) are outside the cache's {cap}")
+    shape = (*cache.shape[:-2], n, 128)
     if out is None:
-        out = torch.empty((*lead, n, 128), dtype=torch.bfloat16, device=dev)
-    if out.shape != (*lead, n, 128) or out.dtype != torch.bfloat16 or not out.is_contiguous():
-        raise RuntimeError(f"out must be contiguous bf16 {[*lead, n, 128]}")
-    _same_device(dev, out=out)
-    if out.numel() == 0:
+        out = torch.empty(shape, dtype=torch.bfloat16, device=dev)
+    elif out.shape != shape or out.dtype is not torch.bfloat16 or not out.is_contiguous() or out.device != dev:
+        raise RuntimeError(f"{what}: out must be contiguous bf16 {list(shape)} on {dev}")
+    if heads == 0 or n == 0:
         return out
-    with torch.cuda.device(dev):
-        rc = lib.rt_kv_read_q4(c.data_ptr(), c.stride(0), out.data_ptr(), n * 256, 256, c.shape[0], n, 128,
-                               c.shape[1], start, _stream(dev))
-    _lib.check(rc, "rt_kv_read_q4")
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return kv_read_q4(cache, start, n, out)
+    rc = _lib.load().rt_kv_read_q4(c.data_ptr(), c.stride(0) if heads > 1 else cap * Q4_ROW_BYTES, out.data_ptr(),
+                                   n * 256, 256, heads, n, 128, cap, start, _raw_stream(dev))
+    if rc:
+        _lib.check(rc, "rt_kv_read_q4")
     _count()
     return out
 
@@ -807,40 +861,53 @@ def tree_attention_q4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask_bi
     length at run time; ``prefix_len`` is then its upper bound.  Returns ``out``
     ``[n, Hq, 128]`` bf16.
     """
-    lib = _lib.load()
-    _require_cuda(q, k, v, mask_bits, out, prefix_len_dev)
-    _no_grad(q)
-    q = _query(q)
-    if q.dtype != torch.bfloat16:
-        raise RuntimeError("tree attention runs on bf16 queries")
-    q = _rows_apart(q)
-    k, v = _q4_cache(k, "k"), _q4_cache(v, "v")
-    if k.shape != v.shape or k.stride() != v.stride():
-        raise RuntimeError("K and V caches must share shape and strides")
-    n, hq, d = q.shape
-    hkv, cap = k.shape[:2]
-    if n == 0 or hkv == 0 or hq == 0 or hq % hkv:
-        raise RuntimeError("at least one node, and key heads that divide the query heads")
-    if mask_bits.dtype != torch.int32 or mask_bits.dim() != 2 or mask_bits.shape[0] < n or \
-            mask_bits.shape[1] * 32 < n:
-        raise RuntimeError("mask_bits must be int32 [n, at least ceil(n / 32)]")
-    if prefix_len_dev is not None and prefix_len_dev.dtype != torch.int64:
-        raise RuntimeError("prefix_len_dev must be int64")
-    if mask_bits.stride(-1) != 1 or mask_bits.stride(0) < mask_bits.shape[1]:
-        mask_bits = mask_bits.contiguous()
+    what = "tree_attention_q4"
+    q = _query(q, what)
     dev = q.device
-    _same_device(dev, k=k, v=v, mask_bits=mask_bits, out=out, prefix_len_dev=prefix_len_dev)
-    out = _attn_out(out, q)
-    prefix_len = int(prefix_len)
-    with torch.cuda.device(dev):
-        nbytes = lib.rt_tree_attn_q4_workspace_size(n, hq, hkv, d, prefix_len, int(num_splits))
-        ws = _workspace(nbytes, dev)
-        rc = lib.rt_tree_attn_q4(q.data_ptr(), *_byte_strides(q), k.data_ptr(), v.data_ptr(),
-                                 k.stride(0) if hkv > 1 else cap * Q4_ROW_BYTES, cap, out.data_ptr(),
-                                 *_byte_strides(out), mask_bits.data_ptr(), mask_bits.stride(0), n, prefix_len,
-                                 _ptr(prefix_len_dev), hq, hkv, d, d ** -0.5 if scale is None else float(scale),
-                                 int(num_splits), _ptr(ws), nbytes, _STATE.status(dev).data_ptr(), _stream(dev))
-    _lib.check(rc, "rt_tree_attn_q4")
+    n, hq, d = q.shape
+    if not (_q4_rows(k) and _q4_rows(v) and q.is_cuda and q.dtype is torch.bfloat16 and d == 128 and q.stride(2) == 1
+            and k.shape == v.shape and k.stride() == v.stride() and k.device == dev and v.device == dev
+            and mask_bits.device == dev and n and hq and k.shape[0] and hq % k.shape[0] == 0
+            and mask_bits.dtype is torch.int32 and mask_bits.dim() == 2 and mask_bits.shape[0] >= n
+            and mask_bits.shape[1] * 32 >= n and not _needs_grad(q)
+            and (prefix_len_dev is None or (prefix_len_dev.dtype is torch.int64 and prefix_len_dev.device == dev))):
+        _refuse(what,
+                (q.is_cuda and k.is_cuda and v.is_cuda and mask_bits.is_cuda, "takes CUDA tensors (no CPU path)"),
+                (not _needs_grad(q), "inference-only (no gradient)"),
+                (q.dtype == torch.bfloat16, "runs on bf16 queries"),
+                (d == 128 and q.stride(2) == 1, "head_dim must be 128 and contiguous"),
+                (_q4_rows(k) and _q4_rows(v),
+                 f"caches must be uint8 [heads, capacity, {Q4_ROW_BYTES}] with contiguous rows"),
+                (k.shape == v.shape and k.stride() == v.stride(), "K and V caches must share shape and strides"),
+                (n and hq and k.shape[0] and hq % k.shape[0] == 0,
+                 "at least one node, and key heads that divide the query heads"),
+                (mask_bits.dtype == torch.int32 and mask_bits.dim() == 2 and mask_bits.shape[0] >= n
+                 and mask_bits.shape[1] * 32 >= n, "mask_bits must be int32 [n, at least ceil(n / 32)]"),
+                (prefix_len_dev is None or prefix_len_dev.dtype == torch.int64, "prefix_len_dev must be int64"))
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return tree_attention_q4(q, k, v, mask_bits, prefix_len, scale, out, num_splits, prefix_len_dev)
+    words, unit = mask_bits.stride()
+    if unit != 1 or words < mask_bits.shape[1]:
+        mask_bits = mask_bits.contiguous()
+        words = mask_bits.shape[1]
+    q, q0, q1 = _rows(q)
+    out = _attn_out(out, q, what)
+    _, o0, o1 = _rows(out)
+    hkv, cap, _ = k.shape
+    lib = _lib.load()
+    prefix_len, num_splits = int(prefix_len), int(num_splits)
+    nbytes = lib.rt_tree_attn_q4_workspace_size(n, hq, hkv, d, prefix_len, num_splits)
+    ws = _workspace(nbytes, dev)
+    rc = lib.rt_tree_attn_q4(q.data_ptr(), q0, q1, k.data_ptr(), v.data_ptr(),
+                             k.stride(0) if hkv > 1 else cap * Q4_ROW_BYTES, cap, out.data_ptr(), o0, o1,
+                             mask_bits.data_ptr(), words, n, prefix_len,
+                             None if prefix_len_dev is None else prefix_len_dev.data_ptr(), hq, hkv, d,
+                             128 ** -0.5 if scale is None else float(scale), num_splits,
+                             None if ws is None else ws.data_ptr(), nbytes, _STATE.status(dev).data_ptr(),
+                             _raw_stream(dev))
+    if rc:
+        _lib.check(rc, "rt_tree_attn_q4")
     _count(2 if nbytes else 1)
     return out
 
