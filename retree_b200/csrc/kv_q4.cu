@@ -83,6 +83,20 @@ __global__ void __launch_bounds__(256) kv_append_q4_kernel(char* k_cache, char* 
   }
 }
 
+// Every scale the format holds, the largest too: 0x4300 | u is 128 + u, and the
+// difference to 128 + z and its product with s are exact.
+__device__ __forceinline__ uint4 q4_decode8_any(uint32_t word, uint32_t w) {
+  const uint32_t z2 = 0x43004300u | ((w & 15u) * 0x00010001u), s2 = q4_scale2(w);
+  auto value = [&](uint32_t x) {
+    x = (x & 0x000F000Fu) | 0x43004300u;
+    const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x),
+                                     *reinterpret_cast<const __nv_bfloat162*>(&z2));
+    const __nv_bfloat162 v = __hmul2(d, *reinterpret_cast<const __nv_bfloat162*>(&s2));
+    return *reinterpret_cast<const uint32_t*>(&v);
+  };
+  return make_uint4(value(word), value(word >> 4), value(word >> 8), value(word >> 12));
+}
+
 __global__ void __launch_bounds__(256) kv_read_q4_kernel(const char* cache, int64_t c_head_stride, char* out,
                                                          int64_t o_head_stride, int64_t o_row_stride, int n_heads,
                                                          int n, int64_t start) {
@@ -98,7 +112,7 @@ __global__ void __launch_bounds__(256) kv_read_q4_kernel(const char* cache, int6
     const uint32_t code = *reinterpret_cast<const uint32_t*>(src + lane * 4);
     const uint32_t word = *reinterpret_cast<const uint16_t*>(src + kQ4Codes + (lane >> 2) * 2);
     *(reinterpret_cast<uint4*>(out + h * o_head_stride + r * o_row_stride) + lane) =
-        q4_decode8(code, q4_zero2(word), q4_scale2(word));
+        q4_decode8_any(code, word);
   }
 }
 

@@ -27,32 +27,48 @@ constexpr int kQ4Row = 72;
 constexpr int kQ4Codes = 64;
 constexpr uint32_t kQ4NanWord = 0x7FF0;
 
-// The 16-bit word's scale as bf16 in both halves, and 128 + z likewise.
+// The 16-bit word's scale as bf16 in both halves.
 __device__ __forceinline__ uint32_t q4_scale2(uint32_t w) {
   const uint32_t s = w & 0x7FF0u;
   return s | (s << 16);
 }
-__device__ __forceinline__ uint32_t q4_zero2(uint32_t w) { return 0x43004300u | ((w & 15u) * 0x00010001u); }
 
-// Values 2j, 2j+1 of a code word as a bf16 pair: 0x4300 | u is 128 + u, the
-// difference to 128 + z and the product are exact.
-__device__ __forceinline__ uint32_t q4_pair(uint32_t shifted, uint32_t zero2, uint32_t scale2) {
-  uint32_t t;
-  asm("lop3.b32 %0, %1, 0x000F000F, 0x43004300, 0xEA;" : "=r"(t) : "r"(shifted));  // (a & b) | c
-  const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&t),
-                                   *reinterpret_cast<const __nv_bfloat162*>(&zero2));
-  const __nv_bfloat162 v = __hmul2(d, *reinterpret_cast<const __nv_bfloat162*>(&scale2));
-  return *reinterpret_cast<const uint32_t*>(&v);
+// Eight values of a code word as four bf16 pairs (16 bytes, in order), three and
+// a quarter instructions a pair: the nibbles as bytes, 64 - z added to each,
+// then 0x43 above a byte b makes the bf16 number 128 + b = 192 + (u - z),
+// and (192 + (u - z)) * s - 192 * s is one fused multiply-add whose result
+// (u - z) * s is representable, so it is exact.  192 * s has as few bits as s, but
+// must not overflow: s < 2^120.
+struct Q4Group {
+  uint32_t add4, scale2, shift2;  // 64 - z in four bytes, s and -192 s in two halves
+};
+__device__ __forceinline__ uint32_t q4_shift(uint32_t scale2) {
+  const __nv_bfloat162 c = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&scale2),
+                                   __floats2bfloat162_rn(-192.f, -192.f));
+  return *reinterpret_cast<const uint32_t*>(&c);
 }
-
-// Eight values of a code word as four bf16 pairs (16 bytes, in order).
-__device__ __forceinline__ uint4 q4_decode8(uint32_t word, uint32_t zero2, uint32_t scale2) {
-  uint4 r;
-  r.x = q4_pair(word, zero2, scale2);
-  r.y = q4_pair(word >> 4, zero2, scale2);
-  r.z = q4_pair(word >> 8, zero2, scale2);
-  r.w = q4_pair(word >> 12, zero2, scale2);
-  return r;
+__device__ __forceinline__ Q4Group q4_group(uint32_t w) {
+  const uint32_t s2 = q4_scale2(w);
+  return {0x40404040u - (w & 15u) * 0x01010101u, s2, q4_shift(s2)};
+}
+// The same for a word whose low half comes from one row and high half from another.
+__device__ __forceinline__ Q4Group q4_group2(uint32_t wlo, uint32_t whi) {
+  const uint32_t s2 = (wlo & 0x7FF0u) | ((whi & 0x7FF0u) << 16);
+  return {0x40404040u - ((wlo & 15u) | ((whi & 15u) << 16)) * 0x0101u, s2, q4_shift(s2)};
+}
+// x43: 0x43434343 in a register.  (Read it from memory: a constant that the
+// compiler can see is copied from a uniform register before every permute, one
+// instruction in seven of the decode.)
+__device__ __forceinline__ uint4 q4_decode8(uint32_t word, const Q4Group& g, uint32_t x43) {
+  const uint32_t lo = (word & 0x0F0F0F0Fu) + g.add4, hi = ((word >> 4) & 0x0F0F0F0Fu) + g.add4;
+  auto value = [&](uint32_t bytes, uint32_t sel) {
+    const uint32_t x = __byte_perm(bytes, x43, sel);
+    const __nv_bfloat162 v = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x),
+                                     *reinterpret_cast<const __nv_bfloat162*>(&g.scale2),
+                                     *reinterpret_cast<const __nv_bfloat162*>(&g.shift2));
+    return *reinterpret_cast<const uint32_t*>(&v);
+  };
+  return make_uint4(value(lo, 0x4240), value(hi, 0x4240), value(lo, 0x4341), value(hi, 0x4341));
 }
 
 }  // namespace rt

@@ -57,7 +57,8 @@ constexpr int kQsStages = 3;
 constexpr uint32_t kQsRing = kQsStages * 2 * kQsHalf;     // of one warp
 constexpr uint32_t kQsOffQ = kQsWarps * kQsRing;          // Q fragments [8-row tile][code word][32 lanes] x 16 bytes
 constexpr uint32_t kQsOffBar = kQsOffQ + 2 * 4 * 32 * 16;
-constexpr uint32_t kQsSmem = kQsOffBar + kQsWarps * kQsStages * 8 + 16 + 128;
+constexpr uint32_t kQsOffX43 = kQsOffBar + kQsWarps * kQsStages * 8 + 8;
+constexpr uint32_t kQsSmem = kQsOffX43 + 8 + 128;
 // after the key loop the rings hold the warps' results, then the CTA's
 constexpr int kQsRows = 16;
 constexpr uint32_t kQsOffPart = 0;                                        // [warp][fragment][lane] x 16 bytes
@@ -70,7 +71,7 @@ static_assert(kQsOffStageMl + kQsRows * 8 <= kQsOffQ, "results fit in the rings"
 
 __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -79,14 +80,10 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1
 // Transpose of an 8 x 8 tile of 16-bit values, two of a row in each lane.
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
   uint32_t d;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
 
-__device__ __forceinline__ uint32_t q4_zero_pair(uint32_t a, uint32_t b) {
-  return 0x43004300u | (a & 15u) | ((b & 15u) << 16);
-}
-__device__ __forceinline__ uint32_t q4_scale_pair(uint32_t a, uint32_t b) { return (a & 0x7FF0u) | ((b & 0x7FF0u) << 16); }
 __device__ __forceinline__ bool q4_is_nan(uint32_t w) { return (w & 0x7F80u) == 0x7F80u; }
 
 __device__ __forceinline__ void store_bf16x4(char* dst, const float4& v) {
@@ -105,7 +102,10 @@ __global__ void __launch_bounds__(kQsThreads, 1) tree_attn_q4_small_kernel(const
   const int split = blockIdx.x, kvh = blockIdx.y, G = p.group, rows = p.n * G;
   if (lane == 0) {
     for (int i = 0; i < kQsStages; ++i) mbar_init(&full[i], 1);
-    if (warp == 0) *abort_word = 0;
+    if (warp == 0) {
+      *abort_word = 0;
+      *reinterpret_cast<uint2*>(smem + kQsOffX43) = make_uint2(0x43434343u, 0);
+    }
     fence_mbar_init();
     fence_proxy_async_smem();
   }
@@ -147,11 +147,13 @@ __global__ void __launch_bounds__(kQsThreads, 1) tree_attn_q4_small_kernel(const
   }
   __syncthreads();
 
+  const uint32_t sbase = smem_u32(smem);
+  const uint32_t x43 = lds64(sbase + kQsOffX43).x;
   const float sl2 = p.scale_log2;
   uint4 qr[NT == 1 ? 4 : 1];  // one tile of queries stays in registers
   if constexpr (NT == 1) {
 #pragma unroll
-    for (int wd = 0; wd < 4; ++wd) qr[wd] = qs[wd * 32 + lane];
+    for (int wd = 0; wd < 4; ++wd) qr[wd] = lds128(sbase + kQsOffQ + (wd * 32 + lane) * 16);
   }
   float O[8][NT][4];
   float m[NT][2], l[NT][2];  // rows 8nt + 2t, + 1
@@ -173,25 +175,23 @@ __global__ void __launch_bounds__(kQsThreads, 1) tree_attn_q4_small_kernel(const
     ok = __all_sync(0xFFFFFFFFu, ok);
     if (!ok) break;
     const int64_t key0 = (b0 + warp + static_cast<int64_t>(i) * kQsWarps) * kQsKeys;
-    const unsigned char* kt = ring + s * 2 * kQsHalf;
-    const unsigned char* vt = kt + kQsHalf;
+    const uint32_t kt = sbase + warp * kQsRing + s * 2 * kQsHalf, vt = kt + kQsHalf;
     // ---- S^T = K Q^T: 16 keys (rows g, g + 8) a step
     float S[2][NT][4];
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) {
-      uint32_t kw[2][4], z2[2], s2[2];
+      uint32_t kw[2][4];
+      Q4Group kg[2];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const unsigned char* row = kt + (mt * 16 + e * 8 + g) * kQ4Row;
-        const uint2 a = *reinterpret_cast<const uint2*>(row + t * 16);
-        const uint2 b = *reinterpret_cast<const uint2*>(row + t * 16 + 8);
-        const uint32_t w = *reinterpret_cast<const uint16_t*>(row + kQ4Codes + t * 2);
+        const uint32_t row = kt + (mt * 16 + e * 8 + g) * kQ4Row;
+        const uint2 a = lds64(row + t * 16), b = lds64(row + t * 16 + 8);
+        const uint32_t w = lds16(row + kQ4Codes + t * 2);
         kw[e][0] = a.x;
         kw[e][1] = a.y;
         kw[e][2] = b.x;
         kw[e][3] = b.y;
-        z2[e] = q4_zero2(w);
-        s2[e] = q4_scale2(w);
+        kg[e] = q4_group(w);
       }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -199,10 +199,10 @@ __global__ void __launch_bounds__(kQsThreads, 1) tree_attn_q4_small_kernel(const
         for (int c = 0; c < 4; ++c) S[mt][nt][c] = 0.f;
 #pragma unroll
       for (int wd = 0; wd < 4; ++wd) {
-        const uint4 a = q4_decode8(kw[0][wd], z2[0], s2[0]), b = q4_decode8(kw[1][wd], z2[1], s2[1]);
+        const uint4 a = q4_decode8(kw[0][wd], kg[0], x43), b = q4_decode8(kw[1][wd], kg[1], x43);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          const uint4 q = NT == 1 ? qr[wd] : qs[(nt * 4 + wd) * 32 + lane];
+          const uint4 q = NT == 1 ? qr[wd] : lds128(sbase + kQsOffQ + ((nt * 4 + wd) * 32 + lane) * 16);
           mma_bf16(S[mt][nt], a.x, b.x, a.y, b.y, q.x, q.y);
           mma_bf16(S[mt][nt], a.z, b.z, a.w, b.w, q.z, q.w);
         }
@@ -215,9 +215,9 @@ __global__ void __launch_bounds__(kQsThreads, 1) tree_attn_q4_small_kernel(const
     for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        const unsigned char* row = vt + (ks * 16 + 2 * t + (c & 1) + 8 * (c >> 1)) * kQ4Row;
-        vw[ks][c] = *reinterpret_cast<const uint2*>(row + g * 8);
-        vm[ks][c] = *reinterpret_cast<const uint16_t*>(row + kQ4Codes + (g >> 1) * 2);
+        const uint32_t row = vt + (ks * 16 + 2 * t + (c & 1) + 8 * (c >> 1)) * kQ4Row;
+        vw[ks][c] = lds64(row + g * 8);
+        vm[ks][c] = lds16(row + kQ4Codes + (g >> 1) * 2);
       }
     // ---- hide, online softmax
     if (key0 + kQsKeys > L) {
@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(kQsThreads, 1) tree_attn_q4_small_kernel(const
       for (int e = 0; e < 4; ++e) {
         const int key = e * 8 + g;
         if (key0 + key >= L && key0 + key < total &&
-            q4_is_nan(*reinterpret_cast<const uint16_t*>(vt + key * kQ4Row + kQ4Codes)))
+            q4_is_nan(lds16(vt + key * kQ4Row + kQ4Codes)))
           bad |= 1u << e;
       }
 #pragma unroll
@@ -300,8 +300,7 @@ __global__ void __launch_bounds__(kQsThreads, 1) tree_attn_q4_small_kernel(const
     // ---- O^T += V^T P^T: a step is 16 keys; an m-tile two values of every lane g's sixteen
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
-      const uint32_t za = q4_zero_pair(vm[ks][0], vm[ks][1]), sa = q4_scale_pair(vm[ks][0], vm[ks][1]);
-      const uint32_t zb = q4_zero_pair(vm[ks][2], vm[ks][3]), sb = q4_scale_pair(vm[ks][2], vm[ks][3]);
+      const Q4Group ga = q4_group2(vm[ks][0], vm[ks][1]), gb = q4_group2(vm[ks][2], vm[ks][3]);
 #pragma unroll
       for (int wd = 0; wd < 2; ++wd) {
         const uint32_t w0 = wd ? vw[ks][0].y : vw[ks][0].x, w1 = wd ? vw[ks][1].y : vw[ks][1].x;
@@ -309,8 +308,8 @@ __global__ void __launch_bounds__(kQsThreads, 1) tree_attn_q4_small_kernel(const
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
           // nibbles of two keys: the words' low (or high) halves side by side
-          const uint4 x = q4_decode8(__byte_perm(w0, w1, hf ? 0x7632 : 0x5410), za, sa);
-          const uint4 y = q4_decode8(__byte_perm(w2, w3, hf ? 0x7632 : 0x5410), zb, sb);
+          const uint4 x = q4_decode8(__byte_perm(w0, w1, hf ? 0x7632 : 0x5410), ga, x43);
+          const uint4 y = q4_decode8(__byte_perm(w2, w3, hf ? 0x7632 : 0x5410), gb, x43);
           const int o = wd * 4 + hf * 2;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
@@ -453,26 +452,25 @@ struct Q4Bars {
       p_full[2], o_full[2], fin;
   uint32_t tmem_base;
   int abort_flag;
+  uint2 x43;  // (.x)
 };
 
 // A key's row of a decoded tile: 128 bf16 values in two SW128 halves.
-__device__ __forceinline__ void q4_decode_row(const unsigned char* src, unsigned char* tile, int r, bool zero,
-                                              bool nan) {
-  const uint2 mw = *reinterpret_cast<const uint2*>(src + kQ4Codes);
+__device__ __forceinline__ void q4_decode_row(uint32_t src, uint32_t tile, int r, bool zero, bool nan, uint32_t x43) {
+  const uint2 mw = lds64(src + kQ4Codes);
   const uint32_t meta[4] = {mw.x & 0xFFFFu, mw.x >> 16, mw.y & 0xFFFFu, mw.y >> 16};
-  unsigned char* dst = tile + r * 128;
+  const uint32_t dst = tile + r * 128;
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
     // (a row that must read as zero or NaN does so through its scale)
-    const uint32_t z2 = q4_zero2(meta[g]);
-    const uint32_t s2 = nan ? 0x7FC07FC0u : (zero ? 0u : q4_scale2(meta[g]));
+    const Q4Group q = q4_group(nan ? 0x7FF0u : (zero ? 0u : meta[g]));
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const uint2 w = *reinterpret_cast<const uint2*>(src + g * 16 + i * 8);
+      const uint2 w = lds64(src + g * 16 + i * 8);
       const int ch = g * 4 + i * 2;
-      unsigned char* half = dst + (ch >> 3) * kQtHalf;
-      *reinterpret_cast<uint4*>(half + (((ch & 7) ^ (r & 7)) << 4)) = q4_decode8(w.x, z2, s2);
-      *reinterpret_cast<uint4*>(half + ((((ch + 1) & 7) ^ (r & 7)) << 4)) = q4_decode8(w.y, z2, s2);
+      const uint32_t half = dst + (ch >> 3) * kQtHalf;
+      sts128(half + (((ch & 7) ^ (r & 7)) << 4), q4_decode8(w.x, q, x43));
+      sts128(half + ((((ch + 1) & 7) ^ (r & 7)) << 4), q4_decode8(w.y, q, x43));
     }
   }
 }
@@ -505,6 +503,7 @@ __global__ void __launch_bounds__(kQtThreads, 1)
     }
     mbar_init(&bar.fin, 1);
     bar.abort_flag = 0;
+    bar.x43 = make_uint2(0x43434343u, 0);
     fence_mbar_init();
     fence_proxy_async_smem();
   }
@@ -612,6 +611,7 @@ __global__ void __launch_bounds__(kQtThreads, 1)
     // ---------------- decode ----------------
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kQtRegsDecode));
     const int r = tid & 127;
+    const uint32_t sbase = smem_u32(smem), x43 = lds64(smem_u32(&bar.x43)).x;
     const char* vb = p.v + kvh * p.kv_head_stride;
     for (int n = 0; n < 2 * nb; ++n) {
       const int si = n % kQtPacked, so = n % kQtStages;
@@ -626,7 +626,7 @@ __global__ void __launch_bounds__(kQtThreads, 1)
         zero = (n & 1) != 0;
         nan = !zero;
       }
-      q4_decode_row(smem + kQtOffPacked + si * kQtBlock + r * kQ4Row, smem + kQtOffKV + so * kQtTile, r, zero, nan);
+      q4_decode_row(sbase + kQtOffPacked + si * kQtBlock + r * kQ4Row, sbase + kQtOffKV + so * kQtTile, r, zero, nan, x43);
       fence_proxy_async_smem();
       mbar_arrive(&bar.in_empty[si]);
       mbar_arrive(&bar.kv_full[so]);
