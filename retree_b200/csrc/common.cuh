@@ -201,6 +201,20 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
       : "memory");
 }
 
+// One lane of a converged warp.  The MMA warps run their loops with all lanes and
+// issue under this: operands that the compiler knows to be the same in every
+// lane (warp_uniform) go straight into uniform registers, where an operand of a
+// lane-0 branch costs a loop over the lanes per instruction.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+template <typename V>
+__device__ __forceinline__ V warp_uniform(V x) {
+  return __shfl_sync(0xFFFFFFFFu, x, 0);
+}
+
 // Arrive on `bar` once every tcgen05 op issued so far by this thread completes.
 __device__ __forceinline__ void umma_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))

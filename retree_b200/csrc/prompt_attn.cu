@@ -13,7 +13,7 @@
 //                   rescale of O in TMEM, P back into S's own columns, and the
 //                   tile's output rows;
 //   warp 8          TMA producer: Q tiles, and K / V blocks into a 4-stage ring;
-//   warp 9          MMA issuer (one lane): per block PV of tile 0, next QK of
+//   warp 9          MMA issuer: per block PV of tile 0, next QK of
 //                   tile 0, PV of tile 1, next QK of tile 1 -- while one tile's
 //                   softmax runs the tensor core has the other tile's products;
 //   warp 10         checks the V blocks that some row must not see in full
@@ -280,82 +280,96 @@ __global__ void __launch_bounds__(kPThreads, 1)
   } else if (warp == 9) {
     // ---------------- MMA issuer ----------------
     fewer_registers();
-    if (lane == 0) {
-      constexpr uint32_t kFmt = std::is_same_v<T, __half> ? (1u << 7 | 1u << 10) : 0u;  // clears the bf16 format bits
-      constexpr uint32_t idesc_qk = idesc_bf16_f32(kPB, kPB, false, false) & ~kFmt;
-      constexpr uint32_t idesc_pv = idesc_bf16_f32(kPB, kPD, false, true) & ~kFmt;
-      const uint32_t sq = smem_u32(smem + kPOffQ), skv = smem_u32(smem + kPOffKV);
-      int n = 0;  // ring loads consumed
-      int nq[2] = {0, 0}, np[2] = {0, 0};
-      uint32_t looks = 0;  // V blocks handed to warp 10
-      bool ok = true;
-      auto wait = [&](uint64_t* b, uint32_t ph) {
-        ok = ok && mbar_wait(b, ph & 1, abort_flag, p.status, RT_DEV_WAIT_TIMEOUT);
-        return ok;
-      };
-      auto qk = [&](int t, int stage) {
-        const uint32_t a = sq + t * kPTile, b = skv + stage * kPTile;
+    constexpr uint32_t kFmt = std::is_same_v<T, __half> ? (1u << 7 | 1u << 10) : 0u;  // clears the bf16 format bits
+    constexpr uint32_t idesc_qk = idesc_bf16_f32(kPB, kPB, false, false) & ~kFmt;
+    constexpr uint32_t idesc_pv = idesc_bf16_f32(kPB, kPD, false, true) & ~kFmt;
+    const uint32_t tm = warp_uniform(tmem);
+    const uint64_t dq = warp_uniform(smem_desc_sw128(smem_u32(smem + kPOffQ), 16, 1024));
+    const uint64_t dk = warp_uniform(smem_desc_sw128(smem_u32(smem + kPOffKV), 16, 1024));
+    const uint64_t dv = warp_uniform(smem_desc_sw128(smem_u32(smem + kPOffKV), kPHalf, 1024));
+    int n = 0;  // ring loads consumed
+    int nq[2] = {0, 0}, np[2] = {0, 0};
+    uint32_t looks = 0;  // V blocks handed to warp 10
+    bool ok = true;
+    auto wait = [&](uint64_t* b, uint32_t ph) {
+      ok = ok && mbar_wait(b, ph & 1, abort_flag, p.status, RT_DEV_WAIT_TIMEOUT);
+      ok = __all_sync(0xFFFFFFFFu, ok);
+      return ok;
+    };
+    // S_t = Q_t K^T of the block in `stage`; the last one of an item frees Q_t
+    auto qk = [&](int t, int stage, bool last) {
+      const uint64_t b = dk + static_cast<uint64_t>(warp_uniform(stage) * (kPTile >> 4));
+      if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < kPD / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * kPHalf + (kk & 3) * 32;
-          umma_f16(tmem + t * kPB, smem_desc_sw128(a + off, 16, 1024), smem_desc_sw128(b + off, 16, 1024), idesc_qk,
-                   kk > 0);
+          const uint32_t off = ((kk >> 2) * kPHalf + (kk & 3) * 32) >> 4;
+          umma_f16(tm + t * kPB, dq + t * (kPTile >> 4) + off, b + off, idesc_qk, kk > 0);
         }
         umma_commit(&bar.s_full[t]);
-      };
-      for (int it = 0; ok && prompt_item(p, tab, it, w); ++it) {
-        const int nb = max(w.nb[0], w.nb[1]);
-        if (nb == 0) continue;
-        int s = n % kPStages;
-        if (!wait(&bar.kv_full[s], n / kPStages)) break;
+        if (last) umma_commit(&bar.q_empty[t]);
+      }
+    };
+    auto commit = [&](uint64_t* b) {
+      if (elect_one()) umma_commit(b);
+    };
+    for (int it = 0; ok && prompt_item(p, tab, it, w); ++it) {
+      const int nb = max(w.nb[0], w.nb[1]);
+      if (nb == 0) continue;
+      int s = n % kPStages;
+      if (!wait(&bar.kv_full[s], n / kPStages)) break;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if (w.nb[t] == 0) continue;
+        if (!wait(&bar.q_full[t], nq[t]++)) break;
+        tc_fence_after();
+        qk(t, s, w.nb[t] == 1);
+      }
+      if (!ok) break;
+      commit(&bar.kv_empty[s]);
+      ++n;
+      for (int j = 0; j < nb && ok; ++j) {
+        const int sv = n % kPStages, sk = (n + 1) % kPStages;
+        const bool more = j + 1 < nb;
+        if (!wait(&bar.kv_full[sv], n / kPStages)) break;
+        bool look = j >= w.jm;
+        if (look && lane == 0) mbar_arrive(&bar.v_look);
+        __syncwarp();
+        const uint64_t b = dv + static_cast<uint64_t>(warp_uniform(sv) * (kPTile >> 4));
+        bool have_k = false;
+#pragma unroll
         for (int t = 0; t < 2; ++t) {
-          if (w.nb[t] == 0) continue;
-          if (!wait(&bar.q_full[t], nq[t]++)) break;
-          tc_fence_after();
-          qk(t, s);
-          if (w.nb[t] == 1) umma_commit(&bar.q_empty[t]);
-        }
-        if (!ok) break;
-        umma_commit(&bar.kv_empty[s]);
-        ++n;
-        for (int j = 0; j < nb && ok; ++j) {
-          const int sv = n % kPStages, sk = (n + 1) % kPStages;
-          const bool more = j + 1 < nb;
-          if (!wait(&bar.kv_full[sv], n / kPStages)) break;
-          bool look = j >= w.jm;
-          if (look) mbar_arrive(&bar.v_look);
-          bool have_k = false;
-          for (int t = 0; t < 2; ++t) {
-            if (j < w.nb[t]) {
-              if (!wait(&bar.p_full[t], np[t]++)) break;
-              if (look && !wait(&bar.v_ok, looks++)) break;
-              look = false;
-              tc_fence_after();
-              const uint32_t b = skv + sv * kPTile;
+          if (j < w.nb[t]) {
+            if (!wait(&bar.p_full[t], np[t]++)) break;
+            if (look && !wait(&bar.v_ok, looks++)) break;
+            look = false;
+            tc_fence_after();
+            if (elect_one()) {
 #pragma unroll
               for (int kk = 0; kk < kPB / 16; ++kk)
-                umma_f16_ts(tmem + kPTmemO + t * kPD, tmem + t * kPB + kk * 8,
-                            smem_desc_sw128(b + kk * 2048, kPHalf, 1024), idesc_pv, (j > 0 || kk > 0) ? 1u : 0u);
+                umma_f16_ts(tm + kPTmemO + t * kPD, tm + t * kPB + kk * 8, b + kk * (2048 >> 4), idesc_pv,
+                            (j > 0 || kk > 0) ? 1u : 0u);
               if (j + 1 == w.nb[t]) umma_commit(&bar.o_full[t]);
             }
-            if (t == 1) umma_commit(&bar.kv_empty[sv]);
-            if (j + 1 < w.nb[t]) {
-              if (!have_k && !wait(&bar.kv_full[sk], (n + 1) / kPStages)) break;
-              have_k = true;
-              tc_fence_after();
-              qk(t, sk);
-              if (j + 2 == w.nb[t]) umma_commit(&bar.q_empty[t]);
-            }
           }
-          if (!ok) break;
-          if (more) umma_commit(&bar.kv_empty[sk]);
-          n += more ? 2 : 1;
+          if (t == 1) commit(&bar.kv_empty[sv]);
+          if (j + 1 < w.nb[t]) {
+            if (!have_k && !wait(&bar.kv_full[sk], (n + 1) / kPStages)) break;
+            have_k = true;
+            tc_fence_after();
+            qk(t, sk, j + 2 == w.nb[t]);
+          }
         }
+        if (!ok) break;
+        if (more) commit(&bar.kv_empty[sk]);
+        n += more ? 2 : 1;
       }
-      // all issued MMAs complete before TMEM is released
+    }
+    // all issued MMAs complete before TMEM is released
+    if (elect_one()) {
       umma_commit(&bar.fin);
       mbar_wait_drain(&bar.fin, 0);
     }
+    __syncwarp();
   } else if (warp == 10) {
     // ---------------- V blocks that are partly hidden: values that are not finite ----------------
     fewer_registers();

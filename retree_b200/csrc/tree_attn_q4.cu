@@ -455,9 +455,17 @@ struct Q4Bars {
   uint2 x43;  // (.x)
 };
 
-// A key's row of a decoded tile: 128 bf16 values in two SW128 halves.
-__device__ __forceinline__ void q4_decode_row(uint32_t src, uint32_t tile, int r, bool zero, bool nan, uint32_t x43) {
+// A key's row of a decoded tile: 128 bf16 values in two SW128 halves.  All of
+// the row is read before anything is decoded (`loaded` runs in between): one
+// warp a scheduler decodes, so its words have to overlap one another.
+template <typename Loaded>
+__device__ __forceinline__ void q4_decode_row(uint32_t src, uint32_t tile, int r, bool zero, bool nan, uint32_t x43,
+                                              Loaded loaded) {
+  uint2 w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = lds64(src + i * 8);
   const uint2 mw = lds64(src + kQ4Codes);
+  loaded();
   const uint32_t meta[4] = {mw.x & 0xFFFFu, mw.x >> 16, mw.y & 0xFFFFu, mw.y >> 16};
   const uint32_t dst = tile + r * 128;
 #pragma unroll
@@ -466,11 +474,10 @@ __device__ __forceinline__ void q4_decode_row(uint32_t src, uint32_t tile, int r
     const Q4Group q = q4_group(nan ? 0x7FF0u : (zero ? 0u : meta[g]));
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const uint2 w = lds64(src + g * 16 + i * 8);
       const int ch = g * 4 + i * 2;
       const uint32_t half = dst + (ch >> 3) * kQtHalf;
-      sts128(half + (((ch & 7) ^ (r & 7)) << 4), q4_decode8(w.x, q, x43));
-      sts128(half + ((((ch + 1) & 7) ^ (r & 7)) << 4), q4_decode8(w.y, q, x43));
+      sts128(half + (((ch & 7) ^ (r & 7)) << 4), q4_decode8(w[g * 2 + i].x, q, x43));
+      sts128(half + ((((ch + 1) & 7) ^ (r & 7)) << 4), q4_decode8(w[g * 2 + i].y, q, x43));
     }
   }
 }
@@ -626,9 +633,9 @@ __global__ void __launch_bounds__(kQtThreads, 1)
         zero = (n & 1) != 0;
         nan = !zero;
       }
-      q4_decode_row(sbase + kQtOffPacked + si * kQtBlock + r * kQ4Row, sbase + kQtOffKV + so * kQtTile, r, zero, nan, x43);
+      q4_decode_row(sbase + kQtOffPacked + si * kQtBlock + r * kQ4Row, sbase + kQtOffKV + so * kQtTile, r, zero, nan, x43,
+                    [&] { mbar_arrive(&bar.in_empty[si]); });
       fence_proxy_async_smem();
-      mbar_arrive(&bar.in_empty[si]);
       mbar_arrive(&bar.kv_full[so]);
     }
   } else {

@@ -8,6 +8,7 @@ is no CPU path, and a missing library raises (``retree_b200._lib.load``).
 from __future__ import annotations
 
 import ctypes
+import functools
 import threading
 
 import numpy as np
@@ -621,12 +622,29 @@ def recovery_walk(parents: torch.Tensor, tokens: torch.Tensor, posterior: torch.
 Q4_ROW_BYTES = _lib.RT_Q4_ROW_BYTES
 
 
-def _raw_stream(dev) -> int:
-    return torch._C._cuda_getCurrentRawStream(dev.index)
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch.cuda.current_device
+_grad_enabled = torch.is_grad_enabled
+_BF16, _F16 = torch.bfloat16, torch.float16
+_STATUS_PTR: dict = {}  # device index -> address of its status word (kept for the process's life)
+_SCALE = 128 ** -0.5
 
 
-def _elsewhere(dev) -> bool:
-    return torch.cuda.current_device() != dev.index
+def _status_ptr(dev) -> int:
+    ptr = _STATUS_PTR.get(dev.index)
+    if ptr is None:
+        ptr = _STATUS_PTR[dev.index] = _STATE.status(dev).data_ptr()
+    return ptr
+
+
+@functools.lru_cache(maxsize=1024)
+def _prompt_workspace(index, *shape) -> int:
+    return _lib.load().rt_prompt_attn_workspace_size(*shape)
+
+
+@functools.lru_cache(maxsize=1024)
+def _tree_q4_workspace(index, *shape) -> int:
+    return _lib.load().rt_tree_attn_q4_workspace_size(*shape)
 
 
 def _refuse(what: str, *conditions) -> None:
@@ -638,7 +656,7 @@ def _refuse(what: str, *conditions) -> None:
 
 
 def _needs_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+    return _grad_enabled() and any(t.requires_grad for t in tensors)
 
 
 def _workspace(nbytes: int, dev) -> torch.Tensor | None:
@@ -680,7 +698,7 @@ def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int, int]:
 
 def _attn_out(out: torch.Tensor | None, q: torch.Tensor, what: str) -> torch.Tensor:
     if out is None:
-        return q.new_empty(q.shape)
+        return q.new_empty(tuple(q.shape))
     if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(-1) != 1 or \
             any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
         raise RuntimeError(f"{what}: out must be {q.dtype} {list(q.shape)} on {q.device} with contiguous head_dim and "
@@ -712,11 +730,15 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     hkv, tk, dk = k.shape
     dt = q.dtype
     cq, ck = cu_seqlens_q, cu_seqlens_k
-    if not (q.is_cuda and k.device == dev and v.device == dev and (dt is torch.bfloat16 or dt is torch.float16)
-            and k.dtype is dt and v.dtype is dt and d == 128 and dk == 128 and q.stride(2) == 1 and k.stride(2) == 1
-            and k.shape == v.shape and v.stride(2) == 1 and hq and hkv and hq % hkv == 0
+    q0, q1, q2 = q.stride()
+    k0, k1, k2 = ks = k.stride()
+    vs = v.stride()
+    if not (q.is_cuda and k.device == dev and v.device == dev and (dt is _BF16 or dt is _F16) and k.dtype is dt
+            and v.dtype is dt and d == 128 and dk == 128 and q2 == 1 and k2 == 1 and vs[2] == 1 and k.shape == v.shape
+            and hq and hkv and hq % hkv == 0
             and (ck is None or (cq is not None and _offsets(ck) and ck.device == dev and ck.numel() == cq.numel()))
-            and (cq is None or (_offsets(cq) and cq.device == dev)) and not _needs_grad(q, k, v)):
+            and (cq is None or (_offsets(cq) and cq.device == dev))
+            and not (_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad))):
         _refuse(what,
                 (q.is_cuda and k.is_cuda and v.is_cuda, "takes CUDA tensors (no CPU path)"),
                 (not _needs_grad(q, k, v), "inference-only (no gradient)"),
@@ -730,27 +752,34 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
                 (all(x is None or _offsets(x) for x in (cq, ck)),
                  "cu_seqlens must be contiguous int32 tensors of at least two offsets"),
                 (ck is None or cq is None or ck.numel() == cq.numel(), "cu_seqlens must name the same number of sequences"))
-    if _elsewhere(dev):
+    index = dev.index
+    if _current_device() != index:
         with torch.cuda.device(dev):
             return prompt_attention(q, k, v, cq, ck, scale, out)
-    q, q0, q1 = _rows(q)
-    k, k0, k1 = _rows(k)
-    v, v0, v1 = _rows(v)
-    if (k0, k1) != (v0, v1):
-        raise RuntimeError(f"{what}: K and V must share strides")
-    out = _attn_out(out, q, what)
+    if ks == vs and t > 1 and hq > 1 and tk > 1 and hkv > 1 and q0 and q1 and k0 and k1:
+        q0, q1, k0, k1 = 2 * q0, 2 * q1, 2 * k0, 2 * k1
+    else:
+        q, q0, q1 = _rows(q)
+        k, k0, k1 = _rows(k)
+        v, v0, v1 = _rows(v)
+        if (k0, k1) != (v0, v1):
+            raise RuntimeError(f"{what}: K and V must share strides")
+    if out is None:
+        out = q.new_empty((t, hq, 128))
+        o0, o1 = hq * 256, 256
+    else:
+        _, o0, o1 = _rows(_attn_out(out, q, what))
     if t == 0:
         return out
-    _, o0, o1 = _rows(out)
     seqs = 1 if cq is None else cq.numel() - 1
-    lib = _lib.load()
-    nbytes = lib.rt_prompt_attn_workspace_size(t, tk, seqs, hq, hkv)
+    nbytes = _prompt_workspace(index, t, tk, seqs, hq, hkv)
     ws = _workspace(nbytes, dev)
-    rc = lib.rt_prompt_attn(q.data_ptr(), q0, q1, k.data_ptr(), v.data_ptr(), k0, k1, out.data_ptr(), o0, o1,
-                            _DTYPE_CODE[dt], None if cq is None else cq.data_ptr(),
-                            None if ck is None else ck.data_ptr(), seqs, t, tk, hq, hkv, d,
-                            128 ** -0.5 if scale is None else float(scale), None if ws is None else ws.data_ptr(), nbytes,
-                            _STATE.status(dev).data_ptr(), _raw_stream(dev))
+    rc = _lib.load().rt_prompt_attn(q.data_ptr(), q0, q1, k.data_ptr(), v.data_ptr(), k0, k1, out.data_ptr(), o0, o1,
+                                    1 if dt is _BF16 else 2, None if cq is None else cq.data_ptr(),
+                                    None if ck is None else ck.data_ptr(), seqs, t, tk, hq, hkv, 128,
+                                    _SCALE if scale is None else float(scale),
+                                    None if ws is None else ws.data_ptr(), nbytes, _status_ptr(dev),
+                                    _raw_stream(index))
     if rc:
         _lib.check(rc, "rt_prompt_attn")
     _count(2 if nbytes else 1)
@@ -759,8 +788,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
 
 def _q4_rows(t: torch.Tensor) -> bool:
     """Whether ``t`` is a 4-bit cache ``[heads, capacity, 72]`` with contiguous rows."""
-    return t.is_cuda and t.dtype is torch.uint8 and t.dim() == 3 and t.shape[2] == Q4_ROW_BYTES and \
-        t.stride()[1:] == (Q4_ROW_BYTES, 1)
+    return t.is_cuda and t.dtype is torch.uint8 and t.dim() == 3 and t.shape[2] == 72 and t.stride()[1:] == (72, 1)
 
 
 def kv_append_q4(k_cache: torch.Tensor, v_cache: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor,
@@ -775,13 +803,15 @@ def kv_append_q4(k_cache: torch.Tensor, v_cache: torch.Tensor, k_new: torch.Tens
         k_new, v_new = _one_batch(k_new, what), _one_batch(v_new, what)
     dev = k_cache.device
     heads, n, d = k_new.shape
-    bf16 = torch.bfloat16
+    cache_heads, cap, _ = k_cache.shape if k_cache.dim() == 3 else (-1, 0, 0)
+    s0, s1, s2 = ss = k_new.stride()
+    sv = v_new.stride()
     if not (_q4_rows(k_cache) and _q4_rows(v_cache) and k_cache.shape == v_cache.shape
-            and k_cache.stride() == v_cache.stride() and k_new.dtype is bf16 and v_new.dtype is bf16
-            and k_new.shape == v_new.shape and heads == k_cache.shape[0] and d == 128 and k_new.stride(2) == 1
-            and v_new.stride(2) == 1 and v_cache.device == dev and k_new.device == dev and v_new.device == dev
+            and k_cache.stride() == v_cache.stride() and k_new.dtype is _BF16 and v_new.dtype is _BF16
+            and k_new.shape == v_new.shape and heads == cache_heads and d == 128 and s2 == 1 and sv[2] == 1
+            and v_cache.device == dev and k_new.device == dev and v_new.device == dev
             and (offset_dev is None or (offset_dev.dtype is torch.int64 and offset_dev.device == dev))
-            and not _needs_grad(k_new, v_new)):
+            and not (_grad_enabled() and (k_new.requires_grad or v_new.requires_grad))):
         _refuse(what,
                 (all(x.is_cuda for x in (k_cache, v_cache, k_new, v_new)), "takes CUDA tensors (no CPU path)"),
                 (not _needs_grad(k_new, v_new), "inference-only (no gradient)"),
@@ -789,24 +819,26 @@ def kv_append_q4(k_cache: torch.Tensor, v_cache: torch.Tensor, k_new: torch.Tens
                  f"caches must be uint8 [heads, capacity, {Q4_ROW_BYTES}] with contiguous rows"),
                 (k_cache.shape == v_cache.shape and k_cache.stride() == v_cache.stride(),
                  "K and V caches must share shape and strides"),
-                (k_new.dtype == bf16 and v_new.dtype == bf16, "takes bf16 rows"),
-                (k_new.shape == v_new.shape and heads == k_cache.shape[0] and d == 128 and k_new.stride(2) == 1
-                 and v_new.stride(2) == 1,
+                (k_new.dtype == _BF16 and v_new.dtype == _BF16, "takes bf16 rows"),
+                (k_new.shape == v_new.shape and heads == cache_heads and d == 128 and s2 == 1 and sv[2] == 1,
                  "new rows must be [cache heads, n, 128] with contiguous head_dim, the same for K and V"),
                 (offset_dev is None or offset_dev.dtype == torch.int64, "offset_dev must be int64"))
-    if _elsewhere(dev):
+    index = dev.index
+    if _current_device() != index:
         with torch.cuda.device(dev):
             return kv_append_q4(k_cache, v_cache, k_new, v_new, offset, offset_dev)
-    k_new, s0, s1 = _rows(k_new)
-    v_new, *sv = _rows(v_new)
-    if sv != [s0, s1]:
-        k_new, v_new, s0, s1 = k_new.contiguous(), v_new.contiguous(), n * 256, 256
-    cap = k_cache.shape[1]
+    if ss == sv and heads > 1 and n > 1 and s0 and s1:
+        s0, s1 = 2 * s0, 2 * s1
+    else:
+        k_new, s0, s1 = _rows(k_new)
+        v_new, *sv = _rows(v_new)
+        if sv != [s0, s1]:
+            k_new, v_new, s0, s1 = k_new.contiguous(), v_new.contiguous(), n * 256, 256
     rc = _lib.load().rt_kv_append_q4(k_cache.data_ptr(), v_cache.data_ptr(),
                                      k_cache.stride(0) if heads > 1 else cap * Q4_ROW_BYTES, k_new.data_ptr(),
                                      v_new.data_ptr(), s0, s1, heads, n, d, cap, int(offset),
                                      None if offset_dev is None else offset_dev.data_ptr(),
-                                     _STATE.status(dev).data_ptr(), _raw_stream(dev))
+                                     _status_ptr(dev), _raw_stream(index))
     if rc:
         _lib.check(rc, "rt_kv_append_q4")
     _count()
@@ -831,18 +863,19 @@ def kv_read_q4(cache: torch.Tensor, start: int, n: int, out: torch.Tensor | None
     start, n = int(start), int(n)
     if start < 0 or n < 0 or start + n > cap:
         raise RuntimeError(f"{what}: rows [{start}, {start + n}) are outside the cache's {cap}")
-    shape = (*cache.shape[:-2], n, 128)
+    shape = (heads, n, 128) if c is cache else (*cache.shape[:-2], n, 128)
     if out is None:
-        out = torch.empty(shape, dtype=torch.bfloat16, device=dev)
+        out = torch.empty(shape, dtype=_BF16, device=dev)
     elif out.shape != shape or out.dtype is not torch.bfloat16 or not out.is_contiguous() or out.device != dev:
         raise RuntimeError(f"{what}: out must be contiguous bf16 {list(shape)} on {dev}")
     if heads == 0 or n == 0:
         return out
-    if _elsewhere(dev):
+    index = dev.index
+    if _current_device() != index:
         with torch.cuda.device(dev):
             return kv_read_q4(cache, start, n, out)
     rc = _lib.load().rt_kv_read_q4(c.data_ptr(), c.stride(0) if heads > 1 else cap * Q4_ROW_BYTES, out.data_ptr(),
-                                   n * 256, 256, heads, n, 128, cap, start, _raw_stream(dev))
+                                   n * 256, 256, heads, n, 128, cap, start, _raw_stream(index))
     if rc:
         _lib.check(rc, "rt_kv_read_q4")
     _count()
@@ -865,11 +898,13 @@ def tree_attention_q4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask_bi
     q = _query(q, what)
     dev = q.device
     n, hq, d = q.shape
-    if not (_q4_rows(k) and _q4_rows(v) and q.is_cuda and q.dtype is torch.bfloat16 and d == 128 and q.stride(2) == 1
+    q0, q1, q2 = q.stride()
+    hkv, cap, _ = k.shape if k.dim() == 3 else (0, 0, 0)
+    if not (_q4_rows(k) and _q4_rows(v) and q.is_cuda and q.dtype is _BF16 and d == 128 and q2 == 1
             and k.shape == v.shape and k.stride() == v.stride() and k.device == dev and v.device == dev
-            and mask_bits.device == dev and n and hq and k.shape[0] and hq % k.shape[0] == 0
+            and mask_bits.device == dev and n and hq and hkv and hq % hkv == 0
             and mask_bits.dtype is torch.int32 and mask_bits.dim() == 2 and mask_bits.shape[0] >= n
-            and mask_bits.shape[1] * 32 >= n and not _needs_grad(q)
+            and mask_bits.shape[1] * 32 >= n and not (_grad_enabled() and q.requires_grad)
             and (prefix_len_dev is None or (prefix_len_dev.dtype is torch.int64 and prefix_len_dev.device == dev))):
         _refuse(what,
                 (q.is_cuda and k.is_cuda and v.is_cuda and mask_bits.is_cuda, "takes CUDA tensors (no CPU path)"),
@@ -879,33 +914,38 @@ def tree_attention_q4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask_bi
                 (_q4_rows(k) and _q4_rows(v),
                  f"caches must be uint8 [heads, capacity, {Q4_ROW_BYTES}] with contiguous rows"),
                 (k.shape == v.shape and k.stride() == v.stride(), "K and V caches must share shape and strides"),
-                (n and hq and k.shape[0] and hq % k.shape[0] == 0,
+                (n and hq and hkv and hq % hkv == 0,
                  "at least one node, and key heads that divide the query heads"),
                 (mask_bits.dtype == torch.int32 and mask_bits.dim() == 2 and mask_bits.shape[0] >= n
                  and mask_bits.shape[1] * 32 >= n, "mask_bits must be int32 [n, at least ceil(n / 32)]"),
                 (prefix_len_dev is None or prefix_len_dev.dtype == torch.int64, "prefix_len_dev must be int64"))
-    if _elsewhere(dev):
+    index = dev.index
+    if _current_device() != index:
         with torch.cuda.device(dev):
             return tree_attention_q4(q, k, v, mask_bits, prefix_len, scale, out, num_splits, prefix_len_dev)
     words, unit = mask_bits.stride()
     if unit != 1 or words < mask_bits.shape[1]:
         mask_bits = mask_bits.contiguous()
         words = mask_bits.shape[1]
-    q, q0, q1 = _rows(q)
-    out = _attn_out(out, q, what)
-    _, o0, o1 = _rows(out)
-    hkv, cap, _ = k.shape
-    lib = _lib.load()
+    if n > 1 and hq > 1 and q0 and q1:
+        q0, q1 = 2 * q0, 2 * q1
+    else:
+        q, q0, q1 = _rows(q)
+    if out is None:
+        out = q.new_empty((n, hq, 128))
+        o0, o1 = hq * 256, 256
+    else:
+        _, o0, o1 = _rows(_attn_out(out, q, what))
     prefix_len, num_splits = int(prefix_len), int(num_splits)
-    nbytes = lib.rt_tree_attn_q4_workspace_size(n, hq, hkv, d, prefix_len, num_splits)
+    nbytes = _tree_q4_workspace(index, n, hq, hkv, 128, prefix_len, num_splits)
     ws = _workspace(nbytes, dev)
-    rc = lib.rt_tree_attn_q4(q.data_ptr(), q0, q1, k.data_ptr(), v.data_ptr(),
-                             k.stride(0) if hkv > 1 else cap * Q4_ROW_BYTES, cap, out.data_ptr(), o0, o1,
-                             mask_bits.data_ptr(), words, n, prefix_len,
-                             None if prefix_len_dev is None else prefix_len_dev.data_ptr(), hq, hkv, d,
-                             128 ** -0.5 if scale is None else float(scale), num_splits,
-                             None if ws is None else ws.data_ptr(), nbytes, _STATE.status(dev).data_ptr(),
-                             _raw_stream(dev))
+    rc = _lib.load().rt_tree_attn_q4(q.data_ptr(), q0, q1, k.data_ptr(), v.data_ptr(),
+                                     k.stride(0) if hkv > 1 else cap * 72, cap, out.data_ptr(), o0, o1,
+                                     mask_bits.data_ptr(), words, n, prefix_len,
+                                     None if prefix_len_dev is None else prefix_len_dev.data_ptr(), hq, hkv, 128,
+                                     _SCALE if scale is None else float(scale), num_splits,
+                                     None if ws is None else ws.data_ptr(), nbytes, _status_ptr(dev),
+                                     _raw_stream(index))
     if rc:
         _lib.check(rc, "rt_tree_attn_q4")
     _count(2 if nbytes else 1)
