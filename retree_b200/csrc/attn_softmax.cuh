@@ -30,9 +30,13 @@ constexpr float kLazyRescale = 8.0f;  // log2 units
 // weights in fp32, before they are rounded.  fp16 weights sit 2^6 above the
 // maximum's 1 (2^14 at most), which keeps weights down to 2^-20 of it out of the
 // subnormal range.
-template <typename T>
+// part1() runs once the weights of the first kPart1 keys are in TMEM, so that
+// their product can start under the last quarter's exponentials; the caller
+// announces the rest.
+constexpr int kPart1 = 96;
+template <typename T, typename Part1>
 __device__ __forceinline__ void softmax_block(const uint32_t (&sr)[4][32], uint32_t ts, uint32_t to, bool rescale,
-                                              float sl2, float& m, float& l) {
+                                              float sl2, float& m, float& l, Part1 part1) {
   constexpr float kLift = std::is_same_v<T, __half> ? 6.f : 0.f;
   float a[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -72,7 +76,14 @@ __device__ __forceinline__ void softmax_block(const uint32_t (&sr)[4][32], uint3
       pk[i] = pack2<T>(p0, p1);
     }
     tmem_st16(ts + c * 16, pk);
+    if (c == kPart1 / 32 - 1) {
+      tmem_wait_st();
+      tc_fence_before();
+      part1();
+    }
   }
+  tmem_wait_st();
+  tc_fence_before();
   l += (acc[0].x + acc[1].x) + (acc[0].y + acc[1].y);
 }
 

@@ -69,6 +69,13 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
+// One arrival for a converged warp (lane 0, after every lane's earlier accesses):
+// arrivals on one barrier are serial, 32 of them cost a warp over 100 cycles.
+__device__ __forceinline__ void mbar_arrive_warp(uint64_t* bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
+
 __device__ __forceinline__ void mbar_arrive_expect_tx(uint64_t* bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes)
                : "memory");
@@ -103,6 +110,32 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
   *abort = 1;
   set_status(status, code);
   return false;
+}
+
+// The same for the hot loops of converged warps: a phase that is (nearly) there
+// costs one poll, about a third of mbar_wait's loop and its checks.  The loops do
+// not branch on the result: after a time-out their (bounded) waits fall through
+// and they finish on whatever is in shared memory, and the results are dropped
+// (*abort).
+__device__ __forceinline__ void mbar_wait_fast(uint64_t* bar, uint32_t parity, volatile int* abort, int* status) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .u32 i, a;\n\tmov.u32 i, 0;\n"
+      "POLL:\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "@p bra DONE;\n\t"
+      "add.u32 i, i, 1;\n\tsetp.lt.u32 q, i, %4;\n\t@!q bra DONE;\n\t"
+      "and.b32 a, i, 1023;\n\tsetp.ne.u32 q, a, 0;\n\t@q bra POLL;\n\t"
+      "ld.volatile.shared.u32 a, [%3];\n\tsetp.eq.u32 q, a, 0;\n\t@q bra POLL;\n"
+      "DONE:\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity), "r"(smem_u32(const_cast<int*>(abort))), "n"(kWaitLimit)
+      : "memory");
+  if (!ok) {
+    *abort = 1;
+    set_status(status, RT_DEV_WAIT_TIMEOUT);
+  }
 }
 
 // Wait (bounded, ignoring the abort flag) for copies a CTA issued itself to

@@ -66,7 +66,7 @@ struct PromptParams {
 };
 
 struct PromptBars {
-  uint64_t q_full[2], q_empty[2], kv_full[kPStages], kv_empty[kPStages], s_full[2], p_full[2], o_full[2],
+  uint64_t q_full[2], q_empty[2], kv_full[kPStages], kv_empty[kPStages], s_full[2], p_part[2], p_full[2], o_full[2],
       v_look, v_ok, fin;
   uint32_t tmem_base;
   int abort_flag;
@@ -183,7 +183,8 @@ __global__ void __launch_bounds__(kPThreads, 1)
       mbar_init(&bar.q_full[t], 1);
       mbar_init(&bar.q_empty[t], 1);
       mbar_init(&bar.s_full[t], 1);
-      mbar_init(&bar.p_full[t], 128);
+      mbar_init(&bar.p_part[t], 4);
+      mbar_init(&bar.p_full[t], 4);
       mbar_init(&bar.o_full[t], 1);
     }
     for (int s = 0; s < kPStages; ++s) {
@@ -290,12 +291,7 @@ __global__ void __launch_bounds__(kPThreads, 1)
     int n = 0;  // ring loads consumed
     int nq[2] = {0, 0}, np[2] = {0, 0};
     uint32_t looks = 0;  // V blocks handed to warp 10
-    bool ok = true;
-    auto wait = [&](uint64_t* b, uint32_t ph) {
-      ok = ok && mbar_wait(b, ph & 1, abort_flag, p.status, RT_DEV_WAIT_TIMEOUT);
-      ok = __all_sync(0xFFFFFFFFu, ok);
-      return ok;
-    };
+    auto wait = [&](uint64_t* b, uint32_t ph) { mbar_wait_fast(b, ph & 1, abort_flag, p.status); };
     // S_t = Q_t K^T of the block in `stage`; the last one of an item frees Q_t
     auto qk = [&](int t, int stage, bool last) {
       const uint64_t b = dk + static_cast<uint64_t>(warp_uniform(stage) * (kPTile >> 4));
@@ -312,54 +308,59 @@ __global__ void __launch_bounds__(kPThreads, 1)
     auto commit = [&](uint64_t* b) {
       if (elect_one()) umma_commit(b);
     };
-    for (int it = 0; ok && prompt_item(p, tab, it, w); ++it) {
+    for (int it = 0; prompt_item(p, tab, it, w); ++it) {
+      if (__any_sync(0xFFFFFFFFu, *abort_flag)) break;
       const int nb = max(w.nb[0], w.nb[1]);
       if (nb == 0) continue;
-      int s = n % kPStages;
-      if (!wait(&bar.kv_full[s], n / kPStages)) break;
+      const int s = n % kPStages;
+      wait(&bar.kv_full[s], n / kPStages);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         if (w.nb[t] == 0) continue;
-        if (!wait(&bar.q_full[t], nq[t]++)) break;
+        wait(&bar.q_full[t], nq[t]++);
         tc_fence_after();
         qk(t, s, w.nb[t] == 1);
       }
-      if (!ok) break;
       commit(&bar.kv_empty[s]);
       ++n;
-      for (int j = 0; j < nb && ok; ++j) {
+      for (int j = 0; j < nb; ++j) {
         const int sv = n % kPStages, sk = (n + 1) % kPStages;
         const bool more = j + 1 < nb;
-        if (!wait(&bar.kv_full[sv], n / kPStages)) break;
+        wait(&bar.kv_full[sv], n / kPStages);
         bool look = j >= w.jm;
-        if (look && lane == 0) mbar_arrive(&bar.v_look);
-        __syncwarp();
+        if (look && elect_one()) mbar_arrive(&bar.v_look);
+        if (more) wait(&bar.kv_full[sk], (n + 1) / kPStages);
         const uint64_t b = dv + static_cast<uint64_t>(warp_uniform(sv) * (kPTile >> 4));
-        bool have_k = false;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           if (j < w.nb[t]) {
-            if (!wait(&bar.p_full[t], np[t]++)) break;
-            if (look && !wait(&bar.v_ok, looks++)) break;
+            auto pv = [&](int kk) {
+              umma_f16_ts(tm + kPTmemO + t * kPD, tm + t * kPB + kk * 8, b + kk * (2048 >> 4), idesc_pv,
+                          (j > 0 || kk > 0) ? 1u : 0u);
+            };
+            if (kPart1 < kPB) {
+              wait(&bar.p_part[t], np[t]);
+              if (look) wait(&bar.v_ok, looks++);
+              look = false;
+              tc_fence_after();
+              if (elect_one()) {
+#pragma unroll
+                for (int kk = 0; kk < kPart1 / 16; ++kk) pv(kk);
+              }
+            }
+            wait(&bar.p_full[t], np[t]++);
+            if (look) wait(&bar.v_ok, looks++);
             look = false;
             tc_fence_after();
             if (elect_one()) {
 #pragma unroll
-              for (int kk = 0; kk < kPB / 16; ++kk)
-                umma_f16_ts(tm + kPTmemO + t * kPD, tm + t * kPB + kk * 8, b + kk * (2048 >> 4), idesc_pv,
-                            (j > 0 || kk > 0) ? 1u : 0u);
+              for (int kk = (kPart1 < kPB ? kPart1 / 16 : 0); kk < kPB / 16; ++kk) pv(kk);
               if (j + 1 == w.nb[t]) umma_commit(&bar.o_full[t]);
             }
           }
+          if (j + 1 < w.nb[t]) qk(t, sk, j + 2 == w.nb[t]);
           if (t == 1) commit(&bar.kv_empty[sv]);
-          if (j + 1 < w.nb[t]) {
-            if (!have_k && !wait(&bar.kv_full[sk], (n + 1) / kPStages)) break;
-            have_k = true;
-            tc_fence_after();
-            qk(t, sk, j + 2 == w.nb[t]);
-          }
         }
-        if (!ok) break;
         if (more) commit(&bar.kv_empty[sk]);
         n += more ? 2 : 1;
       }
@@ -378,14 +379,12 @@ __global__ void __launch_bounds__(kPThreads, 1)
     int n = 0;
     uint32_t looks = 0;
     for (int it = 0; prompt_item(p, tab, it, w); ++it) {
+      if (__any_sync(0xFFFFFFFFu, *abort_flag)) break;
       const int nb = max(w.nb[0], w.nb[1]);
-      bool ok = true;
       for (int j = min(w.jm, nb); j < nb; ++j) {
         const int m = n + 2 * j + 1, s = m % kPStages;
-        ok = mbar_wait(&bar.v_look, looks++ & 1, abort_flag, p.status, RT_DEV_WAIT_TIMEOUT) &&
-             mbar_wait(&bar.kv_full[s], (m / kPStages) & 1, abort_flag, p.status, RT_DEV_WAIT_TIMEOUT);
-        ok = __all_sync(0xFFFFFFFFu, ok);
-        if (!ok) break;
+        mbar_wait_fast(&bar.v_look, looks++ & 1, abort_flag, p.status);
+        mbar_wait_fast(&bar.kv_full[s], (m / kPStages) & 1, abort_flag, p.status);
         uint4* v = reinterpret_cast<uint4*>(smem + kPOffKV + s * kPTile) + lane;
         uint32_t bad = 0;
 #pragma unroll 8
@@ -413,7 +412,6 @@ __global__ void __launch_bounds__(kPThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar.v_ok);
       }
-      if (!ok) break;
       n += 2 * nb;
     }
   } else if (warp < 8) {
@@ -426,8 +424,8 @@ __global__ void __launch_bounds__(kPThreads, 1)
     const int rt = r / p.group, rh = r - rt * p.group;
     const float sl2 = p.scale_log2;
     int ns = 0, no = 0;
-    bool ok = true;
-    for (int it = 0; ok && prompt_item(p, tab, it, w); ++it) {
+    for (int it = 0; prompt_item(p, tab, it, w); ++it) {
+      if (__any_sync(0xFFFFFFFFu, *abort_flag)) break;
       const int tok = w.tok0 + t * p.tok + rt;
       const bool valid = t < p.tiles && rt < p.tok && tok < w.lq;
       const int lim = valid ? min(max(tok + 1 + w.lk - w.lq, 0), w.lk) : 0;  // keys this row sees
@@ -435,10 +433,7 @@ __global__ void __launch_bounds__(kPThreads, 1)
       const int nb = t == 0 ? w.nb[0] : w.nb[1];
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < nb; ++j) {
-        ok = mbar_wait(&bar.s_full[t], ns & 1, abort_flag, p.status, RT_DEV_WAIT_TIMEOUT);
-        ok = __all_sync(0xFFFFFFFFu, ok);
-        if (!ok) break;
-        ++ns;
+        mbar_wait_fast(&bar.s_full[t], ns++ & 1, abort_flag, p.status);
         tc_fence_after();
         uint32_t sr[4][32];
 #pragma unroll
@@ -452,12 +447,9 @@ __global__ void __launch_bounds__(kPThreads, 1)
             for (int i = 0; i < 32; ++i)
               if (c * 32 + i >= left) sr[c][i] = __float_as_uint(-INFINITY);
         }
-        softmax_block<T>(sr, ts, to, j > 0, sl2, m, l);
-        tmem_wait_st();
-        tc_fence_before();
-        mbar_arrive(&bar.p_full[t]);
+        softmax_block<T>(sr, ts, to, j > 0, sl2, m, l, [&] { mbar_arrive_warp(&bar.p_part[t]); });
+        mbar_arrive_warp(&bar.p_full[t]);
       }
-      if (!ok) break;
       char* dst = p.out + static_cast<int64_t>(w.q0 + tok) * p.out_tok_stride +
                   static_cast<int64_t>(w.g * p.group + rh) * p.out_head_stride;
       if (nb == 0) {
@@ -465,10 +457,8 @@ __global__ void __launch_bounds__(kPThreads, 1)
           for (int c = 0; c < 16; ++c) *reinterpret_cast<uint4*>(dst + c * 16) = make_uint4(0, 0, 0, 0);
         continue;
       }
-      ok = mbar_wait(&bar.o_full[t], no & 1, abort_flag, p.status, RT_DEV_WAIT_TIMEOUT);
-      ok = __all_sync(0xFFFFFFFFu, ok);
-      if (!ok) break;
-      ++no;
+      mbar_wait_fast(&bar.o_full[t], no++ & 1, abort_flag, p.status);
+      if (__any_sync(0xFFFFFFFFu, *abort_flag)) break;
       tc_fence_after();
       const float inv = lim > 0 ? 1.f / l : 0.f;
       const bool poison = *const_cast<volatile int*>(&bar.poison) != 0;

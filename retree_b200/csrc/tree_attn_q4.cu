@@ -449,7 +449,7 @@ constexpr uint32_t kQtTmemO = 256;                    // S0 | S1 | O0 | O1, P_t 
 
 struct Q4Bars {
   uint64_t q_full[2], in_full[kQtPacked], in_empty[kQtPacked], kv_full[kQtStages], kv_empty[kQtStages], s_full[2],
-      p_full[2], o_full[2], fin;
+      p_part[2], p_full[2], o_full[2], fin;
   uint32_t tmem_base;
   int abort_flag;
   uint2 x43;  // (.x)
@@ -497,15 +497,16 @@ __global__ void __launch_bounds__(kQtThreads, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bar.q_full[i], 1);
       mbar_init(&bar.s_full[i], 1);
-      mbar_init(&bar.p_full[i], 128);
+      mbar_init(&bar.p_part[i], 4);
+      mbar_init(&bar.p_full[i], 4);
       mbar_init(&bar.o_full[i], 1);
     }
     for (int i = 0; i < kQtPacked; ++i) {
       mbar_init(&bar.in_full[i], 1);
-      mbar_init(&bar.in_empty[i], 128);
+      mbar_init(&bar.in_empty[i], 4);
     }
     for (int i = 0; i < kQtStages; ++i) {
-      mbar_init(&bar.kv_full[i], 128);
+      mbar_init(&bar.kv_full[i], 4);
       mbar_init(&bar.kv_empty[i], 1);
     }
     mbar_init(&bar.fin, 1);
@@ -563,56 +564,73 @@ __global__ void __launch_bounds__(kQtThreads, 1)
         for (int i = max(0, n - kQtPacked); i < n; ++i)
           mbar_wait_drain(&bar.in_full[i % kQtPacked], (i / kQtPacked) & 1);
       }
-    } else if (warp == 13 && lane == 0) {
+    } else if (warp == 13) {
       // ---------------- MMA issuer ----------------
       constexpr uint32_t idesc_qk = idesc_bf16_f32(kBM, kQtKeys, false, false);
       constexpr uint32_t idesc_pv = idesc_bf16_f32(kBM, kHD, false, true);
-      const uint32_t sq = smem_u32(smem + kQtOffQ), skv = smem_u32(smem + kQtOffKV);
-      bool ok = true;
-      auto wait = [&](uint64_t* b, uint32_t ph) {
-        ok = ok && mbar_wait(b, ph & 1, abort_flag, p.status, RT_DEV_WAIT_TIMEOUT);
-        return ok;
-      };
-      auto qk = [&](int t, int stage) {
-        const uint32_t a = sq + t * kQtTile, b = skv + stage * kQtTile;
-#pragma unroll
-        for (int kk = 0; kk < kHD / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * kQtHalf + (kk & 3) * 32;
-          umma_f16(tmem + t * 128, smem_desc_sw128(a + off, 16, 1024), smem_desc_sw128(b + off, 16, 1024), idesc_qk,
-                   kk > 0);
-        }
-        umma_commit(&bar.s_full[t]);
-      };
-      for (int j = -1; j < nb && ok && nb > 0; ++j) {
+      const uint32_t tm = warp_uniform(tmem);
+      const uint64_t dq = warp_uniform(smem_desc_sw128(smem_u32(smem + kQtOffQ), 16, 1024));
+      const uint64_t dk = warp_uniform(smem_desc_sw128(smem_u32(smem + kQtOffKV), 16, 1024));
+      const uint64_t dv = warp_uniform(smem_desc_sw128(smem_u32(smem + kQtOffKV), kQtHalf, 1024));
+      auto wait = [&](uint64_t* b, uint32_t ph) { mbar_wait_fast(b, ph & 1, abort_flag, p.status); };
+      for (int j = -1; j < nb && nb > 0; ++j) {
         // loads 2j+1 = V_j and 2j+2 = K_{j+1}
         const int nv = 2 * j + 1, nk = 2 * j + 2;
         const int sv = nv & (kQtStages - 1), sk = nk % kQtStages;
         const bool more = j + 1 < nb;
-        if (j >= 0 && !wait(&bar.kv_full[sv], nv / kQtStages)) break;
-        for (int t = 0; t < tiles; ++t) {
-          if (j >= 0) {
-            if (!wait(&bar.p_full[t], j)) break;
-            tc_fence_after();
-            const uint32_t b = skv + sv * kQtTile;
+        if (j >= 0) wait(&bar.kv_full[sv], nv / kQtStages);
+        if (more) wait(&bar.kv_full[sk], nk / kQtStages);
+        const uint64_t bk = dk + static_cast<uint64_t>(warp_uniform(sk) * (kQtTile >> 4));
+        const uint64_t bv = dv + static_cast<uint64_t>(warp_uniform(sv) * (kQtTile >> 4));
 #pragma unroll
-            for (int kk = 0; kk < kQtKeys / 16; ++kk)
-              umma_f16_ts(tmem + kQtTmemO + t * kHD, tmem + t * 128 + kk * 8,
-                          smem_desc_sw128(b + kk * 2048, kQtHalf, 1024), idesc_pv, (j > 0 || kk > 0) ? 1u : 0u);
-            if (!more) umma_commit(&bar.o_full[t]);
-            if (t + 1 == tiles) umma_commit(&bar.kv_empty[sv]);
-          }
-          if (more) {
-            if (t == 0 && !wait(&bar.kv_full[sk], nk / kQtStages)) break;
-            if (j < 0 && !wait(&bar.q_full[t], 0)) break;
+        for (int t = 0; t < 2; ++t) {
+          if (t >= tiles) continue;
+          if (j >= 0) {
+            auto pv = [&](int kk) {
+              umma_f16_ts(tm + kQtTmemO + t * kHD, tm + t * 128 + kk * 8, bv + kk * (2048 >> 4), idesc_pv,
+                          (j > 0 || kk > 0) ? 1u : 0u);
+            };
+            if (kPart1 < kQtKeys) {
+              wait(&bar.p_part[t], j);
+              tc_fence_after();
+              if (elect_one()) {
+#pragma unroll
+                for (int kk = 0; kk < kPart1 / 16; ++kk) pv(kk);
+              }
+            }
+            wait(&bar.p_full[t], j);
             tc_fence_after();
-            qk(t, sk);
+            if (elect_one()) {
+#pragma unroll
+              for (int kk = (kPart1 < kQtKeys ? kPart1 / 16 : 0); kk < kQtKeys / 16; ++kk) pv(kk);
+              if (!more) umma_commit(&bar.o_full[t]);
+            }
+          } else {
+            wait(&bar.q_full[t], 0);
+            tc_fence_after();
           }
+          if (more && elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < kHD / 16; ++kk) {
+              const uint32_t off = ((kk >> 2) * kQtHalf + (kk & 3) * 32) >> 4;
+              umma_f16(tm + t * 128, dq + t * (kQtTile >> 4) + off, bk + off, idesc_qk, kk > 0);
+            }
+            umma_commit(&bar.s_full[t]);
+          }
+          __syncwarp();
         }
-        if (ok && more) umma_commit(&bar.kv_empty[sk]);
+        if (elect_one()) {
+          if (j >= 0) umma_commit(&bar.kv_empty[sv]);
+          if (more) umma_commit(&bar.kv_empty[sk]);
+        }
+        __syncwarp();
       }
       // all issued MMAs complete before TMEM is released
-      umma_commit(&bar.fin);
-      mbar_wait_drain(&bar.fin, 0);
+      if (elect_one()) {
+        umma_commit(&bar.fin);
+        mbar_wait_drain(&bar.fin, 0);
+      }
+      __syncwarp();
     }
   } else if (warp >= 8) {
     // ---------------- decode ----------------
@@ -623,9 +641,8 @@ __global__ void __launch_bounds__(kQtThreads, 1)
     for (int n = 0; n < 2 * nb; ++n) {
       const int si = n % kQtPacked, so = n % kQtStages;
       const int64_t key = (b0 + (n >> 1)) * kQtKeys + r;
-      bool ok = mbar_wait(&bar.in_full[si], (n / kQtPacked) & 1, abort_flag, p.status, RT_DEV_WAIT_TIMEOUT) &&
-                mbar_wait(&bar.kv_empty[so], ((n / kQtStages) & 1) ^ 1, abort_flag, p.status, RT_DEV_WAIT_TIMEOUT);
-      if (!ok) break;
+      mbar_wait_fast(&bar.in_full[si], (n / kQtPacked) & 1, abort_flag, p.status);
+      mbar_wait_fast(&bar.kv_empty[so], ((n / kQtStages) & 1) ^ 1, abort_flag, p.status);
       // behind the tree: zero.  A tree row of V that reads as NaN: zero in V, and
       // NaN in K, so that only the nodes that see the key get it.
       bool zero = key >= total, nan = false;
@@ -634,9 +651,9 @@ __global__ void __launch_bounds__(kQtThreads, 1)
         nan = !zero;
       }
       q4_decode_row(sbase + kQtOffPacked + si * kQtBlock + r * kQ4Row, sbase + kQtOffKV + so * kQtTile, r, zero, nan, x43,
-                    [&] { mbar_arrive(&bar.in_empty[si]); });
+                    [&] { mbar_arrive_warp(&bar.in_empty[si]); });
       fence_proxy_async_smem();
-      mbar_arrive(&bar.kv_full[so]);
+      mbar_arrive_warp(&bar.kv_full[so]);
     }
   } else {
     // ---------------- softmax and result of tile t ----------------
@@ -654,11 +671,8 @@ __global__ void __launch_bounds__(kQtThreads, 1)
     const bool warp_live = t < tiles && ((warp & 3) * 32) / G < tok && node0 + t * tok + ((warp & 3) * 32) / G < p.n;
     const float sl2 = p.scale_log2;
     float m = -INFINITY, l = 0.f;
-    bool ok = true;
     for (int j = 0; j < nb && t < tiles; ++j) {
-      ok = mbar_wait(&bar.s_full[t], j & 1, abort_flag, p.status, RT_DEV_WAIT_TIMEOUT);
-      ok = __all_sync(0xFFFFFFFFu, ok);
-      if (!ok) break;
+      mbar_wait_fast(&bar.s_full[t], j & 1, abort_flag, p.status);
       if (warp_live) {
         tc_fence_after();
         uint32_t sr[4][32];
@@ -675,19 +689,18 @@ __global__ void __launch_bounds__(kQtThreads, 1)
               if (!((vm >> i) & 1u)) sr[c][i] = __float_as_uint(-INFINITY);
           }
         }
-        softmax_block<__nv_bfloat16>(sr, ts, to, j > 0, sl2, m, l);
-        tmem_wait_st();
-        tc_fence_before();
+        softmax_block<__nv_bfloat16>(sr, ts, to, j > 0, sl2, m, l, [&] { mbar_arrive_warp(&bar.p_part[t]); });
+      } else {
+        mbar_arrive_warp(&bar.p_part[t]);
       }
-      mbar_arrive(&bar.p_full[t]);
+      mbar_arrive_warp(&bar.p_full[t]);
     }
     const int64_t rows_ws = static_cast<int64_t>(p.tiles) * kBM;
     const int64_t slot = (static_cast<int64_t>(split) * p.num_kv_heads + kvh) * rows_ws + R;
     if (l != l) m = INFINITY;  // a NaN weight wins the merge
-    if (ok && inside && warp_live && nb > 0) {
-      ok = mbar_wait(&bar.o_full[t], 0, abort_flag, p.status, RT_DEV_WAIT_TIMEOUT);
-      ok = __all_sync(0xFFFFFFFFu, ok);
-      if (ok) {
+    if (inside && warp_live && nb > 0) {
+      mbar_wait_fast(&bar.o_full[t], 0, abort_flag, p.status);
+      if (!__any_sync(0xFFFFFFFFu, *abort_flag)) {
         tc_fence_after();
         const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll 1
