@@ -6,13 +6,18 @@
 //
 // A work item is 256 query rows of one kv head -- two 128-row tiles, row r of a
 // tile being (token r / G, query head r % G) of G = Hq / Hkv, so the heads of a
-// group share every K/V tile -- and all the 128-key blocks they see.  CTAs are
-// persistent (one per SM) and take items longest first.  Twelve warps:
+// group share every K/V tile -- and all the 128-key blocks they see (or one of
+// `splits` shares of them, when the items alone would leave SMs without work; the
+// shares are merged through the workspace by prompt_combine_kernel).  The items
+// are ordered longest first and handed out by the hardware: a CTA runs the item
+// of its own block index, then takes over the next block that has not started.
+// Twelve warps:
 //   warps 0-3, 4-7  softmax of tile 0 / 1, one thread per row: S from TMEM, the
 //                   online softmax in the exp2 domain with a lazy (> 8 in log2)
 //                   rescale of O in TMEM, P back into S's own columns, and the
 //                   tile's output rows;
-//   warp 8          TMA producer: Q tiles, and K / V blocks into a 4-stage ring;
+//   warp 8          producer: Q tiles and K / V blocks (a 4-stage ring) by TMA, and
+//                   the requests for further items (cluster launch control);
 //   warp 9          MMA issuer: per block PV of tile 0, next QK of
 //                   tile 0, PV of tile 1, next QK of tile 1 -- while one tile's
 //                   softmax runs the tensor core has the other tile's products;
@@ -47,7 +52,8 @@ constexpr uint32_t kPOffQ = 0;
 constexpr uint32_t kPOffKV = 2 * kPTile;
 constexpr uint32_t kPOffTab = kPOffKV + kPStages * kPTile;  // prefix sums of the sequences' pair counts
 constexpr int kPMaxSeqs = 4096;
-constexpr uint32_t kPOffBar = kPOffTab + (kPMaxSeqs + 1) * 4 + 12;
+constexpr uint32_t kPOffOrd = kPOffTab + (kPMaxSeqs + 1) * 4 + 12;  // up to 32 sequences, longest first
+constexpr uint32_t kPOffBar = kPOffOrd + 32 * 4;
 constexpr uint32_t kPSmem = kPOffBar + 512 + 1024;
 constexpr uint32_t kPTmemO = 256;              // S0 | S1 | O0 | O1, P_t in S_t's first 64 columns
 constexpr int kPSms = 148;
@@ -61,22 +67,28 @@ struct PromptParams {
   const int32_t* cu_k;
   int num_seqs, total_q, total_k, hkv, group, tok;  // tok: tokens per 128-row tile
   int tiles;                                        // tiles per item: 2, or 1 when the call is small
+  int splits;                                       // shares of an item's keys
+  int hq;
+  float* ws_o;                                      // [split][token][head][128]
+  float2* ws_ml;                                    // [split][token][head] (m in log2 units, l)
   float scale_log2;
   int* status;
 };
 
 struct PromptBars {
   uint64_t q_full[2], q_empty[2], kv_full[kPStages], kv_empty[kPStages], s_full[2], p_part[2], p_full[2], o_full[2],
-      v_look, v_ok, fin;
+      v_look, v_ok, clc_full[2], clc_empty[2], fin;
+  uint4 clc[2];
   uint32_t tmem_base;
   int abort_flag;
   int poison;  // set once a checked V block held a value that is not finite
 };
 
 struct PromptItem {
-  int q0, lq, k0, lk, tok0, g;
-  int nb[2];  // key blocks of each tile
-  int jm;     // first block that some row of the item hides in part
+  int q0, lq, k0, lk, tok0, g, split;
+  int jb;     // first key block of this share
+  int nb[2];  // its blocks in each tile
+  int jm;     // the first of them that some row of the item hides in part
 };
 
 __device__ __forceinline__ bool prompt_seq(const PromptParams& p, int b, int& q0, int& lq, int& k0, int& lk) {
@@ -93,35 +105,60 @@ __device__ __forceinline__ bool prompt_seq(const PromptParams& p, int b, int& q0
   return q0 >= 0 && q1 >= q0 && q1 <= p.total_q && k0 >= 0 && k1 >= k0 && k1 <= p.total_k;
 }
 
-// Item `it` of this CTA: round r runs through the list forwards or backwards
-// (the list is sorted by length within a sequence, so a CTA's items average out).
-__device__ __forceinline__ bool prompt_item(const PromptParams& p, const int* tab, int it, PromptItem& w) {
-  const int grid = gridDim.x;
-  const int64_t idx = static_cast<int64_t>(it) * grid + ((it & 1) ? grid - 1 - blockIdx.x : blockIdx.x);
-  const int64_t pos64 = idx / p.hkv;
-  const int total = tab[p.num_seqs];
-  if (static_cast<int64_t>(it) * grid >= static_cast<int64_t>(total) * p.hkv) return false;
+// The item of block index `idx`: kv head fastest, then share, then tile (the
+// last, longest one of a sequence first), then sequence.
+__device__ __forceinline__ void prompt_item(const PromptParams& p, const int* tab, const int* ord, int idx,
+                                            PromptItem& w) {
   w.nb[0] = w.nb[1] = 0;
-  w.jm = 0;
-  w.lq = w.tok0 = 0;
-  if (pos64 >= total) return true;  // an empty place of the last round
-  const int pos = static_cast<int>(pos64);
-  w.g = static_cast<int>(idx - pos64 * p.hkv);
-  int lo = 0, hi = p.num_seqs;  // tab[lo] <= pos < tab[hi]
+  w.jm = w.jb = w.lq = w.tok0 = 0;
+  int pos = idx / p.hkv;
+  w.g = idx - pos * p.hkv;
+  w.split = pos % p.splits;
+  pos /= p.splits;
+  if (pos >= tab[p.num_seqs]) return;  // (the grid is sized for the most items there can be)
+  int lo = 0, hi = p.num_seqs;         // tab[lo] <= pos < tab[hi]
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (tab[mid] <= pos) lo = mid; else hi = mid;
   }
-  prompt_seq(p, lo, w.q0, w.lq, w.k0, w.lk);
-  const int tile = tab[lo + 1] - 1 - pos;  // the longest (last) tiles first
+  prompt_seq(p, p.num_seqs <= 32 ? ord[lo] : lo, w.q0, w.lq, w.k0, w.lk);
+  const int tile = tab[lo + 1] - 1 - pos;
   w.tok0 = tile * p.tiles * p.tok;
   const int shift = w.lk - w.lq;
-  for (int t = 0; t < p.tiles; ++t) {
+  int nb[2] = {0, 0};
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
     const int first = w.tok0 + t * p.tok;
     const int lim = min(first + p.tok, w.lq) + shift;  // keys the tile's last token sees
-    w.nb[t] = (first < w.lq && lim > 0) ? (lim + kPB - 1) / kPB : 0;
+    if (t < p.tiles && first < w.lq && lim > 0) nb[t] = (lim + kPB - 1) / kPB;
   }
-  w.jm = max(w.tok0 + 1 + shift, 0) / kPB;
+  const int all = max(nb[0], nb[1]);
+  w.jb = all * w.split / p.splits;
+  const int je = all * (w.split + 1) / p.splits;
+  w.nb[0] = max(min(nb[0], je) - w.jb, 0);
+  w.nb[1] = max(min(nb[1], je) - w.jb, 0);
+  w.jm = max(max(w.tok0 + 1 + shift, 0) / kPB - w.jb, 0);
+}
+
+// The `it`-th item of this CTA for one converged warp (or one lane that acts for
+// it): its own block's, then those taken over.  False when there is none.
+template <bool kWarp>
+__device__ __forceinline__ bool prompt_next(const PromptParams& p, PromptBars& bar, const int* tab, const int* ord,
+                                            int it, PromptItem& w) {
+  int idx = blockIdx.x;
+  if (it > 0) {
+    const int s = (it - 1) & 1;
+    mbar_wait_fast(&bar.clc_full[s], ((it - 1) >> 1) & 1, &bar.abort_flag, p.status);
+    idx = *const_cast<volatile int*>(&bar.abort_flag) ? -1 : clc_taken(smem_u32(&bar.clc[s]));
+    if constexpr (kWarp) {
+      idx = __reduce_min_sync(0xFFFFFFFFu, idx);  // (the same in every lane but for an abort in between)
+      mbar_arrive_warp(&bar.clc_empty[s]);
+    } else {
+      mbar_arrive(&bar.clc_empty[s]);
+    }
+  }
+  if (idx < 0) return false;
+  prompt_item(p, tab, ord, idx, w);
   return true;
 }
 
@@ -173,6 +210,7 @@ __global__ void __launch_bounds__(kPThreads, 1)
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   PromptBars& bar = *reinterpret_cast<PromptBars*>(smem + kPOffBar);
   int* tab = reinterpret_cast<int*>(smem + kPOffTab);
+  int* ord = reinterpret_cast<int*>(smem + kPOffOrd);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (warp == 8 && lane == 0) {
@@ -191,6 +229,10 @@ __global__ void __launch_bounds__(kPThreads, 1)
       mbar_init(&bar.kv_full[s], 1);
       mbar_init(&bar.kv_empty[s], 1);
     }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bar.clc_full[i], 1);
+      mbar_init(&bar.clc_empty[i], 11);  // warps 0-10
+    }
     mbar_init(&bar.v_look, 1);
     mbar_init(&bar.v_ok, 1);
     mbar_init(&bar.fin, 1);
@@ -207,12 +249,22 @@ __global__ void __launch_bounds__(kPThreads, 1)
   // prefix sums of the sequences' item counts, by warp 10
   if (warp == 10) {
     const int span = p.tiles * p.tok;
+    int q0, lq, k0, lk;
+    if (p.num_seqs <= 32) {  // longest keys first (stable)
+      const int key = lane < p.num_seqs ? (prompt_seq(p, lane, q0, lq, k0, lk) ? lk : -1) : -2;
+      int rank = 0;
+      for (int i = 0; i < p.num_seqs; ++i) {
+        const int other = __shfl_sync(0xFFFFFFFFu, key, i);
+        rank += other > key || (other == key && i < lane);
+      }
+      if (lane < p.num_seqs) ord[rank] = lane;
+      __syncwarp();
+    }
     int carry = 0;
     for (int b0 = 0; b0 < p.num_seqs; b0 += 32) {
       int n = 0;
       if (b0 + lane < p.num_seqs) {
-        int q0, lq, k0, lk;
-        if (prompt_seq(p, b0 + lane, q0, lq, k0, lk)) n = (lq + span - 1) / span;
+        if (prompt_seq(p, p.num_seqs <= 32 ? ord[lane] : b0 + lane, q0, lq, k0, lk)) n = (lq + span - 1) / span;
         else set_status(p.status, RT_DEV_BAD_INDEX);
       }
 #pragma unroll
@@ -252,10 +304,28 @@ __global__ void __launch_bounds__(kPThreads, 1)
         tma_load_3d(dst + kPHalf, map, &bar.kv_full[s], 64, row, w.g);
         ++n;
       };
-      for (int it = 0; ok && prompt_item(p, tab, it, w); ++it) {
+      // The next item is asked for when three blocks of this one are left to load:
+      // late, so that whoever is done first gets it, and early enough that the
+      // answer is there in time.  (Asked for at once, 256 items on 148 CTAs were
+      // all handed out in the first microsecond: 2048 tokens took 52 us, not 43.)
+      int asked = 0;
+      auto take_over = [&](int it) {
+        const int s = it & 1;
+        if (!mbar_wait(&bar.clc_empty[s], ((it >> 1) & 1) ^ 1, abort_flag, p.status, RT_DEV_WAIT_TIMEOUT)) return false;
+        mbar_arrive_expect_tx(&bar.clc_full[s], 16);
+        clc_try_cancel(smem_u32(&bar.clc[s]), &bar.clc_full[s]);
+        asked = it + 1;
+        return true;
+      };
+      for (int it = 0; ok && prompt_next<false>(p, bar, tab, ord, it, w); ++it) {
         const int nb = max(w.nb[0], w.nb[1]);
+        if (nb == 0) ok = take_over(it);
         for (int j = 0; j < nb && ok; ++j) {
-          load(&tmap_k, w.k0 + j * kPB);
+          if (j == max(nb - 3, 0)) {
+            ok = take_over(it);
+            if (!ok) break;
+          }
+          load(&tmap_k, w.k0 + (w.jb + j) * kPB);
           if (j == 0) {
             for (int t = 0; t < 2 && ok; ++t) {
               if (w.nb[t] == 0) continue;
@@ -268,7 +338,7 @@ __global__ void __launch_bounds__(kPThreads, 1)
               ++nq[t];
             }
           }
-          if (ok) load(&tmap_v, w.k0 + j * kPB);
+          if (ok) load(&tmap_v, w.k0 + (w.jb + j) * kPB);
         }
       }
       if (*abort_flag) {
@@ -276,6 +346,7 @@ __global__ void __launch_bounds__(kPThreads, 1)
           mbar_wait_drain(&bar.kv_full[i % kPStages], (i / kPStages) & 1);
         for (int t = 0; t < 2; ++t)
           if (nq[t] > 0) mbar_wait_drain(&bar.q_full[t], (nq[t] - 1) & 1);
+        if (asked > 0) mbar_wait_drain(&bar.clc_full[(asked - 1) & 1], ((asked - 1) >> 1) & 1);
       }
     }
   } else if (warp == 9) {
@@ -308,8 +379,7 @@ __global__ void __launch_bounds__(kPThreads, 1)
     auto commit = [&](uint64_t* b) {
       if (elect_one()) umma_commit(b);
     };
-    for (int it = 0; prompt_item(p, tab, it, w); ++it) {
-      if (__any_sync(0xFFFFFFFFu, *abort_flag)) break;
+    for (int it = 0; prompt_next<true>(p, bar, tab, ord, it, w); ++it) {
       const int nb = max(w.nb[0], w.nb[1]);
       if (nb == 0) continue;
       const int s = n % kPStages;
@@ -378,8 +448,7 @@ __global__ void __launch_bounds__(kPThreads, 1)
     // the check runs beside the block's softmax)
     int n = 0;
     uint32_t looks = 0;
-    for (int it = 0; prompt_item(p, tab, it, w); ++it) {
-      if (__any_sync(0xFFFFFFFFu, *abort_flag)) break;
+    for (int it = 0; prompt_next<true>(p, bar, tab, ord, it, w); ++it) {
       const int nb = max(w.nb[0], w.nb[1]);
       for (int j = min(w.jm, nb); j < nb; ++j) {
         const int m = n + 2 * j + 1, s = m % kPStages;
@@ -424,12 +493,11 @@ __global__ void __launch_bounds__(kPThreads, 1)
     const int rt = r / p.group, rh = r - rt * p.group;
     const float sl2 = p.scale_log2;
     int ns = 0, no = 0;
-    for (int it = 0; prompt_item(p, tab, it, w); ++it) {
-      if (__any_sync(0xFFFFFFFFu, *abort_flag)) break;
+    for (int it = 0; prompt_next<true>(p, bar, tab, ord, it, w); ++it) {
       const int tok = w.tok0 + t * p.tok + rt;
       const bool valid = t < p.tiles && rt < p.tok && tok < w.lq;
       const int lim = valid ? min(max(tok + 1 + w.lk - w.lq, 0), w.lk) : 0;  // keys this row sees
-      const int jmask = max(w.tok0 + t * p.tok + 1 + w.lk - w.lq, 0) / kPB;
+      const int jmask = max(w.tok0 + t * p.tok + 1 + w.lk - w.lq, 0) / kPB - w.jb;
       const int nb = t == 0 ? w.nb[0] : w.nb[1];
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < nb; ++j) {
@@ -440,7 +508,7 @@ __global__ void __launch_bounds__(kPThreads, 1)
         for (int c = 0; c < 4; ++c) tmem_ld32(ts + c * 32, sr[c]);
         tmem_wait_ld();
         if (j >= jmask) {
-          const int left = lim - j * kPB;
+          const int left = lim - (w.jb + j) * kPB;
 #pragma unroll
           for (int c = 0; c < 4; ++c)
 #pragma unroll
@@ -450,17 +518,21 @@ __global__ void __launch_bounds__(kPThreads, 1)
         softmax_block<T>(sr, ts, to, j > 0, sl2, m, l, [&] { mbar_arrive_warp(&bar.p_part[t]); });
         mbar_arrive_warp(&bar.p_full[t]);
       }
-      char* dst = p.out + static_cast<int64_t>(w.q0 + tok) * p.out_tok_stride +
-                  static_cast<int64_t>(w.g * p.group + rh) * p.out_head_stride;
+      const int64_t row = static_cast<int64_t>(w.q0 + tok), head = w.g * p.group + rh;
+      char* dst = p.out + row * p.out_tok_stride + head * p.out_head_stride;
+      const int64_t slot = (static_cast<int64_t>(w.split) * p.total_q + row) * p.hq + head;
       if (nb == 0) {
-        if (valid)
+        if (valid && p.splits > 1) p.ws_ml[slot] = make_float2(-INFINITY, 0.f);
+        if (valid && p.splits == 1)
           for (int c = 0; c < 16; ++c) *reinterpret_cast<uint4*>(dst + c * 16) = make_uint4(0, 0, 0, 0);
         continue;
       }
       mbar_wait_fast(&bar.o_full[t], no++ & 1, abort_flag, p.status);
       if (__any_sync(0xFFFFFFFFu, *abort_flag)) break;
       tc_fence_after();
-      const float inv = lim > 0 ? 1.f / l : 0.f;
+      // (a row that sees no key of this share has l == 0, and its O is 0 or not a number)
+      const float inv = p.splits > 1 ? 1.f : 1.f / l;
+      const bool none = lim <= w.jb * kPB;
       const bool poison = *const_cast<volatile int*>(&bar.poison) != 0;
 #pragma unroll 1
       for (int c = 0; c < 4; ++c) {
@@ -470,16 +542,25 @@ __global__ void __launch_bounds__(kPThreads, 1)
         if (!valid) continue;
         float x[32];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) x[i] = lim > 0 ? __uint_as_float(o[i]) * inv : 0.f;
+        for (int i = 0; i < 32; ++i) x[i] = none ? 0.f : __uint_as_float(o[i]) * inv;
         if (poison)
           add_not_finite<T>(p.v + w.g * p.kv_head_stride + w.k0 * p.kv_row_stride + c * 64, p.kv_row_stride,
-                            w.jm * kPB, lim, x);
+                            (w.jb + w.jm) * kPB, min(lim, (w.jb + nb) * kPB), x);
+        if (p.splits == 1) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          *reinterpret_cast<uint4*>(dst + c * 64 + q * 16) =
-              make_uint4(pack2<T>(x[q * 8], x[q * 8 + 1]), pack2<T>(x[q * 8 + 2], x[q * 8 + 3]),
-                         pack2<T>(x[q * 8 + 4], x[q * 8 + 5]), pack2<T>(x[q * 8 + 6], x[q * 8 + 7]));
+          for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<uint4*>(dst + c * 64 + q * 16) =
+                make_uint4(pack2<T>(x[q * 8], x[q * 8 + 1]), pack2<T>(x[q * 8 + 2], x[q * 8 + 3]),
+                           pack2<T>(x[q * 8 + 4], x[q * 8 + 5]), pack2<T>(x[q * 8 + 6], x[q * 8 + 7]));
+        } else {
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+            *reinterpret_cast<float4*>(p.ws_o + slot * kPD + c * 32 + q * 4) =
+                make_float4(x[q * 4], x[q * 4 + 1], x[q * 4 + 2], x[q * 4 + 3]);
+        }
       }
+      // (a NaN weight wins the merge)
+      if (valid && p.splits > 1) p.ws_ml[slot] = none ? make_float2(-INFINITY, 0.f) : make_float2(l == l ? m : INFINITY, l);
       tc_fence_before();
     }
   } else {
@@ -491,6 +572,56 @@ __global__ void __launch_bounds__(kPThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
+}
+
+// One warp per (token, query head): the sum of the row's shares.  Tokens outside
+// every (valid) sequence have none and are left alone.
+template <typename T>
+__global__ void __launch_bounds__(128) prompt_combine_kernel(const PromptParams p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int64_t gw = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
+  const int lane = threadIdx.x & 31;
+  if (gw >= static_cast<int64_t>(p.total_q) * p.hq) return;
+  const int row = static_cast<int>(gw / p.hq), head = static_cast<int>(gw - static_cast<int64_t>(row) * p.hq);
+  bool mine = false;
+  for (int b = lane; b < p.num_seqs; b += 32) {
+    int q0, lq, k0, lk;
+    mine |= prompt_seq(p, b, q0, lq, k0, lk) && row >= q0 && row < q0 + lq;
+  }
+  if (!__any_sync(0xFFFFFFFFu, mine)) return;
+  const int64_t step = static_cast<int64_t>(p.total_q) * p.hq, slot = static_cast<int64_t>(row) * p.hq + head;
+  const float2 ml = lane < p.splits ? p.ws_ml[slot + lane * step] : make_float2(-INFINITY, 0.f);
+  float M = ml.x;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xFFFFFFFFu, M, o));
+  const float wt = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
+  float lsum = wt * ml.y;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) lsum += __shfl_xor_sync(0xFFFFFFFFu, lsum, o);
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s0 = 0; s0 < p.splits; s0 += 4) {
+    float4 o[4];
+    float w[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      w[u] = __shfl_sync(0xFFFFFFFFu, wt, (s0 + u) & 31);
+      o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (s0 + u < p.splits && w[u] != 0.f)
+        o[u] = *reinterpret_cast<const float4*>(p.ws_o + (slot + (s0 + u) * step) * kPD + lane * 4);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (s0 + u >= p.splits || w[u] == 0.f) continue;
+      acc.x = fmaf(w[u], o[u].x, acc.x);
+      acc.y = fmaf(w[u], o[u].y, acc.y);
+      acc.z = fmaf(w[u], o[u].z, acc.z);
+      acc.w = fmaf(w[u], o[u].w, acc.w);
+    }
+  }
+  const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
+  *reinterpret_cast<uint2*>(p.out + row * p.out_tok_stride + head * p.out_head_stride + lane * 8) =
+      make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
 }
 
 // [rows of 128][mid][outer] of 16-bit values read in boxes of 64 columns x
@@ -510,11 +641,43 @@ static int make_prompt_tmap(CUtensorMap* m, const void* base, bool half, int64_t
   return r == CUDA_SUCCESS ? RT_OK : RT_ERR_INVALID_ARGUMENT;
 }
 
+struct PromptPlan {
+  int tiles, splits;
+  int64_t items;
+};
+
+// Two tiles an item when that fills the GPU.  When it does not, an item's keys
+// are split if there are enough of them (at least eight blocks a share; twice the
+// SMs' number of shares), and short prompts go one tile an item.  The sequences'
+// lengths are on the device, so their mean stands for them.
+static PromptPlan prompt_plan(int64_t total_q, int64_t total_k, int seqs, int hkv, int tok) {
+  PromptPlan pl{2, 1, (total_q / (2 * tok) + seqs) * hkv};
+  if (pl.items >= kPSms) return pl;
+  const int64_t blocks = total_k / seqs / kPB;
+  if (blocks < 16 || total_q / seqs <= tok) {
+    pl.tiles = 1;
+    pl.items = (total_q / tok + seqs) * hkv;
+  }
+  if (blocks >= 16)
+    pl.splits = static_cast<int>(
+        std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(32, blocks / 8), (2 * kPSms + pl.items - 1) / pl.items)));
+  return pl;
+}
+
 }  // namespace rt
 
 using namespace rt;
 
-extern "C" size_t rt_prompt_attn_workspace_size(int64_t, int64_t, int, int, int) { return 0; }
+extern "C" size_t rt_prompt_attn_workspace_size(int64_t total_q, int64_t total_k, int num_seqs, int num_q_heads,
+                                                int num_kv_heads) {
+  if (total_q <= 0 || total_k < 0 || num_seqs <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 ||
+      num_q_heads % num_kv_heads || num_q_heads / num_kv_heads > kPB)
+    return 0;
+  const PromptPlan pl = prompt_plan(total_q, total_k, num_seqs, num_kv_heads, kPB / (num_q_heads / num_kv_heads));
+  if (pl.splits == 1) return 0;
+  const size_t rows = static_cast<size_t>(pl.splits) * total_q * num_q_heads;
+  return align_up(rows * kPD * 4, 256) + align_up(rows * 8, 256);
+}
 
 extern "C" int rt_prompt_attn(const void* q, int64_t q_tok_stride, int64_t q_head_stride, const void* k,
                               const void* v, int64_t kv_head_stride, int64_t kv_row_stride, void* out,
@@ -552,6 +715,7 @@ extern "C" int rt_prompt_attn(const void* q, int64_t q_tok_stride, int64_t q_hea
   if (rc != RT_OK) return rc;
   if (!keys) tk = tv = tq;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  const PromptPlan plan = prompt_plan(total_q, total_k, num_seqs, num_kv_heads, tok);
   for (int b0 = 0; b0 < num_seqs; b0 += kPMaxSeqs) {
     const int nb = std::min(kPMaxSeqs, num_seqs - b0);
     PromptParams p{};
@@ -567,23 +731,38 @@ extern "C" int rt_prompt_attn(const void* q, int64_t q_tok_stride, int64_t q_hea
     p.total_q = static_cast<int>(total_q);
     p.total_k = static_cast<int>(total_k);
     p.hkv = num_kv_heads;
+    p.hq = num_q_heads;
     p.group = G;
     p.tok = tok;
-    // items, at most: full ones and one partial a sequence
-    const int64_t pairs = (total_q / (2 * tok) + nb) * num_kv_heads;
-    p.tiles = pairs >= kPSms ? 2 : 1;
+    p.tiles = plan.tiles;
+    p.splits = plan.splits;
     // (never 0: a hidden score is -inf and stays so; scores times 2^-126 are 0 in the sum)
     p.scale_log2 = std::max(scale * 1.4426950408889634f, 1.17549435e-38f);
     p.status = status;
-    const int64_t items = (total_q / (p.tiles * tok) + nb) * num_kv_heads;
-    const dim3 grid(static_cast<unsigned>(std::min<int64_t>(items, kPSms)));
+    if (plan.splits > 1) {  // (fewer than kPMaxSeqs sequences: one launch)
+      const size_t rows = static_cast<size_t>(plan.splits) * total_q * num_q_heads;
+      if (workspace == nullptr ||
+          workspace_bytes < rt_prompt_attn_workspace_size(total_q, total_k, num_seqs, num_q_heads, num_kv_heads))
+        return RT_ERR_WORKSPACE;
+      p.ws_o = static_cast<float*>(workspace);
+      p.ws_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + align_up(rows * kPD * 4, 256));
+    }
+    // items, at most: full ones and one partial a sequence
+    const int64_t items = (total_q / (plan.tiles * tok) + nb) * num_kv_heads * plan.splits;
+    if (items > INT32_MAX) return RT_ERR_UNSUPPORTED;
+    const dim3 grid(static_cast<unsigned>(items));
+    const dim3 rows_grid(static_cast<unsigned>((total_q * num_q_heads + 3) / 4));
     if (half) {
       set_smem_limit(prompt_attn_kernel<__half>, kPSmem);
       rc = record_cuda(launch_ex(prompt_attn_kernel<__half>, grid, dim3(kPThreads), kPSmem, s, 1, tq, tk, tv, p));
+      if (rc == RT_OK && plan.splits > 1)
+        rc = record_cuda(launch_ex(prompt_combine_kernel<__half>, rows_grid, dim3(128), 0, s, 1, p));
     } else {
       set_smem_limit(prompt_attn_kernel<__nv_bfloat16>, kPSmem);
       rc = record_cuda(
           launch_ex(prompt_attn_kernel<__nv_bfloat16>, grid, dim3(kPThreads), kPSmem, s, 1, tq, tk, tv, p));
+      if (rc == RT_OK && plan.splits > 1)
+        rc = record_cuda(launch_ex(prompt_combine_kernel<__nv_bfloat16>, rows_grid, dim3(128), 0, s, 1, p));
     }
     if (rc != RT_OK) return rc;
   }
