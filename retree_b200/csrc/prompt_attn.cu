@@ -304,7 +304,7 @@ __global__ void __launch_bounds__(kPThreads, 1)
         tma_load_3d(dst + kPHalf, map, &bar.kv_full[s], 64, row, w.g);
         ++n;
       };
-      // The next item is asked for when three blocks of this one are left to load:
+      // The next item is asked for when five blocks of this one are left to load:
       // late, so that whoever is done first gets it, and early enough that the
       // answer is there in time.  (Asked for at once, 256 items on 148 CTAs were
       // all handed out in the first microsecond: 2048 tokens took 52 us, not 43.)
@@ -321,7 +321,7 @@ __global__ void __launch_bounds__(kPThreads, 1)
         const int nb = max(w.nb[0], w.nb[1]);
         if (nb == 0) ok = take_over(it);
         for (int j = 0; j < nb && ok; ++j) {
-          if (j == max(nb - 3, 0)) {
+          if (j == max(nb - 5, 0)) {
             ok = take_over(it);
             if (!ok) break;
           }
