@@ -32,6 +32,10 @@
 //   warp 12         producer: Q by TMA, the blocks' bytes by bulk copies (9216
 //                   contiguous bytes each) into a 3-stage ring;
 //   warp 13         MMA issuer.
+// When only one tile has queries (n * group <= 128, or the last rows) the two
+// softmax groups take turns at its key blocks instead: two chains of S, P and O
+// for the same queries, merged at the end, so that one chain's softmax still runs
+// under the other's products.
 //
 // What hides: the rows behind the tree are stale bytes, so the last tile reads
 // their scales as zero; a tree row that reads as NaN turns the scores of the
@@ -444,7 +448,8 @@ constexpr uint32_t kQtOffQ = 0;
 constexpr uint32_t kQtOffKV = 2 * kQtTile;
 constexpr uint32_t kQtOffPacked = kQtOffKV + kQtStages * kQtTile;
 constexpr uint32_t kQtOffBar = kQtOffPacked + kQtPacked * kQtBlock;
-constexpr uint32_t kQtSmem = kQtOffBar + 512 + 1024;
+constexpr uint32_t kQtOffMl = kQtOffBar + 512;        // [chain][row] (m, l)
+constexpr uint32_t kQtSmem = kQtOffMl + 2 * 128 * 8 + 1024;
 constexpr uint32_t kQtTmemO = 256;                    // S0 | S1 | O0 | O1, P_t in S_t's first 64 columns
 
 struct Q4Bars {
@@ -454,6 +459,15 @@ struct Q4Bars {
   int abort_flag;
   uint2 x43;  // (.x)
 };
+
+// Order in which the blocks' bytes are loaded, decoded and consumed: K of the
+// first `ahead` blocks (1, or 2 with two chains), then V_b and K_{b + ahead} in turn.
+__device__ __forceinline__ int q4_entry(int n, int nb, int ahead, bool& is_v) {
+  const int a = min(ahead, nb), m = n - a, pairs = nb - a;
+  is_v = m >= 2 * pairs || (m >= 0 && !(m & 1));
+  if (m < 0) return n;
+  return m >= 2 * pairs ? m - pairs : (m >> 1) + ((m & 1) ? a : 0);
+}
 
 // A key's row of a decoded tile: 128 bf16 values in two SW128 halves.  All of
 // the row is read before anything is decoded (`loaded` runs in between): one
@@ -492,6 +506,8 @@ __global__ void __launch_bounds__(kQtThreads, 1)
   const int split = blockIdx.x, kvh = blockIdx.y, G = p.group;
   const int node0 = blockIdx.z * 2 * tok;               // first node of tile 0
   const int tiles = node0 + tok < p.n ? 2 : 1;
+  const bool dual = tiles == 1;                         // two chains over one tile's keys
+  const int ahead = dual ? 2 : 1;
   if (warp == 12 && lane == 0) {
     prefetch_tmap(&tmap_q);
     for (int i = 0; i < 2; ++i) {
@@ -552,12 +568,13 @@ __global__ void __launch_bounds__(kQtThreads, 1)
         const int s = n % kQtPacked;
         ok = mbar_wait(&bar.in_empty[s], ((n / kQtPacked) & 1) ^ 1, abort_flag, p.status, RT_DEV_WAIT_TIMEOUT);
         if (!ok) break;
-        const int64_t key0 = (b0 + (n >> 1)) * kQtKeys;
+        bool is_v;
+        const int64_t key0 = (b0 + q4_entry(n, nb, ahead, is_v)) * kQtKeys;
         // an even number of rows: 16-byte pieces that end inside the (even) capacity
         const uint32_t bytes =
             static_cast<uint32_t>((min(static_cast<int64_t>(kQtKeys), total - key0) + 1) & ~int64_t(1)) * kQ4Row;
         mbar_arrive_expect_tx(&bar.in_full[s], bytes);
-        bulk_load(smem + kQtOffPacked + s * kQtBlock, ((n & 1) ? vb : kb) + key0 * kQ4Row, bytes, &bar.in_full[s]);
+        bulk_load(smem + kQtOffPacked + s * kQtBlock, (is_v ? vb : kb) + key0 * kQ4Row, bytes, &bar.in_full[s]);
       }
       if (*abort_flag) {
         for (int t = 0; t < tiles; ++t) mbar_wait_drain(&bar.q_full[t], 0);
@@ -573,57 +590,77 @@ __global__ void __launch_bounds__(kQtThreads, 1)
       const uint64_t dk = warp_uniform(smem_desc_sw128(smem_u32(smem + kQtOffKV), 16, 1024));
       const uint64_t dv = warp_uniform(smem_desc_sw128(smem_u32(smem + kQtOffKV), kQtHalf, 1024));
       auto wait = [&](uint64_t* b, uint32_t ph) { mbar_wait_fast(b, ph & 1, abort_flag, p.status); };
-      for (int j = -1; j < nb && nb > 0; ++j) {
-        // loads 2j+1 = V_j and 2j+2 = K_{j+1}
+      auto qk = [&](int t, int qt, int stage) {
+        const uint64_t a = dq + static_cast<uint64_t>(qt * (kQtTile >> 4));
+        const uint64_t b = dk + static_cast<uint64_t>(warp_uniform(stage) * (kQtTile >> 4));
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < kHD / 16; ++kk) {
+            const uint32_t off = ((kk >> 2) * kQtHalf + (kk & 3) * 32) >> 4;
+            umma_f16(tm + t * 128, a + off, b + off, idesc_qk, kk > 0);
+          }
+          umma_commit(&bar.s_full[t]);
+        }
+      };
+      auto pv = [&](int t, int stage, int j, bool last) {
+        const uint64_t b = dv + static_cast<uint64_t>(warp_uniform(stage) * (kQtTile >> 4));
+        auto mma = [&](int kk) {
+          umma_f16_ts(tm + kQtTmemO + t * kHD, tm + t * 128 + kk * 8, b + kk * (2048 >> 4), idesc_pv,
+                      (j > 0 || kk > 0) ? 1u : 0u);
+        };
+        wait(&bar.p_part[t], j);
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < kPart1 / 16; ++kk) mma(kk);
+        }
+        wait(&bar.p_full[t], j);
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int kk = kPart1 / 16; kk < kQtKeys / 16; ++kk) mma(kk);
+          if (last) umma_commit(&bar.o_full[t]);
+        }
+      };
+      auto release = [&](int stage) {
+        if (elect_one()) umma_commit(&bar.kv_empty[stage]);
+      };
+      if (dual && nb > 0) {
+        wait(&bar.q_full[0], 0);
+        int n = 0;
+        for (; n < min(2, nb); ++n) {
+          wait(&bar.kv_full[n], 0);
+          qk(n, 0, n);
+          release(n);
+        }
+        for (int b = 0; b < nb; ++b) {
+          const int t = b & 1, sv = n % kQtStages, sk = (n + 1) % kQtStages;
+          const bool more = b + 2 < nb;
+          wait(&bar.kv_full[sv], n / kQtStages);
+          if (more) wait(&bar.kv_full[sk], (n + 1) / kQtStages);
+          pv(t, sv, b >> 1, !more);
+          if (more) qk(t, 0, sk);
+          release(sv);
+          if (more) release(sk);
+          n += more ? 2 : 1;
+        }
+      }
+      for (int j = -1; j < nb && nb > 0 && !dual; ++j) {
+        // entries 2j+1 = V_j and 2j+2 = K_{j+1}
         const int nv = 2 * j + 1, nk = 2 * j + 2;
         const int sv = nv & (kQtStages - 1), sk = nk % kQtStages;
         const bool more = j + 1 < nb;
         if (j >= 0) wait(&bar.kv_full[sv], nv / kQtStages);
         if (more) wait(&bar.kv_full[sk], nk / kQtStages);
-        const uint64_t bk = dk + static_cast<uint64_t>(warp_uniform(sk) * (kQtTile >> 4));
-        const uint64_t bv = dv + static_cast<uint64_t>(warp_uniform(sv) * (kQtTile >> 4));
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          if (t >= tiles) continue;
-          if (j >= 0) {
-            auto pv = [&](int kk) {
-              umma_f16_ts(tm + kQtTmemO + t * kHD, tm + t * 128 + kk * 8, bv + kk * (2048 >> 4), idesc_pv,
-                          (j > 0 || kk > 0) ? 1u : 0u);
-            };
-            if (kPart1 < kQtKeys) {
-              wait(&bar.p_part[t], j);
-              tc_fence_after();
-              if (elect_one()) {
-#pragma unroll
-                for (int kk = 0; kk < kPart1 / 16; ++kk) pv(kk);
-              }
-            }
-            wait(&bar.p_full[t], j);
-            tc_fence_after();
-            if (elect_one()) {
-#pragma unroll
-              for (int kk = (kPart1 < kQtKeys ? kPart1 / 16 : 0); kk < kQtKeys / 16; ++kk) pv(kk);
-              if (!more) umma_commit(&bar.o_full[t]);
-            }
-          } else {
-            wait(&bar.q_full[t], 0);
-            tc_fence_after();
-          }
-          if (more && elect_one()) {
-#pragma unroll
-            for (int kk = 0; kk < kHD / 16; ++kk) {
-              const uint32_t off = ((kk >> 2) * kQtHalf + (kk & 3) * 32) >> 4;
-              umma_f16(tm + t * 128, dq + t * (kQtTile >> 4) + off, bk + off, idesc_qk, kk > 0);
-            }
-            umma_commit(&bar.s_full[t]);
-          }
-          __syncwarp();
+          if (j >= 0) pv(t, sv, j, !more);
+          else wait(&bar.q_full[t], 0);
+          if (more) qk(t, t, sk);
         }
-        if (elect_one()) {
-          if (j >= 0) umma_commit(&bar.kv_empty[sv]);
-          if (more) umma_commit(&bar.kv_empty[sk]);
-        }
-        __syncwarp();
+        if (j >= 0) release(sv);
+        if (more) release(sk);
       }
       // all issued MMAs complete before TMEM is released
       if (elect_one()) {
@@ -640,15 +677,16 @@ __global__ void __launch_bounds__(kQtThreads, 1)
     const char* vb = p.v + kvh * p.kv_head_stride;
     for (int n = 0; n < 2 * nb; ++n) {
       const int si = n % kQtPacked, so = n % kQtStages;
-      const int64_t key = (b0 + (n >> 1)) * kQtKeys + r;
+      bool is_v;
+      const int64_t key = (b0 + q4_entry(n, nb, ahead, is_v)) * kQtKeys + r;
       mbar_wait_fast(&bar.in_full[si], (n / kQtPacked) & 1, abort_flag, p.status);
       mbar_wait_fast(&bar.kv_empty[so], ((n / kQtStages) & 1) ^ 1, abort_flag, p.status);
       // behind the tree: zero.  A tree row of V that reads as NaN: zero in V, and
       // NaN in K, so that only the nodes that see the key get it.
       bool zero = key >= total, nan = false;
       if (key >= L && !zero && q4_is_nan(*reinterpret_cast<const uint16_t*>(vb + key * kQ4Row + kQ4Codes))) {
-        zero = (n & 1) != 0;
-        nan = !zero;
+        zero = is_v;
+        nan = !is_v;
       }
       q4_decode_row(sbase + kQtOffPacked + si * kQtBlock + r * kQ4Row, sbase + kQtOffKV + so * kQtTile, r, zero, nan, x43,
                     [&] { mbar_arrive_warp(&bar.in_empty[si]); });
@@ -656,22 +694,25 @@ __global__ void __launch_bounds__(kQtThreads, 1)
       mbar_arrive_warp(&bar.kv_full[so]);
     }
   } else {
-    // ---------------- softmax and result of tile t ----------------
+    // ---------------- softmax and result of tile (or chain) t ----------------
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kQtRegsSoftmax));
     const int t = warp >> 2, r = tid & 127;
     const int rt = r / G;
-    const int node = node0 + t * tok + rt;
-    const bool valid = t < tiles && rt < tok && node < p.n;
+    const int first = node0 + (dual ? 0 : t * tok);     // first node of the tile
+    const int node = first + rt;
+    const bool valid = rt < tok && node < p.n;
     const int h = kvh * G + (r - rt * G);
     const int64_t R = static_cast<int64_t>(node) * G + (r - rt * G);
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t ts = tmem + lane_base + t * 128, to = tmem + lane_base + kQtTmemO + t * kHD;
+    const uint32_t ts = tmem + lane_base + t * 128, tmo = tmem + lane_base + kQtTmemO, to = tmo + t * kHD;
     const uint32_t* mrow = p.mask + static_cast<int64_t>(valid ? node : 0) * p.mask_words;
     // a warp without a query only keeps the barriers' count
-    const bool warp_live = t < tiles && ((warp & 3) * 32) / G < tok && node0 + t * tok + ((warp & 3) * 32) / G < p.n;
+    const bool warp_live = ((warp & 3) * 32) / G < tok && first + ((warp & 3) * 32) / G < p.n;
     const float sl2 = p.scale_log2;
     float m = -INFINITY, l = 0.f;
-    for (int j = 0; j < nb && t < tiles; ++j) {
+    const int step = dual ? 2 : 1;
+    int j = 0;
+    for (int b = dual ? t : 0; b < nb; b += step, ++j) {
       mbar_wait_fast(&bar.s_full[t], j & 1, abort_flag, p.status);
       if (warp_live) {
         tc_fence_after();
@@ -679,7 +720,7 @@ __global__ void __launch_bounds__(kQtThreads, 1)
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld32(ts + c * 32, sr[c]);
         tmem_wait_ld();
-        const int64_t key0 = (b0 + j) * kQtKeys;
+        const int64_t key0 = (b0 + b) * kQtKeys;
         if (key0 + kQtKeys > L) {
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
@@ -695,45 +736,63 @@ __global__ void __launch_bounds__(kQtThreads, 1)
       }
       mbar_arrive_warp(&bar.p_full[t]);
     }
+    if (l != l) m = INFINITY;  // a NaN weight wins the merges
+    float w0 = 1.f, w1 = 0.f;  // of the two O tiles; with one chain t's own is the first
+    if (j > 0) mbar_wait_fast(&bar.o_full[t], 0, abort_flag, p.status);
+    if (dual) {
+      float2* ml = reinterpret_cast<float2*>(smem + kQtOffMl);
+      ml[t * 128 + r] = make_float2(m, l);
+      tc_fence_before();
+      asm volatile("bar.sync 1, 256;" ::: "memory");  // both chains' products are done, too
+      const float2 x0 = ml[r], x1 = ml[128 + r];
+      m = fmaxf(x0.x, x1.x);
+      w0 = x0.x == -INFINITY ? 0.f : ex2(x0.x - m);
+      w1 = x1.x == -INFINITY ? 0.f : ex2(x1.x - m);
+      l = fmaf(w0, x0.y, w1 * x1.y);
+    }
     const int64_t rows_ws = static_cast<int64_t>(p.tiles) * kBM;
     const int64_t slot = (static_cast<int64_t>(split) * p.num_kv_heads + kvh) * rows_ws + R;
-    if (l != l) m = INFINITY;  // a NaN weight wins the merge
-    if (inside && warp_live && nb > 0) {
-      mbar_wait_fast(&bar.o_full[t], 0, abort_flag, p.status);
-      if (!__any_sync(0xFFFFFFFFu, *abort_flag)) {
-        tc_fence_after();
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (inside && nb == 0) {
+      if (valid && p.num_splits > 1 && (t == 0 || !dual)) p.ws_ml[slot] = make_float2(-INFINITY, 0.f);
+    } else if (inside && warp_live && !__any_sync(0xFFFFFFFFu, *abort_flag)) {
+      tc_fence_after();
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      // one chain: all four column groups of the tile's O; two: half of them, of both O
 #pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          uint32_t o[32];
-          tmem_ld32(to + c * 32, o);
+      for (int c = dual ? 2 * t : 0; c < (dual ? 2 * t + 2 : 4); ++c) {
+        float x[32];
+        uint32_t o[32];
+        tmem_ld32((dual ? tmo : to) + c * 32, o);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) x[i] = w0 == 0.f ? 0.f : __uint_as_float(o[i]) * w0;
+        if (dual) {
+          tmem_ld32(tmo + kHD + c * 32, o);
           tmem_wait_ld();
-          if (!valid) continue;
-          if (p.num_splits == 1) {
-            char* dst = p.out + node * p.out_tok_stride + h * p.out_head_stride + c * 64;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              uint32_t w[4];
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                w[i] = l == 0.f ? 0u
-                                : pack_bf16x2(__uint_as_float(o[q * 8 + 2 * i]) * inv,
-                                              __uint_as_float(o[q * 8 + 2 * i + 1]) * inv);
-              *reinterpret_cast<uint4*>(dst + q * 16) = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-          } else {
-#pragma unroll
-            for (int q = 0; q < 8; ++q)
-              *reinterpret_cast<uint4*>(p.ws_o + slot * kHD + c * 32 + q * 4) =
-                  make_uint4(o[q * 4], o[q * 4 + 1], o[q * 4 + 2], o[q * 4 + 3]);
-          }
+          for (int i = 0; i < 32; ++i) x[i] = w1 == 0.f ? x[i] : fmaf(w1, __uint_as_float(o[i]), x[i]);
         }
-        if (valid && p.num_splits > 1) p.ws_ml[slot] = make_float2(m, l);
-        tc_fence_before();
+        if (!valid) continue;
+        if (p.num_splits == 1) {
+          char* dst = p.out + node * p.out_tok_stride + h * p.out_head_stride + c * 64;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              w[i] = l == 0.f ? 0u : pack_bf16x2(x[q * 8 + 2 * i] * inv, x[q * 8 + 2 * i + 1] * inv);
+            *reinterpret_cast<uint4*>(dst + q * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        } else {
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+            *reinterpret_cast<float4*>(p.ws_o + slot * kHD + c * 32 + q * 4) =
+                make_float4(x[q * 4], x[q * 4 + 1], x[q * 4 + 2], x[q * 4 + 3]);
+        }
       }
-    } else if (inside && valid && nb == 0 && p.num_splits > 1) {
-      p.ws_ml[slot] = make_float2(-INFINITY, 0.f);
+      if (valid && p.num_splits > 1 && (t == 0 || !dual)) p.ws_ml[slot] = make_float2(m, l);
     }
+    tc_fence_before();
   }
   __syncthreads();
   if (warp == 13) {
