@@ -117,6 +117,103 @@ __device__ __forceinline__ void merge_weights(const float2 (&ml)[kMaxMerge], flo
   for (int u = 0; u < kMaxMerge; ++u) w[u] = w[u] * inv;
 }
 
+// In-kernel split merge: once a CTA's last PV product is final, the Q / K / V
+// ring is idle and holds the CTA's unnormalised fp32 O tile (rows of 512 B,
+// 16-byte chunks XOR-swizzled by row) and its rows' (m, l).
+constexpr uint32_t kOffStage = 0;
+constexpr uint32_t kOffMl = 65536;
+constexpr uint32_t kOffWeights = 98304;  // [owned rows][kMaxMerge] fp32 merge weights
+
+// Byte offset of 16-byte chunk `c` (0..31) of row `r` in the merge's O stage.
+__device__ __forceinline__ uint32_t stage_off(int r, int c) {
+  return kOffStage + static_cast<uint32_t>(r) * 512u + static_cast<uint32_t>((c ^ (r & 31)) << 4);
+}
+
+// The split merge inside the cluster (every thread of every CTA calls it, or the
+// first kThreads of each while the others pass its two cluster barriers; the
+// cluster is the S = num_splits CTAs of one (kv head, tile), rank = split).
+// Each CTA has staged its unnormalised O rows and (m, l) in its own shared
+// memory.  Rank c merges the tile rows r = c, c + S, ...: the rank weights of
+// a row are 2^(m_s - M) / L (L = sum_s 2^(m_s - M) l_s, in rank order), and the
+// chunks are summed in rank order (a rank of weight 0 -- no key of the row, or
+// a row it did not stage -- is skipped, never multiplied) into the bf16
+// output.  When every thread has at most one (row, 4-dim chunk) item, each
+// item's thread loads every rank's (m, l) and chunk at once and forms the
+// weights itself: one distributed-shared-memory round trip.  Otherwise one
+// thread per row forms the weights into a shared table first and the item
+// threads then load only the chunks.  The last barrier keeps every CTA's
+// shared memory until all ranks have read it.
+template <int kThreads, bool kWholeBlock = true>
+__device__ __forceinline__ void merge_splits(const AttnParams& p, unsigned char* smem, int rank, int kvh, int row0,
+                                             int rows_total) {
+  __syncwarp();
+  cluster_sync_all();
+  const int tid = threadIdx.x;
+  const int S = p.num_splits, G = p.group;
+  const int rows_here = min(kBM, rows_total - row0);
+  const int owned = rows_here > rank ? (rows_here - rank + S - 1) / S : 0;
+  const uint32_t base = smem_u32(smem);
+  float* wtab = reinterpret_cast<float*>(smem + kOffWeights);
+  auto store = [&](int rr, int c, const float4& acc) {
+    const int R = row0 + rr;
+    const int node = R / G, h = kvh * G + (R - node * G);
+    uint2 pk;
+    pk.x = pack_bf16x2(acc.x, acc.y);
+    pk.y = pack_bf16x2(acc.z, acc.w);
+    *reinterpret_cast<uint2*>(p.out + node * p.out_tok_stride + h * p.out_head_stride + c * 8) = pk;
+  };
+  if (owned * 32 <= kThreads) {  // the same in every thread of the CTA
+    const int it = tid;
+    if (it < owned * 32) {
+      const int i = it >> 5, c = it & 31;
+      const int rr = rank + S * i;
+      const uint32_t off = base + stage_off(rr, c);
+      float2 ml[kMaxMerge];
+      float4 o[kMaxMerge];
+#pragma unroll
+      for (int u = 0; u < kMaxMerge; ++u) {
+        ml[u] = make_float2(-INFINITY, 0.f);
+        o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (u < S) {
+          ml[u] = ld_cluster_f32x2(cluster_map(base + kOffMl + rr * 8, u));
+          o[u] = ld_cluster_f32x4(cluster_map(off, u));
+        }
+      }
+      float w[kMaxMerge];
+      merge_weights(ml, w);
+      store(rr, c, merge_chunk(o, S, w));
+    }
+  } else {
+    for (int i = tid; i < owned; i += kThreads) {
+      const int rr = rank + S * i;
+      float2 ml[kMaxMerge];
+#pragma unroll
+      for (int u = 0; u < kMaxMerge; ++u)
+        ml[u] = u < S ? ld_cluster_f32x2(cluster_map(base + kOffMl + rr * 8, u)) : make_float2(-INFINITY, 0.f);
+      float w[kMaxMerge];
+      merge_weights(ml, w);
+#pragma unroll
+      for (int u = 0; u < kMaxMerge; ++u) wtab[i * kMaxMerge + u] = w[u];
+    }
+    if constexpr (kWholeBlock) __syncthreads();
+    else asm volatile("bar.sync 2, %0;" ::"n"(kThreads) : "memory");
+    for (int it = tid; it < owned * 32; it += kThreads) {
+      const int i = it >> 5, c = it & 31;
+      const int rr = rank + S * i;
+      const uint32_t off = base + stage_off(rr, c);
+      float4 o[kMaxMerge];
+#pragma unroll
+      for (int u = 0; u < kMaxMerge; ++u) {
+        o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (u < S && wtab[i * kMaxMerge + u] != 0.f) o[u] = ld_cluster_f32x4(cluster_map(off, u));
+      }
+      store(rr, c, merge_chunk(o, S, wtab + i * kMaxMerge));
+    }
+  }
+  __syncwarp();
+  cluster_sync_all();
+}
+
 // ---------------------------------------------------------------------------
 // Split merge: one warp per (kv head, tile row); lane owns 4 dims.
 // ---------------------------------------------------------------------------

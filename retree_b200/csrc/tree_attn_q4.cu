@@ -25,13 +25,14 @@
 // ---------------------------------------------------------------------------
 // One CTA per (key split, kv head, 256 query rows): two 128-row tiles (row r of
 // a tile is (node r / group, query head r % group)) in ping-pong on tcgen05 as in
-// the prompt attention.  Sixteen warps:
+// the prompt attention.  Warps:
 //   warps 0-3, 4-7  softmax of tile 0 / 1, one thread per row;
-//   warps 8-11      decode: a thread per key turns the 72 bytes of K (then V) of
-//                   a 128-key block into its row of a bf16 SW128 tile;
-//   warp 12         producer: Q by TMA, the blocks' bytes by bulk copies (9216
+//   warps 8-11 (15) decode, one group of four warps or two that take turns: a
+//                   thread per key turns the 72 bytes of K (or V) of a 128-key
+//                   block into its row of a bf16 SW128 tile;
+//   next warp       producer: Q by TMA, the blocks' bytes by bulk copies (9216
 //                   contiguous bytes each) into a 3-stage ring;
-//   warp 13         MMA issuer.
+//   next warp       MMA issuer.
 // When only one tile has queries (n * group <= 128, or the last rows) the two
 // softmax groups take turns at its key blocks instead: two chains of S, P and O
 // for the same queries, merged at the end, so that one chain's softmax still runs
@@ -436,9 +437,15 @@ __global__ void __launch_bounds__(kQsThreads, 1) tree_attn_q4_small_kernel(const
 // ---------------------------------------------------------------------------
 // More query rows: decoded tiles on tcgen05
 // ---------------------------------------------------------------------------
-constexpr int kQtThreads = 512;
-// registers a thread; the block is launched with 128 x 512 (2 x 176 + 88 + 72 = 4 x 128)
-constexpr int kQtRegsSoftmax = 176, kQtRegsDecode = 88, kQtRegsOther = 72;
+// With one decode group the block is launched with 128 registers x 512 threads
+// (2 x 176 + 88 + 72 = 4 x 128), with two 96 x 640 (2 x 168 + 2 x 48 + 48 = 5 x 96).
+template <int kDec>
+struct Q4Tile {
+  static constexpr int kThreads = 384 + 128 * kDec;
+  static constexpr int kProducerWarp = 8 + 4 * kDec, kMmaWarp = kProducerWarp + 1;
+  static constexpr int kRegsSoftmax = kDec == 1 ? 176 : 168, kRegsDecode = kDec == 1 ? 88 : 48,
+                       kRegsOther = kDec == 1 ? 72 : 48;
+};
 constexpr int kQtKeys = 128;
 constexpr uint32_t kQtTile = 128 * 128 * 2, kQtHalf = kQtTile / 2;
 constexpr int kQtStages = 4;                          // decoded tiles
@@ -496,19 +503,21 @@ __device__ __forceinline__ void q4_decode_row(uint32_t src, uint32_t tile, int r
   }
 }
 
-__global__ void __launch_bounds__(kQtThreads, 1)
+template <int kDec>
+__global__ void __launch_bounds__(Q4Tile<kDec>::kThreads, 1)
     tree_attn_q4_tile_kernel(const __grid_constant__ CUtensorMap tmap_q, const AttnParams p, const int tok) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   Q4Bars& bar = *reinterpret_cast<Q4Bars*>(smem + kQtOffBar);
+  constexpr int kProducerWarp = Q4Tile<kDec>::kProducerWarp, kMmaWarp = Q4Tile<kDec>::kMmaWarp;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int split = blockIdx.x, kvh = blockIdx.y, G = p.group;
   const int node0 = blockIdx.z * 2 * tok;               // first node of tile 0
   const int tiles = node0 + tok < p.n ? 2 : 1;
   const bool dual = tiles == 1;                         // two chains over one tile's keys
   const int ahead = dual ? 2 : 1;
-  if (warp == 12 && lane == 0) {
+  if (warp == kProducerWarp && lane == 0) {
     prefetch_tmap(&tmap_q);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bar.q_full[i], 1);
@@ -531,7 +540,7 @@ __global__ void __launch_bounds__(kQtThreads, 1)
     fence_mbar_init();
     fence_proxy_async_smem();
   }
-  if (warp == 13) {
+  if (warp == kMmaWarp) {
     tmem_alloc(&bar.tmem_base, 512);
     tmem_relinquish();
   }
@@ -549,9 +558,9 @@ __global__ void __launch_bounds__(kQtThreads, 1)
   if (inside) split_range(total, split, p.num_splits, kQtKeys, b0, b1);
   const int nb = static_cast<int>(b1 - b0);
 
-  if (warp >= 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kQtRegsOther));
-    if (warp == 12 && lane == 0 && nb > 0) {
+  if (warp >= kProducerWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Q4Tile<kDec>::kRegsOther));
+    if (warp == kProducerWarp && lane == 0 && nb > 0) {
       // ---------------- producer ----------------
       bool ok = true;
       const uint32_t qbytes = static_cast<uint32_t>(tok * G) * 256u;
@@ -581,7 +590,7 @@ __global__ void __launch_bounds__(kQtThreads, 1)
         for (int i = max(0, n - kQtPacked); i < n; ++i)
           mbar_wait_drain(&bar.in_full[i % kQtPacked], (i / kQtPacked) & 1);
       }
-    } else if (warp == 13) {
+    } else if (warp == kMmaWarp) {
       // ---------------- MMA issuer ----------------
       constexpr uint32_t idesc_qk = idesc_bf16_f32(kBM, kQtKeys, false, false);
       constexpr uint32_t idesc_pv = idesc_bf16_f32(kBM, kHD, false, true);
@@ -640,8 +649,8 @@ __global__ void __launch_bounds__(kQtThreads, 1)
           wait(&bar.kv_full[sv], n / kQtStages);
           if (more) wait(&bar.kv_full[sk], (n + 1) / kQtStages);
           pv(t, sv, b >> 1, !more);
-          if (more) qk(t, 0, sk);
           release(sv);
+          if (more) qk(t, 0, sk);
           if (more) release(sk);
           n += more ? 2 : 1;
         }
@@ -671,11 +680,11 @@ __global__ void __launch_bounds__(kQtThreads, 1)
     }
   } else if (warp >= 8) {
     // ---------------- decode ----------------
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kQtRegsDecode));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Q4Tile<kDec>::kRegsDecode));
     const int r = tid & 127;
     const uint32_t sbase = smem_u32(smem), x43 = lds64(smem_u32(&bar.x43)).x;
     const char* vb = p.v + kvh * p.kv_head_stride;
-    for (int n = 0; n < 2 * nb; ++n) {
+    for (int n = (warp >> 2) - 2; n < 2 * nb; n += kDec) {  // (two groups take turns)
       const int si = n % kQtPacked, so = n % kQtStages;
       bool is_v;
       const int64_t key = (b0 + q4_entry(n, nb, ahead, is_v)) * kQtKeys + r;
@@ -695,7 +704,7 @@ __global__ void __launch_bounds__(kQtThreads, 1)
     }
   } else {
     // ---------------- softmax and result of tile (or chain) t ----------------
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kQtRegsSoftmax));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Q4Tile<kDec>::kRegsSoftmax));
     const int t = warp >> 2, r = tid & 127;
     const int rt = r / G;
     const int first = node0 + (dual ? 0 : t * tok);     // first node of the tile
@@ -752,7 +761,35 @@ __global__ void __launch_bounds__(kQtThreads, 1)
     }
     const int64_t rows_ws = static_cast<int64_t>(p.tiles) * kBM;
     const int64_t slot = (static_cast<int64_t>(split) * p.num_kv_heads + kvh) * rows_ws + R;
-    if (inside && nb == 0) {
+    if (p.merge > 1) {
+      // park the unnormalised O rows and (m, l) for the merge in the cluster: the
+      // rings are idle, every load was consumed and the last products are done
+      const bool have = inside && warp_live && nb > 0 && !__any_sync(0xFFFFFFFFu, *abort_flag);
+      if (have) {
+        tc_fence_after();
+#pragma unroll 1
+        for (int c = 2 * t; c < 2 * t + 2; ++c) {
+          uint32_t o[32], o1[32];
+          tmem_ld32(tmo + c * 32, o);
+          tmem_ld32(tmo + kHD + c * 32, o1);
+          tmem_wait_ld();
+          float x[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            x[i] = w0 == 0.f ? 0.f : __uint_as_float(o[i]) * w0;
+            if (w1 != 0.f) x[i] = fmaf(w1, __uint_as_float(o1[i]), x[i]);
+          }
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+            *reinterpret_cast<float4*>(smem + stage_off(r, c * 8 + q)) =
+                make_float4(x[q * 4], x[q * 4 + 1], x[q * 4 + 2], x[q * 4 + 3]);
+        }
+      }
+      if (t == 0)
+        reinterpret_cast<float2*>(smem + kOffMl)[r] = have ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
+      // (one tile, so the launch's rows are the tile's)
+      if (inside) merge_splits<256, false>(p, smem, split, kvh, 0, p.n * G);
+    } else if (inside && nb == 0) {
       if (valid && p.num_splits > 1 && (t == 0 || !dual)) p.ws_ml[slot] = make_float2(-INFINITY, 0.f);
     } else if (inside && warp_live && !__any_sync(0xFFFFFFFFu, *abort_flag)) {
       tc_fence_after();
@@ -794,8 +831,13 @@ __global__ void __launch_bounds__(kQtThreads, 1)
     }
     tc_fence_before();
   }
+  if (p.merge > 1 && inside && warp >= 8) {  // the merge's two cluster barriers
+    __syncwarp();
+    cluster_sync_all();
+    cluster_sync_all();
+  }
   __syncthreads();
-  if (warp == 13) {
+  if (warp == kMmaWarp) {
     __syncwarp();
     tc_fence_after();
     tmem_dealloc(tmem, 512);
@@ -826,22 +868,18 @@ struct Q4Plan {
   bool merge;
 };
 
-static int q4_clusters_fit(int c) {
-  static std::mutex mu;
-  static int cache[kMaxMerge + 1] = {};
-  static bool done[kMaxMerge + 1] = {};
-  std::lock_guard<std::mutex> lock(mu);
-  if (c < 2 || c > kMaxMerge) return 0;
-  if (done[c]) return cache[c];
+// Clusters of `c` CTAs of `kernel` that fit on the GPU at once (0 when the query
+// fails, e.g. without a device).
+template <typename Kernel>
+static int clusters_fit(Kernel kernel, int threads, uint32_t smem, int c) {
   int n = 0;
-  if (cudaFuncSetAttribute(tree_attn_q4_small_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           static_cast<int>(kQsSmem)) == cudaSuccess &&
-      (c <= 8 || cudaFuncSetAttribute(tree_attn_q4_small_kernel<2>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) ==
-                     cudaSuccess)) {
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) ==
+          cudaSuccess &&
+      (c <= 8 || cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess)) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(c, 1, 1);
-    cfg.blockDim = dim3(kQsThreads);
-    cfg.dynamicSmemBytes = kQsSmem;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.x = static_cast<unsigned>(c);
@@ -849,12 +887,25 @@ static int q4_clusters_fit(int c) {
     attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    if (cudaOccupancyMaxActiveClusters(&n, tree_attn_q4_small_kernel<2>, &cfg) != cudaSuccess) n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) n = 0;
   }
   cudaGetLastError();
-  cache[c] = n;
-  done[c] = true;
   return n;
+}
+
+// ... of the few-rows kernel, or of the tile kernel with two decode groups (cached per size).
+static int q4_clusters_fit(bool small, int c) {
+  static std::mutex mu;
+  static int cache[2][kMaxMerge + 1] = {};
+  static bool done[2][kMaxMerge + 1] = {};
+  std::lock_guard<std::mutex> lock(mu);
+  if (c < 2 || c > kMaxMerge) return 0;
+  if (!done[small][c]) {
+    cache[small][c] = small ? clusters_fit(tree_attn_q4_small_kernel<2>, kQsThreads, kQsSmem, c)
+                            : clusters_fit(tree_attn_q4_tile_kernel<2>, Q4Tile<2>::kThreads, kQtSmem, c);
+    done[small][c] = true;
+  }
+  return cache[small][c];
 }
 
 template <int NT>
@@ -865,6 +916,15 @@ static int launch_q4_small(dim3 grid, dim3 cluster, cudaStream_t s, const AttnPa
       launch_ex_cluster(tree_attn_q4_small_kernel<NT>, grid, dim3(kQsThreads), kQsSmem, s, cluster, p));
 }
 
+template <int kDec>
+static int launch_q4_tile(dim3 grid, dim3 cluster, cudaStream_t s, const CUtensorMap& tq, const AttnParams& p, int tok) {
+  set_smem_limit(tree_attn_q4_tile_kernel<kDec>, kQtSmem);
+  if (cluster.x > 8)
+    cudaFuncSetAttribute(tree_attn_q4_tile_kernel<kDec>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  return record_cuda(launch_ex_cluster(tree_attn_q4_tile_kernel<kDec>, grid, dim3(Q4Tile<kDec>::kThreads), kQtSmem, s,
+                                       cluster, tq, p, tok));
+}
+
 static Q4Plan q4_plan(int n, int G, int hkv, int64_t prefix_len, int num_splits) {
   const bool small = n * G <= kQsRows;
   if (small) {
@@ -873,7 +933,7 @@ static Q4Plan q4_plan(int n, int G, int hkv, int64_t prefix_len, int num_splits)
     if (want <= 0) want = std::max<int64_t>(1, std::min<int64_t>(148 / hkv, (tiles + 7) / 8));
     want = std::min<int64_t>(std::min<int64_t>(want, tiles), 256);
     const int s = static_cast<int>(want);
-    return {true, s, s >= 2 && s <= kMaxMerge && hkv <= q4_clusters_fit(s)};
+    return {true, s, s >= 2 && s <= kMaxMerge && hkv <= q4_clusters_fit(true, s)};
   }
   const int64_t blocks = (prefix_len + n + kQtKeys - 1) / kQtKeys;
   const int tok = kBM / G;
@@ -881,6 +941,15 @@ static Q4Plan q4_plan(int n, int G, int hkv, int64_t prefix_len, int num_splits)
   int64_t want = num_splits;
   if (want <= 0) want = std::max<int64_t>(1, 148 / ctas);
   want = std::min<int64_t>(std::min<int64_t>(want, blocks), 256);
+  if (n <= tok && want > 1) {
+    // one tile: its splits merge in a cluster when it takes all of them, or (where
+    // the count is ours to choose) leaves each CTA three blocks at most
+    int c = static_cast<int>(std::min<int64_t>(want, kMaxMerge));
+    if (num_splits <= 0)
+      while (c >= 2 && hkv > q4_clusters_fit(false, c)) --c;
+    if (c >= 2 && hkv <= q4_clusters_fit(false, c) && (c == want || (num_splits <= 0 && blocks <= 3 * c)))
+      return {false, c, true};
+  }
   return {false, static_cast<int>(want), false};
 }
 
@@ -963,9 +1032,11 @@ extern "C" int rt_tree_attn_q4(const void* q, int64_t q_tok_stride, int64_t q_he
     CUtensorMap tq;
     rc = make_q4_query_tmap(&tq, q, q_tok_stride, q_head_stride, n, num_q_heads, G, tok);
     if (rc != RT_OK) return rc;
-    set_smem_limit(tree_attn_q4_tile_kernel, kQtSmem);
     const dim3 grid(pl.splits, num_kv_heads, (n + 2 * tok - 1) / (2 * tok));
-    rc = record_cuda(launch_ex(tree_attn_q4_tile_kernel, grid, dim3(kQtThreads), kQtSmem, s, 1, tq, p, tok));
+    // One tile (two chains) wants two decode groups, two tiles the registers:
+    // 32768 rows, 17 nodes 31.5 us with one group, 29.4 with two; 257 nodes 205, 217.
+    rc = n <= tok ? launch_q4_tile<2>(grid, dim3(pl.merge ? pl.splits : 1, 1, 1), s, tq, p, tok)
+                  : launch_q4_tile<1>(grid, dim3(1, 1, 1), s, tq, p, tok);
   }
   if (rc != RT_OK || pl.merge || pl.splits == 1) return rc;
   const int warps = num_kv_heads * n * G * (pl.splits <= kFastSplits ? 2 : 1);
