@@ -112,7 +112,7 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
   return false;
 }
 
-// The same for the hot loops of converged warps: a phase that is (nearly) there
+// The same for the hot loops of whole warps (every lane calls it): a phase that is (nearly) there
 // costs one poll, about a third of mbar_wait's loop and its checks.  The loops do
 // not branch on the result: after a time-out their (bounded) waits fall through
 // and they finish on whatever is in shared memory, and the results are dropped
@@ -136,6 +136,7 @@ __device__ __forceinline__ void mbar_wait_fast(uint64_t* bar, uint32_t parity, v
     *abort = 1;
     set_status(status, RT_DEV_WAIT_TIMEOUT);
   }
+  __syncwarp();  // lanes may leave the poll apart; what follows (tcgen05.ld and the like) needs them together
 }
 
 // Wait (bounded, ignoring the abort flag) for copies a CTA issued itself to

@@ -148,7 +148,8 @@ __device__ __forceinline__ bool prompt_next(const PromptParams& p, PromptBars& b
   int idx = blockIdx.x;
   if (it > 0) {
     const int s = (it - 1) & 1;
-    mbar_wait_fast(&bar.clc_full[s], ((it - 1) >> 1) & 1, &bar.abort_flag, p.status);
+    if constexpr (kWarp) mbar_wait_fast(&bar.clc_full[s], ((it - 1) >> 1) & 1, &bar.abort_flag, p.status);
+    else mbar_wait(&bar.clc_full[s], ((it - 1) >> 1) & 1, &bar.abort_flag, p.status, RT_DEV_WAIT_TIMEOUT);
     idx = *const_cast<volatile int*>(&bar.abort_flag) ? -1 : clc_taken(smem_u32(&bar.clc[s]));
     if constexpr (kWarp) {
       idx = __reduce_min_sync(0xFFFFFFFFu, idx);  // (the same in every lane but for an abort in between)

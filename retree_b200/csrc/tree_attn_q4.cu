@@ -438,13 +438,13 @@ __global__ void __launch_bounds__(kQsThreads, 1) tree_attn_q4_small_kernel(const
 // More query rows: decoded tiles on tcgen05
 // ---------------------------------------------------------------------------
 // With one decode group the block is launched with 128 registers x 512 threads
-// (2 x 176 + 88 + 72 = 4 x 128), with two 96 x 640 (2 x 168 + 2 x 48 + 48 = 5 x 96).
+// (2 x 176 + 88 + 72 = 4 x 128), with two 96 x 640 (2 x 168 + 2 x 40 + 64 = 5 x 96).
 template <int kDec>
 struct Q4Tile {
   static constexpr int kThreads = 384 + 128 * kDec;
   static constexpr int kProducerWarp = 8 + 4 * kDec, kMmaWarp = kProducerWarp + 1;
-  static constexpr int kRegsSoftmax = kDec == 1 ? 176 : 168, kRegsDecode = kDec == 1 ? 88 : 48,
-                       kRegsOther = kDec == 1 ? 72 : 48;
+  static constexpr int kRegsSoftmax = kDec == 1 ? 176 : 168, kRegsDecode = kDec == 1 ? 88 : 40,
+                       kRegsOther = kDec == 1 ? 72 : 64;
 };
 constexpr int kQtKeys = 128;
 constexpr uint32_t kQtTile = 128 * 128 * 2, kQtHalf = kQtTile / 2;
