@@ -519,7 +519,9 @@ int rt_prompt_attn(const void* q, int64_t q_tok_stride, int64_t q_head_stride, c
  *   scales s below 2^120 (values below 2^119); a node that sees no
  *   key gets a zero row; a prefix length outside the cache writes nothing
  *   (RT_DEV_BAD_INDEX).  workspace must hold
- *   rt_tree_attn_q4_workspace_size(...) bytes (alignment 256).
+ *   rt_tree_attn_q4_workspace_size(...) bytes (alignment 256);
+ *   rt_tree_attn_q4_default_splits is the split count of num_splits = 0 (a count
+ *   given to two launches splits the same keys the same way in both).
  * ---------------------------------------------------------------------- */
 #define RT_Q4_ROW_BYTES 72
 int rt_kv_append_q4(void* k_cache, void* v_cache, int64_t cache_head_stride, const void* k_new, const void* v_new,
@@ -528,6 +530,7 @@ int rt_kv_append_q4(void* k_cache, void* v_cache, int64_t cache_head_stride, con
 int rt_kv_read_q4(const void* cache, int64_t cache_head_stride, void* out, int64_t out_head_stride,
                   int64_t out_row_stride, int n_heads, int n, int head_dim, int64_t capacity, int64_t start,
                   rt_stream_t stream);
+int rt_tree_attn_q4_default_splits(int n, int num_q_heads, int num_kv_heads, int64_t prefix_len);
 size_t rt_tree_attn_q4_workspace_size(int n, int num_q_heads, int num_kv_heads, int head_dim, int64_t prefix_len,
                                       int num_splits);
 int rt_tree_attn_q4(const void* q, int64_t q_tok_stride, int64_t q_head_stride, const void* k, const void* v,

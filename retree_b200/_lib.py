@@ -67,6 +67,7 @@ SIGNATURES = {
                             _I, _F, _P, _SZ, _P, _P]),
     "rt_kv_append_q4": (_I, [_P, _P, _I64, _P, _P, _I64, _I64, _I, _I, _I, _I64, _I64, _P, _P, _P]),
     "rt_kv_read_q4": (_I, [_P, _I64, _P, _I64, _I64, _I, _I, _I, _I64, _I64, _P]),
+    "rt_tree_attn_q4_default_splits": (_I, [_I, _I, _I, _I64]),
     "rt_tree_attn_q4_workspace_size": (_SZ, [_I, _I, _I, _I, _I64, _I]),
     "rt_tree_attn_q4": (_I, [_P, _I64, _I64, _P, _P, _I64, _I64, _P, _I64, _I64, _P, _I, _I, _I64, _P, _I, _I, _I,
                              _F, _I, _P, _SZ, _P, _P]),

@@ -20,14 +20,26 @@ masking_utils.py:827-829):
     ``is_causal=False`` (the DFlash draft's attention, model/dflash.py:47 and
     its callers' kwargs), which the SDPA backend honours the same way
     (sdpa_attention.py:64-77): then every new token sees every key.
+
+Whole prompts can take their own kernel (``kernels.prompt_attention``: the hidden
+half of the scores is not computed and no mask is read): always when the call
+carries transformers' packed-sequence offsets (``cu_seq_lens_q`` and
+``cu_seq_lens_k``, which a plain causal mask would mix up) or a prompt starts a
+4-bit cache, and otherwise inside ``prompt_kernel()``.  Over a 4-bit cache
+(``TreeKVCacheQ4``) trees and later tokens read the cached rows
+(``kernels.tree_attention_q4``).
 """
 
 from __future__ import annotations
+
+import contextlib
+import contextvars
 
 import numpy as np
 import torch
 
 from . import kernels
+from .cache import Q4_ATTR
 
 NAME = "retree_tree"
 
@@ -35,6 +47,24 @@ _CAUSAL_BITS: dict = {}
 
 #: when a list, every call appends (start event, end event, prefix_len, n, q heads, kv heads)
 PROFILE: list | None = None
+
+
+#: whether an unmasked causal call runs prompt_attention (set by prompt_kernel())
+_PROMPT_KERNEL = contextvars.ContextVar("retree_prompt_kernel", default=False)
+
+#: new tokens over a 4-bit cache above which a causal call reads the cache's values
+#: once and runs prompt_attention, instead of a chain-shaped tree over the 4-bit rows
+_Q4_CHAIN_MAX = 256
+
+
+@contextlib.contextmanager
+def prompt_kernel(enabled: bool = True):
+    """Inside, calls without a mask (prompts, chunks of prompts) run ``kernels.prompt_attention``."""
+    token = _PROMPT_KERNEL.set(bool(enabled))
+    try:
+        yield
+    finally:
+        _PROMPT_KERNEL.reset(token)
 
 
 class TreeMask:
@@ -92,6 +122,63 @@ def _bits_for(mask, n: int, key_len: int, device, causal: bool = True):
     return kernels.mask_from_dense(m2, key_len - n, n), None
 
 
+class _Timer:
+    """Events around a call's attention kernel, for PROFILE (records nothing when that is None)."""
+
+    def __init__(self):
+        self.on = PROFILE is not None
+        self.events = [torch.cuda.Event(enable_timing=True) for _ in range(2)] if self.on else None
+
+    def start(self) -> None:
+        if self.on:
+            self.events[0].record()
+
+    def stop(self, *shape) -> None:
+        if self.on:
+            self.events[1].record()
+            PROFILE.append((*self.events, *shape))
+
+
+def _q4_forward(query, key, value, attention_mask, scaling, causal: bool, rows, timer) -> torch.Tensor:
+    """Attention of new tokens over a 4-bit cache that already holds their rows."""
+    n, hq = query.shape[2], query.shape[1]
+    if attention_mask is None and not rows.device_length and causal:
+        if rows.prefix_len == 0:
+            timer.start()
+            return kernels.prompt_attention(query, key, value, scale=scaling)
+        if n > _Q4_CHAIN_MAX:
+            timer.start()
+            k, v = (kernels.kv_read_q4(x, 0, rows.prefix_len + n) for x in (rows.k, rows.v))
+            return kernels.prompt_attention(query, k, v, scale=scaling)
+    bits, prefix_dev = _bits_for(attention_mask, n, rows.prefix_len + n, query.device, causal=causal)
+    if rows.device_length and prefix_dev is None:
+        raise RuntimeError("a cache in device-length mode needs a tree mask with its prefix length")
+    splits = kernels.default_splits_q4(n, hq, rows.k.shape[0], rows.k.shape[1] - n)
+    timer.start()
+    return kernels.tree_attention_q4(query, rows.k, rows.v, bits, rows.prefix_len, scale=scaling, num_splits=splits,
+                                     prefix_len_dev=prefix_dev)
+
+
+def _tree_forward(query, key, value, attention_mask, scaling, causal: bool, timer) -> torch.Tensor:
+    """rt_tree_attn over bf16 K/V: the mask's tree, or the new tokens as a chain."""
+    n = query.shape[2]
+    bits, prefix_dev = _bits_for(attention_mask, n, key.shape[2], query.device, causal=causal)
+    timer.start()
+    # rows allocated per head: the launch (and its split of the keys) is sized
+    # for the cache's capacity, so host-length and device-length rounds over the
+    # same cache run the identical launch
+    cap = key.shape[2]
+    if key.stride(-1) == 1 and key.stride(2) > 0 and key.stride(1) % key.stride(2) == 0:
+        cap = max(cap, key.stride(1) // key.stride(2))
+    splits = kernels.default_splits(n, query.shape[1], key.shape[1], cap - n)
+    if prefix_dev is not None:
+        # full-capacity K/V views; the real prefix length lives on the device
+        return kernels.tree_attention(query, key, value, bits, prefix_len=cap - n, scale=scaling,
+                                      prefix_len_dev=prefix_dev, kv_capacity=cap, num_splits=splits)
+    return kernels.tree_attention(query, key, value, bits, prefix_len=key.shape[2] - n, scale=scaling,
+                                  kv_capacity=cap, num_splits=splits)
+
+
 def tree_attention_forward(module, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
                            attention_mask, dropout: float = 0.0, scaling: float | None = None,
                            sliding_window=None, **kwargs):
@@ -107,28 +194,24 @@ def tree_attention_forward(module, query: torch.Tensor, key: torch.Tensor, value
     causal = kwargs.get("is_causal", None)
     if causal is None:
         causal = getattr(module, "is_causal", True)
-    bits, prefix_dev = _bits_for(attention_mask, n, key.shape[2], query.device, causal=bool(causal))
-    if PROFILE is not None:
-        ev0 = torch.cuda.Event(enable_timing=True)
-        ev1 = torch.cuda.Event(enable_timing=True)
-        ev0.record()
-    # rows allocated per head: the launch (and its split of the keys) is sized
-    # for the cache's capacity, so host-length and device-length rounds over the
-    # same cache run the identical launch
-    cap = key.shape[2]
-    if key.stride(-1) == 1 and key.stride(2) > 0 and key.stride(1) % key.stride(2) == 0:
-        cap = max(cap, key.stride(1) // key.stride(2))
-    splits = kernels.default_splits(n, query.shape[1], key.shape[1], cap - n)
-    if prefix_dev is not None:
-        # full-capacity K/V views; the real prefix length lives on the device
-        out = kernels.tree_attention(query, key, value, bits, prefix_len=cap - n, scale=scaling,
-                                     prefix_len_dev=prefix_dev, kv_capacity=cap, num_splits=splits)
+    causal = bool(causal)
+    rows = getattr(key, Q4_ATTR, None)
+    cu_q, cu_k = kwargs.get("cu_seq_lens_q"), kwargs.get("cu_seq_lens_k")
+    prefix = key.shape[2] - n if rows is None else rows.prefix_len
+    timer = _Timer()
+    if cu_q is not None and attention_mask is None:
+        if not causal or (rows is not None and rows.prefix_len > 0):
+            raise RuntimeError("packed sequences run causally over keys of their own (no cached prefix)")
+        timer.start()
+        out = kernels.prompt_attention(query, key, value, cu_seqlens_q=cu_q, cu_seqlens_k=cu_k, scale=scaling)
+    elif rows is not None:
+        out = _q4_forward(query, key, value, attention_mask, scaling, causal, rows, timer)
+    elif _PROMPT_KERNEL.get() and attention_mask is None and causal:
+        timer.start()
+        out = kernels.prompt_attention(query, key, value, scale=scaling)
     else:
-        out = kernels.tree_attention(query, key, value, bits, prefix_len=key.shape[2] - n, scale=scaling,
-                                     kv_capacity=cap, num_splits=splits)
-    if PROFILE is not None:
-        ev1.record()
-        PROFILE.append((ev0, ev1, key.shape[2] - n, n, query.shape[1], key.shape[1]))
+        out = _tree_forward(query, key, value, attention_mask, scaling, causal, timer)
+    timer.stop(prefix, n, query.shape[1], key.shape[1])
     return out.unsqueeze(0), None
 
 

@@ -24,6 +24,8 @@ length from the same device word.
 
 from __future__ import annotations
 
+from types import SimpleNamespace
+
 import torch
 from transformers.cache_utils import Cache, CacheLayerMixin
 
@@ -124,11 +126,22 @@ class TreeKVCache(Cache):
         self.device = torch.device(device if device is not None else "cuda")
         if self.device.type != "cuda":
             raise RuntimeError("TreeKVCache lives on a CUDA device")
-        self.slab = torch.zeros((2 * self.num_layers, self.num_kv_heads, self.capacity, self.head_dim),
-                                dtype=dtype, device=self.device)
+        self.slab = self._make_slab()
         self.length_dev = torch.zeros(1, dtype=torch.int64, device=self.device)
         self.device_length = False
-        super().__init__(layers=[TreeKVLayer(self, i) for i in range(self.num_layers)])
+        super().__init__(layers=[self.layer_class(self, i) for i in range(self.num_layers)])
+
+    layer_class = TreeKVLayer
+
+    def _make_slab(self) -> torch.Tensor:
+        return torch.zeros((2 * self.num_layers, self.num_kv_heads, self.capacity, self.head_dim), dtype=self.dtype,
+                           device=self.device)
+
+    def append(self, layer: int, k_new: torch.Tensor, v_new: torch.Tensor, offset: int = 0,
+               offset_dev: torch.Tensor | None = None) -> None:
+        """Write ``[heads, n, head_dim]`` rows of one layer at ``offset`` (the layer's length is not changed)."""
+        kernels.kv_append(self.slab[2 * layer], self.slab[2 * layer + 1], k_new, v_new, offset=offset,
+                          offset_dev=offset_dev)
 
     @classmethod
     def for_model(cls, config, capacity: int, dtype=torch.bfloat16, device=None) -> "TreeKVCache":
@@ -175,3 +188,73 @@ class TreeKVCache(Cache):
 
     def batch_select_indices(self, indices):
         raise NotImplementedError("TreeKVCache holds one sequence")
+
+
+class TreeKVLayerQ4(TreeKVLayer):
+    """One layer of a ``TreeKVCacheQ4``; ``keys`` / ``values`` are decoded copies."""
+
+    def _view(self, kv: int, length: int) -> torch.Tensor:
+        return kernels.kv_read_q4(self._cache.slab[2 * self.index + kv], 0, length).unsqueeze(0)
+
+    def update(self, key_states: torch.Tensor, value_states: torch.Tensor, *args, **kwargs):
+        """Quantise the new rows into the cache; returns them, tagged with where the cache's rows are.
+
+        The attention backend reads the cache itself (``Q4_ATTR``), so no bf16
+        copy of the cached rows is made.
+        """
+        c = self._cache
+        n = key_states.shape[-2]
+        before = self.length
+        if c.device_length:
+            c.append(self.index, key_states, value_states, offset_dev=c.length_dev)
+            self.length = c.capacity
+            prefix = c.capacity - n
+        else:
+            if before + n > c.capacity:
+                raise RuntimeError(f"TreeKVCache capacity {c.capacity} exceeded ({before} + {n})")
+            c.append(self.index, key_states, value_states, offset=before)
+            self.length += n
+            prefix = before
+        tagged = key_states.view(key_states.shape)  # (a tensor of its own to carry the tag)
+        setattr(tagged, Q4_ATTR, SimpleNamespace(k=c.slab[2 * self.index], v=c.slab[2 * self.index + 1],
+                                                 prefix_len=prefix, device_length=c.device_length))
+        return tagged, value_states
+
+
+#: attribute of the key tensor a 4-bit cache hands to the attention backend
+Q4_ATTR = "_rt_q4"
+
+
+class TreeKVCacheQ4(TreeKVCache):
+    """The same cache with rows of 4 bits: 72 bytes a head and token instead of 256.
+
+    ``slab`` is uint8 ``[2 * layers, kv_heads, capacity, 72]`` (the row's layout is
+    in ``include/retree_b200.h``, RT_Q4_ROW_BYTES); the capacity is rounded up to
+    an even number.  Appending quantises (``kernels.kv_append_q4``), the
+    ``retree_tree`` attention reads the 4-bit rows (``kernels.tree_attention_q4``),
+    compaction moves them as they are.  A prompt over an empty cache attends to
+    its own bf16 keys and values; whatever comes later attends to the cached
+    rows, its own among them, so a token's result does not depend on whether its
+    ancestors were committed or are still in the tree.
+    """
+
+    layer_class = TreeKVLayerQ4
+
+    def _make_slab(self) -> torch.Tensor:
+        if self.head_dim != 128 or self.dtype != torch.bfloat16:
+            raise RuntimeError("the 4-bit cache holds bf16 rows of head_dim 128")
+        self.capacity += self.capacity & 1
+        return torch.zeros((2 * self.num_layers, self.num_kv_heads, self.capacity, kernels.Q4_ROW_BYTES),
+                           dtype=torch.uint8, device=self.device)
+
+    def append(self, layer: int, k_new: torch.Tensor, v_new: torch.Tensor, offset: int = 0,
+               offset_dev: torch.Tensor | None = None) -> None:
+        kernels.kv_append_q4(self.slab[2 * layer], self.slab[2 * layer + 1], k_new, v_new, offset=offset,
+                             offset_dev=offset_dev)
+
+
+def make_cache(kv_bits: int, *args, **kwargs) -> TreeKVCache:
+    """A ``TreeKVCache`` (16 bits) or a ``TreeKVCacheQ4`` (4 bits)."""
+    if kv_bits not in (16, 4):
+        raise ValueError("kv_bits must be 16 or 4")
+    return (TreeKVCacheQ4 if kv_bits == 4 else TreeKVCache)(*args, **kwargs)

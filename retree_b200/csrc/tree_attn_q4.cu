@@ -931,7 +931,7 @@ static Q4Plan q4_plan(int n, int G, int hkv, int64_t prefix_len, int num_splits)
     const int64_t tiles = (prefix_len + n + kQsKeys - 1) / kQsKeys;
     int64_t want = num_splits;
     if (want <= 0) want = std::max<int64_t>(1, std::min<int64_t>(148 / hkv, (tiles + 7) / 8));
-    want = std::min<int64_t>(std::min<int64_t>(want, tiles), 256);
+    want = std::min<int64_t>(want, 256);
     const int s = static_cast<int>(want);
     return {true, s, s >= 2 && s <= kMaxMerge && hkv <= q4_clusters_fit(true, s)};
   }
@@ -940,7 +940,8 @@ static Q4Plan q4_plan(int n, int G, int hkv, int64_t prefix_len, int num_splits)
   const int64_t ctas = static_cast<int64_t>(hkv) * ((n + 2 * tok - 1) / (2 * tok));
   int64_t want = num_splits;
   if (want <= 0) want = std::max<int64_t>(1, 148 / ctas);
-  want = std::min<int64_t>(std::min<int64_t>(want, blocks), 256);
+  if (num_splits <= 0) want = std::min<int64_t>(want, blocks);  // (a given count is kept: empty splits are fine)
+  want = std::min<int64_t>(want, 256);
   if (n <= tok && want > 1) {
     // one tile: its splits merge in a cluster when it takes all of them, or (where
     // the count is ours to choose) leaves each CTA three blocks at most
@@ -956,6 +957,11 @@ static Q4Plan q4_plan(int n, int G, int hkv, int64_t prefix_len, int num_splits)
 }  // namespace rt
 
 using namespace rt;
+
+extern "C" int rt_tree_attn_q4_default_splits(int n, int num_q_heads, int num_kv_heads, int64_t prefix_len) {
+  if (n <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads || prefix_len < 0) return 1;
+  return q4_plan(n, num_q_heads / num_kv_heads, num_kv_heads, prefix_len, 0).splits;
+}
 
 extern "C" size_t rt_tree_attn_q4_workspace_size(int n, int num_q_heads, int num_kv_heads, int head_dim,
                                                  int64_t prefix_len, int num_splits) {

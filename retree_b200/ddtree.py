@@ -303,7 +303,8 @@ def allocate_tree_buffers(tree_budget: int, device):
 def ddtree_generate(model, target, input_ids: torch.Tensor, mask_token_id: int, max_new_tokens: int,
                     block_size: int, stop_token_ids, temperature: float = 0.0, tree_budget: int | None = None,
                     save_tree_traces: bool = False, draft_fn=None, fused: bool | None = None,
-                    fused_draft: bool = False) -> SimpleNamespace:
+                    fused_draft: bool = False, kv_bits: int = 16,
+                    prompt_attention: bool = False) -> SimpleNamespace:
     """The DDTree decode loop of ddtree.py:734-968 on the device kernels.
 
     ``target`` is a causal LM whose attention backend is ``"retree_tree"``.
@@ -313,18 +314,21 @@ def ddtree_generate(model, target, input_ids: torch.Tensor, mask_token_id: int, 
     [block_size-1, vocab]`` logits callable may replace it.  ``fused`` picks
     the verify forward (None: the fused stages when the model allows them and
     no hidden states are needed), ``fused_draft`` runs the draft module on the
-    fused stages (``retree_b200.draft.FusedDraft``).
+    fused stages (``retree_b200.draft.FusedDraft``).  ``kv_bits`` / ``prompt_attention``
+    as in ``TreeVerifier``: a target cache of 4 bits, the prompt on its own kernel.
     """
     from .verify import TreeVerifier
 
     if block_size <= 1:  # ddtree.py:747-757: the linear path
         return dflash_generate(model, target, input_ids, mask_token_id, max_new_tokens, block_size, stop_token_ids,
-                               temperature=temperature, draft_fn=draft_fn, fused=fused, fused_draft=fused_draft)
+                               temperature=temperature, draft_fn=draft_fn, fused=fused, fused_draft=fused_draft,
+                               kv_bits=kv_bits, prompt_attention=prompt_attention)
     layer_ids = None if (model is None or draft_fn is not None) else list(model.target_layer_ids)
     verifier = TreeVerifier(target, tree_budget=(block_size - 1) if tree_budget is None else max(tree_budget, 0),
                             max_length=input_ids.shape[1] + max_new_tokens + 2 * block_size + 8,
                             draft_horizon=block_size - 1, temperature=temperature, target_layer_ids=layer_ids,
-                            fused=fused, fused_draft=fused_draft)
+                            fused=fused, fused_draft=fused_draft, kv_bits=kv_bits,
+                            prompt_attention=prompt_attention)
     return verifier.generate(input_ids, mask_token_id, max_new_tokens, block_size, stop_token_ids,
                              draft_model=model, draft_fn=draft_fn, save_tree_traces=save_tree_traces)
 
@@ -332,7 +336,8 @@ def ddtree_generate(model, target, input_ids: torch.Tensor, mask_token_id: int, 
 @torch.inference_mode()
 def dflash_generate(model, target, input_ids: torch.Tensor, mask_token_id: int, max_new_tokens: int,
                     block_size: int, stop_token_ids, temperature: float = 0.0, draft_fn=None,
-                    fused: bool | None = None, fused_draft: bool = False) -> SimpleNamespace:
+                    fused: bool | None = None, fused_draft: bool = False, kv_bits: int = 16,
+                    prompt_attention: bool = False) -> SimpleNamespace:
     """The linear DFlash decode loop of dflash.py:14-162 on the device kernels.
 
     Each round verifies the chain of the draft rows' argmax tokens (a tree with
@@ -347,6 +352,7 @@ def dflash_generate(model, target, input_ids: torch.Tensor, mask_token_id: int, 
     verifier = TreeVerifier(target, tree_budget=chain,
                             max_length=input_ids.shape[1] + max_new_tokens + 2 * max(block_size, 1) + 8,
                             draft_horizon=max(chain, 1), temperature=temperature, target_layer_ids=layer_ids,
-                            fused=fused, fused_draft=fused_draft, chain=True)
+                            fused=fused, fused_draft=fused_draft, chain=True, kv_bits=kv_bits,
+                            prompt_attention=prompt_attention)
     return verifier.generate(input_ids, mask_token_id, max_new_tokens, max(int(block_size), 1), stop_token_ids,
                              draft_model=model, draft_fn=draft_fn)

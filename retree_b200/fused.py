@@ -12,7 +12,9 @@ projections.  Here a layer is seven launches:
   rt_add_rmsnorm     residual += mlp_out; x = rmsnorm(residual) * w_in
   rt_linear QKV      x @ [Wq;Wk;Wv]^T, epilogue: q/k head norms + rotary,
                      q out, k/v into the cache
-  rt_tree_attn       the tree-masked attention kernel (+ split combine)
+  rt_tree_attn       the tree-masked attention kernel (+ split combine); over a
+                     4-bit cache rt_kv_append_q4 (from bf16 rows the QKV stage
+                     leaves in a buffer) and rt_tree_attn_q4
   rt_linear          attn @ Wo^T
   rt_add_rmsnorm     residual += o; x = rmsnorm(residual) * w_post
   rt_linear SILU     x @ [Wg;Wu]^T, epilogue: silu(gate) * up
@@ -42,6 +44,7 @@ import torch
 from torch import nn
 
 from . import kernels
+from .cache import TreeKVCacheQ4
 from .headsplit import gather_heads
 
 SUPPORTED_MODEL_TYPES = ("qwen3", "qwen2", "llama")
@@ -166,6 +169,9 @@ class FusedTarget:
         self.xnorm = torch.empty((n, self.hidden), **e)
         self.qkv = torch.empty((n, (hq + 2 * hkv) * d), **e)
         self.q = torch.empty((n, hq, d), **e)
+        # over a 4-bit cache the layer's new K/V rows come here in bf16 and are quantised from here
+        self.q4 = isinstance(cache, TreeKVCacheQ4)
+        self.kv_new = torch.empty((2, hkv, n, d), **e) if self.q4 else None
         self.attn = torch.empty((n, hq, d), **e)
         self.o = torch.empty((n, self.hidden), **e)
         self.gate_up = torch.empty((n, 2 * self.inter), **e)
@@ -218,7 +224,8 @@ class FusedTarget:
         return rope_tables(model.model.rotary_emb, next(model.parameters()).device, max_positions)
 
     def _splits(self, n: int) -> int:
-        return kernels.default_splits(n, self.hq, self.hkv, self.cache.capacity - n)
+        pick = kernels.default_splits_q4 if self.q4 else kernels.default_splits
+        return pick(n, self.hq, self.hkv, self.cache.capacity - n)
 
     @torch.inference_mode()
     def _autotune(self, n: int) -> dict:
@@ -314,7 +321,16 @@ class FusedTarget:
     def _qkv(self, L, xn, positions, offset, offset_dev):
         """Packed q/k/v projection + head norms + rotary + cache append."""
         n = xn.shape[0]
-        kc, vc = self.cache.slab[2 * L.index], self.cache.slab[2 * L.index + 1]
+        if self.q4:
+            k_new, v_new = self.kv_new[0, :, :n], self.kv_new[1, :, :n]
+            self._qkv_rows(L, xn, positions, k_new, v_new, 0, None)
+            self.cache.append(L.index, k_new, v_new, offset=offset, offset_dev=offset_dev)
+            return
+        self._qkv_rows(L, xn, positions, self.cache.slab[2 * L.index], self.cache.slab[2 * L.index + 1], offset,
+                       offset_dev)
+
+    def _qkv_rows(self, L, xn, positions, kc, vc, offset, offset_dev):
+        n = xn.shape[0]
         if self.use_rt["qkv"] and L.qkv_b is None and kernels.linear_supported(n, L.qkv_w.shape[0], xn.shape[1], 2):
             kernels.linear(xn, L.qkv_w, epilogue=2,
                            qkv=dict(num_q_heads=L.hq, num_kv_heads=L.hkv, q_norm=L.q_norm, k_norm=L.k_norm,
@@ -362,7 +378,10 @@ class FusedTarget:
             kc, vc = slab[2 * L.index], slab[2 * L.index + 1]
             # this rank's heads go straight into its exchange slot under the peer exchange
             attn_out = self.attn[:n] if self.peer is None else self.peer.slot(L.index, n).view(n, L.hq, -1)
-            if offset_dev is not None:
+            if self.q4:
+                kernels.tree_attention_q4(self.q[:n], kc, vc, bits, offset if offset_dev is None else cap - n,
+                                          scale=L.scale, out=attn_out, num_splits=splits, prefix_len_dev=offset_dev)
+            elif offset_dev is not None:
                 kernels.tree_attention(self.q[:n], kc, vc, bits, cap - n, scale=L.scale, out=attn_out,
                                        num_splits=splits, prefix_len_dev=offset_dev, kv_capacity=cap)
             else:

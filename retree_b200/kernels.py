@@ -850,22 +850,26 @@ def kv_read_q4(cache: torch.Tensor, start: int, n: int, out: torch.Tensor | None
     if not cache.is_cuda:
         raise RuntimeError(f"{what}: takes CUDA tensors (no CPU path)")
     dev = cache.device
-    c = cache
-    if c.dim() != 3:
-        try:
-            c = cache.view(-1, *cache.shape[-2:]) if cache.dim() > 1 else None
-        except RuntimeError:
-            c = None
-    if c is None or not _q4_rows(c):
+    *lead, cap, row = cache.shape if cache.dim() > 1 else (0, 0)
+    *outer, s1, s0 = cache.stride() if cache.dim() > 1 else (0, 0)
+    # the leading axes as one: heads `step` bytes apart
+    heads, step = 1, cap * 72
+    fold = row == 72 and s0 == 1 and s1 == 72 and cache.dtype is torch.uint8
+    for size, stride in zip(reversed(lead), reversed(outer)):
+        if size > 1:
+            if heads == 1:
+                step = stride
+            fold = fold and stride == heads * step
+        heads *= size
+    if not fold:
         raise RuntimeError(f"{what}: the cache must be uint8 [..., capacity, {Q4_ROW_BYTES}] with contiguous rows and "
                            "leading dimensions of one stride")
-    heads, cap, _ = c.shape
     start, n = int(start), int(n)
     if start < 0 or n < 0 or start + n > cap:
         raise RuntimeError(f"{what}: rows [{start}, {start + n}) are outside the cache's {cap}")
-    shape = (heads, n, 128) if c is cache else (*cache.shape[:-2], n, 128)
+    shape = (*lead, n, 128)
     if out is None:
-        out = torch.empty(shape, dtype=_BF16, device=dev)
+        out = cache.new_empty(shape, dtype=_BF16)
     elif out.shape != shape or out.dtype is not torch.bfloat16 or not out.is_contiguous() or out.device != dev:
         raise RuntimeError(f"{what}: out must be contiguous bf16 {list(shape)} on {dev}")
     if heads == 0 or n == 0:
@@ -874,8 +878,8 @@ def kv_read_q4(cache: torch.Tensor, start: int, n: int, out: torch.Tensor | None
     if _current_device() != index:
         with torch.cuda.device(dev):
             return kv_read_q4(cache, start, n, out)
-    rc = _lib.load().rt_kv_read_q4(c.data_ptr(), c.stride(0) if heads > 1 else cap * Q4_ROW_BYTES, out.data_ptr(),
-                                   n * 256, 256, heads, n, 128, cap, start, _raw_stream(index))
+    rc = _lib.load().rt_kv_read_q4(cache.data_ptr(), step, out.data_ptr(), n * 256, 256, heads, n, 128, cap, start,
+                                   _raw_stream(index))
     if rc:
         _lib.check(rc, "rt_kv_read_q4")
     _count()
@@ -952,4 +956,10 @@ def tree_attention_q4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask_bi
     return out
 
 
-__all__ += ["prompt_attention", "kv_append_q4", "kv_read_q4", "tree_attention_q4", "Q4_ROW_BYTES"]
+def default_splits_q4(n: int, num_q_heads: int, num_kv_heads: int, prefix_len: int) -> int:
+    """Key splits ``tree_attention_q4`` picks for this shape."""
+    return int(_lib.load().rt_tree_attn_q4_default_splits(n, num_q_heads, num_kv_heads, int(prefix_len)))
+
+
+__all__ += ["prompt_attention", "kv_append_q4", "kv_read_q4", "tree_attention_q4", "default_splits_q4",
+            "Q4_ROW_BYTES"]

@@ -89,7 +89,8 @@ def retree_generate(model, target, input_ids, mask_token_id, max_new_tokens, blo
                     recovery_memory: RecoveryMemory | None = None, gate_threshold: float = 0.01,
                     recovery_online_update: bool = True, recovery_record_top_k: int = 8,
                     recovery_rescue_top_k: int = 8, draft_fn=None, device_recovery: bool = True,
-                    fused: bool | None = None, fused_draft: bool = False):
+                    fused: bool | None = None, fused_draft: bool = False, kv_bits: int = 16,
+                    prompt_attention: bool = False):
     """ReTree decode loop (retree.py:193-444); ``total_rescued`` counts sibling rescues.
 
     ``device_recovery`` (the default) runs the recovery walk on the GPU
@@ -97,14 +98,15 @@ def retree_generate(model, target, input_ids, mask_token_id, max_new_tokens, blo
     is one graph replay with no per-candidate host round trip; its online
     counts are applied to ``recovery_memory`` when the request ends.  False
     walks on the host with the reference's control flow.  ``fused`` /
-    ``fused_draft`` as in ``ddtree_generate``.
+    ``fused_draft`` / ``kv_bits`` / ``prompt_attention`` as in ``ddtree_generate``.
     """
     from .verify import TreeVerifier
 
     if block_size <= 1:  # retree.py:210-219: the linear path
         from .ddtree import dflash_generate
         out = dflash_generate(model, target, input_ids, mask_token_id, max_new_tokens, block_size, stop_token_ids,
-                              temperature=temperature, draft_fn=draft_fn, fused=fused, fused_draft=fused_draft)
+                              temperature=temperature, draft_fn=draft_fn, fused=fused, fused_draft=fused_draft,
+                              kv_bits=kv_bits, prompt_attention=prompt_attention)
         out.total_rescued = 0
         return out
     stop_set = None if stop_token_ids is None else {int(t) for t in stop_token_ids if t is not None}
@@ -122,7 +124,8 @@ def retree_generate(model, target, input_ids, mask_token_id, max_new_tokens, blo
                             max_length=input_ids.shape[1] + max_new_tokens + 2 * block_size + 8,
                             draft_horizon=block_size - 1, temperature=temperature,
                             target_layer_ids=None if (model is None or draft_fn is not None)
-                            else list(model.target_layer_ids), fused=fused, fused_draft=fused_draft)
+                            else list(model.target_layer_ids), fused=fused, fused_draft=fused_draft,
+                            kv_bits=kv_bits, prompt_attention=prompt_attention)
     if device_recovery and recovery_memory is not None:
         from .recovery_device import DeviceRecoveryMemory
         dm = DeviceRecoveryMemory(recovery_memory, verifier.device, stop_ids=stop_set)

@@ -2,7 +2,7 @@
 
 ``TreeVerifier`` holds what the reference's decode loops keep between rounds
 (ddtree.py:765-795, retree.py:228-264): the output-id buffer, the target KV
-cache (a ``TreeKVCache`` here), the tree buffers, and the stage timers.  One
+cache (a ``TreeKVCache`` here, or its 4-bit form), the tree buffers, and the stage timers.  One
 ``round(draft_logits)`` is the verification hot path:
 
   1. draft top-k + best-first expansion   (kernels: rt_draft_topk, rt_tree_build)
@@ -31,8 +31,8 @@ from . import fused as fused_mod
 from . import kernels
 from .attention import NAME as ATTN_NAME
 from .headsplit import NAME as HEADSPLIT_NAME
-from .attention import attach
-from .cache import TreeKVCache
+from .attention import attach, prompt_kernel
+from .cache import make_cache
 from .ddtree import (DDTREE_STAGE_ORDER, DDTREE_TREE_BUILD_STAGE_ORDER, build_tree_device, cuda_time,
                      empty_stage_times, resolve_strategy, sample)
 
@@ -59,7 +59,10 @@ class TreeVerifier:
     def __init__(self, target, tree_budget: int, max_length: int, draft_horizon: int = 15,
                  temperature: float = 0.0, target_layer_ids=None, device=None, fused: bool | None = None,
                  gemm: str = "auto", fused_draft: bool = False, exchange: str = "nccl", chain: bool = False,
-                 fused_argmax: bool = False):
+                 fused_argmax: bool = False, kv_bits: int = 16, prompt_attention: bool = False):
+        """``kv_bits=4`` keeps the target's cache in 4 bits (``TreeKVCacheQ4``);
+        ``prompt_attention=True`` runs the prompt forward on ``kernels.prompt_attention``
+        (a 4-bit cache's prompt always does)."""
         cfg = target.config
         if getattr(cfg, "_attn_implementation", None) not in (ATTN_NAME, HEADSPLIT_NAME):
             raise RuntimeError(f"target must use attn_implementation={ATTN_NAME!r} (retree_b200.attention.register())")
@@ -75,8 +78,10 @@ class TreeVerifier:
         # a target split by KV head (retree_b200.headsplit) caches only its own heads
         kv_heads = getattr(target, "_rt_local_kv_heads", cfg.num_key_value_heads)
         head_dim = getattr(cfg, "head_dim", None) or cfg.hidden_size // cfg.num_attention_heads
-        self.cache = TreeKVCache(cfg.num_hidden_layers, kv_heads, head_dim, self.max_length + self.n_max + 128,
-                                 device=self.device)
+        self.kv_bits = int(kv_bits)
+        self.prompt_attention = bool(prompt_attention)
+        self.cache = make_cache(self.kv_bits, cfg.num_hidden_layers, kv_heads, head_dim,
+                                self.max_length + self.n_max + 128, device=self.device)
         self.output_ids = torch.zeros(self.max_length + self.n_max + 1, dtype=torch.long, device=self.device)
         # [start, start before the last commit]; in graph mode the cache appends at start_dev[0]
         self.start_dev = torch.zeros(2, dtype=torch.int64, device=self.device)
@@ -143,8 +148,9 @@ class TreeVerifier:
         self.cache.use_device_length(False)  # the prompt is causal over an empty cache
         self.cache.set_length(0)
         pos = torch.arange(n, device=self.device).unsqueeze(0)
-        out = self.target(ids, position_ids=pos, past_key_values=self.cache, use_cache=True, logits_to_keep=1,
-                          output_hidden_states=self.target_layer_ids is not None)
+        with prompt_kernel(self.prompt_attention):
+            out = self.target(ids, position_ids=pos, past_key_values=self.cache, use_cache=True, logits_to_keep=1,
+                              output_hidden_states=self.target_layer_ids is not None)
         self.output_ids[:n] = ids[0]
         self.output_ids[n: n + 1] = sample(out.logits, self.temperature)[0]
         if self.target_layer_ids is not None:
@@ -168,8 +174,14 @@ class TreeVerifier:
         vocab = vocab or self.target.config.vocab_size
         g = torch.Generator(device=self.device).manual_seed(seed)
         slab = self.cache.slab
-        for i in range(slab.shape[0]):
-            slab[i, :, :length].copy_(torch.randn(slab[i, :, :length].shape, device=self.device, generator=g))
+        if self.kv_bits == 4:
+            shape = (2, slab.shape[1], length, self.cache.head_dim)
+            for i in range(self.cache.num_layers):
+                k, v = torch.randn(shape, device=self.device, generator=g).to(torch.bfloat16)
+                self.cache.append(i, k, v)
+        else:
+            for i in range(slab.shape[0]):
+                slab[i, :, :length].copy_(torch.randn(slab[i, :, :length].shape, device=self.device, generator=g))
         self.output_ids[: length + 1] = torch.randint(0, vocab, (length + 1,), device=self.device, generator=g)
         self.cache.set_length(length)
         self.start = length
