@@ -25,14 +25,12 @@
 // ---------------------------------------------------------------------------
 // One CTA per (key split, kv head, 256 query rows): two 128-row tiles (row r of
 // a tile is (node r / group, query head r % group)) in ping-pong on tcgen05 as in
-// the prompt attention.  Warps:
+// the prompt attention.  Sixteen warps:
 //   warps 0-3, 4-7  softmax of tile 0 / 1, one thread per row;
-//   warps 8-11 (15) decode, one group of four warps or two that take turns: a
-//                   thread per key turns the 72 bytes of K (or V) of a 128-key
-//                   block into its row of a bf16 SW128 tile;
-//   next warp       producer: Q by TMA, the blocks' bytes by bulk copies (9216
-//                   contiguous bytes each) into a 3-stage ring;
-//   next warp       MMA issuer.
+//   warps 8-14      decode: a lane turns the 72 bytes of a key's K (or V) into its
+//                   row of a bf16 SW128 tile, 32 keys a task, the next task's
+//                   bytes already on their way from global memory;
+//   warp 15         Q by TMA, MMA issuer.
 // When only one tile has queries (n * group <= 128, or the last rows) the two
 // softmax groups take turns at its key blocks instead: two chains of S, P and O
 // for the same queries, merged at the end, so that one chain's softmax still runs
@@ -437,37 +435,31 @@ __global__ void __launch_bounds__(kQsThreads, 1) tree_attn_q4_small_kernel(const
 // ---------------------------------------------------------------------------
 // More query rows: decoded tiles on tcgen05
 // ---------------------------------------------------------------------------
-// With one decode group the block is launched with 128 registers x 512 threads
-// (2 x 176 + 88 + 72 = 4 x 128), with two 96 x 640 (2 x 168 + 2 x 40 + 64 = 5 x 96).
-template <int kDec>
-struct Q4Tile {
-  static constexpr int kThreads = 384 + 128 * kDec;
-  static constexpr int kProducerWarp = 8 + 4 * kDec, kMmaWarp = kProducerWarp + 1;
-  static constexpr int kRegsSoftmax = kDec == 1 ? 176 : 168, kRegsDecode = kDec == 1 ? 88 : 40,
-                       kRegsOther = kDec == 1 ? 72 : 64;
-};
+constexpr int kQtThreads = 512;
+constexpr int kQtDecodeWarps = 7, kQtMmaWarp = 15;    // warps 8-14, 15
+// registers a thread; the block is launched with 128 x 512 (2 x 176 + 2 x 80 = 4 x 128).
+// (Spilling on either side shows: 257 nodes over 32768 rows 204 us, 222 with 168 / 88,
+// 216 with 184 / 72.  With 4 / 5 / 6 / 7 decode warps 17 nodes take 33.8 / 33.8 / 30.5 / 28.7.)
+constexpr int kQtRegsSoftmax = 176, kQtRegsOther = 80;
 constexpr int kQtKeys = 128;
 constexpr uint32_t kQtTile = 128 * 128 * 2, kQtHalf = kQtTile / 2;
 constexpr int kQtStages = 4;                          // decoded tiles
-constexpr int kQtPacked = 3;                          // blocks of bytes
-constexpr uint32_t kQtBlock = kQtKeys * kQ4Row;
 constexpr uint32_t kQtOffQ = 0;
 constexpr uint32_t kQtOffKV = 2 * kQtTile;
-constexpr uint32_t kQtOffPacked = kQtOffKV + kQtStages * kQtTile;
-constexpr uint32_t kQtOffBar = kQtOffPacked + kQtPacked * kQtBlock;
+constexpr uint32_t kQtOffBar = kQtOffKV + kQtStages * kQtTile;
 constexpr uint32_t kQtOffMl = kQtOffBar + 512;        // [chain][row] (m, l)
 constexpr uint32_t kQtSmem = kQtOffMl + 2 * 128 * 8 + 1024;
 constexpr uint32_t kQtTmemO = 256;                    // S0 | S1 | O0 | O1, P_t in S_t's first 64 columns
 
 struct Q4Bars {
-  uint64_t q_full[2], in_full[kQtPacked], in_empty[kQtPacked], kv_full[kQtStages], kv_empty[kQtStages], s_full[2],
+  uint64_t q_full[2], kv_full[kQtStages], kv_empty[kQtStages], s_full[2],
       p_part[2], p_full[2], o_full[2], fin;
   uint32_t tmem_base;
   int abort_flag;
   uint2 x43;  // (.x)
 };
 
-// Order in which the blocks' bytes are loaded, decoded and consumed: K of the
+// Order in which the blocks are decoded and consumed: K of the
 // first `ahead` blocks (1, or 2 with two chains), then V_b and K_{b + ahead} in turn.
 __device__ __forceinline__ int q4_entry(int n, int nb, int ahead, bool& is_v) {
   const int a = min(ahead, nb), m = n - a, pairs = nb - a;
@@ -476,48 +468,48 @@ __device__ __forceinline__ int q4_entry(int n, int nb, int ahead, bool& is_v) {
   return m >= 2 * pairs ? m - pairs : (m >> 1) + ((m & 1) ? a : 0);
 }
 
-// A key's row of a decoded tile: 128 bf16 values in two SW128 halves.  All of
-// the row is read before anything is decoded (`loaded` runs in between): one
-// warp a scheduler decodes, so its words have to overlap one another.
-template <typename Loaded>
-__device__ __forceinline__ void q4_decode_row(uint32_t src, uint32_t tile, int r, bool zero, bool nan, uint32_t x43,
-                                              Loaded loaded) {
-  uint2 w[8];
+// A key's row as its thread holds it.
+struct Q4Packed {
+  uint2 w[8];  // code words
+  uint2 meta;  // group words
+};
+
+__device__ __forceinline__ void q4_load_row(const char* src, bool have, Q4Packed& x) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) w[i] = lds64(src + i * 8);
-  const uint2 mw = lds64(src + kQ4Codes);
-  loaded();
-  const uint32_t meta[4] = {mw.x & 0xFFFFu, mw.x >> 16, mw.y & 0xFFFFu, mw.y >> 16};
+  for (int i = 0; i < 8; ++i) x.w[i] = have ? *reinterpret_cast<const uint2*>(src + i * 8) : make_uint2(0, 0);
+  x.meta = have ? *reinterpret_cast<const uint2*>(src + kQ4Codes) : make_uint2(0, 0);  // (scale 0: reads as zero)
+}
+
+// Its 128 bf16 values into row r of a decoded tile (two SW128 halves).
+__device__ __forceinline__ void q4_decode_row(const Q4Packed& x, uint32_t tile, int r, uint32_t x43) {
+  const uint32_t meta[4] = {x.meta.x & 0xFFFFu, x.meta.x >> 16, x.meta.y & 0xFFFFu, x.meta.y >> 16};
   const uint32_t dst = tile + r * 128;
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
-    // (a row that must read as zero or NaN does so through its scale)
-    const Q4Group q = q4_group(nan ? 0x7FF0u : (zero ? 0u : meta[g]));
+    const Q4Group q = q4_group(meta[g]);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int ch = g * 4 + i * 2;
       const uint32_t half = dst + (ch >> 3) * kQtHalf;
-      sts128(half + (((ch & 7) ^ (r & 7)) << 4), q4_decode8(w[g * 2 + i].x, q, x43));
-      sts128(half + ((((ch + 1) & 7) ^ (r & 7)) << 4), q4_decode8(w[g * 2 + i].y, q, x43));
+      sts128(half + (((ch & 7) ^ (r & 7)) << 4), q4_decode8(x.w[g * 2 + i].x, q, x43));
+      sts128(half + ((((ch + 1) & 7) ^ (r & 7)) << 4), q4_decode8(x.w[g * 2 + i].y, q, x43));
     }
   }
 }
 
-template <int kDec>
-__global__ void __launch_bounds__(Q4Tile<kDec>::kThreads, 1)
+__global__ void __launch_bounds__(kQtThreads, 1)
     tree_attn_q4_tile_kernel(const __grid_constant__ CUtensorMap tmap_q, const AttnParams p, const int tok) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   Q4Bars& bar = *reinterpret_cast<Q4Bars*>(smem + kQtOffBar);
-  constexpr int kProducerWarp = Q4Tile<kDec>::kProducerWarp, kMmaWarp = Q4Tile<kDec>::kMmaWarp;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int split = blockIdx.x, kvh = blockIdx.y, G = p.group;
   const int node0 = blockIdx.z * 2 * tok;               // first node of tile 0
   const int tiles = node0 + tok < p.n ? 2 : 1;
   const bool dual = tiles == 1;                         // two chains over one tile's keys
   const int ahead = dual ? 2 : 1;
-  if (warp == kProducerWarp && lane == 0) {
+  if (warp == 8 && lane == 0) {
     prefetch_tmap(&tmap_q);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bar.q_full[i], 1);
@@ -525,10 +517,6 @@ __global__ void __launch_bounds__(Q4Tile<kDec>::kThreads, 1)
       mbar_init(&bar.p_part[i], 4);
       mbar_init(&bar.p_full[i], 4);
       mbar_init(&bar.o_full[i], 1);
-    }
-    for (int i = 0; i < kQtPacked; ++i) {
-      mbar_init(&bar.in_full[i], 1);
-      mbar_init(&bar.in_empty[i], 4);
     }
     for (int i = 0; i < kQtStages; ++i) {
       mbar_init(&bar.kv_full[i], 4);
@@ -540,7 +528,7 @@ __global__ void __launch_bounds__(Q4Tile<kDec>::kThreads, 1)
     fence_mbar_init();
     fence_proxy_async_smem();
   }
-  if (warp == kMmaWarp) {
+  if (warp == kQtMmaWarp) {
     tmem_alloc(&bar.tmem_base, 512);
     tmem_relinquish();
   }
@@ -558,40 +546,20 @@ __global__ void __launch_bounds__(Q4Tile<kDec>::kThreads, 1)
   if (inside) split_range(total, split, p.num_splits, kQtKeys, b0, b1);
   const int nb = static_cast<int>(b1 - b0);
 
-  if (warp >= kProducerWarp) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Q4Tile<kDec>::kRegsOther));
-    if (warp == kProducerWarp && lane == 0 && nb > 0) {
-      // ---------------- producer ----------------
-      bool ok = true;
-      const uint32_t qbytes = static_cast<uint32_t>(tok * G) * 256u;
-      for (int t = 0; t < tiles; ++t) {
-        unsigned char* dst = smem + kQtOffQ + t * kQtTile;
-        mbar_arrive_expect_tx(&bar.q_full[t], qbytes);
-        tma_load_3d(dst, &tmap_q, &bar.q_full[t], 0, kvh * G, node0 + t * tok);
-        tma_load_3d(dst + kQtHalf, &tmap_q, &bar.q_full[t], 64, kvh * G, node0 + t * tok);
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kQtRegsOther));
+    if (warp == kQtMmaWarp) {
+      // ---------------- MMA issuer (and Q by TMA) ----------------
+      if (lane == 0 && nb > 0) {
+        const uint32_t qbytes = static_cast<uint32_t>(tok * G) * 256u;
+        for (int t = 0; t < tiles; ++t) {
+          unsigned char* dst = smem + kQtOffQ + t * kQtTile;
+          mbar_arrive_expect_tx(&bar.q_full[t], qbytes);
+          tma_load_3d(dst, &tmap_q, &bar.q_full[t], 0, kvh * G, node0 + t * tok);
+          tma_load_3d(dst + kQtHalf, &tmap_q, &bar.q_full[t], 64, kvh * G, node0 + t * tok);
+        }
       }
-      const char* kb = p.k + kvh * p.kv_head_stride;
-      const char* vb = p.v + kvh * p.kv_head_stride;
-      int n = 0;
-      for (; n < 2 * nb; ++n) {
-        const int s = n % kQtPacked;
-        ok = mbar_wait(&bar.in_empty[s], ((n / kQtPacked) & 1) ^ 1, abort_flag, p.status, RT_DEV_WAIT_TIMEOUT);
-        if (!ok) break;
-        bool is_v;
-        const int64_t key0 = (b0 + q4_entry(n, nb, ahead, is_v)) * kQtKeys;
-        // an even number of rows: 16-byte pieces that end inside the (even) capacity
-        const uint32_t bytes =
-            static_cast<uint32_t>((min(static_cast<int64_t>(kQtKeys), total - key0) + 1) & ~int64_t(1)) * kQ4Row;
-        mbar_arrive_expect_tx(&bar.in_full[s], bytes);
-        bulk_load(smem + kQtOffPacked + s * kQtBlock, (is_v ? vb : kb) + key0 * kQ4Row, bytes, &bar.in_full[s]);
-      }
-      if (*abort_flag) {
-        for (int t = 0; t < tiles; ++t) mbar_wait_drain(&bar.q_full[t], 0);
-        for (int i = max(0, n - kQtPacked); i < n; ++i)
-          mbar_wait_drain(&bar.in_full[i % kQtPacked], (i / kQtPacked) & 1);
-      }
-    } else if (warp == kMmaWarp) {
-      // ---------------- MMA issuer ----------------
+      __syncwarp();
       constexpr uint32_t idesc_qk = idesc_bf16_f32(kBM, kQtKeys, false, false);
       constexpr uint32_t idesc_pv = idesc_bf16_f32(kBM, kHD, false, true);
       const uint32_t tm = warp_uniform(tmem);
@@ -677,34 +645,42 @@ __global__ void __launch_bounds__(Q4Tile<kDec>::kThreads, 1)
         mbar_wait_drain(&bar.fin, 0);
       }
       __syncwarp();
-    }
-  } else if (warp >= 8) {
-    // ---------------- decode ----------------
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Q4Tile<kDec>::kRegsDecode));
-    const int r = tid & 127;
-    const uint32_t sbase = smem_u32(smem), x43 = lds64(smem_u32(&bar.x43)).x;
-    const char* vb = p.v + kvh * p.kv_head_stride;
-    for (int n = (warp >> 2) - 2; n < 2 * nb; n += kDec) {  // (two groups take turns)
-      const int si = n % kQtPacked, so = n % kQtStages;
-      bool is_v;
-      const int64_t key = (b0 + q4_entry(n, nb, ahead, is_v)) * kQtKeys + r;
-      mbar_wait_fast(&bar.in_full[si], (n / kQtPacked) & 1, abort_flag, p.status);
-      mbar_wait_fast(&bar.kv_empty[so], ((n / kQtStages) & 1) ^ 1, abort_flag, p.status);
-      // behind the tree: zero.  A tree row of V that reads as NaN: zero in V, and
-      // NaN in K, so that only the nodes that see the key get it.
-      bool zero = key >= total, nan = false;
-      if (key >= L && !zero && q4_is_nan(*reinterpret_cast<const uint16_t*>(vb + key * kQ4Row + kQ4Codes))) {
-        zero = is_v;
-        nan = !is_v;
+      if (nb > 0)
+        for (int t = 0; t < tiles; ++t) mbar_wait_drain(&bar.q_full[t], 0);  // (long done, but for an abort)
+    } else if (warp < 8 + kQtDecodeWarps) {
+      // ---------------- decode ----------------
+      // A task is 32 keys of K or V of a block, a lane a key; the warps take turns.
+      // The next task's rows are on their way from global memory meanwhile.
+      const uint32_t sbase = smem_u32(smem), x43 = lds64(smem_u32(&bar.x43)).x;
+      const char* kb = p.k + kvh * p.kv_head_stride;
+      const char* vb = p.v + kvh * p.kv_head_stride;
+      const int tasks = 8 * nb;
+      Q4Packed next;
+      auto load = [&](int task) {
+        bool is_v;
+        const int64_t key = (b0 + q4_entry(task >> 2, nb, ahead, is_v)) * kQtKeys + (task & 3) * 32 + lane;
+        // (behind the tree: zeros)
+        q4_load_row((is_v ? vb : kb) + key * kQ4Row, task < tasks && key < total, next);
+        // A tree row of V that reads as NaN: zero in V, and NaN in K, so that only
+        // the nodes that see the key get it.
+        if (task < tasks && key >= L && key < total &&
+            q4_is_nan(*reinterpret_cast<const uint16_t*>(vb + key * kQ4Row + kQ4Codes)))
+          next.meta = is_v ? make_uint2(0, 0) : make_uint2(0x7FF07FF0u, 0x7FF07FF0u);
+      };
+      load(warp - 8);
+      for (int task = warp - 8; task < tasks; task += kQtDecodeWarps) {
+        const Q4Packed x = next;
+        load(task + kQtDecodeWarps);
+        const int n = task >> 2, so = n % kQtStages;
+        mbar_wait_fast(&bar.kv_empty[so], ((n / kQtStages) & 1) ^ 1, abort_flag, p.status);
+        q4_decode_row(x, sbase + kQtOffKV + so * kQtTile, (task & 3) * 32 + lane, x43);
+        fence_proxy_async_smem();
+        mbar_arrive_warp(&bar.kv_full[so]);
       }
-      q4_decode_row(sbase + kQtOffPacked + si * kQtBlock + r * kQ4Row, sbase + kQtOffKV + so * kQtTile, r, zero, nan, x43,
-                    [&] { mbar_arrive_warp(&bar.in_empty[si]); });
-      fence_proxy_async_smem();
-      mbar_arrive_warp(&bar.kv_full[so]);
     }
   } else {
     // ---------------- softmax and result of tile (or chain) t ----------------
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Q4Tile<kDec>::kRegsSoftmax));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kQtRegsSoftmax));
     const int t = warp >> 2, r = tid & 127;
     const int rt = r / G;
     const int first = node0 + (dual ? 0 : t * tok);     // first node of the tile
@@ -837,7 +813,7 @@ __global__ void __launch_bounds__(Q4Tile<kDec>::kThreads, 1)
     cluster_sync_all();
   }
   __syncthreads();
-  if (warp == kMmaWarp) {
+  if (warp == kQtMmaWarp) {
     __syncwarp();
     tc_fence_after();
     tmem_dealloc(tmem, 512);
@@ -893,7 +869,7 @@ static int clusters_fit(Kernel kernel, int threads, uint32_t smem, int c) {
   return n;
 }
 
-// ... of the few-rows kernel, or of the tile kernel with two decode groups (cached per size).
+// ... of the few-rows kernel, or of the tile kernel (cached per size).
 static int q4_clusters_fit(bool small, int c) {
   static std::mutex mu;
   static int cache[2][kMaxMerge + 1] = {};
@@ -902,7 +878,7 @@ static int q4_clusters_fit(bool small, int c) {
   if (c < 2 || c > kMaxMerge) return 0;
   if (!done[small][c]) {
     cache[small][c] = small ? clusters_fit(tree_attn_q4_small_kernel<2>, kQsThreads, kQsSmem, c)
-                            : clusters_fit(tree_attn_q4_tile_kernel<2>, Q4Tile<2>::kThreads, kQtSmem, c);
+                            : clusters_fit(tree_attn_q4_tile_kernel, kQtThreads, kQtSmem, c);
     done[small][c] = true;
   }
   return cache[small][c];
@@ -916,13 +892,31 @@ static int launch_q4_small(dim3 grid, dim3 cluster, cudaStream_t s, const AttnPa
       launch_ex_cluster(tree_attn_q4_small_kernel<NT>, grid, dim3(kQsThreads), kQsSmem, s, cluster, p));
 }
 
-template <int kDec>
-static int launch_q4_tile(dim3 grid, dim3 cluster, cudaStream_t s, const CUtensorMap& tq, const AttnParams& p, int tok) {
-  set_smem_limit(tree_attn_q4_tile_kernel<kDec>, kQtSmem);
-  if (cluster.x > 8)
-    cudaFuncSetAttribute(tree_attn_q4_tile_kernel<kDec>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  return record_cuda(launch_ex_cluster(tree_attn_q4_tile_kernel<kDec>, grid, dim3(Q4Tile<kDec>::kThreads), kQtSmem, s,
-                                       cluster, tq, p, tok));
+// Splits of a launch of two-tile CTAs ("heavy") and, where the last nodes fill one
+// tile only, single-tile ones ("light", started last): the count with the
+// shortest estimated time on 148 SMs, from a block's cost in either (2.3 and
+// 1.24 us) and a CTA's fixed cost (6 us) as measured at 32768 rows.  257 nodes
+// (4 heavy CTAs and a light one a kv head): 204 us with one wave of 3 splits, 172 with 4, 179 with 8.
+static int tile_splits(int n, int tok, int hkv, int64_t blocks) {
+  const int rest = n % (2 * tok);
+  const int heavy = hkv * (n / (2 * tok) + (rest > tok)), light = hkv * (rest > 0 && rest <= tok);
+  int best = 1;
+  double best_t = 1e30;
+  for (int s = 1; s <= 32 && s <= blocks; ++s) {
+    const double each = static_cast<double>((blocks + s - 1) / s), h = 2.3 * each + 6, l = 1.24 * each + 6;
+    const int64_t H = static_cast<int64_t>(heavy) * s, Lc = static_cast<int64_t>(light) * s;
+    const int64_t rounds = (H + 147) / 148, idle = rounds * 148 - H, fit = static_cast<int64_t>(h / l);
+    // the light ones run on the SMs without a heavy one in the last round, then on all
+    double t = rounds * h;
+    const int64_t left = Lc - idle * fit;
+    if (left > 0 && left <= idle) t = std::max(t, (rounds - 1) * h + (fit + 1) * l);
+    else if (left > 0) t += l * ((left + 147) / 148);
+    if (t < best_t) {
+      best_t = t;
+      best = s;
+    }
+  }
+  return best;
 }
 
 static Q4Plan q4_plan(int n, int G, int hkv, int64_t prefix_len, int num_splits) {
@@ -939,8 +933,7 @@ static Q4Plan q4_plan(int n, int G, int hkv, int64_t prefix_len, int num_splits)
   const int tok = kBM / G;
   const int64_t ctas = static_cast<int64_t>(hkv) * ((n + 2 * tok - 1) / (2 * tok));
   int64_t want = num_splits;
-  if (want <= 0) want = std::max<int64_t>(1, 148 / ctas);
-  if (num_splits <= 0) want = std::min<int64_t>(want, blocks);  // (a given count is kept: empty splits are fine)
+  if (want <= 0) want = n <= tok ? std::min<int64_t>(std::max<int64_t>(1, 148 / ctas), blocks) : tile_splits(n, tok, hkv, blocks);
   want = std::min<int64_t>(want, 256);
   if (n <= tok && want > 1) {
     // one tile: its splits merge in a cluster when it takes all of them, or (where
@@ -1039,10 +1032,11 @@ extern "C" int rt_tree_attn_q4(const void* q, int64_t q_tok_stride, int64_t q_he
     rc = make_q4_query_tmap(&tq, q, q_tok_stride, q_head_stride, n, num_q_heads, G, tok);
     if (rc != RT_OK) return rc;
     const dim3 grid(pl.splits, num_kv_heads, (n + 2 * tok - 1) / (2 * tok));
-    // One tile (two chains) wants two decode groups, two tiles the registers:
-    // 32768 rows, 17 nodes 31.5 us with one group, 29.4 with two; 257 nodes 205, 217.
-    rc = n <= tok ? launch_q4_tile<2>(grid, dim3(pl.merge ? pl.splits : 1, 1, 1), s, tq, p, tok)
-                  : launch_q4_tile<1>(grid, dim3(1, 1, 1), s, tq, p, tok);
+    set_smem_limit(tree_attn_q4_tile_kernel, kQtSmem);
+    if (pl.merge && pl.splits > 8)
+      cudaFuncSetAttribute(tree_attn_q4_tile_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    rc = record_cuda(launch_ex_cluster(tree_attn_q4_tile_kernel, grid, dim3(kQtThreads), kQtSmem, s,
+                                       dim3(pl.merge ? pl.splits : 1, 1, 1), tq, p, tok));
   }
   if (rc != RT_OK || pl.merge || pl.splits == 1) return rc;
   const int warps = num_kv_heads * n * G * (pl.splits <= kFastSplits ? 2 : 1);
