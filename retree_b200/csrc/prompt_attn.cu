@@ -53,7 +53,8 @@ constexpr uint32_t kPOffKV = 2 * kPTile;
 constexpr uint32_t kPOffTab = kPOffKV + kPStages * kPTile;  // prefix sums of the sequences' pair counts
 constexpr int kPMaxSeqs = 4096;
 constexpr uint32_t kPOffOrd = kPOffTab + (kPMaxSeqs + 1) * 4 + 12;  // up to 32 sequences, longest first
-constexpr uint32_t kPOffBar = kPOffOrd + 32 * 4;
+constexpr uint32_t kPOffOut = kPOffOrd + 32 * 4;                       // a warp's 32 rows x 64 bytes of output
+constexpr uint32_t kPOffBar = kPOffOut + 8 * 2048;
 constexpr uint32_t kPSmem = kPOffBar + 512 + 1024;
 constexpr uint32_t kPTmemO = 256;              // S0 | S1 | O0 | O1, P_t in S_t's first 64 columns
 constexpr int kPSms = 148;
@@ -494,6 +495,7 @@ __global__ void __launch_bounds__(kPThreads, 1)
     const int rt = r / p.group, rh = r - rt * p.group;
     const float sl2 = p.scale_log2;
     int ns = 0, no = 0;
+    const uint32_t stage = smem_u32(smem + kPOffOut + warp * 2048);
     for (int it = 0; prompt_next<true>(p, bar, tab, ord, it, w); ++it) {
       const int tok = w.tok0 + t * p.tok + rt;
       const bool valid = t < p.tiles && rt < p.tok && tok < w.lq;
@@ -520,7 +522,7 @@ __global__ void __launch_bounds__(kPThreads, 1)
         mbar_arrive_warp(&bar.p_full[t]);
       }
       const int64_t row = static_cast<int64_t>(w.q0 + tok), head = w.g * p.group + rh;
-      char* dst = p.out + row * p.out_tok_stride + head * p.out_head_stride;
+      char* dst = valid ? p.out + row * p.out_tok_stride + head * p.out_head_stride : nullptr;
       const int64_t slot = (static_cast<int64_t>(w.split) * p.total_q + row) * p.hq + head;
       if (nb == 0) {
         if (valid && p.splits > 1) p.ws_ml[slot] = make_float2(-INFINITY, 0.f);
@@ -540,20 +542,30 @@ __global__ void __launch_bounds__(kPThreads, 1)
         uint32_t o[32];
         tmem_ld32(to + c * 32, o);
         tmem_wait_ld();
-        if (!valid) continue;
         float x[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) x[i] = none ? 0.f : __uint_as_float(o[i]) * inv;
-        if (poison)
+        if (poison && valid)
           add_not_finite<T>(p.v + w.g * p.kv_head_stride + w.k0 * p.kv_row_stride + c * 64, p.kv_row_stride,
                             (w.jb + w.jm) * kPB, min(lim, (w.jb + nb) * kPB), x);
         if (p.splits == 1) {
+          // through shared memory, so that four lanes write a row's 64 bytes together
+          // (a lane a row would touch 32 rows with every store)
 #pragma unroll
           for (int q = 0; q < 4; ++q)
-            *reinterpret_cast<uint4*>(dst + c * 64 + q * 16) =
-                make_uint4(pack2<T>(x[q * 8], x[q * 8 + 1]), pack2<T>(x[q * 8 + 2], x[q * 8 + 3]),
-                           pack2<T>(x[q * 8 + 4], x[q * 8 + 5]), pack2<T>(x[q * 8 + 6], x[q * 8 + 7]));
-        } else {
+            sts128(stage + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4),
+                   make_uint4(pack2<T>(x[q * 8], x[q * 8 + 1]), pack2<T>(x[q * 8 + 2], x[q * 8 + 3]),
+                              pack2<T>(x[q * 8 + 4], x[q * 8 + 5]), pack2<T>(x[q * 8 + 6], x[q * 8 + 7])));
+          __syncwarp();
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int from = q * 8 + (lane >> 2), ch = lane & 3;
+            const uint4 v = lds128(stage + from * 64 + ((ch ^ ((from >> 1) & 3)) << 4));
+            const uint64_t to_row = __shfl_sync(0xFFFFFFFFu, reinterpret_cast<uint64_t>(dst), from);
+            if (to_row != 0) *reinterpret_cast<uint4*>(to_row + c * 64 + ch * 16) = v;
+          }
+          __syncwarp();
+        } else if (valid) {
 #pragma unroll
           for (int q = 0; q < 8; ++q)
             *reinterpret_cast<float4*>(p.ws_o + slot * kPD + c * 32 + q * 4) =
