@@ -498,7 +498,8 @@ __device__ __forceinline__ void q4_decode_row(const Q4Packed& x, uint32_t tile, 
 }
 
 __global__ void __launch_bounds__(kQtThreads, 1)
-    tree_attn_q4_tile_kernel(const __grid_constant__ CUtensorMap tmap_q, const AttnParams p, const int tok) {
+    tree_attn_q4_tile_kernel(const __grid_constant__ CUtensorMap tmap_q, const AttnParams p, const int tok, const int heavy,
+                             const int tail) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -543,7 +544,8 @@ __global__ void __launch_bounds__(kQtThreads, 1)
   const bool inside = L >= 0 && total <= p.capacity;    // the same in every thread of the launch
   if (!inside && tid == 0) set_status(p.status, RT_DEV_BAD_INDEX);
   int64_t b0 = 0, b1 = 0;
-  if (inside) split_range(total, split, p.num_splits, kQtKeys, b0, b1);
+  const int mine = dual ? tail : heavy;                 // this tile's splits; the launch has the larger count
+  if (inside && split < mine) split_range(total, split, mine, kQtKeys, b0, b1);
   const int nb = static_cast<int>(b1 - b0);
 
   if (warp >= 8) {
@@ -840,8 +842,9 @@ static int make_q4_query_tmap(CUtensorMap* m, const void* q, int64_t tok_stride,
 
 struct Q4Plan {
   bool small;  // the mma.sync path
-  int splits;
+  int splits;  // of the keys, the most any tile has
   bool merge;
+  int heavy, tail;  // of the two-tile CTAs, of a last single-tile one
 };
 
 // Clusters of `c` CTAs of `kernel` that fit on the GPU at once (0 when the query
@@ -893,30 +896,34 @@ static int launch_q4_small(dim3 grid, dim3 cluster, cudaStream_t s, const AttnPa
 }
 
 // Splits of a launch of two-tile CTAs ("heavy") and, where the last nodes fill one
-// tile only, single-tile ones ("light", started last): the count with the
-// shortest estimated time on 148 SMs, from a block's cost in either (2.3 and
-// 1.24 us) and a CTA's fixed cost (6 us) as measured at 32768 rows.  257 nodes
-// (4 heavy CTAs and a light one a kv head): 204 us with one wave of 3 splits, 172 with 4, 179 with 8.
-static int tile_splits(int n, int tok, int hkv, int64_t blocks) {
+// tile only (a root and a power of two of others, say), single-tile ones ("light",
+// started last): the counts with the shortest estimated time on 148 SMs, from a
+// block's cost in either (2.3 and 1.24 us) and a CTA's fixed cost (6 us) as
+// measured at 32768 rows.  257 nodes (4 heavy CTAs and a light one a kv head): 204 us
+// with 3 splits of both, 172 with 4, 179 with 8, 161 with 4 of the heavy and 5 of the light ones.
+static void tile_splits(int n, int tok, int hkv, int64_t blocks, int& splits, int& tail) {
   const int rest = n % (2 * tok);
   const int heavy = hkv * (n / (2 * tok) + (rest > tok)), light = hkv * (rest > 0 && rest <= tok);
-  int best = 1;
-  double best_t = 1e30;
-  for (int s = 1; s <= 32 && s <= blocks; ++s) {
-    const double each = static_cast<double>((blocks + s - 1) / s), h = 2.3 * each + 6, l = 1.24 * each + 6;
-    const int64_t H = static_cast<int64_t>(heavy) * s, Lc = static_cast<int64_t>(light) * s;
-    const int64_t rounds = (H + 147) / 148, idle = rounds * 148 - H, fit = static_cast<int64_t>(h / l);
-    // the light ones run on the SMs without a heavy one in the last round, then on all
-    double t = rounds * h;
-    const int64_t left = Lc - idle * fit;
-    if (left > 0 && left <= idle) t = std::max(t, (rounds - 1) * h + (fit + 1) * l);
-    else if (left > 0) t += l * ((left + 147) / 148);
-    if (t < best_t) {
-      best_t = t;
-      best = s;
+  const int most = static_cast<int>(std::min<int64_t>(32, blocks));
+  auto cost = [&](double block, int s) { return block * static_cast<double>((blocks + s - 1) / s) + 6; };
+  double best = 1e30;
+  for (int s = 1; s <= most; ++s) {
+    const double h = cost(2.3, s);
+    const int H = heavy * s, rounds = (H + 147) / 148, idle = rounds * 148 - H;
+    if (rounds * h >= best) continue;
+    for (int sl = 1; sl <= (light > 0 ? most : 1); ++sl) {
+      // the light ones take the SMs as they come free
+      const double l = cost(1.24, sl);
+      double t_idle = (rounds - 1) * h, t_busy = rounds * h;
+      for (int left = light * sl; left > 0;) {
+        const bool on_idle = idle > 0 && t_idle <= t_busy;
+        left -= on_idle ? idle : 148 - idle;
+        (on_idle ? t_idle : t_busy) += l;
+      }
+      const double t = std::max(t_idle, t_busy);
+      if (t < best) best = t, splits = s, tail = light > 0 ? sl : s;
     }
   }
-  return best;
 }
 
 static Q4Plan q4_plan(int n, int G, int hkv, int64_t prefix_len, int num_splits) {
@@ -927,13 +934,17 @@ static Q4Plan q4_plan(int n, int G, int hkv, int64_t prefix_len, int num_splits)
     if (want <= 0) want = std::max<int64_t>(1, std::min<int64_t>(148 / hkv, (tiles + 7) / 8));
     want = std::min<int64_t>(want, 256);
     const int s = static_cast<int>(want);
-    return {true, s, s >= 2 && s <= kMaxMerge && hkv <= q4_clusters_fit(true, s)};
+    return {true, s, s >= 2 && s <= kMaxMerge && hkv <= q4_clusters_fit(true, s), s, s};
   }
   const int64_t blocks = (prefix_len + n + kQtKeys - 1) / kQtKeys;
   const int tok = kBM / G;
-  const int64_t ctas = static_cast<int64_t>(hkv) * ((n + 2 * tok - 1) / (2 * tok));
   int64_t want = num_splits;
-  if (want <= 0) want = n <= tok ? std::min<int64_t>(std::max<int64_t>(1, 148 / ctas), blocks) : tile_splits(n, tok, hkv, blocks);
+  if (want <= 0 && n > tok) {
+    int heavy = 1, tail = 1;
+    tile_splits(n, tok, hkv, blocks, heavy, tail);
+    return {false, std::max(heavy, tail), false, heavy, tail};
+  }
+  if (want <= 0) want = std::min<int64_t>(std::max<int64_t>(1, 148 / hkv), blocks);
   want = std::min<int64_t>(want, 256);
   if (n <= tok && want > 1) {
     // one tile: its splits merge in a cluster when it takes all of them, or (where
@@ -942,9 +953,10 @@ static Q4Plan q4_plan(int n, int G, int hkv, int64_t prefix_len, int num_splits)
     if (num_splits <= 0)
       while (c >= 2 && hkv > q4_clusters_fit(false, c)) --c;
     if (c >= 2 && hkv <= q4_clusters_fit(false, c) && (c == want || (num_splits <= 0 && blocks <= 3 * c)))
-      return {false, c, true};
+      return {false, c, true, c, c};
   }
-  return {false, static_cast<int>(want), false};
+  const int s = static_cast<int>(want);
+  return {false, s, false, s, s};
 }
 
 }  // namespace rt
@@ -1036,7 +1048,7 @@ extern "C" int rt_tree_attn_q4(const void* q, int64_t q_tok_stride, int64_t q_he
     if (pl.merge && pl.splits > 8)
       cudaFuncSetAttribute(tree_attn_q4_tile_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     rc = record_cuda(launch_ex_cluster(tree_attn_q4_tile_kernel, grid, dim3(kQtThreads), kQtSmem, s,
-                                       dim3(pl.merge ? pl.splits : 1, 1, 1), tq, p, tok));
+                                       dim3(pl.merge ? pl.splits : 1, 1, 1), tq, p, tok, pl.heavy, pl.tail));
   }
   if (rc != RT_OK || pl.merge || pl.splits == 1) return rc;
   const int warps = num_kv_heads * n * G * (pl.splits <= kFastSplits ? 2 : 1);
