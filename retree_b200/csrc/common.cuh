@@ -112,15 +112,32 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
   return false;
 }
 
+// Whether the phase is there, without waiting: asked some instructions ahead of
+// mbar_wait_fast, the answer's latency (over 200 cycles beside busy softmax warps) is hidden.
+__device__ __forceinline__ uint32_t mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok;
+}
+
 // The same for the hot loops of whole warps (every lane calls it): a phase that is (nearly) there
 // costs one poll, about a third of mbar_wait's loop and its checks.  The loops do
 // not branch on the result: after a time-out their (bounded) waits fall through
 // and they finish on whatever is in shared memory, and the results are dropped
 // (*abort).
-__device__ __forceinline__ void mbar_wait_fast(uint64_t* bar, uint32_t parity, volatile int* abort, int* status) {
+// `known`: what an earlier mbar_test of the phase said.
+__device__ __forceinline__ void mbar_wait_fast(uint64_t* bar, uint32_t parity, volatile int* abort, int* status,
+                                               uint32_t known = 0) {
   uint32_t ok;
   asm volatile(
-      "{\n\t.reg .pred p, q;\n\t.reg .u32 i, a;\n\tmov.u32 i, 0;\n"
+      "{\n\t.reg .pred p, q;\n\t.reg .u32 i, a;\n\tmov.u32 i, 0;\n\t"
+      "setp.ne.u32 p, %5, 0;\n\t@p bra DONE;\n"
       "POLL:\n\t"
       "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
       "@p bra DONE;\n\t"
@@ -130,7 +147,8 @@ __device__ __forceinline__ void mbar_wait_fast(uint64_t* bar, uint32_t parity, v
       "DONE:\n\t"
       "selp.b32 %0, 1, 0, p;\n\t}"
       : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity), "r"(smem_u32(const_cast<int*>(abort))), "n"(kWaitLimit)
+      : "r"(smem_u32(bar)), "r"(parity), "r"(smem_u32(const_cast<int*>(abort))), "n"(kWaitLimit),
+        "r"(known)
       : "memory");
   if (!ok) {
     *abort = 1;

@@ -364,7 +364,10 @@ __global__ void __launch_bounds__(kPThreads, 1)
     int n = 0;  // ring loads consumed
     int nq[2] = {0, 0}, np[2] = {0, 0};
     uint32_t looks = 0;  // V blocks handed to warp 10
-    auto wait = [&](uint64_t* b, uint32_t ph) { mbar_wait_fast(b, ph & 1, abort_flag, p.status); };
+    auto wait = [&](uint64_t* b, uint32_t ph, uint32_t known = 0) {
+      mbar_wait_fast(b, ph & 1, abort_flag, p.status, known);
+    };
+    auto test = [](uint64_t* b, uint32_t ph) { return mbar_test(b, ph & 1); };
     // S_t = Q_t K^T of the block in `stage`; the last one of an item frees Q_t
     auto qk = [&](int t, int stage, bool last) {
       const uint64_t b = dk + static_cast<uint64_t>(warp_uniform(stage) * (kPTile >> 4));
@@ -395,13 +398,16 @@ __global__ void __launch_bounds__(kPThreads, 1)
       }
       commit(&bar.kv_empty[s]);
       ++n;
+      // Each wait's barrier is asked some products ahead (`known`), so that the answer
+      // of one that is there does not hold up the tensor core.
+      uint32_t known_v = 0, known_p = 0;
       for (int j = 0; j < nb; ++j) {
         const int sv = n % kPStages, sk = (n + 1) % kPStages;
         const bool more = j + 1 < nb;
-        wait(&bar.kv_full[sv], n / kPStages);
         bool look = j >= w.jm;
+        wait(&bar.kv_full[sv], n / kPStages, known_v);
         if (look && elect_one()) mbar_arrive(&bar.v_look);
-        if (more) wait(&bar.kv_full[sk], (n + 1) / kPStages);
+        uint32_t known_k = more ? test(&bar.kv_full[sk], (n + 1) / kPStages) : 0;
         const uint64_t b = dv + static_cast<uint64_t>(warp_uniform(sv) * (kPTile >> 4));
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
@@ -410,26 +416,26 @@ __global__ void __launch_bounds__(kPThreads, 1)
               umma_f16_ts(tm + kPTmemO + t * kPD, tm + t * kPB + kk * 8, b + kk * (2048 >> 4), idesc_pv,
                           (j > 0 || kk > 0) ? 1u : 0u);
             };
-            if (kPart1 < kPB) {
-              wait(&bar.p_part[t], np[t]);
-              if (look) wait(&bar.v_ok, looks++);
-              look = false;
-              tc_fence_after();
-              if (elect_one()) {
-#pragma unroll
-                for (int kk = 0; kk < kPart1 / 16; ++kk) pv(kk);
-              }
-            }
-            wait(&bar.p_full[t], np[t]++);
+            wait(&bar.p_part[t], np[t], known_p);
             if (look) wait(&bar.v_ok, looks++);
             look = false;
             tc_fence_after();
+            const uint32_t known = test(&bar.p_full[t], np[t]);
             if (elect_one()) {
 #pragma unroll
-              for (int kk = (kPart1 < kPB ? kPart1 / 16 : 0); kk < kPB / 16; ++kk) pv(kk);
+              for (int kk = 0; kk < kPart1 / 16; ++kk) pv(kk);
+            }
+            wait(&bar.p_full[t], np[t]++, known);
+            tc_fence_after();
+            if (elect_one()) {
+#pragma unroll
+              for (int kk = kPart1 / 16; kk < kPB / 16; ++kk) pv(kk);
               if (j + 1 == w.nb[t]) umma_commit(&bar.o_full[t]);
             }
           }
+          if (more && t == 0) wait(&bar.kv_full[sk], (n + 1) / kPStages, known_k);
+          known_p = test(&bar.p_part[t ^ 1], np[t ^ 1]);
+          if (t == 1 && more) known_v = test(&bar.kv_full[(n + 2) % kPStages], (n + 2) / kPStages);
           if (j + 1 < w.nb[t]) qk(t, sk, j + 2 == w.nb[t]);
           if (t == 1) commit(&bar.kv_empty[sv]);
         }
