@@ -625,15 +625,15 @@ Q4_ROW_BYTES = _lib.RT_Q4_ROW_BYTES
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch.cuda.current_device
 _grad_enabled = torch.is_grad_enabled
-_BF16, _F16 = torch.bfloat16, torch.float16
+_BF16, _F16, _U8 = torch.bfloat16, torch.float16, torch.uint8
 _STATUS_PTR: dict = {}  # device index -> address of its status word (kept for the process's life)
 _SCALE = 128 ** -0.5
 
 
-def _status_ptr(dev) -> int:
-    ptr = _STATUS_PTR.get(dev.index)
+def _status_ptr(index: int) -> int:
+    ptr = _STATUS_PTR.get(index)
     if ptr is None:
-        ptr = _STATUS_PTR[dev.index] = _STATE.status(dev).data_ptr()
+        ptr = _STATUS_PTR[index] = _STATE.status(torch.device("cuda", index)).data_ptr()
     return ptr
 
 
@@ -659,9 +659,9 @@ def _needs_grad(*tensors) -> bool:
     return _grad_enabled() and any(t.requires_grad for t in tensors)
 
 
-def _workspace(nbytes: int, dev) -> torch.Tensor | None:
+def _workspace(nbytes: int, dev) -> torch.Tensor:
     """Scratch of one call, from the caching allocator: ordered by the call's stream, the graph's own in a capture."""
-    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    return torch.empty(nbytes, dtype=torch.uint8, device=dev)
 
 
 def _offsets(t) -> bool:
@@ -722,22 +722,24 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     Returns ``out`` ``[T, Hq, 128]``.
     """
     what = "prompt_attention"
-    q = _query(q, what)
+    if q.dim() != 3:
+        q = _query(q, what)
     if k.dim() != 3 or v.dim() != 3:
         k, v = _one_batch(k, what), _one_batch(v, what)
-    dev = q.device
+    index = q.get_device()
     t, hq, d = q.shape
-    hkv, tk, dk = k.shape
+    hkv, tk, dk = k_shape = k.shape
     dt = q.dtype
     cq, ck = cu_seqlens_q, cu_seqlens_k
     q0, q1, q2 = q.stride()
     k0, k1, k2 = ks = k.stride()
     vs = v.stride()
-    if not (q.is_cuda and k.device == dev and v.device == dev and (dt is _BF16 or dt is _F16) and k.dtype is dt
-            and v.dtype is dt and d == 128 and dk == 128 and q2 == 1 and k2 == 1 and vs[2] == 1 and k.shape == v.shape
-            and hq and hkv and hq % hkv == 0
-            and (ck is None or (cq is not None and _offsets(ck) and ck.device == dev and ck.numel() == cq.numel()))
-            and (cq is None or (_offsets(cq) and cq.device == dev))
+    if not (q.is_cuda and k.is_cuda and k.get_device() == index and v.is_cuda and v.get_device() == index
+            and (dt is _BF16 or dt is _F16) and k.dtype is dt and v.dtype is dt and d == 128 and dk == 128
+            and q2 == 1 and k2 == 1 and vs[2] == 1 and k_shape == v.shape and hq and hkv and hq % hkv == 0
+            and (ck is None or (cq is not None and _offsets(ck) and ck.get_device() == index
+                                and ck.numel() == cq.numel()))
+            and (cq is None or (_offsets(cq) and cq.get_device() == index))
             and not (_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad))):
         _refuse(what,
                 (q.is_cuda and k.is_cuda and v.is_cuda, "takes CUDA tensors (no CPU path)"),
@@ -752,9 +754,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
                 (all(x is None or _offsets(x) for x in (cq, ck)),
                  "cu_seqlens must be contiguous int32 tensors of at least two offsets"),
                 (ck is None or cq is None or ck.numel() == cq.numel(), "cu_seqlens must name the same number of sequences"))
-    index = dev.index
     if _current_device() != index:
-        with torch.cuda.device(dev):
+        with torch.cuda.device(index):
             return prompt_attention(q, k, v, cq, ck, scale, out)
     if ks == vs and t > 1 and hq > 1 and tk > 1 and hkv > 1 and q0 and q1 and k0 and k1:
         q0, q1, k0, k1 = 2 * q0, 2 * q1, 2 * k0, 2 * k1
@@ -773,12 +774,12 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         return out
     seqs = 1 if cq is None else cq.numel() - 1
     nbytes = _prompt_workspace(index, t, tk, seqs, hq, hkv)
-    ws = _workspace(nbytes, dev)
+    ws = _workspace(nbytes, q.device) if nbytes else None
     rc = _lib.load().rt_prompt_attn(q.data_ptr(), q0, q1, k.data_ptr(), v.data_ptr(), k0, k1, out.data_ptr(), o0, o1,
                                     1 if dt is _BF16 else 2, None if cq is None else cq.data_ptr(),
                                     None if ck is None else ck.data_ptr(), seqs, t, tk, hq, hkv, 128,
                                     _SCALE if scale is None else float(scale),
-                                    None if ws is None else ws.data_ptr(), nbytes, _status_ptr(dev),
+                                    None if ws is None else ws.data_ptr(), nbytes, _status_ptr(index),
                                     _raw_stream(index))
     if rc:
         _lib.check(rc, "rt_prompt_attn")
@@ -801,16 +802,20 @@ def kv_append_q4(k_cache: torch.Tensor, v_cache: torch.Tensor, k_new: torch.Tens
     what = "kv_append_q4"
     if k_new.dim() != 3 or v_new.dim() != 3:
         k_new, v_new = _one_batch(k_new, what), _one_batch(v_new, what)
-    dev = k_cache.device
-    heads, n, d = k_new.shape
-    cache_heads, cap, _ = k_cache.shape if k_cache.dim() == 3 else (-1, 0, 0)
+    index = k_cache.get_device()
+    heads, n, d = new_shape = k_new.shape
+    c_shape, c_stride = k_cache.shape, k_cache.stride()
+    cache_heads, cap, row = c_shape if len(c_shape) == 3 else (-1, 0, 0)
     s0, s1, s2 = ss = k_new.stride()
     sv = v_new.stride()
-    if not (_q4_rows(k_cache) and _q4_rows(v_cache) and k_cache.shape == v_cache.shape
-            and k_cache.stride() == v_cache.stride() and k_new.dtype is _BF16 and v_new.dtype is _BF16
-            and k_new.shape == v_new.shape and heads == cache_heads and d == 128 and s2 == 1 and sv[2] == 1
-            and v_cache.device == dev and k_new.device == dev and v_new.device == dev
-            and (offset_dev is None or (offset_dev.dtype is torch.int64 and offset_dev.device == dev))
+    if not (k_cache.is_cuda and k_cache.dtype is _U8 and v_cache.dtype is _U8 and row == 72
+            and c_stride[1:] == (72, 1) and c_shape == v_cache.shape and c_stride == v_cache.stride()
+            and k_new.dtype is _BF16 and v_new.dtype is _BF16
+            and new_shape == v_new.shape and heads == cache_heads and d == 128 and s2 == 1 and sv[2] == 1
+            and v_cache.is_cuda and v_cache.get_device() == index and k_new.is_cuda and k_new.get_device() == index
+            and v_new.is_cuda and v_new.get_device() == index
+            and (offset_dev is None or (offset_dev.dtype is torch.int64 and offset_dev.is_cuda
+                                        and offset_dev.get_device() == index))
             and not (_grad_enabled() and (k_new.requires_grad or v_new.requires_grad))):
         _refuse(what,
                 (all(x.is_cuda for x in (k_cache, v_cache, k_new, v_new)), "takes CUDA tensors (no CPU path)"),
@@ -823,9 +828,8 @@ def kv_append_q4(k_cache: torch.Tensor, v_cache: torch.Tensor, k_new: torch.Tens
                 (k_new.shape == v_new.shape and heads == cache_heads and d == 128 and s2 == 1 and sv[2] == 1,
                  "new rows must be [cache heads, n, 128] with contiguous head_dim, the same for K and V"),
                 (offset_dev is None or offset_dev.dtype == torch.int64, "offset_dev must be int64"))
-    index = dev.index
     if _current_device() != index:
-        with torch.cuda.device(dev):
+        with torch.cuda.device(index):
             return kv_append_q4(k_cache, v_cache, k_new, v_new, offset, offset_dev)
     if ss == sv and heads > 1 and n > 1 and s0 and s1:
         s0, s1 = 2 * s0, 2 * s1
@@ -835,10 +839,10 @@ def kv_append_q4(k_cache: torch.Tensor, v_cache: torch.Tensor, k_new: torch.Tens
         if sv != [s0, s1]:
             k_new, v_new, s0, s1 = k_new.contiguous(), v_new.contiguous(), n * 256, 256
     rc = _lib.load().rt_kv_append_q4(k_cache.data_ptr(), v_cache.data_ptr(),
-                                     k_cache.stride(0) if heads > 1 else cap * Q4_ROW_BYTES, k_new.data_ptr(),
+                                     c_stride[0] if heads > 1 else cap * Q4_ROW_BYTES, k_new.data_ptr(),
                                      v_new.data_ptr(), s0, s1, heads, n, d, cap, int(offset),
                                      None if offset_dev is None else offset_dev.data_ptr(),
-                                     _status_ptr(dev), _raw_stream(index))
+                                     _status_ptr(index), _raw_stream(index))
     if rc:
         _lib.check(rc, "rt_kv_append_q4")
     _count()
@@ -899,17 +903,21 @@ def tree_attention_q4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask_bi
     ``[n, Hq, 128]`` bf16.
     """
     what = "tree_attention_q4"
-    q = _query(q, what)
-    dev = q.device
+    if q.dim() != 3:
+        q = _query(q, what)
+    index = q.get_device()
     n, hq, d = q.shape
     q0, q1, q2 = q.stride()
-    hkv, cap, _ = k.shape if k.dim() == 3 else (0, 0, 0)
-    if not (_q4_rows(k) and _q4_rows(v) and q.is_cuda and q.dtype is _BF16 and d == 128 and q2 == 1
-            and k.shape == v.shape and k.stride() == v.stride() and k.device == dev and v.device == dev
-            and mask_bits.device == dev and n and hq and hkv and hq % hkv == 0
-            and mask_bits.dtype is torch.int32 and mask_bits.dim() == 2 and mask_bits.shape[0] >= n
-            and mask_bits.shape[1] * 32 >= n and not (_grad_enabled() and q.requires_grad)
-            and (prefix_len_dev is None or (prefix_len_dev.dtype is torch.int64 and prefix_len_dev.device == dev))):
+    k_shape, k_stride, m_shape = k.shape, k.stride(), mask_bits.shape
+    hkv, cap, row = k_shape if len(k_shape) == 3 else (0, 0, 0)
+    if not (q.is_cuda and q.dtype is _BF16 and d == 128 and q2 == 1 and k.dtype is _U8 and v.dtype is _U8
+            and row == 72 and k_stride[1:] == (72, 1) and k_shape == v.shape and k_stride == v.stride()
+            and k.is_cuda and k.get_device() == index and v.is_cuda and v.get_device() == index
+            and mask_bits.is_cuda and mask_bits.get_device() == index and n and hq and hkv and hq % hkv == 0
+            and mask_bits.dtype is torch.int32 and len(m_shape) == 2 and m_shape[0] >= n and m_shape[1] * 32 >= n
+            and not (_grad_enabled() and q.requires_grad)
+            and (prefix_len_dev is None or (prefix_len_dev.dtype is torch.int64 and prefix_len_dev.is_cuda
+                                            and prefix_len_dev.get_device() == index))):
         _refuse(what,
                 (q.is_cuda and k.is_cuda and v.is_cuda and mask_bits.is_cuda, "takes CUDA tensors (no CPU path)"),
                 (not _needs_grad(q), "inference-only (no gradient)"),
@@ -923,16 +931,15 @@ def tree_attention_q4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask_bi
                 (mask_bits.dtype == torch.int32 and mask_bits.dim() == 2 and mask_bits.shape[0] >= n
                  and mask_bits.shape[1] * 32 >= n, "mask_bits must be int32 [n, at least ceil(n / 32)]"),
                 (prefix_len_dev is None or prefix_len_dev.dtype == torch.int64, "prefix_len_dev must be int64"))
-    index = dev.index
     if _current_device() != index:
-        with torch.cuda.device(dev):
+        with torch.cuda.device(index):
             return tree_attention_q4(q, k, v, mask_bits, prefix_len, scale, out, num_splits, prefix_len_dev)
     words, unit = mask_bits.stride()
-    if unit != 1 or words < mask_bits.shape[1]:
+    if unit != 1 or words < m_shape[1]:
         mask_bits = mask_bits.contiguous()
-        words = mask_bits.shape[1]
-    if n > 1 and hq > 1 and q0 and q1:
-        q0, q1 = 2 * q0, 2 * q1
+        words = m_shape[1]
+    if (q0 or n == 1) and (q1 or hq == 1):
+        q0, q1 = 2 * q0 if n > 1 else 256, 2 * q1 if hq > 1 else 256
     else:
         q, q0, q1 = _rows(q)
     if out is None:
@@ -942,13 +949,13 @@ def tree_attention_q4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask_bi
         _, o0, o1 = _rows(_attn_out(out, q, what))
     prefix_len, num_splits = int(prefix_len), int(num_splits)
     nbytes = _tree_q4_workspace(index, n, hq, hkv, 128, prefix_len, num_splits)
-    ws = _workspace(nbytes, dev)
+    ws = _workspace(nbytes, q.device) if nbytes else None
     rc = _lib.load().rt_tree_attn_q4(q.data_ptr(), q0, q1, k.data_ptr(), v.data_ptr(),
-                                     k.stride(0) if hkv > 1 else cap * 72, cap, out.data_ptr(), o0, o1,
+                                     k_stride[0] if hkv > 1 else cap * 72, cap, out.data_ptr(), o0, o1,
                                      mask_bits.data_ptr(), words, n, prefix_len,
                                      None if prefix_len_dev is None else prefix_len_dev.data_ptr(), hq, hkv, 128,
                                      _SCALE if scale is None else float(scale), num_splits,
-                                     None if ws is None else ws.data_ptr(), nbytes, _status_ptr(dev),
+                                     None if ws is None else ws.data_ptr(), nbytes, _status_ptr(index),
                                      _raw_stream(index))
     if rc:
         _lib.check(rc, "rt_tree_attn_q4")
