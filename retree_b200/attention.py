@@ -200,7 +200,7 @@ def tree_attention_forward(module, query: torch.Tensor, key: torch.Tensor, value
     prefix = key.shape[2] - n if rows is None else rows.prefix_len
     timer = _Timer()
     if cu_q is not None and attention_mask is None:
-        if not causal or (rows is not None and rows.prefix_len > 0):
+        if not causal or (rows is not None and rows.prefix_len > 0) or (cu_k is None and key.shape[2] != n):
             raise RuntimeError("packed sequences run causally over keys of their own (no cached prefix)")
         timer.start()
         out = kernels.prompt_attention(query, key, value, cu_seqlens_q=cu_q, cu_seqlens_k=cu_k, scale=scaling)

@@ -241,3 +241,22 @@ def test_prefill_random_fills_a_4bit_cache(model):
     assert keys.shape == (1, 2, 200, 128) and 0.9 < float(keys.float().std()) < 1.1
     v.round(torch.from_numpy(synthetic.draft_logits(1, 15, VOCAB, amp=6.0)).to(dev).to(torch.bfloat16))
     kernels.check_device_status(dev)
+
+
+def test_packed_queries_over_earlier_keys_need_their_offsets():
+    """Without the keys' own offsets the queries' would point at the first keys of the cache."""
+    dev = cuda()
+    c = TreeKVCache(1, 2, 128, 64, device=dev)
+    c.update(_rows(1, 2, 4, dev), _rows(2, 2, 4, dev), 0)
+    key, value = c.update(_rows(3, 2, 6, dev), _rows(4, 2, 6, dev), 0)
+    cu = torch.tensor([0, 6], dtype=torch.int32, device=dev)
+    q = _rows(5, 8, 6, dev)
+    with pytest.raises(RuntimeError, match="packed"):
+        attention.tree_attention_forward(_Module(), q, key, value, None, scaling=0.1, cu_seq_lens_q=cu)
+    cu_k = torch.tensor([0, 10], dtype=torch.int32, device=dev)
+    out, _ = attention.tree_attention_forward(_Module(), q, key, value, None, scaling=0.1, cu_seq_lens_q=cu,
+                                              cu_seq_lens_k=cu_k)
+    with attention.prompt_kernel():
+        one, _ = attention.tree_attention_forward(_Module(), q, key, value, None, scaling=0.1)
+    kernels.check_device_status(dev)
+    assert torch.equal(out, one)
