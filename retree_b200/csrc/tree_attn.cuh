@@ -33,6 +33,9 @@ struct AttnParams {
   int64_t kv_head_stride, kv_row_stride;
   // 4-bit cache: rows of a head; a prefix length that does not fit writes nothing (0: not checked)
   int64_t capacity;
+  // with tail_splits > 0 the rows from tail_row on have so many splits and those before
+  // them row_splits; num_splits is the larger count
+  int row_splits, tail_splits, tail_row;
 };
 
 __device__ __forceinline__ int64_t key_count(const AttnParams& p) {
@@ -226,9 +229,11 @@ static __global__ void __launch_bounds__(128) attn_combine_kernel(const AttnPara
   const int rows = p.n * p.group;
   if (p.capacity > 0 && (key_count(p) < p.n || key_count(p) > p.capacity)) return;
   const int64_t rows_ws = static_cast<int64_t>(p.tiles) * kBM;
-  const int S = p.num_splits;
+  auto splits_of = [&](int R) {
+    return p.tail_splits == 0 ? p.num_splits : R >= p.tail_row ? p.tail_splits : p.row_splits;
+  };
   const float2 none = make_float2(-INFINITY, 0.f);
-  if (S <= kFastSplits) {
+  if (p.num_splits <= kFastSplits) {
     // Two warps per (kv head, row), one per 64-dim half, lane owns 2 dims.
     // Every load of the row is independent of the others, so all of them --
     // the splits' partial rows and (max, sum) pairs -- go out at once: one
@@ -238,7 +243,7 @@ static __global__ void __launch_bounds__(128) attn_combine_kernel(const AttnPara
     const int gw = (blockIdx.x * blockDim.x + threadIdx.x) >> 5;
     if (gw >= 2 * p.num_kv_heads * rows) return;
     const int half = gw & 1, pair = gw >> 1;
-    const int kvh = pair / rows, R = pair - kvh * rows;
+    const int kvh = pair / rows, R = pair - kvh * rows, S = splits_of(R);
     auto slot = [&](int s) { return (static_cast<int64_t>(s) * p.num_kv_heads + kvh) * rows_ws + R; };
     const int d0 = half * 64 + lane * 2;
     float2 o[kFastSplits];
@@ -273,7 +278,7 @@ static __global__ void __launch_bounds__(128) attn_combine_kernel(const AttnPara
   }
   const int gw = (blockIdx.x * blockDim.x + threadIdx.x) >> 5;
   if (gw >= p.num_kv_heads * rows) return;
-  const int kvh = gw / rows, R = gw - kvh * rows;
+  const int kvh = gw / rows, R = gw - kvh * rows, S = splits_of(R);
   auto slot = [&](int s) { return (static_cast<int64_t>(s) * p.num_kv_heads + kvh) * rows_ws + R; };
   // lane s holds split s's (max, sum); one load per lane instead of a serial walk
   const float2 first = lane < S ? p.ws_ml[slot(lane)] : none;

@@ -498,17 +498,20 @@ __device__ __forceinline__ void q4_decode_row(const Q4Packed& x, uint32_t tile, 
 }
 
 __global__ void __launch_bounds__(kQtThreads, 1)
-    tree_attn_q4_tile_kernel(const __grid_constant__ CUtensorMap tmap_q, const AttnParams p, const int tok, const int heavy,
-                             const int tail) {
+    tree_attn_q4_tile_kernel(const __grid_constant__ CUtensorMap tmap_q, const AttnParams p, const int tok, const int pairs,
+                             const int heavy) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   Q4Bars& bar = *reinterpret_cast<Q4Bars*>(smem + kQtOffBar);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int split = blockIdx.x, kvh = blockIdx.y, G = p.group;
-  const int node0 = blockIdx.z * 2 * tok;               // first node of tile 0
-  const int tiles = node0 + tok < p.n ? 2 : 1;
-  const bool dual = tiles == 1;                         // two chains over one tile's keys
+  // CTAs of two tiles (`pairs` a kv head and split), then those of a last single one
+  const int two = pairs * heavy * p.num_kv_heads, G = p.group;
+  const bool dual = static_cast<int>(blockIdx.x) >= two;  // two chains over one tile's keys
+  const int tiles = dual ? 1 : 2, mine = dual ? p.tail_splits : heavy;
+  const int rank = blockIdx.x - (dual ? two : 0), split = rank % mine;
+  const int kvh = rank / mine % p.num_kv_heads;
+  const int node0 = (dual ? pairs : rank / (mine * p.num_kv_heads)) * 2 * tok;  // first node of tile 0
   const int ahead = dual ? 2 : 1;
   if (warp == 8 && lane == 0) {
     prefetch_tmap(&tmap_q);
@@ -544,8 +547,7 @@ __global__ void __launch_bounds__(kQtThreads, 1)
   const bool inside = L >= 0 && total <= p.capacity;    // the same in every thread of the launch
   if (!inside && tid == 0) set_status(p.status, RT_DEV_BAD_INDEX);
   int64_t b0 = 0, b1 = 0;
-  const int mine = dual ? tail : heavy;                 // this tile's splits; the launch has the larger count
-  if (inside && split < mine) split_range(total, split, mine, kQtKeys, b0, b1);
+  if (inside) split_range(total, split, mine, kQtKeys, b0, b1);
   const int nb = static_cast<int>(b1 - b0);
 
   if (warp >= 8) {
@@ -844,7 +846,7 @@ struct Q4Plan {
   bool small;  // the mma.sync path
   int splits;  // of the keys, the most any tile has
   bool merge;
-  int heavy, tail;  // of the two-tile CTAs, of a last single-tile one
+  int heavy, tail;  // of the tiles of two-tile CTAs, of a last single one
 };
 
 // Clusters of `c` CTAs of `kernel` that fit on the GPU at once (0 when the query
@@ -895,35 +897,56 @@ static int launch_q4_small(dim3 grid, dim3 cluster, cudaStream_t s, const AttnPa
       launch_ex_cluster(tree_attn_q4_small_kernel<NT>, grid, dim3(kQsThreads), kQsSmem, s, cluster, p));
 }
 
-// Splits of a launch of two-tile CTAs ("heavy") and, where the last nodes fill one
-// tile only (a root and a power of two of others, say), single-tile ones ("light",
-// started last): the counts with the shortest estimated time on 148 SMs, from a
-// block's cost in either (2.3 and 1.24 us) and a CTA's fixed cost (6 us) as
-// measured at 32768 rows.  257 nodes (4 heavy CTAs and a light one a kv head): 204 us
-// with 3 splits of both, 172 with 4, 179 with 8, 161 with 4 of the heavy and 5 of the light ones.
-static void tile_splits(int n, int tok, int hkv, int64_t blocks, int& splits, int& tail) {
-  const int rest = n % (2 * tok);
-  const int heavy = hkv * (n / (2 * tok) + (rest > tok)), light = hkv * (rest > 0 && rest <= tok);
-  const int most = static_cast<int>(std::min<int64_t>(32, blocks));
-  auto cost = [&](double block, int s) { return block * static_cast<double>((blocks + s - 1) / s) + 6; };
-  double best = 1e30;
-  for (int s = 1; s <= most; ++s) {
-    const double h = cost(2.3, s);
-    const int H = heavy * s, rounds = (H + 147) / 148, idle = rounds * 148 - H;
-    if (rounds * h >= best) continue;
-    for (int sl = 1; sl <= (light > 0 ? most : 1); ++sl) {
-      // the light ones take the SMs as they come free
-      const double l = cost(1.24, sl);
-      double t_idle = (rounds - 1) * h, t_busy = rounds * h;
-      for (int left = light * sl; left > 0;) {
-        const bool on_idle = idle > 0 && t_idle <= t_busy;
-        left -= on_idle ? idle : 148 - idle;
-        (on_idle ? t_idle : t_busy) += l;
-      }
-      const double t = std::max(t_idle, t_busy);
-      if (t < best) best = t, splits = s, tail = light > 0 ? sl : s;
-    }
+// A launch of two-tile CTAs ("heavy") may end in a single-tile one a kv head
+// ("light", started last): a root and a power of two of others leave just that.
+// A block costs them 2.3 and 1.24 us (measured at 32768 rows), a CTA 6 us besides.
+struct Q4Load {
+  int heavy, light;  // CTAs for each split
+};
+constexpr double kQtHeavyBlock = 2.3, kQtLightBlock = 1.24, kQtCta = 6;
+
+// Time on 148 SMs of heavy CTAs of `h` and light ones of `l`, which take the SMs as they come free.
+static double q4_time(int heavy, double h, int light, double l) {
+  const int rounds = (heavy + 147) / 148, idle = rounds * 148 - heavy;
+  double t_idle = (rounds - 1) * h, t_busy = rounds * h;
+  while (light > 0) {
+    const bool on_idle = idle > 0 && t_idle <= t_busy;
+    light -= on_idle ? idle : 148 - idle;
+    (on_idle ? t_idle : t_busy) += l;
   }
+  return std::max(t_idle, t_busy);
+}
+
+// Splits of the light CTAs beside heavy ones of `s` splits: the fewest that come within 2 % of
+// the shortest time over many blocks (no use of the prefix length: launches that are given
+// one count split alike).  257 nodes over 32768 rows: 172 us with 4 splits of both, 161 with
+// 4 of the heavy and 5 of the light ones.
+static int tail_splits(const Q4Load& w, int s) {
+  if (w.light == 0 || w.heavy == 0 || s == 1) return s;
+  double t[33], best = 1e30;
+  for (int i = 1; i <= 32; ++i) {
+    t[i] = q4_time(w.heavy * s, kQtHeavyBlock / s, w.light * i, kQtLightBlock / i);
+    best = std::min(best, t[i]);
+  }
+  int tail = 1;
+  while (t[tail] > 1.02 * best) ++tail;
+  return tail;
+}
+
+// The split count with the shortest estimated time.  257 nodes over 32768 rows: 4 (161 us);
+// 205 with 3, 179 with 8 (of both kinds).
+static int tile_splits(const Q4Load& w, int64_t blocks) {
+  int best_s = 1;
+  double best = 1e30;
+  auto cost = [&](double block, int s) { return block * static_cast<double>((blocks + s - 1) / s) + kQtCta; };
+  for (int s = 1; s <= 32 && s <= blocks; ++s) {
+    const double h = cost(kQtHeavyBlock, s);
+    if ((w.heavy * s + 147) / 148 * h >= best) continue;
+    const int tail = tail_splits(w, s);
+    const double t = q4_time(w.heavy * s, h, w.light * tail, cost(kQtLightBlock, tail));
+    if (t < best) best = t, best_s = s;
+  }
+  return best_s;
 }
 
 static Q4Plan q4_plan(int n, int G, int hkv, int64_t prefix_len, int num_splits) {
@@ -939,14 +962,16 @@ static Q4Plan q4_plan(int n, int G, int hkv, int64_t prefix_len, int num_splits)
   const int64_t blocks = (prefix_len + n + kQtKeys - 1) / kQtKeys;
   const int tok = kBM / G;
   int64_t want = num_splits;
-  if (want <= 0 && n > tok) {
-    int heavy = 1, tail = 1;
-    tile_splits(n, tok, hkv, blocks, heavy, tail);
+  if (n > tok) {
+    const int rest = n % (2 * tok);
+    const Q4Load w = {hkv * (n / (2 * tok) + (rest > tok)), hkv * (rest > 0 && rest <= tok)};
+    const int heavy = want > 0 ? static_cast<int>(std::min<int64_t>(want, 256)) : tile_splits(w, blocks);
+    const int tail = tail_splits(w, heavy);
     return {false, std::max(heavy, tail), false, heavy, tail};
   }
   if (want <= 0) want = std::min<int64_t>(std::max<int64_t>(1, 148 / hkv), blocks);
   want = std::min<int64_t>(want, 256);
-  if (n <= tok && want > 1) {
+  if (want > 1) {
     // one tile: its splits merge in a cluster when it takes all of them, or (where
     // the count is ours to choose) leaves each CTA three blocks at most
     int c = static_cast<int>(std::min<int64_t>(want, kMaxMerge));
@@ -965,7 +990,7 @@ using namespace rt;
 
 extern "C" int rt_tree_attn_q4_default_splits(int n, int num_q_heads, int num_kv_heads, int64_t prefix_len) {
   if (n <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads || prefix_len < 0) return 1;
-  return q4_plan(n, num_q_heads / num_kv_heads, num_kv_heads, prefix_len, 0).splits;
+  return q4_plan(n, num_q_heads / num_kv_heads, num_kv_heads, prefix_len, 0).heavy;
 }
 
 extern "C" size_t rt_tree_attn_q4_workspace_size(int n, int num_q_heads, int num_kv_heads, int head_dim,
@@ -1017,6 +1042,7 @@ extern "C" int rt_tree_attn_q4(const void* q, int64_t q_tok_stride, int64_t q_he
   p.num_kv_heads = num_kv_heads;
   p.tiles = tiles_for(n, G);
   p.num_splits = pl.splits;
+  p.row_splits = pl.heavy;
   p.merge = pl.merge ? pl.splits : 1;
   // (never 0: a hidden score is -inf and stays so; scores times 2^-126 are 0 in the sum)
   p.scale_log2 = std::max(scale * 1.4426950408889634f, 1.17549435e-38f);
@@ -1043,12 +1069,16 @@ extern "C" int rt_tree_attn_q4(const void* q, int64_t q_tok_stride, int64_t q_he
     CUtensorMap tq;
     rc = make_q4_query_tmap(&tq, q, q_tok_stride, q_head_stride, n, num_q_heads, G, tok);
     if (rc != RT_OK) return rc;
-    const dim3 grid(pl.splits, num_kv_heads, (n + 2 * tok - 1) / (2 * tok));
+    const int pairs = n / (2 * tok) + (n % (2 * tok) > tok);
+    const bool last = n > pairs * 2 * tok;
+    p.tail_splits = last ? pl.tail : 0;
+    p.tail_row = pairs * 2 * tok * G;
+    const dim3 grid(num_kv_heads * (pairs * pl.heavy + p.tail_splits));
     set_smem_limit(tree_attn_q4_tile_kernel, kQtSmem);
     if (pl.merge && pl.splits > 8)
       cudaFuncSetAttribute(tree_attn_q4_tile_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     rc = record_cuda(launch_ex_cluster(tree_attn_q4_tile_kernel, grid, dim3(kQtThreads), kQtSmem, s,
-                                       dim3(pl.merge ? pl.splits : 1, 1, 1), tq, p, tok, pl.heavy, pl.tail));
+                                       dim3(pl.merge ? pl.splits : 1, 1, 1), tq, p, tok, pairs, pl.heavy));
   }
   if (rc != RT_OK || pl.merge || pl.splits == 1) return rc;
   const int warps = num_kv_heads * n * G * (pl.splits <= kFastSplits ? 2 : 1);

@@ -896,7 +896,7 @@ def tree_attention_q4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask_bi
     """``tree_attention`` over a 4-bit cache.
 
     q: bf16 ``[n, Hq, 128]`` or HF's ``[1, Hq, n, 128]``; k, v: uint8 caches
-    ``[Hkv, capacity, 72]`` of which rows ``[0, prefix_len + n)`` are used;
+    ``[Hkv, capacity, 72]`` (an even capacity) of which rows ``[0, prefix_len + n)`` are used;
     mask_bits: int32 ``[n, W]`` ancestor bits of the tree block (one bit, set,
     for a single token).  ``prefix_len_dev`` (int64[1]) supplies the prefix
     length at run time; ``prefix_len`` is then its upper bound.  Returns ``out``
@@ -911,7 +911,7 @@ def tree_attention_q4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask_bi
     k_shape, k_stride, m_shape = k.shape, k.stride(), mask_bits.shape
     hkv, cap, row = k_shape if len(k_shape) == 3 else (0, 0, 0)
     if not (q.is_cuda and q.dtype is _BF16 and d == 128 and q2 == 1 and k.dtype is _U8 and v.dtype is _U8
-            and row == 72 and k_stride[1:] == (72, 1) and k_shape == v.shape and k_stride == v.stride()
+            and row == 72 and not cap & 1 and k_stride[1:] == (72, 1) and k_shape == v.shape and k_stride == v.stride()
             and k.is_cuda and k.get_device() == index and v.is_cuda and v.get_device() == index
             and mask_bits.is_cuda and mask_bits.get_device() == index and n and hq and hkv and hq % hkv == 0
             and mask_bits.dtype is torch.int32 and len(m_shape) == 2 and m_shape[0] >= n and m_shape[1] * 32 >= n
@@ -925,6 +925,7 @@ def tree_attention_q4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask_bi
                 (d == 128 and q.stride(2) == 1, "head_dim must be 128 and contiguous"),
                 (_q4_rows(k) and _q4_rows(v),
                  f"caches must be uint8 [heads, capacity, {Q4_ROW_BYTES}] with contiguous rows"),
+                (not cap & 1, "the caches' capacity must be even"),
                 (k.shape == v.shape and k.stride() == v.stride(), "K and V caches must share shape and strides"),
                 (n and hq and hkv and hq % hkv == 0,
                  "at least one node, and key heads that divide the query heads"),

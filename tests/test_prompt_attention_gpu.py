@@ -272,3 +272,23 @@ def test_refusals():
         kernels.prompt_attention(flat[4:].view(20, 8, 128), k, v)
     assert kernels.prompt_attention(q[:0], k, v).shape == (0, 8, 128)
     assert kernels.prompt_attention(q, k[:, :0], v[:, :0]).abs().sum() == 0
+
+
+def test_calls_on_two_streams_at_once():
+    """Launches with and without key splits (their workspace) side by side: each as when it runs alone."""
+    dev = cuda()
+    sets = []
+    for t, tk in ((64, 9000), (300, 300), (1500, 2100)):
+        args = make(t, t, tk, 8, 2, torch.bfloat16, dev)
+        offs = (cu([t], dev), cu([tk], dev))
+        sets.append((args, offs, kernels.prompt_attention(*args, *offs)))
+    streams = [torch.cuda.Stream(dev) for _ in range(2)]
+    outs = [[], []]
+    torch.cuda.synchronize(dev)
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                outs[i] += [(kernels.prompt_attention(*args, *offs), want) for args, offs, want in sets[::1 - 2 * i]]
+    torch.cuda.synchronize(dev)
+    kernels.check_device_status(dev)
+    assert all(torch.equal(got, want) for o in outs for got, want in o)

@@ -318,3 +318,48 @@ def test_attention_refusals():
     for scale in (-0.1, float("nan"), float("inf")):
         with pytest.raises(RuntimeError, match="invalid argument"):
             kernels.tree_attention_q4(q, slab[0], slab[1], bits, 10, scale=scale)
+
+
+def test_an_odd_capacity_is_refused():
+    dev = cuda()
+    slab = torch.zeros((2, 1, 41, 72), dtype=torch.uint8, device=dev)
+    bits = bits_tensor(np.ones((1, 1), bool), dev)
+    with pytest.raises(RuntimeError, match="even"):
+        kernels.tree_attention_q4(rows(1, dev, 1, 4), slab[0], slab[1], bits, 10)
+
+
+@pytest.mark.parametrize("n,prefix", [(1, 3000), (17, 3000), (33, 9000), (65, 4096), (129, 3000), (257, 2075)])
+def test_a_given_split_count_splits_like_the_one_picked(n, prefix):
+    """One launch sized by its prefix, one given that launch's count and sized for the capacity: the same bits."""
+    dev = cuda()
+    _, vis = random_tree(n, n - 1)
+    slab = caches(n, dev, 8, prefix + n, extra=4000)
+    q, bits = rows(n, dev, n, 32), bits_tensor(vis, dev)
+    count = kernels.default_splits_q4(n, 32, 8, prefix)
+    a = kernels.tree_attention_q4(q, slab[0], slab[1], bits, prefix, num_splits=count)
+    b = kernels.tree_attention_q4(q, slab[0], slab[1], bits, slab.shape[2] - n, num_splits=count,
+                                  prefix_len_dev=torch.tensor([prefix], device=dev))
+    kernels.check_device_status(dev)
+    assert torch.equal(a, b)
+    check(a, q, slab, prefix, vis)
+
+
+def test_calls_on_two_streams_at_once():
+    """Launches with workspaces, clusters and neither, side by side: each as when it runs alone."""
+    dev = cuda()
+    sets = []
+    for n, prefix in ((1, 3000), (17, 6000), (40, 2000), (129, 5000)):
+        _, vis = random_tree(n, n - 1)
+        slab = caches(n, dev, 8, prefix + n)
+        args = (rows(n, dev, n, 32), slab[0], slab[1], bits_tensor(vis, dev), prefix)
+        sets.append((args, kernels.tree_attention_q4(*args)))
+    streams = [torch.cuda.Stream(dev) for _ in range(2)]
+    outs = [[], []]
+    torch.cuda.synchronize(dev)
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                outs[i] += [(kernels.tree_attention_q4(*args), want) for args, want in sets[::1 - 2 * i]]
+    torch.cuda.synchronize(dev)
+    kernels.check_device_status(dev)
+    assert all(torch.equal(got, want) for o in outs for got, want in o)
