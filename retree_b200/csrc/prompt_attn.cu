@@ -528,7 +528,7 @@ __global__ void __launch_bounds__(kPThreads, 1)
         mbar_arrive_warp(&bar.p_full[t]);
       }
       const int64_t row = static_cast<int64_t>(w.q0 + tok), head = w.g * p.group + rh;
-      char* dst = valid ? p.out + row * p.out_tok_stride + head * p.out_head_stride : nullptr;
+      char* dst = p.out + row * p.out_tok_stride + head * p.out_head_stride;
       const int64_t slot = (static_cast<int64_t>(w.split) * p.total_q + row) * p.hq + head;
       if (nb == 0) {
         if (valid && p.splits > 1) p.ws_ml[slot] = make_float2(-INFINITY, 0.f);
@@ -554,29 +554,10 @@ __global__ void __launch_bounds__(kPThreads, 1)
         if (poison && valid)
           add_not_finite<T>(p.v + w.g * p.kv_head_stride + w.k0 * p.kv_row_stride + c * 64, p.kv_row_stride,
                             (w.jb + w.jm) * kPB, min(lim, (w.jb + nb) * kPB), x);
-        if (p.splits == 1) {
-          // through shared memory, so that four lanes write a row's 64 bytes together
-          // (a lane a row would touch 32 rows with every store)
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            sts128(stage + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4),
-                   make_uint4(pack2<T>(x[q * 8], x[q * 8 + 1]), pack2<T>(x[q * 8 + 2], x[q * 8 + 3]),
-                              pack2<T>(x[q * 8 + 4], x[q * 8 + 5]), pack2<T>(x[q * 8 + 6], x[q * 8 + 7])));
-          __syncwarp();
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int from = q * 8 + (lane >> 2), ch = lane & 3;
-            const uint4 v = lds128(stage + from * 64 + ((ch ^ ((from >> 1) & 3)) << 4));
-            const uint64_t to_row = __shfl_sync(0xFFFFFFFFu, reinterpret_cast<uint64_t>(dst), from);
-            if (to_row != 0) *reinterpret_cast<uint4*>(to_row + c * 64 + ch * 16) = v;
-          }
-          __syncwarp();
-        } else if (valid) {
-#pragma unroll
-          for (int q = 0; q < 8; ++q)
-            *reinterpret_cast<float4*>(p.ws_o + slot * kPD + c * 32 + q * 4) =
-                make_float4(x[q * 4], x[q * 4 + 1], x[q * 4 + 2], x[q * 4 + 3]);
-        }
+        if (p.splits == 1)
+          store_row32<T>(stage, x, valid ? reinterpret_cast<uint64_t>(dst + c * 64) : 0);
+        else
+          store_row32<float>(stage, x, valid ? reinterpret_cast<uint64_t>(p.ws_o + slot * kPD + c * 32) : 0);
       }
       // (a NaN weight wins the merge)
       if (valid && p.splits > 1) p.ws_ml[slot] = none ? make_float2(-INFINITY, 0.f) : make_float2(l == l ? m : INFINITY, l);

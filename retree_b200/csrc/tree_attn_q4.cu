@@ -774,6 +774,9 @@ __global__ void __launch_bounds__(kQtThreads, 1)
     } else if (inside && warp_live && !__any_sync(0xFFFFFFFFu, *abort_flag)) {
       tc_fence_after();
       const float inv = l == 0.f ? 0.f : 1.f / l;
+      const uint32_t stage = smem_u32(smem) + kQtOffQ + (dual ? warp : t * 8 + (warp & 3)) * 4096;  // (Q is done with)
+      char* row = p.num_splits > 1 ? reinterpret_cast<char*>(p.ws_o + slot * kHD)
+                                   : p.out + node * p.out_tok_stride + h * p.out_head_stride;
       // one chain: all four column groups of the tile's O; two: half of them, of both O
 #pragma unroll 1
       for (int c = dual ? 2 * t : 0; c < (dual ? 2 * t + 2 : 4); ++c) {
@@ -789,22 +792,12 @@ __global__ void __launch_bounds__(kQtThreads, 1)
 #pragma unroll
           for (int i = 0; i < 32; ++i) x[i] = w1 == 0.f ? x[i] : fmaf(w1, __uint_as_float(o[i]), x[i]);
         }
-        if (!valid) continue;
         if (p.num_splits == 1) {
-          char* dst = p.out + node * p.out_tok_stride + h * p.out_head_stride + c * 64;
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint32_t w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              w[i] = l == 0.f ? 0u : pack_bf16x2(x[q * 8 + 2 * i] * inv, x[q * 8 + 2 * i + 1] * inv);
-            *reinterpret_cast<uint4*>(dst + q * 16) = make_uint4(w[0], w[1], w[2], w[3]);
-          }
+          for (int i = 0; i < 32; ++i) x[i] = l == 0.f ? 0.f : x[i] * inv;
+          store_row32<__nv_bfloat16>(stage, x, valid ? reinterpret_cast<uint64_t>(row + c * 64) : 0);
         } else {
-#pragma unroll
-          for (int q = 0; q < 8; ++q)
-            *reinterpret_cast<float4*>(p.ws_o + slot * kHD + c * 32 + q * 4) =
-                make_float4(x[q * 4], x[q * 4 + 1], x[q * 4 + 2], x[q * 4 + 3]);
+          store_row32<float>(stage, x, valid ? reinterpret_cast<uint64_t>(row + c * 128) : 0);
         }
       }
       if (valid && p.num_splits > 1 && (t == 0 || !dual)) p.ws_ml[slot] = make_float2(m, l);
