@@ -253,10 +253,7 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
       : "memory");
 }
 
-// One lane of a converged warp.  The MMA warps run their loops with all lanes and
-// issue under this: operands that the compiler knows to be the same in every
-// lane (warp_uniform) go straight into uniform registers, where an operand of a
-// lane-0 branch costs a loop over the lanes per instruction.
+// One lane of a converged warp.
 __device__ __forceinline__ bool elect_one() {
   uint32_t p;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(p));
@@ -265,6 +262,45 @@ __device__ __forceinline__ bool elect_one() {
 template <typename V>
 __device__ __forceinline__ V warp_uniform(V x) {
   return __shfl_sync(0xFFFFFFFFu, x, 0);
+}
+// The same for a number below 4, by votes: a shuffle queues behind the exponentials of
+// the warps beside it.
+__device__ __forceinline__ int warp_uniform2(int x) {
+  return (__any_sync(0xFFFFFFFFu, x & 1) ? 1 : 0) + (__any_sync(0xFFFFFFFFu, x & 2) ? 2 : 0);
+}
+
+// Products issued by a whole converged warp, of which one lane (`me`, elect_one)
+// acts: the operands of tcgen05.mma are uniform registers, and without a branch
+// the compiler computes them there.  Eight products took 418 cycles to issue in a
+// branch of the elected lane, 187 in this form (descriptors by their low words,
+// `hi` the common high one); the tensor core runs them in 512.
+__device__ __forceinline__ void umma_f16_if(bool me, uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t hi,
+                                            uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\t"
+      "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(static_cast<uint32_t>(accumulate)),
+      "r"(static_cast<uint32_t>(me))
+      : "memory");
+}
+__device__ __forceinline__ void umma_f16_ts_if(bool me, uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t hi,
+                                               uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 b;\n\tmov.b64 b, {%2, %3};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "r"(b_lo), "r"(hi), "r"(idesc), "r"(static_cast<uint32_t>(accumulate)),
+      "r"(static_cast<uint32_t>(me))
+      : "memory");
+}
+__device__ __forceinline__ void umma_commit_if(bool me, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+      "r"(static_cast<uint32_t>(me))
+      : "memory");
 }
 
 // Arrive on `bar` once every tcgen05 op issued so far by this thread completes.

@@ -357,10 +357,14 @@ __global__ void __launch_bounds__(kPThreads, 1)
     constexpr uint32_t kFmt = std::is_same_v<T, __half> ? (1u << 7 | 1u << 10) : 0u;  // clears the bf16 format bits
     constexpr uint32_t idesc_qk = idesc_bf16_f32(kPB, kPB, false, false) & ~kFmt;
     constexpr uint32_t idesc_pv = idesc_bf16_f32(kPB, kPD, false, true) & ~kFmt;
+    const bool me = elect_one();
     const uint32_t tm = warp_uniform(tmem);
-    const uint64_t dq = warp_uniform(smem_desc_sw128(smem_u32(smem + kPOffQ), 16, 1024));
-    const uint64_t dk = warp_uniform(smem_desc_sw128(smem_u32(smem + kPOffKV), 16, 1024));
-    const uint64_t dv = warp_uniform(smem_desc_sw128(smem_u32(smem + kPOffKV), kPHalf, 1024));
+    // (descriptors: the low words; Q, K and V differ in the high one)
+    const uint64_t desc_q = smem_desc_sw128(smem_u32(smem + kPOffQ), 16, 1024);
+    const uint64_t desc_v = smem_desc_sw128(smem_u32(smem + kPOffKV), kPHalf, 1024);
+    const uint32_t dq = warp_uniform(static_cast<uint32_t>(desc_q)), hi_qk = warp_uniform(static_cast<uint32_t>(desc_q >> 32));
+    const uint32_t dk = dq + ((kPOffKV - kPOffQ) >> 4);
+    const uint32_t dv = warp_uniform(static_cast<uint32_t>(desc_v)), hi_v = warp_uniform(static_cast<uint32_t>(desc_v >> 32));
     int n = 0;  // ring loads consumed
     int nq[2] = {0, 0}, np[2] = {0, 0};
     uint32_t looks = 0;  // V blocks handed to warp 10
@@ -370,24 +374,19 @@ __global__ void __launch_bounds__(kPThreads, 1)
     auto test = [](uint64_t* b, uint32_t ph) { return mbar_test(b, ph & 1); };
     // S_t = Q_t K^T of the block in `stage`; the last one of an item frees Q_t
     auto qk = [&](int t, int stage, bool last) {
-      const uint64_t b = dk + static_cast<uint64_t>(warp_uniform(stage) * (kPTile >> 4));
-      if (elect_one()) {
+      const uint32_t a = dq + t * (kPTile >> 4), b = dk + stage * (kPTile >> 4);
 #pragma unroll
-        for (int kk = 0; kk < kPD / 16; ++kk) {
-          const uint32_t off = ((kk >> 2) * kPHalf + (kk & 3) * 32) >> 4;
-          umma_f16(tm + t * kPB, dq + t * (kPTile >> 4) + off, b + off, idesc_qk, kk > 0);
-        }
-        umma_commit(&bar.s_full[t]);
-        if (last) umma_commit(&bar.q_empty[t]);
+      for (int kk = 0; kk < kPD / 16; ++kk) {
+        const uint32_t off = ((kk >> 2) * kPHalf + (kk & 3) * 32) >> 4;
+        umma_f16_if(me, tm + t * kPB, a + off, b + off, hi_qk, idesc_qk, kk > 0);
       }
-    };
-    auto commit = [&](uint64_t* b) {
-      if (elect_one()) umma_commit(b);
+      umma_commit_if(me, &bar.s_full[t]);
+      umma_commit_if(me && last, &bar.q_empty[t]);
     };
     for (int it = 0; prompt_next<true>(p, bar, tab, ord, it, w); ++it) {
       const int nb = max(w.nb[0], w.nb[1]);
       if (nb == 0) continue;
-      const int s = n % kPStages;
+      const int s = warp_uniform2(n % kPStages);
       wait(&bar.kv_full[s], n / kPStages);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
@@ -396,58 +395,52 @@ __global__ void __launch_bounds__(kPThreads, 1)
         tc_fence_after();
         qk(t, s, w.nb[t] == 1);
       }
-      commit(&bar.kv_empty[s]);
+      umma_commit_if(me, &bar.kv_empty[s]);
       ++n;
       // Each wait's barrier is asked some products ahead (`known`), so that the answer
       // of one that is there does not hold up the tensor core.
       uint32_t known_v = 0, known_p = 0;
       for (int j = 0; j < nb; ++j) {
-        const int sv = n % kPStages, sk = (n + 1) % kPStages;
+        const int sv = warp_uniform2(n % kPStages), sk = (sv + 1) % kPStages;
         const bool more = j + 1 < nb;
         bool look = j >= w.jm;
         wait(&bar.kv_full[sv], n / kPStages, known_v);
-        if (look && elect_one()) mbar_arrive(&bar.v_look);
+        if (look && me) mbar_arrive(&bar.v_look);
         uint32_t known_k = more ? test(&bar.kv_full[sk], (n + 1) / kPStages) : 0;
-        const uint64_t b = dv + static_cast<uint64_t>(warp_uniform(sv) * (kPTile >> 4));
+        const uint32_t b = dv + sv * (kPTile >> 4);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           if (j < w.nb[t]) {
             auto pv = [&](int kk) {
-              umma_f16_ts(tm + kPTmemO + t * kPD, tm + t * kPB + kk * 8, b + kk * (2048 >> 4), idesc_pv,
-                          (j > 0 || kk > 0) ? 1u : 0u);
+              umma_f16_ts_if(me, tm + kPTmemO + t * kPD, tm + t * kPB + kk * 8, b + kk * (2048 >> 4), hi_v, idesc_pv,
+                             j > 0 || kk > 0);
             };
             wait(&bar.p_part[t], np[t], known_p);
             if (look) wait(&bar.v_ok, looks++);
             look = false;
             tc_fence_after();
             const uint32_t known = test(&bar.p_full[t], np[t]);
-            if (elect_one()) {
 #pragma unroll
-              for (int kk = 0; kk < kPart1 / 16; ++kk) pv(kk);
-            }
+            for (int kk = 0; kk < kPart1 / 16; ++kk) pv(kk);
             wait(&bar.p_full[t], np[t]++, known);
             tc_fence_after();
-            if (elect_one()) {
 #pragma unroll
-              for (int kk = kPart1 / 16; kk < kPB / 16; ++kk) pv(kk);
-              if (j + 1 == w.nb[t]) umma_commit(&bar.o_full[t]);
-            }
+            for (int kk = kPart1 / 16; kk < kPB / 16; ++kk) pv(kk);
+            umma_commit_if(me && j + 1 == w.nb[t], &bar.o_full[t]);
           }
           if (more && t == 0) wait(&bar.kv_full[sk], (n + 1) / kPStages, known_k);
           known_p = test(&bar.p_part[t ^ 1], np[t ^ 1]);
-          if (t == 1 && more) known_v = test(&bar.kv_full[(n + 2) % kPStages], (n + 2) / kPStages);
+          if (t == 1 && more) known_v = test(&bar.kv_full[(sv + 2) % kPStages], (n + 2) / kPStages);
           if (j + 1 < w.nb[t]) qk(t, sk, j + 2 == w.nb[t]);
-          if (t == 1) commit(&bar.kv_empty[sv]);
+          if (t == 1) umma_commit_if(me, &bar.kv_empty[sv]);
         }
-        if (more) commit(&bar.kv_empty[sk]);
+        umma_commit_if(me && more, &bar.kv_empty[sk]);
         n += more ? 2 : 1;
       }
     }
     // all issued MMAs complete before TMEM is released
-    if (elect_one()) {
-      umma_commit(&bar.fin);
-      mbar_wait_drain(&bar.fin, 0);
-    }
+    umma_commit_if(me, &bar.fin);
+    if (me) mbar_wait_drain(&bar.fin, 0);
     __syncwarp();
   } else if (warp == 10) {
     // ---------------- V blocks that are partly hidden: values that are not finite ----------------
