@@ -566,47 +566,43 @@ __global__ void __launch_bounds__(kQtThreads, 1)
       __syncwarp();
       constexpr uint32_t idesc_qk = idesc_bf16_f32(kBM, kQtKeys, false, false);
       constexpr uint32_t idesc_pv = idesc_bf16_f32(kBM, kHD, false, true);
+      const bool me = elect_one();
       const uint32_t tm = warp_uniform(tmem);
-      const uint64_t dq = warp_uniform(smem_desc_sw128(smem_u32(smem + kQtOffQ), 16, 1024));
-      const uint64_t dk = warp_uniform(smem_desc_sw128(smem_u32(smem + kQtOffKV), 16, 1024));
-      const uint64_t dv = warp_uniform(smem_desc_sw128(smem_u32(smem + kQtOffKV), kQtHalf, 1024));
+      // (descriptors: the low words; Q and K differ from V in the high one)
+      const uint64_t desc_q = smem_desc_sw128(smem_u32(smem + kQtOffQ), 16, 1024);
+      const uint64_t desc_v = smem_desc_sw128(smem_u32(smem + kQtOffKV), kQtHalf, 1024);
+      const uint32_t dq = warp_uniform(static_cast<uint32_t>(desc_q)), dk = dq + ((kQtOffKV - kQtOffQ) >> 4);
+      const uint32_t dv = warp_uniform(static_cast<uint32_t>(desc_v));
+      const uint32_t hi_qk = warp_uniform(static_cast<uint32_t>(desc_q >> 32));
+      const uint32_t hi_v = warp_uniform(static_cast<uint32_t>(desc_v >> 32));
       auto wait = [&](uint64_t* b, uint32_t ph) { mbar_wait_fast(b, ph & 1, abort_flag, p.status); };
       auto qk = [&](int t, int qt, int stage) {
-        const uint64_t a = dq + static_cast<uint64_t>(qt * (kQtTile >> 4));
-        const uint64_t b = dk + static_cast<uint64_t>(warp_uniform(stage) * (kQtTile >> 4));
+        const uint32_t a = dq + qt * (kQtTile >> 4), b = dk + stage * (kQtTile >> 4);
         tc_fence_after();
-        if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < kHD / 16; ++kk) {
-            const uint32_t off = ((kk >> 2) * kQtHalf + (kk & 3) * 32) >> 4;
-            umma_f16(tm + t * 128, a + off, b + off, idesc_qk, kk > 0);
-          }
-          umma_commit(&bar.s_full[t]);
+        for (int kk = 0; kk < kHD / 16; ++kk) {
+          const uint32_t off = ((kk >> 2) * kQtHalf + (kk & 3) * 32) >> 4;
+          umma_f16_if(me, tm + t * 128, a + off, b + off, hi_qk, idesc_qk, kk > 0);
         }
+        umma_commit_if(me, &bar.s_full[t]);
       };
       auto pv = [&](int t, int stage, int j, bool last) {
-        const uint64_t b = dv + static_cast<uint64_t>(warp_uniform(stage) * (kQtTile >> 4));
+        const uint32_t b = dv + stage * (kQtTile >> 4);
         auto mma = [&](int kk) {
-          umma_f16_ts(tm + kQtTmemO + t * kHD, tm + t * 128 + kk * 8, b + kk * (2048 >> 4), idesc_pv,
-                      (j > 0 || kk > 0) ? 1u : 0u);
+          umma_f16_ts_if(me, tm + kQtTmemO + t * kHD, tm + t * 128 + kk * 8, b + kk * (2048 >> 4), hi_v, idesc_pv,
+                         j > 0 || kk > 0);
         };
         wait(&bar.p_part[t], j);
         tc_fence_after();
-        if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < kPart1 / 16; ++kk) mma(kk);
-        }
+        for (int kk = 0; kk < kPart1 / 16; ++kk) mma(kk);
         wait(&bar.p_full[t], j);
         tc_fence_after();
-        if (elect_one()) {
 #pragma unroll
-          for (int kk = kPart1 / 16; kk < kQtKeys / 16; ++kk) mma(kk);
-          if (last) umma_commit(&bar.o_full[t]);
-        }
+        for (int kk = kPart1 / 16; kk < kQtKeys / 16; ++kk) mma(kk);
+        umma_commit_if(me && last, &bar.o_full[t]);
       };
-      auto release = [&](int stage) {
-        if (elect_one()) umma_commit(&bar.kv_empty[stage]);
-      };
+      auto release = [&](int stage) { umma_commit_if(me, &bar.kv_empty[stage]); };
       if (dual && nb > 0) {
         wait(&bar.q_full[0], 0);
         int n = 0;
@@ -616,7 +612,7 @@ __global__ void __launch_bounds__(kQtThreads, 1)
           release(n);
         }
         for (int b = 0; b < nb; ++b) {
-          const int t = b & 1, sv = n % kQtStages, sk = (n + 1) % kQtStages;
+          const int t = warp_uniform2(b & 1), sv = warp_uniform2(n % kQtStages), sk = (sv + 1) % kQtStages;
           const bool more = b + 2 < nb;
           wait(&bar.kv_full[sv], n / kQtStages);
           if (more) wait(&bar.kv_full[sk], (n + 1) / kQtStages);
@@ -630,7 +626,7 @@ __global__ void __launch_bounds__(kQtThreads, 1)
       for (int j = -1; j < nb && nb > 0 && !dual; ++j) {
         // entries 2j+1 = V_j and 2j+2 = K_{j+1}
         const int nv = 2 * j + 1, nk = 2 * j + 2;
-        const int sv = nv & (kQtStages - 1), sk = nk % kQtStages;
+        const int sk = warp_uniform2(nk % kQtStages), sv = (sk + kQtStages - 1) % kQtStages;
         const bool more = j + 1 < nb;
         if (j >= 0) wait(&bar.kv_full[sv], nv / kQtStages);
         if (more) wait(&bar.kv_full[sk], nk / kQtStages);
@@ -644,10 +640,8 @@ __global__ void __launch_bounds__(kQtThreads, 1)
         if (more) release(sk);
       }
       // all issued MMAs complete before TMEM is released
-      if (elect_one()) {
-        umma_commit(&bar.fin);
-        mbar_wait_drain(&bar.fin, 0);
-      }
+      umma_commit_if(me, &bar.fin);
+      if (me) mbar_wait_drain(&bar.fin, 0);
       __syncwarp();
       if (nb > 0)
         for (int t = 0; t < tiles; ++t) mbar_wait_drain(&bar.q_full[t], 0);  // (long done, but for an abort)
