@@ -20,6 +20,9 @@
 // heads costs one 8-wide tile, not a 16-wide one.
 // The warps' results are merged in shared memory, the splits' in the cluster
 // (distributed shared memory) or through the workspace (attn_combine_kernel).
+// Measured (32 / 8 heads, in a graph): one token over 2048 rows 7.0 us (launch and
+// merges), over 131071 rows 42.7 us (3.5 TB/s): bound by instruction issue, 735 a
+// tile and warp, 64 % of the issue slots, the ALU pipe 54 % busy.
 //
 // More query rows
 // ---------------------------------------------------------------------------
@@ -35,6 +38,10 @@
 // softmax groups take turns at its key blocks instead: two chains of S, P and O
 // for the same queries, merged at the end, so that one chain's softmax still runs
 // under the other's products.
+// Measured (32 / 8 heads, 32768 rows, in a graph): 17 nodes 28.7 us, of which 12.6 do
+// not depend on the length; decode (2140 cycles a block) and the two chains (2050)
+// bound the rest alike.  257 nodes 157 us (880 TFLOP/s): a tile's chain (softmax 2250 cycles,
+// P to the next S 1500) bounds the block, whose products take 2048.
 //
 // What hides: the rows behind the tree are stale bytes, so the last tile reads
 // their scales as zero; a tree row that reads as NaN turns the scores of the

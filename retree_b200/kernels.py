@@ -853,18 +853,21 @@ def kv_read_q4(cache: torch.Tensor, start: int, n: int, out: torch.Tensor | None
     what = "kv_read_q4"
     if not cache.is_cuda:
         raise RuntimeError(f"{what}: takes CUDA tensors (no CPU path)")
-    dev = cache.device
-    *lead, cap, row = cache.shape if cache.dim() > 1 else (0, 0)
-    *outer, s1, s0 = cache.stride() if cache.dim() > 1 else (0, 0)
+    size, stride = cache.shape, cache.stride()
+    *lead, cap, row = size if len(size) > 1 else (0, 0)
+    fold = row == 72 and stride[-2:] == (72, 1) and cache.dtype is _U8
     # the leading axes as one: heads `step` bytes apart
-    heads, step = 1, cap * 72
-    fold = row == 72 and s0 == 1 and s1 == 72 and cache.dtype is torch.uint8
-    for size, stride in zip(reversed(lead), reversed(outer)):
-        if size > 1:
-            if heads == 1:
-                step = stride
-            fold = fold and stride == heads * step
-        heads *= size
+    if len(lead) == 2 and lead[0] > 1 and lead[1] > 1:
+        heads, step = lead[0] * lead[1], stride[1]
+        fold = fold and stride[0] == lead[1] * step
+    else:
+        heads, step = 1, cap * 72
+        for axis in range(len(lead) - 1, -1, -1):
+            if size[axis] > 1:
+                if heads == 1:
+                    step = stride[axis]
+                fold = fold and stride[axis] == heads * step
+            heads *= size[axis]
     if not fold:
         raise RuntimeError(f"{what}: the cache must be uint8 [..., capacity, {Q4_ROW_BYTES}] with contiguous rows and "
                            "leading dimensions of one stride")
@@ -874,13 +877,13 @@ def kv_read_q4(cache: torch.Tensor, start: int, n: int, out: torch.Tensor | None
     shape = (*lead, n, 128)
     if out is None:
         out = cache.new_empty(shape, dtype=_BF16)
-    elif out.shape != shape or out.dtype is not torch.bfloat16 or not out.is_contiguous() or out.device != dev:
-        raise RuntimeError(f"{what}: out must be contiguous bf16 {list(shape)} on {dev}")
+    elif out.shape != shape or out.dtype is not torch.bfloat16 or not out.is_contiguous() or out.device != cache.device:
+        raise RuntimeError(f"{what}: out must be contiguous bf16 {list(shape)} on {cache.device}")
     if heads == 0 or n == 0:
         return out
-    index = dev.index
+    index = cache.get_device()
     if _current_device() != index:
-        with torch.cuda.device(dev):
+        with torch.cuda.device(index):
             return kv_read_q4(cache, start, n, out)
     rc = _lib.load().rt_kv_read_q4(cache.data_ptr(), step, out.data_ptr(), n * 256, 256, heads, n, 128, cap, start,
                                    _raw_stream(index))
