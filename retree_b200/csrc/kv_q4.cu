@@ -7,7 +7,7 @@
 // kRowsEach rows, whose loads are all in flight at once.
 // Measured, 8191 rows of 8 heads, K and V (43 MB), in a graph: append 13.8 us (3.1
 // TB/s; bound by the quantisation: ALU pipe 67 % and issue slots 74 % busy), read
-// 6.4 us (6.7 TB/s).  A lane a row at a time took 36.9 us for both.
+// 6.4 us (6.7 TB/s).  With one row a lane and fp32 divisions both took 36.9 us.
 #include "common.cuh"
 #include "host_util.h"
 #include "q4_row.cuh"
@@ -176,7 +176,7 @@ extern "C" int rt_kv_append_q4(void* k_cache, void* v_cache, int64_t cache_head_
   if (head_dim != 128) return RT_ERR_UNSUPPORTED;
   if (n_heads == 0 || n_new == 0) return RT_OK;
   if (!k_cache || !v_cache || !k_new || !v_new) return RT_ERR_INVALID_ARGUMENT;
-  if (offset_dev == nullptr && (offset < 0 || offset + n_new > capacity)) return RT_ERR_INVALID_ARGUMENT;
+  if (offset_dev == nullptr && (offset < 0 || offset > capacity - n_new)) return RT_ERR_INVALID_ARGUMENT;
   const uint64_t a16 = reinterpret_cast<uint64_t>(k_new) | reinterpret_cast<uint64_t>(v_new) |
                        static_cast<uint64_t>(new_head_stride) | static_cast<uint64_t>(new_row_stride);
   const uint64_t a8 = reinterpret_cast<uint64_t>(k_cache) | reinterpret_cast<uint64_t>(v_cache) |
@@ -193,7 +193,7 @@ extern "C" int rt_kv_append_q4(void* k_cache, void* v_cache, int64_t cache_head_
 extern "C" int rt_kv_read_q4(const void* cache, int64_t cache_head_stride, void* out, int64_t out_head_stride,
                              int64_t out_row_stride, int n_heads, int n, int head_dim, int64_t capacity,
                              int64_t start, rt_stream_t stream) {
-  if (n_heads < 0 || n < 0 || capacity < 0 || start < 0 || start + n > capacity) return RT_ERR_INVALID_ARGUMENT;
+  if (n_heads < 0 || n < 0 || capacity < 0 || start < 0 || start > capacity - n) return RT_ERR_INVALID_ARGUMENT;
   if (head_dim != 128) return RT_ERR_UNSUPPORTED;
   if (n_heads == 0 || n == 0) return RT_OK;
   if (!cache || !out) return RT_ERR_INVALID_ARGUMENT;

@@ -38,10 +38,12 @@ struct AttnParams {
   int row_splits, tail_splits, tail_row;
 };
 
-__device__ __forceinline__ int64_t key_count(const AttnParams& p) {
-  const int64_t L = p.prefix_len_dev != nullptr ? *p.prefix_len_dev : p.prefix_len;
-  return L + p.n;
+__device__ __forceinline__ int64_t prefix_rows(const AttnParams& p) {
+  return p.prefix_len_dev != nullptr ? *p.prefix_len_dev : p.prefix_len;
 }
+__device__ __forceinline__ int64_t key_count(const AttnParams& p) { return prefix_rows(p) + p.n; }
+// Whether the keys are rows of the cache (asked before a sum that a wild length could overflow).
+__device__ __forceinline__ bool prefix_fits(const AttnParams& p, int64_t L) { return L >= 0 && L <= p.capacity - p.n; }
 
 // Block range [b0, b1) of this split: the blocks spread evenly (range sizes
 // differ by at most one, so no split runs two blocks while another idles).
@@ -227,7 +229,7 @@ static __global__ void __launch_bounds__(128) attn_combine_kernel(const AttnPara
   pdl_wait();
   const int lane = threadIdx.x & 31;
   const int rows = p.n * p.group;
-  if (p.capacity > 0 && (key_count(p) < p.n || key_count(p) > p.capacity)) return;
+  if (p.capacity > 0 && !prefix_fits(p, prefix_rows(p))) return;
   const int64_t rows_ws = static_cast<int64_t>(p.tiles) * kBM;
   auto splits_of = [&](int R) {
     return p.tail_splits == 0 ? p.num_splits : R >= p.tail_row ? p.tail_splits : p.row_splits;

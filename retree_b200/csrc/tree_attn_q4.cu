@@ -121,11 +121,12 @@ __global__ void __launch_bounds__(kQsThreads, 1) tree_attn_q4_small_kernel(const
   }
   pdl_launch_dependents();
   pdl_wait();
-  const int64_t total = key_count(p), L = total - p.n;
-  if (L < 0 || total > p.capacity) {  // the same in every CTA of the launch
+  const int64_t L = prefix_rows(p);
+  if (!prefix_fits(p, L)) {  // the same in every CTA of the launch
     if (tid == 0) set_status(p.status, RT_DEV_BAD_INDEX);
     return;
   }
+  const int64_t total = L + p.n;
   int64_t b0, b1;
   split_range(total, split, p.num_splits, kQsKeys, b0, b1);
   const char* kb = p.k + kvh * p.kv_head_stride;
@@ -550,8 +551,9 @@ __global__ void __launch_bounds__(kQtThreads, 1)
   pdl_launch_dependents();
   const uint32_t tmem = bar.tmem_base;
   volatile int* abort_flag = &bar.abort_flag;
-  const int64_t total = key_count(p), L = total - p.n;
-  const bool inside = L >= 0 && total <= p.capacity;    // the same in every thread of the launch
+  const int64_t L = prefix_rows(p);
+  const bool inside = prefix_fits(p, L);                // the same in every thread of the launch
+  const int64_t total = inside ? L + p.n : 0;
   if (!inside && tid == 0) set_status(p.status, RT_DEV_BAD_INDEX);
   int64_t b0 = 0, b1 = 0;
   if (inside) split_range(total, split, mine, kQtKeys, b0, b1);
@@ -1010,7 +1012,7 @@ extern "C" int rt_tree_attn_q4(const void* q, int64_t q_tok_stride, int64_t q_he
   if (!(scale >= 0.f) || scale > 3e38f) return RT_ERR_INVALID_ARGUMENT;
   if (head_dim != kHD) return RT_ERR_UNSUPPORTED;
   if (mask_words < (n + 31) / 32) return RT_ERR_INVALID_ARGUMENT;
-  if (prefix_len_dev == nullptr && prefix_len + n > kv_capacity) return RT_ERR_INVALID_ARGUMENT;
+  if (prefix_len_dev == nullptr && prefix_len > kv_capacity - n) return RT_ERR_INVALID_ARGUMENT;
   const uint64_t align_bits = reinterpret_cast<uint64_t>(q) | reinterpret_cast<uint64_t>(k) |
                               reinterpret_cast<uint64_t>(v) | reinterpret_cast<uint64_t>(out) |
                               static_cast<uint64_t>(q_tok_stride) | static_cast<uint64_t>(q_head_stride) |

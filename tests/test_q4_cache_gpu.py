@@ -363,3 +363,19 @@ def test_calls_on_two_streams_at_once():
     torch.cuda.synchronize(dev)
     kernels.check_device_status(dev)
     assert all(torch.equal(got, want) for o in outs for got, want in o)
+
+
+@pytest.mark.parametrize("n", [1, 17, 129])
+def test_wild_device_lengths_are_reported(n):
+    """Lengths whose sum with the tree passes 64 bits, on the device: nothing is read or written."""
+    dev = cuda()
+    _, vis = random_tree(n, n - 1)
+    slab = caches(n, dev, 2, 2000 + n)
+    q = rows(n, dev, n, 8)
+    out = torch.full_like(q, 7.0)
+    for prefix in (2 ** 63 - 1, 2 ** 63 - n, -2 ** 63):
+        plen = torch.tensor([prefix], device=dev)
+        kernels.tree_attention_q4(q, slab[0], slab[1], bits_tensor(vis, dev), 2000, prefix_len_dev=plen, out=out)
+        with pytest.raises(RuntimeError, match="index"):
+            kernels.check_device_status(dev)
+    assert bool((out == 7).all())

@@ -96,6 +96,16 @@ def test_q4_host_checks():
     assert attn(d=64) == unsup
 
 
+def test_lengths_whose_sum_passes_64_bits_are_refused():
+    lib = _lib.load()
+    bad, far = _lib.RT_ERR_INVALID_ARGUMENT, 2 ** 63 - 1
+    assert lib.rt_kv_append_q4(P, P, 72 * 64, P, P, 1 << 12, 256, 8, 4, 128, 64, far, None, None, None) == bad
+    assert lib.rt_kv_read_q4(P, 72 * 64, P, 1 << 10, 256, 8, 4, 128, 64, far, None) == bad
+    for n in (1, 40):
+        assert lib.rt_tree_attn_q4(P, 8192, 256, P, P, 72 * 64, 64, P, 8192, 256, P, 2, n, far, None, 32, 8, 128,
+                                   ctypes.c_float(1.0), 0, None, 0, None, None) == bad
+
+
 def test_wrappers_refuse_cpu_tensors():
     q, kv = torch.zeros(2, 8, 128, dtype=torch.bfloat16), torch.zeros(2, 4, 128, dtype=torch.bfloat16)
     c = torch.zeros(2, 4, 72, dtype=torch.uint8)
