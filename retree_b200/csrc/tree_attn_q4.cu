@@ -449,6 +449,7 @@ constexpr int kQtDecodeWarps = 7, kQtMmaWarp = 15;    // warps 8-14, 15
 // (Spilling on either side shows: 257 nodes over 32768 rows 204 us, 222 with 168 / 88,
 // 216 with 184 / 72.  With 4 / 5 / 6 / 7 decode warps 17 nodes take 33.8 / 33.8 / 30.5 / 28.7.)
 constexpr int kQtRegsSoftmax = 176, kQtRegsOther = 80;
+constexpr int kQtAhead = 4;                           // blocks between L2 prefetch and products
 constexpr int kQtKeys = 128;
 constexpr uint32_t kQtTile = 128 * 128 * 2, kQtHalf = kQtTile / 2;
 constexpr int kQtStages = 4;                          // decoded tiles
@@ -612,6 +613,20 @@ __global__ void __launch_bounds__(kQtThreads, 1)
         umma_commit_if(me && last, &bar.o_full[t]);
       };
       auto release = [&](int stage) { umma_commit_if(me, &bar.kv_empty[stage]); };
+      // The blocks some way ahead into L2: the decode warps' registers hold too little
+      // to cover the memory's latency (a cache that is not in L2, 32768 rows: 17 nodes
+      // 33.8 -> 31.5 us, 257 nodes 167 -> 158; 3, 6 and 8 blocks ahead alike; asked
+      // for by the decode warps themselves 34.1 and 174).
+      const char* kb = p.k + kvh * p.kv_head_stride + b0 * kQtKeys * kQ4Row;
+      const char* vb = p.v + kvh * p.kv_head_stride + b0 * kQtKeys * kQ4Row;
+      const int whole = static_cast<int>(min(static_cast<int64_t>(nb), total / kQtKeys - b0));  // blocks of 128 rows
+      auto prefetch = [&](int b) {
+        if (me && b < whole) {
+          prefetch_l2(kb + static_cast<int64_t>(b) * kQtKeys * kQ4Row, kQtKeys * kQ4Row);
+          prefetch_l2(vb + static_cast<int64_t>(b) * kQtKeys * kQ4Row, kQtKeys * kQ4Row);
+        }
+      };
+      for (int b = 0; b < kQtAhead; ++b) prefetch(b);
       if (dual && nb > 0) {
         wait(&bar.q_full[0], 0);
         int n = 0;
@@ -623,6 +638,7 @@ __global__ void __launch_bounds__(kQtThreads, 1)
         for (int b = 0; b < nb; ++b) {
           const int t = warp_uniform2(b & 1), sv = warp_uniform2(n % kQtStages), sk = (sv + 1) % kQtStages;
           const bool more = b + 2 < nb;
+          prefetch(b + kQtAhead);
           wait(&bar.kv_full[sv], n / kQtStages);
           if (more) wait(&bar.kv_full[sk], (n + 1) / kQtStages);
           pv(t, sv, b >> 1, !more);
@@ -637,6 +653,7 @@ __global__ void __launch_bounds__(kQtThreads, 1)
         const int nv = 2 * j + 1, nk = 2 * j + 2;
         const int sk = warp_uniform2(nk % kQtStages), sv = (sk + kQtStages - 1) % kQtStages;
         const bool more = j + 1 < nb;
+        prefetch(j + kQtAhead);
         if (j >= 0) wait(&bar.kv_full[sv], nv / kQtStages);
         if (more) wait(&bar.kv_full[sk], nk / kQtStages);
 #pragma unroll
