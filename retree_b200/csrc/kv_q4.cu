@@ -67,26 +67,32 @@ __device__ __forceinline__ void quantise8(const uint4& raw, uint32_t& code, uint
     x[2 * i] = __uint_as_float(w[i] << 16);
     x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
   }
-  float z = -lo;
+  float z = -lo, top_x = hi;
   if (plain) {
     float inv;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = quotient(x[i], s, inv);
     z = quotient(z, s, inv);
+    top_x = quotient(top_x, s, inv);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = __fdiv_rn(x[i], s);
     z = __fdiv_rn(z, s);
+    top_x = __fdiv_rn(top_x, s);
   }
   // adding 1.5 * 2^23 rounds to the nearest integer (ties to even) in the low
   // bits; the codes are summed with that offset and it is taken off at the end
   constexpr float kRound = 12582912.f;
   const uint32_t zi = __float_as_uint(z + kRound) - __float_as_uint(kRound), base = __float_as_uint(kRound) - zi;
   word = ((__float_as_uint(s) >> 16) & 0x7FF0u) | zi;
+  // (the upper clamp matters only where the group's largest code would be 16)
+  if (__float_as_uint(top_x + kRound) > base + 15u) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    code += min(__float_as_uint(x[i] + kRound), base + 15u) << (4 * ((i >> 1) + 4 * (i & 1)));
+    for (int i = 0; i < 8; ++i) x[i] = fminf(x[i], __uint_as_float(base + 15u) - kRound);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) code += __float_as_uint(x[i] + kRound) << (4 * ((i >> 1) + 4 * (i & 1)));
   code -= base * 0x11111111u;
 }
 

@@ -947,7 +947,7 @@ def tree_attention_q4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask_bi
     else:
         q, q0, q1 = _rows(q)
     if out is None:
-        out = q.new_empty((n, hq, 128))
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((n, hq, 128))
         o0, o1 = hq * 256, 256
     else:
         _, o0, o1 = _rows(_attn_out(out, q, what))

@@ -379,3 +379,18 @@ def test_wild_device_lengths_are_reported(n):
         with pytest.raises(RuntimeError, match="index"):
             kernels.check_device_status(dev)
     assert bool((out == 7).all())
+
+
+def test_codes_of_symmetric_ranges_are_clamped():
+    """hi = -lo = 7.5 s: both ends round away from zero, and the upper one would be code 16."""
+    dev = cuda()
+    x = rows(3, dev, 1, 40).clamp(-7.5, 7.5)
+    x[:, :, ::32], x[:, :, 1::32] = 7.5, -7.5
+    x = torch.where(x.abs() > 7.5, 7.5, x) * (2.0 ** torch.arange(-20, 20, device=dev))[None, :, None].bfloat16()
+    slab = torch.zeros((2, 1, 40, 72), dtype=torch.uint8, device=dev)
+    kernels.kv_append_q4(slab[0], slab[1], x, -x)
+    kernels.check_device_status(dev)
+    want = q4.pack(torch.stack([x, -x]))
+    assert torch.equal(slab, want)
+    top = kernels.kv_read_q4(slab, 0, 40)[0, 0, :, 0].float()
+    assert torch.equal(top, 7 * 2.0 ** torch.arange(-20, 20, device=dev))
