@@ -87,47 +87,52 @@ __device__ __forceinline__ void softmax_block(const uint32_t (&sr)[4][32], uint3
   l += (acc[0].x + acc[1].x) + (acc[0].y + acc[1].y);
 }
 
-// 64 bytes of a row from each lane to `dst` (0: no row), through 2 KB of the warp's
-// at `stage`: four lanes write a row's 64 bytes together, so a store touches 8 rows
-// and not 32.
-__device__ __forceinline__ void store_rows64(uint32_t stage, const uint4 (&v)[4], uint64_t dst) {
-  const int lane = threadIdx.x & 31;
+// A warp's 32 output rows, a lane a row, written through 2 KB of shared memory four
+// lanes a row, so that a store touches 8 rows and not 32.
+struct RowsOut {
+  uint32_t stage;
+  uint64_t to[4];  // rows lane / 4 + 0, 8, 16, 24 (0: no row)
+  __device__ __forceinline__ RowsOut(uint32_t stage, uint64_t row) : stage(stage) {
 #pragma unroll
-  for (int q = 0; q < 4; ++q) sts128(stage + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4), v[q]);
-  __syncwarp();
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int from = q * 8 + (lane >> 2), piece = lane & 3;
-    const uint4 x = lds128(stage + from * 64 + ((piece ^ ((from >> 1) & 3)) << 4));
-    const uint64_t to = __shfl_sync(0xFFFFFFFFu, dst, from);
-    if (to != 0) *reinterpret_cast<uint4*>(to + piece * 16) = x;
+    for (int q = 0; q < 4; ++q) to[q] = __shfl_sync(0xFFFFFFFFu, row, q * 8 + ((threadIdx.x & 31) >> 2));
   }
-  __syncwarp();
-}
-
-// 32 values of a row: in T, or in fp32.
-template <typename T>
-__device__ __forceinline__ void store_row32(uint32_t stage, const float (&x)[32], uint64_t dst) {
-  if constexpr (std::is_same_v<T, float>) {
+  // 64 bytes of each row, `at` bytes into it
+  __device__ __forceinline__ void put(const uint4 (&v)[4], int at) const {
+    const int lane = threadIdx.x & 31, piece = lane & 3;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      uint4 v[4];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float* f = x + h * 16 + q * 4;
-        v[q] = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
-      }
-      store_rows64(stage, v, dst == 0 ? 0 : dst + h * 64);
-    }
-  } else {
-    uint4 v[4];
+    for (int q = 0; q < 4; ++q) sts128(stage + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4), v[q]);
+    __syncwarp();
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const float* f = x + q * 8;
-      v[q] = make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
+      const int from = q * 8 + (lane >> 2);
+      const uint4 x = lds128(stage + from * 64 + ((piece ^ ((from >> 1) & 3)) << 4));
+      if (to[q] != 0) *reinterpret_cast<uint4*>(to[q] + at + piece * 16) = x;
     }
-    store_rows64(stage, v, dst);
+    __syncwarp();
   }
-}
+  // values 32c .. 32c + 31 of each row, in T or in fp32
+  template <typename T>
+  __device__ __forceinline__ void put32(const float (&x)[32], int c) const {
+    uint4 v[4];
+    if constexpr (std::is_same_v<T, float>) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float* f = x + h * 16 + q * 4;
+          v[q] = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+        }
+        put(v, c * 128 + h * 64);
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float* f = x + q * 8;
+        v[q] = make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
+      }
+      put(v, c * 64);
+    }
+  }
+};
 
 }  // namespace rt

@@ -501,7 +501,9 @@ __global__ void __launch_bounds__(kPThreads, 1)
     const float sl2 = p.scale_log2;
     int ns = 0, no = 0;
     const uint32_t stage = smem_u32(smem + kPOffOut + warp * 2048);
-    for (int it = 0; prompt_next<true>(p, bar, tab, ord, it, w); ++it) {
+    bool more = prompt_next<true>(p, bar, tab, ord, 0, w);
+    PromptItem next{};
+    for (int it = 0; more; ++it, w = next) {
       const int tok = w.tok0 + t * p.tok + rt;
       const bool valid = t < p.tiles && rt < p.tok && tok < w.lq;
       const int lim = valid ? min(max(tok + 1 + w.lk - w.lq, 0), w.lk) : 0;  // keys this row sees
@@ -529,6 +531,8 @@ __global__ void __launch_bounds__(kPThreads, 1)
       const int64_t row = static_cast<int64_t>(w.q0 + tok), head = w.g * p.group + rh;
       char* dst = p.out + row * p.out_tok_stride + head * p.out_head_stride;
       const int64_t slot = (static_cast<int64_t>(w.split) * p.total_q + row) * p.hq + head;
+      // (found out while the last products run)
+      more = prompt_next<true>(p, bar, tab, ord, it + 1, next);
       if (nb == 0) {
         if (valid && p.splits > 1) p.ws_ml[slot] = make_float2(-INFINITY, 0.f);
         if (valid && p.splits == 1)
@@ -542,6 +546,9 @@ __global__ void __launch_bounds__(kPThreads, 1)
       const float inv = p.splits > 1 ? 1.f : 1.f / l;
       const bool none = lim <= w.jb * kPB;
       const bool poison = *const_cast<volatile int*>(&bar.poison) != 0;
+      const RowsOut rows(stage, !valid          ? 0
+                                : p.splits == 1 ? reinterpret_cast<uint64_t>(dst)
+                                                : reinterpret_cast<uint64_t>(p.ws_o + slot * kPD));
 #pragma unroll 1
       for (int c = 0; c < 4; ++c) {
         uint32_t o[32];
@@ -553,10 +560,8 @@ __global__ void __launch_bounds__(kPThreads, 1)
         if (poison && valid)
           add_not_finite<T>(p.v + w.g * p.kv_head_stride + w.k0 * p.kv_row_stride + c * 64, p.kv_row_stride,
                             (w.jb + w.jm) * kPB, min(lim, (w.jb + nb) * kPB), x);
-        if (p.splits == 1)
-          store_row32<T>(stage, x, valid ? reinterpret_cast<uint64_t>(dst + c * 64) : 0);
-        else
-          store_row32<float>(stage, x, valid ? reinterpret_cast<uint64_t>(p.ws_o + slot * kPD + c * 32) : 0);
+        if (p.splits == 1) rows.put32<T>(x, c);
+        else rows.put32<float>(x, c);
       }
       // (a NaN weight wins the merge)
       if (valid && p.splits > 1) p.ws_ml[slot] = none ? make_float2(-INFINITY, 0.f) : make_float2(l == l ? m : INFINITY, l);

@@ -797,6 +797,7 @@ __global__ void __launch_bounds__(kQtThreads, 1)
       const uint32_t stage = smem_u32(smem) + kQtOffQ + (dual ? warp : t * 8 + (warp & 3)) * 4096;  // (Q is done with)
       char* row = p.num_splits > 1 ? reinterpret_cast<char*>(p.ws_o + slot * kHD)
                                    : p.out + node * p.out_tok_stride + h * p.out_head_stride;
+      const RowsOut rows(stage, valid ? reinterpret_cast<uint64_t>(row) : 0);
       // one chain: all four column groups of the tile's O; two: half of them, of both O
 #pragma unroll 1
       for (int c = dual ? 2 * t : 0; c < (dual ? 2 * t + 2 : 4); ++c) {
@@ -815,9 +816,9 @@ __global__ void __launch_bounds__(kQtThreads, 1)
         if (p.num_splits == 1) {
 #pragma unroll
           for (int i = 0; i < 32; ++i) x[i] = l == 0.f ? 0.f : x[i] * inv;
-          store_row32<__nv_bfloat16>(stage, x, valid ? reinterpret_cast<uint64_t>(row + c * 64) : 0);
+          rows.put32<__nv_bfloat16>(x, c);
         } else {
-          store_row32<float>(stage, x, valid ? reinterpret_cast<uint64_t>(row + c * 128) : 0);
+          rows.put32<float>(x, c);
         }
       }
       if (valid && p.num_splits > 1 && (t == 0 || !dual)) p.ws_ml[slot] = make_float2(m, l);
