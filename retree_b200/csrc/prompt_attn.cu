@@ -21,11 +21,12 @@
 //   warp 9          MMA issuer: per block PV of tile 0, next QK of
 //                   tile 0, PV of tile 1, next QK of tile 1 -- while one tile's
 //                   softmax runs the tensor core has the other tile's products;
-//   warp 10         checks the V blocks that some row must not see in full
+//   warps 10, 11    check the V blocks that some row must not see in full
 //                   (the causal diagonal, the sequence's end) for values that
 //                   are not finite: 0 * NaN would reach rows that hide the key.
-//                   It zeroes them; rows that do see the key add the value back
-//                   at the end.
+//                   They zero them; rows that do see the key add the value back
+//                   at the end.  (Half a block each: one warp took longer than the
+//                   block's softmax.)
 // Every mbarrier wait is bounded (common.cuh): on time-out the CTA records
 // RT_DEV_WAIT_TIMEOUT, drains what it issued, frees TMEM and exits.
 //
@@ -186,6 +187,19 @@ __device__ __forceinline__ uint32_t not_finite2(uint32_t w) {
   return ((w & kExp) + kOne) & 0x80008000u;
 }
 
+// Larger magnitude of the halves of two 16-bit pairs (NaN stays).
+template <typename T>
+__device__ __forceinline__ uint32_t abs_max2(uint32_t a, uint32_t b) {
+  if constexpr (std::is_same_v<T, __half>) {
+    const __half2 m = __hmax2_nan(*reinterpret_cast<const __half2*>(&a), __habs2(*reinterpret_cast<const __half2*>(&b)));
+    return *reinterpret_cast<const uint32_t*>(&m);
+  } else {
+    const __nv_bfloat162 m = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&a),
+                                         __habs2(*reinterpret_cast<const __nv_bfloat162*>(&b)));
+    return *reinterpret_cast<const uint32_t*>(&m);
+  }
+}
+
 // The values of v rows [key0, key1) that are not finite, added to 32 columns of
 // one output row (the rare path: those values were zero in the product).
 template <typename T>
@@ -239,10 +253,10 @@ __global__ void __launch_bounds__(kPThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bar.clc_full[i], 1);
-      mbar_init(&bar.clc_empty[i], 11);  // warps 0-10
+      mbar_init(&bar.clc_empty[i], 12);  // every warp
     }
     mbar_init(&bar.v_look, 1);
-    mbar_init(&bar.v_ok, 1);
+    mbar_init(&bar.v_ok, 2);
     mbar_init(&bar.fin, 1);
     bar.abort_flag = 0;
     bar.poison = 0;
@@ -373,7 +387,7 @@ __global__ void __launch_bounds__(kPThreads, 1)
     const uint32_t dv = warp_uniform(static_cast<uint32_t>(desc_v)), hi_v = warp_uniform(static_cast<uint32_t>(desc_v >> 32));
     int n = 0;  // ring loads consumed
     int nq[2] = {0, 0}, np[2] = {0, 0};
-    uint32_t looks = 0;  // V blocks handed to warp 10
+    uint32_t looks = 0;  // V blocks handed to warps 10 and 11
     auto wait = [&](uint64_t* b, uint32_t ph, uint32_t known = 0) {
       mbar_wait_fast(b, ph & 1, abort_flag, p.status, known);
     };
@@ -448,7 +462,7 @@ __global__ void __launch_bounds__(kPThreads, 1)
     umma_commit_if(me, &bar.fin);
     if (me) mbar_wait_drain(&bar.fin, 0);
     __syncwarp();
-  } else if (warp == 10) {
+  } else if (warp >= 10) {
     // ---------------- V blocks that are partly hidden: values that are not finite ----------------
     fewer_registers();
     // (the MMA warp hands them over in order, right after the block's QK, so
@@ -461,26 +475,28 @@ __global__ void __launch_bounds__(kPThreads, 1)
         const int m = n + 2 * j + 1, s = m % kPStages;
         mbar_wait_fast(&bar.v_look, looks++ & 1, abort_flag, p.status);
         mbar_wait_fast(&bar.kv_full[s], (m / kPStages) & 1, abort_flag, p.status);
-        uint4* v = reinterpret_cast<uint4*>(smem + kPOffKV + s * kPTile) + lane;
-        uint32_t bad = 0;
+        // this warp's half, 512 bytes a step
+        constexpr int kSteps = static_cast<int>(kPTile / 1024);
+        const uint32_t v = smem_u32(smem + kPOffKV + s * kPTile) + (warp - 10) * (kPTile / 2) + lane * 16;
+        uint32_t top = 0;  // largest magnitudes, NaN above all
 #pragma unroll 8
-        for (int i = 0; i < static_cast<int>(kPTile / 512); ++i) {
-          const uint4 x = v[i * 32];
-          bad |= not_finite2<T>(x.x) | not_finite2<T>(x.y) | not_finite2<T>(x.z) | not_finite2<T>(x.w);
+        for (int i = 0; i < kSteps; ++i) {
+          const uint4 x = lds128(v + i * 512);
+          top = abs_max2<T>(abs_max2<T>(abs_max2<T>(abs_max2<T>(top, x.x), x.y), x.z), x.w);
         }
-        if (__any_sync(0xFFFFFFFFu, bad != 0)) {
+        if (__any_sync(0xFFFFFFFFu, not_finite2<T>(top) != 0)) {
           auto fix = [](uint32_t x) {
             const uint32_t b = not_finite2<T>(x);
             return x & ~(((b >> 15) & 0x00010001u) * 0xFFFFu);
           };
 #pragma unroll 1
-          for (int i = 0; i < static_cast<int>(kPTile / 512); ++i) {
-            uint4 x = v[i * 32];
+          for (int i = 0; i < kSteps; ++i) {
+            uint4 x = lds128(v + i * 512);
             x.x = fix(x.x);
             x.y = fix(x.y);
             x.z = fix(x.z);
             x.w = fix(x.w);
-            v[i * 32] = x;
+            sts128(v + i * 512, x);
           }
           fence_proxy_async_smem();
           if (lane == 0) *const_cast<volatile int*>(&bar.poison) = 1;
@@ -567,8 +583,6 @@ __global__ void __launch_bounds__(kPThreads, 1)
       if (valid && p.splits > 1) p.ws_ml[slot] = none ? make_float2(-INFINITY, 0.f) : make_float2(l == l ? m : INFINITY, l);
       tc_fence_before();
     }
-  } else {
-    fewer_registers();
   }
   __syncthreads();
   if (warp == 9) {
