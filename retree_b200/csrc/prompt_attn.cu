@@ -30,8 +30,8 @@
 // Every mbarrier wait is bounded (common.cuh): on time-out the CTA records
 // RT_DEV_WAIT_TIMEOUT, drains what it issued, frees TMEM and exits.
 //
-// Measured (32 / 8 heads, bf16, in a graph): 2048 tokens 40.8 us, 7122 tokens
-// 348-361 us (1150-1190 TFLOP/s; 244 us at the burst rate of a plain matrix product).  Long
+// Measured (32 / 8 heads, bf16, in a graph): 2048 tokens 39.2-40.3 us, 7122
+// tokens 347-365 us (1140-1200 TFLOP/s; 244 us at the burst rate of a plain matrix product).  Long
 // prompts run at the GPU's power limit (990 W, SM clock 1.65 GHz, tensor pipe 60 %
 // active): 340 us with the exponentials, maxima and sums left out.  A block of two
 // tiles takes the MMA warp 3200 cycles, of which its products fill 2048.

@@ -446,7 +446,7 @@ __global__ void __launch_bounds__(kQsThreads, 1) tree_attn_q4_small_kernel(const
 constexpr int kQtThreads = 512;
 constexpr int kQtDecodeWarps = 7, kQtMmaWarp = 15;    // warps 8-14, 15
 // registers a thread; the block is launched with 128 x 512 (2 x 176 + 2 x 80 = 4 x 128).
-// (Spilling on either side shows: 257 nodes over 32768 rows 204 us, 222 with 168 / 88,
+// (Spilling on either side shows: 257 nodes over 32768 rows, three splits, 204 us, 222 with 168 / 88,
 // 216 with 184 / 72.  With 4 / 5 / 6 / 7 decode warps 17 nodes take 33.8 / 33.8 / 30.5 / 28.7.)
 constexpr int kQtRegsSoftmax = 176, kQtRegsOther = 80;
 constexpr int kQtAhead = 4;                           // blocks between L2 prefetch and products
