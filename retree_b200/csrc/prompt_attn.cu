@@ -30,7 +30,7 @@
 // Every mbarrier wait is bounded (common.cuh): on time-out the CTA records
 // RT_DEV_WAIT_TIMEOUT, drains what it issued, frees TMEM and exits.
 //
-// Measured (32 / 8 heads, bf16, in a graph): 2048 tokens 39.2-40.3 us, 7122
+// Measured (32 / 8 heads, bf16, in a graph): 2048 tokens 39.0-40.3 us, 7122
 // tokens 347-365 us (1140-1200 TFLOP/s; 244 us at the burst rate of a plain matrix product).  Long
 // prompts run at the GPU's power limit (990 W, SM clock 1.65 GHz, tensor pipe 60 %
 // active): 340 us with the exponentials, maxima and sums left out.  A block of two
@@ -223,7 +223,8 @@ __device__ __forceinline__ void add_not_finite(const char* v, int64_t row_stride
   }
 }
 
-template <typename T>
+// kSplit: the items' keys are shared out (splits > 1), and results go to the workspace.
+template <typename T, bool kSplit>
 __global__ void __launch_bounds__(kPThreads, 1)
     prompt_attn_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
                        const __grid_constant__ CUtensorMap tmap_v, const PromptParams p) {
@@ -550,8 +551,8 @@ __global__ void __launch_bounds__(kPThreads, 1)
       // (found out while the last products run)
       more = prompt_next<true>(p, bar, tab, ord, it + 1, next);
       if (nb == 0) {
-        if (valid && p.splits > 1) p.ws_ml[slot] = make_float2(-INFINITY, 0.f);
-        if (valid && p.splits == 1)
+        if (kSplit && valid) p.ws_ml[slot] = make_float2(-INFINITY, 0.f);
+        if (!kSplit && valid)
           for (int c = 0; c < 16; ++c) *reinterpret_cast<uint4*>(dst + c * 16) = make_uint4(0, 0, 0, 0);
         continue;
       }
@@ -559,12 +560,12 @@ __global__ void __launch_bounds__(kPThreads, 1)
       if (__any_sync(0xFFFFFFFFu, *abort_flag)) break;
       tc_fence_after();
       // (a row that sees no key of this share has l == 0, and its O is 0 or not a number)
-      const float inv = p.splits > 1 ? 1.f : 1.f / l;
+      const float inv = kSplit ? 1.f : 1.f / l;
       const bool none = lim <= w.jb * kPB;
       const bool poison = *const_cast<volatile int*>(&bar.poison) != 0;
-      const RowsOut rows(stage, !valid          ? 0
-                                : p.splits == 1 ? reinterpret_cast<uint64_t>(dst)
-                                                : reinterpret_cast<uint64_t>(p.ws_o + slot * kPD));
+      const RowsOut rows(stage, !valid   ? 0
+                                : kSplit ? reinterpret_cast<uint64_t>(p.ws_o + slot * kPD)
+                                         : reinterpret_cast<uint64_t>(dst));
 #pragma unroll 1
       for (int c = 0; c < 4; ++c) {
         uint32_t o[32];
@@ -576,11 +577,10 @@ __global__ void __launch_bounds__(kPThreads, 1)
         if (poison && valid)
           add_not_finite<T>(p.v + w.g * p.kv_head_stride + w.k0 * p.kv_row_stride + c * 64, p.kv_row_stride,
                             (w.jb + w.jm) * kPB, min(lim, (w.jb + nb) * kPB), x);
-        if (p.splits == 1) rows.put32<T>(x, c);
-        else rows.put32<float>(x, c);
+        rows.put32<std::conditional_t<kSplit, float, T>>(x, c);
       }
       // (a NaN weight wins the merge)
-      if (valid && p.splits > 1) p.ws_ml[slot] = none ? make_float2(-INFINITY, 0.f) : make_float2(l == l ? m : INFINITY, l);
+      if (kSplit && valid) p.ws_ml[slot] = none ? make_float2(-INFINITY, 0.f) : make_float2(l == l ? m : INFINITY, l);
       tc_fence_before();
     }
   }
@@ -770,18 +770,18 @@ extern "C" int rt_prompt_attn(const void* q, int64_t q_tok_stride, int64_t q_hea
     if (items > INT32_MAX) return RT_ERR_UNSUPPORTED;
     const dim3 grid(static_cast<unsigned>(items));
     const dim3 rows_grid(static_cast<unsigned>((total_q * num_q_heads + 3) / 4));
-    if (half) {
-      set_smem_limit(prompt_attn_kernel<__half>, kPSmem);
-      rc = record_cuda(launch_ex(prompt_attn_kernel<__half>, grid, dim3(kPThreads), kPSmem, s, 1, tq, tk, tv, p));
-      if (rc == RT_OK && plan.splits > 1)
-        rc = record_cuda(launch_ex(prompt_combine_kernel<__half>, rows_grid, dim3(128), 0, s, 1, p));
-    } else {
-      set_smem_limit(prompt_attn_kernel<__nv_bfloat16>, kPSmem);
-      rc = record_cuda(
-          launch_ex(prompt_attn_kernel<__nv_bfloat16>, grid, dim3(kPThreads), kPSmem, s, 1, tq, tk, tv, p));
-      if (rc == RT_OK && plan.splits > 1)
-        rc = record_cuda(launch_ex(prompt_combine_kernel<__nv_bfloat16>, rows_grid, dim3(128), 0, s, 1, p));
-    }
+    auto launch = [&](auto kernel, auto combine) {
+      set_smem_limit(kernel, kPSmem);
+      int status = record_cuda(launch_ex(kernel, grid, dim3(kPThreads), kPSmem, s, 1, tq, tk, tv, p));
+      if (status == RT_OK && plan.splits > 1) status = record_cuda(launch_ex(combine, rows_grid, dim3(128), 0, s, 1, p));
+      return status;
+    };
+    if (half)
+      rc = plan.splits > 1 ? launch(prompt_attn_kernel<__half, true>, prompt_combine_kernel<__half>)
+                           : launch(prompt_attn_kernel<__half, false>, prompt_combine_kernel<__half>);
+    else
+      rc = plan.splits > 1 ? launch(prompt_attn_kernel<__nv_bfloat16, true>, prompt_combine_kernel<__nv_bfloat16>)
+                           : launch(prompt_attn_kernel<__nv_bfloat16, false>, prompt_combine_kernel<__nv_bfloat16>);
     if (rc != RT_OK) return rc;
   }
   return RT_OK;
