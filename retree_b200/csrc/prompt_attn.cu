@@ -307,207 +307,210 @@ __global__ void __launch_bounds__(kPThreads, 1)
   const uint32_t tmem = bar.tmem_base;
   volatile int* abort_flag = &bar.abort_flag;
   PromptItem w{};
-  // (inside the roles' own branches: ptxas budgets the code after a merge for the smaller count)
-  auto fewer_registers = [] { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPRegsOther)); };
-  if (warp == 8) {
-    // ---------------- TMA producer ----------------
-    fewer_registers();
-    if (lane == 0) {
-      int n = 0;          // ring loads issued
-      int nq[2] = {0, 0};  // Q loads issued per tile
-      bool ok = true;
-      const uint32_t qbytes = static_cast<uint32_t>(p.tok * p.group) * 256u;
-      auto load = [&](const CUtensorMap* map, int row) {
-        const int s = n % kPStages;
-        ok = mbar_wait(&bar.kv_empty[s], ((n / kPStages) & 1) ^ 1, abort_flag, p.status, RT_DEV_WAIT_TIMEOUT);
-        if (!ok) return;
-        unsigned char* dst = smem + kPOffKV + s * kPTile;
-        mbar_arrive_expect_tx(&bar.kv_full[s], kPTile);
-        tma_load_3d(dst, map, &bar.kv_full[s], 0, row, w.g);
-        tma_load_3d(dst + kPHalf, map, &bar.kv_full[s], 64, row, w.g);
-        ++n;
-      };
-      // The next item is asked for when five blocks of this one are left to load:
-      // late, so that whoever is done first gets it, and early enough that the
-      // answer is there in time.  (Asked for at once, 256 items on 148 CTAs were
-      // all handed out in the first microsecond: 2048 tokens took 52 us, not 43.)
-      int asked = 0;
-      auto take_over = [&](int it) {
-        const int s = it & 1;
-        if (!mbar_wait(&bar.clc_empty[s], ((it >> 1) & 1) ^ 1, abort_flag, p.status, RT_DEV_WAIT_TIMEOUT)) return false;
-        mbar_arrive_expect_tx(&bar.clc_full[s], 16);
-        clc_try_cancel(smem_u32(&bar.clc[s]), &bar.clc_full[s]);
-        asked = it + 1;
-        return true;
-      };
-      for (int it = 0; ok && prompt_next<false>(p, bar, tab, ord, it, w); ++it) {
-        const int nb = max(w.nb[0], w.nb[1]);
-        if (nb == 0) ok = take_over(it);
-        for (int j = 0; j < nb && ok; ++j) {
-          if (j == max(nb - 5, 0)) {
-            ok = take_over(it);
-            if (!ok) break;
-          }
-          load(&tmap_k, w.k0 + (w.jb + j) * kPB);
-          if (j == 0) {
-            for (int t = 0; t < 2 && ok; ++t) {
-              if (w.nb[t] == 0) continue;
-              ok = mbar_wait(&bar.q_empty[t], (nq[t] & 1) ^ 1, abort_flag, p.status, RT_DEV_WAIT_TIMEOUT);
+  if (warp >= 8) {
+    // (one instruction for the whole warpgroup; what follows stays inside the branch, as the
+    // compiler budgets code after a merge for the smaller count)
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPRegsOther));
+    if (warp == 8) {
+      // ---------------- TMA producer ----------------
+      if (lane == 0) {
+        int n = 0;          // ring loads issued
+        int nq[2] = {0, 0};  // Q loads issued per tile
+        bool ok = true;
+        const uint32_t qbytes = static_cast<uint32_t>(p.tok * p.group) * 256u;
+        auto load = [&](const CUtensorMap* map, int row) {
+          const int s = n % kPStages;
+          ok = mbar_wait(&bar.kv_empty[s], ((n / kPStages) & 1) ^ 1, abort_flag, p.status, RT_DEV_WAIT_TIMEOUT);
+          if (!ok) return;
+          unsigned char* dst = smem + kPOffKV + s * kPTile;
+          mbar_arrive_expect_tx(&bar.kv_full[s], kPTile);
+          tma_load_3d(dst, map, &bar.kv_full[s], 0, row, w.g);
+          tma_load_3d(dst + kPHalf, map, &bar.kv_full[s], 64, row, w.g);
+          ++n;
+        };
+        // The next item is asked for when five blocks of this one are left to load:
+        // late, so that whoever is done first gets it, and early enough that the
+        // answer is there in time.  (Asked for at once, 256 items on 148 CTAs were
+        // all handed out in the first microsecond: 2048 tokens took 52 us, not 43.)
+        int asked = 0;
+        auto take_over = [&](int it) {
+          const int s = it & 1;
+          if (!mbar_wait(&bar.clc_empty[s], ((it >> 1) & 1) ^ 1, abort_flag, p.status, RT_DEV_WAIT_TIMEOUT))
+            return false;
+          mbar_arrive_expect_tx(&bar.clc_full[s], 16);
+          clc_try_cancel(smem_u32(&bar.clc[s]), &bar.clc_full[s]);
+          asked = it + 1;
+          return true;
+        };
+        for (int it = 0; ok && prompt_next<false>(p, bar, tab, ord, it, w); ++it) {
+          const int nb = max(w.nb[0], w.nb[1]);
+          if (nb == 0) ok = take_over(it);
+          for (int j = 0; j < nb && ok; ++j) {
+            if (j == max(nb - 5, 0)) {
+              ok = take_over(it);
               if (!ok) break;
-              unsigned char* dst = smem + kPOffQ + t * kPTile;
-              mbar_arrive_expect_tx(&bar.q_full[t], qbytes);
-              tma_load_3d(dst, &tmap_q, &bar.q_full[t], 0, w.g * p.group, w.q0 + w.tok0 + t * p.tok);
-              tma_load_3d(dst + kPHalf, &tmap_q, &bar.q_full[t], 64, w.g * p.group, w.q0 + w.tok0 + t * p.tok);
-              ++nq[t];
             }
+            load(&tmap_k, w.k0 + (w.jb + j) * kPB);
+            if (j == 0) {
+              for (int t = 0; t < 2 && ok; ++t) {
+                if (w.nb[t] == 0) continue;
+                ok = mbar_wait(&bar.q_empty[t], (nq[t] & 1) ^ 1, abort_flag, p.status, RT_DEV_WAIT_TIMEOUT);
+                if (!ok) break;
+                unsigned char* dst = smem + kPOffQ + t * kPTile;
+                mbar_arrive_expect_tx(&bar.q_full[t], qbytes);
+                tma_load_3d(dst, &tmap_q, &bar.q_full[t], 0, w.g * p.group, w.q0 + w.tok0 + t * p.tok);
+                tma_load_3d(dst + kPHalf, &tmap_q, &bar.q_full[t], 64, w.g * p.group, w.q0 + w.tok0 + t * p.tok);
+                ++nq[t];
+              }
+            }
+            if (ok) load(&tmap_v, w.k0 + (w.jb + j) * kPB);
           }
-          if (ok) load(&tmap_v, w.k0 + (w.jb + j) * kPB);
+        }
+        if (*abort_flag) {
+          for (int i = max(0, n - kPStages); i < n; ++i)
+            mbar_wait_drain(&bar.kv_full[i % kPStages], (i / kPStages) & 1);
+          for (int t = 0; t < 2; ++t)
+            if (nq[t] > 0) mbar_wait_drain(&bar.q_full[t], (nq[t] - 1) & 1);
+          if (asked > 0) mbar_wait_drain(&bar.clc_full[(asked - 1) & 1], ((asked - 1) >> 1) & 1);
         }
       }
-      if (*abort_flag) {
-        for (int i = max(0, n - kPStages); i < n; ++i)
-          mbar_wait_drain(&bar.kv_full[i % kPStages], (i / kPStages) & 1);
-        for (int t = 0; t < 2; ++t)
-          if (nq[t] > 0) mbar_wait_drain(&bar.q_full[t], (nq[t] - 1) & 1);
-        if (asked > 0) mbar_wait_drain(&bar.clc_full[(asked - 1) & 1], ((asked - 1) >> 1) & 1);
-      }
-    }
-  } else if (warp == 9) {
-    // ---------------- MMA issuer ----------------
-    fewer_registers();
-    constexpr uint32_t kFmt = std::is_same_v<T, __half> ? (1u << 7 | 1u << 10) : 0u;  // clears the bf16 format bits
-    constexpr uint32_t idesc_qk = idesc_bf16_f32(kPB, kPB, false, false) & ~kFmt;
-    constexpr uint32_t idesc_pv = idesc_bf16_f32(kPB, kPD, false, true) & ~kFmt;
-    const bool me = elect_one();
-    const uint32_t tm = warp_uniform(tmem);
-    // (descriptors: the low words; Q, K and V differ in the high one)
-    const uint64_t desc_q = smem_desc_sw128(smem_u32(smem + kPOffQ), 16, 1024);
-    const uint64_t desc_v = smem_desc_sw128(smem_u32(smem + kPOffKV), kPHalf, 1024);
-    const uint32_t dq = warp_uniform(static_cast<uint32_t>(desc_q)), hi_qk = warp_uniform(static_cast<uint32_t>(desc_q >> 32));
-    const uint32_t dk = dq + ((kPOffKV - kPOffQ) >> 4);
-    const uint32_t dv = warp_uniform(static_cast<uint32_t>(desc_v)), hi_v = warp_uniform(static_cast<uint32_t>(desc_v >> 32));
-    int n = 0;  // ring loads consumed
-    int nq[2] = {0, 0}, np[2] = {0, 0};
-    uint32_t looks = 0;  // V blocks handed to warps 10 and 11
-    auto wait = [&](uint64_t* b, uint32_t ph, uint32_t known = 0) {
-      mbar_wait_fast(b, ph & 1, abort_flag, p.status, known);
-    };
-    auto test = [](uint64_t* b, uint32_t ph) { return mbar_test(b, ph & 1); };
-    // S_t = Q_t K^T of the block in `stage`; the last one of an item frees Q_t
-    auto qk = [&](int t, int stage, bool last) {
-      const uint32_t a = dq + t * (kPTile >> 4), b = dk + stage * (kPTile >> 4);
-#pragma unroll
-      for (int kk = 0; kk < kPD / 16; ++kk) {
-        const uint32_t off = ((kk >> 2) * kPHalf + (kk & 3) * 32) >> 4;
-        umma_f16_if(me, tm + t * kPB, a + off, b + off, hi_qk, idesc_qk, kk > 0);
-      }
-      umma_commit_if(me, &bar.s_full[t]);
-      umma_commit_if(me && last, &bar.q_empty[t]);
-    };
-    for (int it = 0; prompt_next<true>(p, bar, tab, ord, it, w); ++it) {
-      const int nb = max(w.nb[0], w.nb[1]);
-      if (nb == 0) continue;
-      const int s = warp_uniform2(n % kPStages);
-      wait(&bar.kv_full[s], n / kPStages);
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        if (w.nb[t] == 0) continue;
-        wait(&bar.q_full[t], nq[t]++);
-        tc_fence_after();
-        qk(t, s, w.nb[t] == 1);
-      }
-      umma_commit_if(me, &bar.kv_empty[s]);
-      ++n;
-      // Each wait's barrier is asked some products ahead (`known`), so that the answer
-      // of one that is there does not hold up the tensor core.
-      uint32_t known_v = 0, known_p = 0;
-      for (int j = 0; j < nb; ++j) {
-        const int sv = warp_uniform2(n % kPStages), sk = (sv + 1) % kPStages;
-        const bool more = j + 1 < nb;
-        bool look = j >= w.jm;
-        wait(&bar.kv_full[sv], n / kPStages, known_v);
-        if (look && me) mbar_arrive(&bar.v_look);
-        uint32_t known_k = more ? test(&bar.kv_full[sk], (n + 1) / kPStages) : 0;
-        const uint32_t b = dv + sv * (kPTile >> 4);
-#pragma unroll
+    } else if (warp == 9) {
+      // ---------------- MMA issuer ----------------
+      constexpr uint32_t kFmt = std::is_same_v<T, __half> ? (1u << 7 | 1u << 10) : 0u;  // clears the bf16 format bits
+      constexpr uint32_t idesc_qk = idesc_bf16_f32(kPB, kPB, false, false) & ~kFmt;
+      constexpr uint32_t idesc_pv = idesc_bf16_f32(kPB, kPD, false, true) & ~kFmt;
+      const bool me = elect_one();
+      const uint32_t tm = warp_uniform(tmem);
+      // (descriptors: the low words; Q, K and V differ in the high one)
+      const uint64_t desc_q = smem_desc_sw128(smem_u32(smem + kPOffQ), 16, 1024);
+      const uint64_t desc_v = smem_desc_sw128(smem_u32(smem + kPOffKV), kPHalf, 1024);
+      const uint32_t dq = warp_uniform(static_cast<uint32_t>(desc_q));
+      const uint32_t hi_qk = warp_uniform(static_cast<uint32_t>(desc_q >> 32));
+      const uint32_t dk = dq + ((kPOffKV - kPOffQ) >> 4);
+      const uint32_t dv = warp_uniform(static_cast<uint32_t>(desc_v));
+      const uint32_t hi_v = warp_uniform(static_cast<uint32_t>(desc_v >> 32));
+      int n = 0;  // ring loads consumed
+      int nq[2] = {0, 0}, np[2] = {0, 0};
+      uint32_t looks = 0;  // V blocks handed to warps 10 and 11
+      auto wait = [&](uint64_t* b, uint32_t ph, uint32_t known = 0) {
+        mbar_wait_fast(b, ph & 1, abort_flag, p.status, known);
+      };
+      auto test = [](uint64_t* b, uint32_t ph) { return mbar_test(b, ph & 1); };
+      // S_t = Q_t K^T of the block in `stage`; the last one of an item frees Q_t
+      auto qk = [&](int t, int stage, bool last) {
+        const uint32_t a = dq + t * (kPTile >> 4), b = dk + stage * (kPTile >> 4);
+  #pragma unroll
+        for (int kk = 0; kk < kPD / 16; ++kk) {
+          const uint32_t off = ((kk >> 2) * kPHalf + (kk & 3) * 32) >> 4;
+          umma_f16_if(me, tm + t * kPB, a + off, b + off, hi_qk, idesc_qk, kk > 0);
+        }
+        umma_commit_if(me, &bar.s_full[t]);
+        umma_commit_if(me && last, &bar.q_empty[t]);
+      };
+      for (int it = 0; prompt_next<true>(p, bar, tab, ord, it, w); ++it) {
+        const int nb = max(w.nb[0], w.nb[1]);
+        if (nb == 0) continue;
+        const int s = warp_uniform2(n % kPStages);
+        wait(&bar.kv_full[s], n / kPStages);
+  #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          if (j < w.nb[t]) {
-            auto pv = [&](int kk) {
-              umma_f16_ts_if(me, tm + kPTmemO + t * kPD, tm + t * kPB + kk * 8, b + kk * (2048 >> 4), hi_v, idesc_pv,
-                             j > 0 || kk > 0);
-            };
-            wait(&bar.p_part[t], np[t], known_p);
-            if (look) wait(&bar.v_ok, looks++);
-            look = false;
-            tc_fence_after();
-            const uint32_t known = test(&bar.p_full[t], np[t]);
-#pragma unroll
-            for (int kk = 0; kk < kPart1 / 16; ++kk) pv(kk);
-            wait(&bar.p_full[t], np[t]++, known);
-            tc_fence_after();
-#pragma unroll
-            for (int kk = kPart1 / 16; kk < kPB / 16; ++kk) pv(kk);
-            umma_commit_if(me && j + 1 == w.nb[t], &bar.o_full[t]);
+          if (w.nb[t] == 0) continue;
+          wait(&bar.q_full[t], nq[t]++);
+          tc_fence_after();
+          qk(t, s, w.nb[t] == 1);
+        }
+        umma_commit_if(me, &bar.kv_empty[s]);
+        ++n;
+        // Each wait's barrier is asked some products ahead (`known`), so that the answer
+        // of one that is there does not hold up the tensor core.
+        uint32_t known_v = 0, known_p = 0;
+        for (int j = 0; j < nb; ++j) {
+          const int sv = warp_uniform2(n % kPStages), sk = (sv + 1) % kPStages;
+          const bool more = j + 1 < nb;
+          bool look = j >= w.jm;
+          wait(&bar.kv_full[sv], n / kPStages, known_v);
+          if (look && me) mbar_arrive(&bar.v_look);
+          uint32_t known_k = more ? test(&bar.kv_full[sk], (n + 1) / kPStages) : 0;
+          const uint32_t b = dv + sv * (kPTile >> 4);
+  #pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (j < w.nb[t]) {
+              auto pv = [&](int kk) {
+                umma_f16_ts_if(me, tm + kPTmemO + t * kPD, tm + t * kPB + kk * 8, b + kk * (2048 >> 4), hi_v, idesc_pv,
+                               j > 0 || kk > 0);
+              };
+              wait(&bar.p_part[t], np[t], known_p);
+              if (look) wait(&bar.v_ok, looks++);
+              look = false;
+              tc_fence_after();
+              const uint32_t known = test(&bar.p_full[t], np[t]);
+  #pragma unroll
+              for (int kk = 0; kk < kPart1 / 16; ++kk) pv(kk);
+              wait(&bar.p_full[t], np[t]++, known);
+              tc_fence_after();
+  #pragma unroll
+              for (int kk = kPart1 / 16; kk < kPB / 16; ++kk) pv(kk);
+              umma_commit_if(me && j + 1 == w.nb[t], &bar.o_full[t]);
+            }
+            if (more && t == 0) wait(&bar.kv_full[sk], (n + 1) / kPStages, known_k);
+            known_p = test(&bar.p_part[t ^ 1], np[t ^ 1]);
+            if (t == 1 && more) known_v = test(&bar.kv_full[(sv + 2) % kPStages], (n + 2) / kPStages);
+            if (j + 1 < w.nb[t]) qk(t, sk, j + 2 == w.nb[t]);
+            if (t == 1) umma_commit_if(me, &bar.kv_empty[sv]);
           }
-          if (more && t == 0) wait(&bar.kv_full[sk], (n + 1) / kPStages, known_k);
-          known_p = test(&bar.p_part[t ^ 1], np[t ^ 1]);
-          if (t == 1 && more) known_v = test(&bar.kv_full[(sv + 2) % kPStages], (n + 2) / kPStages);
-          if (j + 1 < w.nb[t]) qk(t, sk, j + 2 == w.nb[t]);
-          if (t == 1) umma_commit_if(me, &bar.kv_empty[sv]);
+          umma_commit_if(me && more, &bar.kv_empty[sk]);
+          n += more ? 2 : 1;
         }
-        umma_commit_if(me && more, &bar.kv_empty[sk]);
-        n += more ? 2 : 1;
       }
-    }
-    // all issued MMAs complete before TMEM is released
-    umma_commit_if(me, &bar.fin);
-    if (me) mbar_wait_drain(&bar.fin, 0);
-    __syncwarp();
-  } else if (warp >= 10) {
-    // ---------------- V blocks that are partly hidden: values that are not finite ----------------
-    fewer_registers();
-    // (the MMA warp hands them over in order, right after the block's QK, so
-    // the check runs beside the block's softmax)
-    int n = 0;
-    uint32_t looks = 0;
-    for (int it = 0; prompt_next<true>(p, bar, tab, ord, it, w); ++it) {
-      const int nb = max(w.nb[0], w.nb[1]);
-      for (int j = min(w.jm, nb); j < nb; ++j) {
-        const int m = n + 2 * j + 1, s = m % kPStages;
-        mbar_wait_fast(&bar.v_look, looks++ & 1, abort_flag, p.status);
-        mbar_wait_fast(&bar.kv_full[s], (m / kPStages) & 1, abort_flag, p.status);
-        // this warp's half, 512 bytes a step
-        constexpr int kSteps = static_cast<int>(kPTile / 1024);
-        const uint32_t v = smem_u32(smem + kPOffKV + s * kPTile) + (warp - 10) * (kPTile / 2) + lane * 16;
-        uint32_t top = 0;  // largest magnitudes, NaN above all
-#pragma unroll 8
-        for (int i = 0; i < kSteps; ++i) {
-          const uint4 x = lds128(v + i * 512);
-          top = abs_max2<T>(abs_max2<T>(abs_max2<T>(abs_max2<T>(top, x.x), x.y), x.z), x.w);
-        }
-        if (__any_sync(0xFFFFFFFFu, not_finite2<T>(top) != 0)) {
-          auto fix = [](uint32_t x) {
-            const uint32_t b = not_finite2<T>(x);
-            return x & ~(((b >> 15) & 0x00010001u) * 0xFFFFu);
-          };
-#pragma unroll 1
+      // all issued MMAs complete before TMEM is released
+      umma_commit_if(me, &bar.fin);
+      if (me) mbar_wait_drain(&bar.fin, 0);
+      __syncwarp();
+    } else {
+      // ---------------- V blocks that are partly hidden: values that are not finite ----------------
+      // (the MMA warp hands them over in order, right after the block's QK, so
+      // the check runs beside the block's softmax)
+      int n = 0;
+      uint32_t looks = 0;
+      for (int it = 0; prompt_next<true>(p, bar, tab, ord, it, w); ++it) {
+        const int nb = max(w.nb[0], w.nb[1]);
+        for (int j = min(w.jm, nb); j < nb; ++j) {
+          const int m = n + 2 * j + 1, s = m % kPStages;
+          mbar_wait_fast(&bar.v_look, looks++ & 1, abort_flag, p.status);
+          mbar_wait_fast(&bar.kv_full[s], (m / kPStages) & 1, abort_flag, p.status);
+          // this warp's half, 512 bytes a step
+          constexpr int kSteps = static_cast<int>(kPTile / 1024);
+          const uint32_t v = smem_u32(smem + kPOffKV + s * kPTile) + (warp - 10) * (kPTile / 2) + lane * 16;
+          uint32_t top = 0;  // largest magnitudes, NaN above all
+  #pragma unroll 8
           for (int i = 0; i < kSteps; ++i) {
-            uint4 x = lds128(v + i * 512);
-            x.x = fix(x.x);
-            x.y = fix(x.y);
-            x.z = fix(x.z);
-            x.w = fix(x.w);
-            sts128(v + i * 512, x);
+            const uint4 x = lds128(v + i * 512);
+            top = abs_max2<T>(abs_max2<T>(abs_max2<T>(abs_max2<T>(top, x.x), x.y), x.z), x.w);
           }
-          fence_proxy_async_smem();
-          if (lane == 0) *const_cast<volatile int*>(&bar.poison) = 1;
+          if (__any_sync(0xFFFFFFFFu, not_finite2<T>(top) != 0)) {
+            auto fix = [](uint32_t x) {
+              const uint32_t b = not_finite2<T>(x);
+              return x & ~(((b >> 15) & 0x00010001u) * 0xFFFFu);
+            };
+  #pragma unroll 1
+            for (int i = 0; i < kSteps; ++i) {
+              uint4 x = lds128(v + i * 512);
+              x.x = fix(x.x);
+              x.y = fix(x.y);
+              x.z = fix(x.z);
+              x.w = fix(x.w);
+              sts128(v + i * 512, x);
+            }
+            fence_proxy_async_smem();
+            if (lane == 0) *const_cast<volatile int*>(&bar.poison) = 1;
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bar.v_ok);
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bar.v_ok);
+        n += 2 * nb;
       }
-      n += 2 * nb;
     }
-  } else if (warp < 8) {
+  } else {
     // ---------------- softmax and output of tile t ----------------
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPRegsSoftmax));
     const int t = warp >> 2;

@@ -1,0 +1,29 @@
+"""Rules of the kernels' sources that no run shows (CPU only)."""
+
+import re
+from pathlib import Path
+
+import pytest
+
+CSRC = Path(__file__).resolve().parents[1] / "retree_b200" / "csrc"
+
+
+def _code(name: str) -> str:
+    return re.sub(r"//[^\n]*", "", (CSRC / name).read_text())
+
+
+@pytest.mark.parametrize("name", [p.name for p in sorted(CSRC.glob("*.cu")) if "setmaxnreg" in p.read_text()])
+def test_a_warpgroup_changes_its_registers_in_one_instruction(name):
+    """Every thread of a warpgroup has to run the same setmaxnreg: it opens a branch of whole warpgroups."""
+    code = _code(name)
+    sites = [m.start() for m in re.finditer(r"setmaxnreg", code)]
+    assert sites
+    for at in sites:
+        before = code[:at].rstrip()
+        assert before.endswith('asm volatile("'), before[-80:]
+        opening = before[: -len('asm volatile("')].rstrip().splitlines()[-1].strip()
+        split = re.fullmatch(r"(?:\} else )?if \(warp (?:<|>=) (\d+)\) \{", opening)
+        assert opening == "} else {" or (split and int(split.group(1)) % 4 == 0), opening
+    # one for each direction of a kernel
+    kernels = code.count("__global__")
+    assert code.count("setmaxnreg.dec") <= kernels and code.count("setmaxnreg.inc") <= kernels
