@@ -159,6 +159,7 @@ __device__ __forceinline__ bool prompt_next(const PromptParams& p, PromptBars& b
     if constexpr (kWarp) mbar_wait_fast(&bar.clc_full[s], ((it - 1) >> 1) & 1, &bar.abort_flag, p.status);
     else mbar_wait(&bar.clc_full[s], ((it - 1) >> 1) & 1, &bar.abort_flag, p.status, RT_DEV_WAIT_TIMEOUT);
     idx = *const_cast<volatile int*>(&bar.abort_flag) ? -1 : clc_taken(smem_u32(&bar.clc[s]));
+    fence_proxy_async_smem();  // the slot's next answer is an async-proxy write: this read comes first
     if constexpr (kWarp) {
       idx = __reduce_min_sync(0xFFFFFFFFu, idx);  // (the same in every lane but for an abort in between)
       mbar_arrive_warp(&bar.clc_empty[s]);

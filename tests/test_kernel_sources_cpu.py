@@ -27,3 +27,11 @@ def test_a_warpgroup_changes_its_registers_in_one_instruction(name):
     # one for each direction of a kernel
     kernels = code.count("__global__")
     assert code.count("setmaxnreg.dec") <= kernels and code.count("setmaxnreg.inc") <= kernels
+
+
+def test_a_launch_control_answer_is_read_before_its_slot_is_freed():
+    """The next answer is written by the async proxy: a proxy fence orders this one's reads before it."""
+    body = _code("prompt_attn.cu").split("bool prompt_next(", 1)[1].split("return true;", 1)[0]
+    read, fence = body.index("clc_taken("), body.index("fence_proxy_async_smem()")
+    frees = [m.start() for m in re.finditer(r"mbar_arrive(_warp)?\(&bar\.clc_empty", body)]
+    assert len(frees) == 2 and read < fence < min(frees)
