@@ -306,7 +306,8 @@ __global__ void __launch_bounds__(kQsThreads, 1) tree_attn_q4_small_kernel(const
         pf[mt][nt] = make_uint2(transpose8x8(pack_bf16x2(p0, p1)), transpose8x8(pack_bf16x2(p2, p3)));
       }
     }
-    // the stage is read (every lane has taken part in the votes above): refill it
+    // refill the stage once every lane has read it
+    __syncwarp();
     if (lane == 0 && i + kQsStages < tiles) issue(i + kQsStages);
     // ---- O^T += V^T P^T: a step is 16 keys; an m-tile two values of every lane g's sixteen
 #pragma unroll

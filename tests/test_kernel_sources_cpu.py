@@ -35,3 +35,10 @@ def test_a_launch_control_answer_is_read_before_its_slot_is_freed():
     read, fence = body.index("clc_taken("), body.index("fence_proxy_async_smem()")
     frees = [m.start() for m in re.finditer(r"mbar_arrive(_warp)?\(&bar\.clc_empty", body)]
     assert len(frees) == 2 and read < fence < min(frees)
+
+
+def test_a_ring_stage_is_refilled_after_every_lane_has_read_it():
+    """Votes order no memory; a __syncwarp does."""
+    code = _code("tree_attn_q4.cu")
+    refill = code.index("if (lane == 0 && i + kQsStages < tiles) issue(i + kQsStages);")
+    assert code[:refill].rstrip().endswith("__syncwarp();")
