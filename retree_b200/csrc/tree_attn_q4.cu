@@ -557,6 +557,7 @@ __global__ void __launch_bounds__(kQtThreads, 1)
   const bool inside = prefix_fits(p, L);                // the same in every thread of the launch
   const int64_t total = inside ? L + p.n : 0;
   if (!inside && tid == 0) set_status(p.status, RT_DEV_BAD_INDEX);
+  __syncwarp();  // (whole warps for setmaxnreg)
   int64_t b0 = 0, b1 = 0;
   if (inside) split_range(total, split, mine, kQtKeys, b0, b1);
   const int nb = static_cast<int>(b1 - b0);

@@ -42,3 +42,13 @@ def test_a_ring_stage_is_refilled_after_every_lane_has_read_it():
     code = _code("tree_attn_q4.cu")
     refill = code.index("if (lane == 0 && i + kQsStages < tiles) issue(i + kQsStages);")
     assert code[:refill].rstrip().endswith("__syncwarp();")
+
+
+def test_warps_are_whole_where_they_change_their_registers():
+    """A lane's own branch right before an aligned instruction ends in a __syncwarp (or a block barrier)."""
+    for name in ("prompt_attn.cu", "tree_attn_q4.cu"):
+        code = _code(name)
+        for m in re.finditer(r"setmaxnreg\.dec", code):
+            before = code[: m.start()]
+            barrier = max(before.rfind("__syncthreads();"), before.rfind("__syncwarp();"))
+            assert not re.search(r"(tid|lane) == 0", before[barrier:]), name
