@@ -21,6 +21,9 @@ def quantise(x: torch.Tensor):
     hi = torch.maximum(g.amax(-1, keepdim=True), zero)
     mant, expo = torch.frexp((hi - lo) / 15)
     s = torch.ldexp(torch.ceil(mant * 16) / 16, expo)
+    # (hi - lo may have lost its small end even in 64 bits; 15 s less the large end loses nothing)
+    short = 15 * s - torch.maximum(hi, -lo) < torch.minimum(hi, -lo)
+    s = torch.where(short, s + torch.ldexp(torch.full_like(s, 1 / 16), torch.frexp(s)[1]), s)
     s = torch.where(s < 2.0 ** -126, zero, s)
     d = torch.where(s == 0, 1.0, s)
     z = torch.round(-lo / d)

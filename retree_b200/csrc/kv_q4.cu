@@ -53,8 +53,10 @@ __device__ __forceinline__ void quantise8(const uint4& raw, uint32_t& code, uint
   word = kQ4NanWord;
   if (spoilt) return;
   // (hi - lo) / 15, halved first so that the difference cannot overflow, and up to
-  // four significant bits
-  const float d = __fsub_rn(0.5f * hi, 0.5f * lo);
+  // four significant bits.  The difference is rounded up: 7.5 times a scale has 8
+  // bits, so one that the exact difference passes, by however little, d passes by a
+  // step of fp32, and the quotient by more than half a step, which its rounding keeps.
+  const float d = __fsub_ru(0.5f * hi, 0.5f * lo);
   const bool plain = d >= 1.7347235e-17f && d <= 1.2676506e30f;  // 2^-56, 2^100
   float s = plain ? quotient(d, 7.5f, 1.f / 7.5f) : __fdiv_rn(d, 7.5f);
   s = __uint_as_float((__float_as_uint(s) + 0xFFFFFu) & ~0xFFFFFu);

@@ -13,7 +13,8 @@
 //   lo = min(0, min x), hi = max(0, max x)
 //   s  = (hi - lo) / 15 rounded up to four significant bits (0 below 2^-126)
 //   z  = rne(-lo / s),  u = clamp(rne(x / s) + z, 0, 15)
-// Both quotients are correctly rounded in fp32, and x (8 significant bits)
+// hi - lo is rounded up in fp32 and its quotient correctly, which gives the exact s.
+// The other two quotients are correctly rounded in fp32, and x (8 significant bits)
 // either equals a half-integer times s (9 bits) or is off it by 2^-9 or more,
 // so every rounding decision is the exact one.  A row holding a value that is
 // not finite gets NaN scales: all of its 128 values read as NaN.

@@ -394,3 +394,23 @@ def test_codes_of_symmetric_ranges_are_clamped():
     assert torch.equal(slab, want)
     top = kernels.kv_read_q4(slab, 0, 40)[0, 0, :, 0].float()
     assert torch.equal(top, 7 * 2.0 ** torch.arange(-20, 20, device=dev))
+
+
+def _edge_groups(ends):
+    """Rows whose four groups have the given (hi, lo), the values in between among them."""
+    x = torch.zeros((1, len(ends), 128), dtype=torch.float64)
+    for i, (hi, lo) in enumerate(ends):
+        x[0, i, 0::32], x[0, i, 1::32], x[0, i, 2::32] = hi, lo, hi / 3
+    return x.to(torch.bfloat16)
+
+
+def test_scales_of_ranges_whose_small_end_is_below_the_large_ones_last_bit():
+    """15 times a scale of four bits and a little more takes the next scale, however little it is."""
+    dev = cuda()
+    ends = [(15 * m / 8 * 2.0 ** e, -15 * 2.0 ** (e - k)) for m in range(8, 16) for e in (-100, -60, -27, 0, 40, 98, 120)
+            for k in (7, 20, 23, 24, 25, 30, 53, 60, 90)]
+    x = _edge_groups(ends).to(dev)
+    slab = torch.zeros((2, 1, len(ends), 72), dtype=torch.uint8, device=dev)
+    kernels.kv_append_q4(slab[0], slab[1], x, -x)
+    kernels.check_device_status(dev)
+    assert torch.equal(slab, q4.pack(torch.stack([x, -x])))

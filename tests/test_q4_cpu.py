@@ -114,3 +114,19 @@ def test_wrappers_refuse_cpu_tensors():
                  lambda: kernels.tree_attention_q4(q, c, c, torch.ones(2, 1, dtype=torch.int32), 2)):
         with pytest.raises(RuntimeError, match="CUDA"):
             call()
+
+
+def test_a_scale_covers_its_range_to_the_last_bit():
+    """15 s >= hi - lo in exact arithmetic, for a small end of any size, and the scale below does not."""
+    from fractions import Fraction
+    for m in range(8, 16):
+        for k in (7, 20, 24, 25, 30, 53, 60, 120):
+            x = torch.zeros((2, 128), dtype=torch.bfloat16)
+            x[0, ::32], x[0, 1::32] = 15 * m / 8, -15 * 2.0 ** -k
+            x[1] = -x[0]
+            span = Fraction(float(x[0, 0])) - Fraction(float(x[0, 1]))
+            for got in q4.quantise(x)[2][:, 0, 0].tolist():
+                s = Fraction(got)
+                assert 15 * s >= span, (m, k)
+                step = Fraction(1, 4) if s > 2 else Fraction(1, 8)
+                assert 15 * (s - step if s > 1 else Fraction(15, 16)) < span, (m, k)
