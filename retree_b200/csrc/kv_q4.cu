@@ -59,9 +59,12 @@ __device__ __forceinline__ void quantise8(const uint4& raw, uint32_t& code, uint
   const float d = __fsub_ru(0.5f * hi, 0.5f * lo);
   const bool plain = d >= 1.7347235e-17f && d <= 1.2676506e30f;  // 2^-56, 2^100
   float s = plain ? quotient(d, 7.5f, 1.f / 7.5f) : __fdiv_rn(d, 7.5f);
+  // (asked before: below 2^-126 a step of this rounding is 2^-129, not four bits; the
+  // largest four-bit number there is 15/16 of 2^-126)
+  const bool flat = s <= 1.10202596e-38f;
   s = __uint_as_float((__float_as_uint(s) + 0xFFFFFu) & ~0xFFFFFu);
   word = 0;
-  if (s < 1.17549435e-38f) return;
+  if (flat) return;
   float x[8];
   const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll

@@ -414,3 +414,13 @@ def test_scales_of_ranges_whose_small_end_is_below_the_large_ones_last_bit():
     kernels.kv_append_q4(slab[0], slab[1], x, -x)
     kernels.check_device_status(dev)
     assert torch.equal(slab, q4.pack(torch.stack([x, -x])))
+
+
+def test_groups_read_as_zero_below_the_smallest_normal_scale():
+    dev = cuda()
+    ends = [(m / 16 * 2.0 ** -126, 0.0) for m in range(128, 256)] + [(0.0, -m / 16 * 2.0 ** -126) for m in range(200, 256)]
+    x = _edge_groups(ends).to(dev)
+    slab = torch.zeros((2, 1, len(ends), 72), dtype=torch.uint8, device=dev)
+    kernels.kv_append_q4(slab[0], slab[1], x, -x)
+    kernels.check_device_status(dev)
+    assert torch.equal(slab, q4.pack(torch.stack([x, -x])))
