@@ -159,6 +159,20 @@ def _q4_forward(query, key, value, attention_mask, scaling, causal: bool, rows, 
                                      prefix_len_dev=prefix_dev)
 
 
+def _check_key_offsets(cu_q, cu_k, keys: int) -> None:
+    """Packed queries over more keys than queries: the keys' offsets have to reach the last key.
+
+    Callers without a cache pass the queries' offsets for both; over a cache those
+    are in range, but name its first rows.  (One read of an offset, on this path only.)
+    """
+    if cu_k is None or cu_k is cu_q or cu_k.data_ptr() == cu_q.data_ptr():
+        raise RuntimeError("packed queries over cached keys need the keys' own offsets")
+    if cu_k.is_cuda and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("packed queries over cached keys are not captured: their offsets are checked on the host")
+    if int(cu_k[-1]) != keys:
+        raise RuntimeError(f"packed queries over cached keys: cu_seq_lens_k ends before the last of the {keys} keys")
+
+
 def _tree_forward(query, key, value, attention_mask, scaling, causal: bool, timer) -> torch.Tensor:
     """rt_tree_attn over bf16 K/V: the mask's tree, or the new tokens as a chain."""
     n = query.shape[2]
@@ -200,8 +214,10 @@ def tree_attention_forward(module, query: torch.Tensor, key: torch.Tensor, value
     prefix = key.shape[2] - n if rows is None else rows.prefix_len
     timer = _Timer()
     if cu_q is not None and attention_mask is None:
-        if not causal or (rows is not None and rows.prefix_len > 0) or (cu_k is None and key.shape[2] != n):
+        if not causal or (rows is not None and (rows.device_length or rows.prefix_len > 0)):
             raise RuntimeError("packed sequences run causally over keys of their own (no cached prefix)")
+        if rows is None and key.shape[2] != n:
+            _check_key_offsets(cu_q, cu_k, key.shape[2])
         timer.start()
         out = kernels.prompt_attention(query, key, value, cu_seqlens_q=cu_q, cu_seqlens_k=cu_k, scale=scaling)
     elif rows is not None:
