@@ -39,7 +39,7 @@ import numpy as np
 import torch
 
 from . import kernels
-from .cache import Q4_ATTR
+from .cache import Q4Rows
 
 NAME = "retree_tree"
 
@@ -139,13 +139,13 @@ class _Timer:
             PROFILE.append((*self.events, *shape))
 
 
-def _q4_forward(query, key, value, attention_mask, scaling, causal: bool, rows, timer) -> torch.Tensor:
+def _q4_forward(query, attention_mask, scaling, causal: bool, rows: Q4Rows, timer) -> torch.Tensor:
     """Attention of new tokens over a 4-bit cache that already holds their rows."""
     n, hq = query.shape[2], query.shape[1]
     if attention_mask is None and not rows.device_length and causal:
         if rows.prefix_len == 0:
             timer.start()
-            return kernels.prompt_attention(query, key, value, scale=scaling)
+            return kernels.prompt_attention(query, rows.k_new, rows.v_new, scale=scaling)
         if n > _Q4_CHAIN_MAX:
             timer.start()
             k, v = (kernels.kv_read_q4(x, 0, rows.prefix_len + n) for x in (rows.k, rows.v))
@@ -209,7 +209,7 @@ def tree_attention_forward(module, query: torch.Tensor, key: torch.Tensor, value
     if causal is None:
         causal = getattr(module, "is_causal", True)
     causal = bool(causal)
-    rows = getattr(key, Q4_ATTR, None)
+    rows = key if isinstance(key, Q4Rows) else None
     cu_q, cu_k = kwargs.get("cu_seq_lens_q"), kwargs.get("cu_seq_lens_k")
     prefix = key.shape[2] - n if rows is None else rows.prefix_len
     timer = _Timer()
@@ -218,10 +218,11 @@ def tree_attention_forward(module, query: torch.Tensor, key: torch.Tensor, value
             raise RuntimeError("packed sequences run causally over keys of their own (no cached prefix)")
         if rows is None and key.shape[2] != n:
             _check_key_offsets(cu_q, cu_k, key.shape[2])
+        k, v = (key, value) if rows is None else (rows.k_new, rows.v_new)
         timer.start()
-        out = kernels.prompt_attention(query, key, value, cu_seqlens_q=cu_q, cu_seqlens_k=cu_k, scale=scaling)
+        out = kernels.prompt_attention(query, k, v, cu_seqlens_q=cu_q, cu_seqlens_k=cu_k, scale=scaling)
     elif rows is not None:
-        out = _q4_forward(query, key, value, attention_mask, scaling, causal, rows, timer)
+        out = _q4_forward(query, attention_mask, scaling, causal, rows, timer)
     elif _PROMPT_KERNEL.get() and attention_mask is None and causal:
         timer.start()
         out = kernels.prompt_attention(query, key, value, scale=scaling)

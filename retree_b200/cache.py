@@ -24,8 +24,6 @@ length from the same device word.
 
 from __future__ import annotations
 
-from types import SimpleNamespace
-
 import torch
 from transformers.cache_utils import Cache, CacheLayerMixin
 
@@ -197,11 +195,7 @@ class TreeKVLayerQ4(TreeKVLayer):
         return kernels.kv_read_q4(self._cache.slab[2 * self.index + kv], 0, length).unsqueeze(0)
 
     def update(self, key_states: torch.Tensor, value_states: torch.Tensor, *args, **kwargs):
-        """Quantise the new rows into the cache; returns them, tagged with where the cache's rows are.
-
-        The attention backend reads the cache itself (``Q4_ATTR``), so no bf16
-        copy of the cached rows is made.
-        """
+        """Quantise the new rows into the cache; returns what stands for all rows (``Q4Rows``), as keys and values."""
         c = self._cache
         n = key_states.shape[-2]
         before = self.length
@@ -215,14 +209,39 @@ class TreeKVLayerQ4(TreeKVLayer):
             c.append(self.index, key_states, value_states, offset=before)
             self.length += n
             prefix = before
-        tagged = key_states.view(key_states.shape)  # (a tensor of its own to carry the tag)
-        setattr(tagged, Q4_ATTR, SimpleNamespace(k=c.slab[2 * self.index], v=c.slab[2 * self.index + 1],
-                                                 prefix_len=prefix, device_length=c.device_length))
-        return tagged, value_states
+        rows = Q4Rows(c.slab[2 * self.index], c.slab[2 * self.index + 1], key_states, value_states, prefix,
+                      c.device_length)
+        return rows, rows
 
 
-#: attribute of the key tensor a 4-bit cache hands to the attention backend
-Q4_ATTR = "_rt_q4"
+class Q4Rows(torch.Tensor):
+    """The keys (and values) a 4-bit cache hands to the attention backend.
+
+    It has the shape that ``TreeKVCache`` would return, but no data: the
+    ``retree_tree`` backend reads the cache's rows (``k``, ``v``: uint8 ``[heads,
+    capacity, 72]``, of which ``prefix_len`` rows and the new ones are used) or, for a
+    prompt over an empty cache, the new rows (``k_new``, ``v_new``), so no bf16 copy of the cached
+    rows is made.  Any other use, by another backend, is an error.
+    """
+
+    @staticmethod
+    def __new__(cls, k, v, k_new, v_new, prefix_len: int, device_length: bool):
+        shape = (*k_new.shape[:-2], prefix_len + k_new.shape[-2], k_new.shape[-1])
+        self = torch.Tensor._make_wrapper_subclass(cls, shape, dtype=k_new.dtype, device=k_new.device)
+        self.k, self.v, self.k_new, self.v_new = k, v, k_new, v_new
+        self.prefix_len, self.device_length = prefix_len, device_length
+        return self
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise RuntimeError(f"rows of a 4-bit cache are read by the retree_tree attention backend only (asked for "
+                           f"{func}); cache.layers[i].keys and .values are decoded copies")
+
+    def data_ptr(self):
+        raise RuntimeError("rows of a 4-bit cache have no data of their own")
+
+    def __repr__(self, **kwargs):
+        return f"Q4Rows(shape={tuple(self.shape)}, prefix_len={self.prefix_len})"
 
 
 class TreeKVCacheQ4(TreeKVCache):
@@ -232,7 +251,8 @@ class TreeKVCacheQ4(TreeKVCache):
     in ``include/retree_b200.h``, RT_Q4_ROW_BYTES); the capacity is rounded up to
     an even number.  Appending quantises (``kernels.kv_append_q4``), the
     ``retree_tree`` attention reads the 4-bit rows (``kernels.tree_attention_q4``),
-    compaction moves them as they are.  A prompt over an empty cache attends to
+    compaction moves them as they are.  Other attention backends are refused
+    (``for_model``, ``Q4Rows``).  A prompt over an empty cache attends to
     its own bf16 keys and values; whatever comes later attends to the cached
     rows, its own among them, so a token's result does not depend on whether its
     ancestors were committed or are still in the tree.
@@ -246,6 +266,17 @@ class TreeKVCacheQ4(TreeKVCache):
         self.capacity += self.capacity & 1
         return torch.zeros((2 * self.num_layers, self.num_kv_heads, self.capacity, kernels.Q4_ROW_BYTES),
                            dtype=torch.uint8, device=self.device)
+
+    @classmethod
+    def for_model(cls, config, capacity: int, dtype=torch.bfloat16, device=None) -> "TreeKVCacheQ4":
+        from .attention import NAME
+        from .headsplit import NAME as HEADSPLIT_NAME
+
+        impl = getattr(config, "_attn_implementation", None)
+        if impl not in (None, NAME, HEADSPLIT_NAME):
+            raise RuntimeError(f"a 4-bit cache needs attn_implementation={NAME!r} (or {HEADSPLIT_NAME!r}), "
+                               f"not {impl!r}")
+        return super().for_model(config, capacity, dtype, device)
 
     def append(self, layer: int, k_new: torch.Tensor, v_new: torch.Tensor, offset: int = 0,
                offset_dev: torch.Tensor | None = None) -> None:

@@ -260,3 +260,16 @@ def test_packed_queries_over_earlier_keys_need_their_offsets():
         one, _ = attention.tree_attention_forward(_Module(), q, key, value, None, scaling=0.1)
     kernels.check_device_status(dev)
     assert torch.equal(out, one)
+
+
+@torch.inference_mode()
+def test_another_backend_over_a_4bit_cache_is_an_error():
+    """A prompt and a single token after it: neither runs on a part of the keys."""
+    dev = cuda()
+    m = build_target(_cfg(1), device=dev, seed=4, attn_implementation="sdpa")
+    cache = TreeKVCacheQ4(1, 2, 128, 64, device=dev)
+    for n in (5, 1):
+        with pytest.raises(RuntimeError, match="4-bit"):
+            m(_ids(n, n, dev), past_key_values=cache, use_cache=True)
+    with pytest.raises(RuntimeError, match="retree_tree"):
+        TreeKVCacheQ4.for_model(m.config, capacity=64, device=dev)
