@@ -865,11 +865,11 @@ struct Q4Plan {
   int heavy, tail;  // of the tiles of two-tile CTAs, of a last single one
 };
 
-// Clusters of `c` CTAs of `kernel` that fit on the GPU at once (0 when the query
+// Clusters of `c` CTAs of `kernel` that fit on the GPU at once (-1 when the query
 // fails, e.g. without a device).
 template <typename Kernel>
 static int clusters_fit(Kernel kernel, int threads, uint32_t smem, int c) {
-  int n = 0;
+  int n = -1;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) ==
           cudaSuccess &&
       (c <= 8 || cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess)) {
@@ -884,25 +884,31 @@ static int clusters_fit(Kernel kernel, int threads, uint32_t smem, int c) {
     attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) n = -1;
   }
   cudaGetLastError();
   return n;
 }
 
-// ... of the few-rows kernel, or of the tile kernel (cached per size).
+// ... of the few-rows kernel, or of the tile kernel: an answer is kept per device and
+// size, a failed query counts as none and is asked again.
 static int q4_clusters_fit(bool small, int c) {
+  constexpr int kDevices = 64;
   static std::mutex mu;
-  static int cache[2][kMaxMerge + 1] = {};
-  static bool done[2][kMaxMerge + 1] = {};
-  std::lock_guard<std::mutex> lock(mu);
+  static int cache[kDevices][2][kMaxMerge + 1] = {};  // answer + 1, 0: not asked yet
   if (c < 2 || c > kMaxMerge) return 0;
-  if (!done[small][c]) {
-    cache[small][c] = small ? clusters_fit(tree_attn_q4_small_kernel<2>, kQsThreads, kQsSmem, c)
-                            : clusters_fit(tree_attn_q4_tile_kernel, kQtThreads, kQtSmem, c);
-    done[small][c] = true;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kDevices) {
+    cudaGetLastError();
+    return 0;
   }
-  return cache[small][c];
+  std::lock_guard<std::mutex> lock(mu);
+  if (cache[dev][small][c] > 0) return cache[dev][small][c] - 1;
+  const int n = small ? clusters_fit(tree_attn_q4_small_kernel<2>, kQsThreads, kQsSmem, c)
+                      : clusters_fit(tree_attn_q4_tile_kernel, kQtThreads, kQtSmem, c);
+  if (n < 0) return 0;
+  cache[dev][small][c] = n + 1;
+  return n;
 }
 
 template <int NT>

@@ -52,3 +52,9 @@ def test_warps_are_whole_where_they_change_their_registers():
             before = code[: m.start()]
             barrier = max(before.rfind("__syncthreads();"), before.rfind("__syncwarp();"))
             assert not re.search(r"(tid|lane) == 0", before[barrier:]), name
+
+
+def test_a_failed_cluster_query_is_asked_again_and_answers_are_per_device():
+    body = _code("tree_attn_q4.cu").split("static int q4_clusters_fit(", 1)[1].split("\n}\n", 1)[0]
+    assert "cudaGetDevice(&dev)" in body and "cache[dev]" in body
+    assert body.index("if (n < 0) return 0;") < body.rindex("cache[dev]")
