@@ -625,6 +625,7 @@ Q4_ROW_BYTES = _lib.RT_Q4_ROW_BYTES
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch.cuda.current_device
 _grad_enabled = torch.is_grad_enabled
+_forward_ad = torch.autograd.forward_ad
 _BF16, _F16, _U8 = torch.bfloat16, torch.float16, torch.uint8
 _STATUS_PTR: dict = {}  # device index -> address of its status word (kept for the process's life)
 _SCALE = 128 ** -0.5
@@ -655,8 +656,13 @@ def _refuse(what: str, *conditions) -> None:
     raise RuntimeError(f"{what}: tensors must be on one device")
 
 
+def _tangents(*tensors) -> bool:
+    """Whether one carries a forward-mode tangent (there are none outside a dual level)."""
+    return _forward_ad._current_level >= 0 and any(_forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def _needs_grad(*tensors) -> bool:
-    return _grad_enabled() and any(t.requires_grad for t in tensors)
+    return (_grad_enabled() and any(t.requires_grad for t in tensors)) or _tangents(*tensors)
 
 
 def _workspace(nbytes: int, dev) -> torch.Tensor:
@@ -740,7 +746,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
             and (ck is None or (cq is not None and _offsets(ck) and ck.get_device() == index
                                 and ck.numel() == cq.numel()))
             and (cq is None or (_offsets(cq) and cq.get_device() == index))
-            and not (_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad))):
+            and not (_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad))
+            and not (_forward_ad._current_level >= 0 and _tangents(q, k, v))):
         _refuse(what,
                 (q.is_cuda and k.is_cuda and v.is_cuda, "takes CUDA tensors (no CPU path)"),
                 (not _needs_grad(q, k, v), "inference-only (no gradient)"),
@@ -816,7 +823,8 @@ def kv_append_q4(k_cache: torch.Tensor, v_cache: torch.Tensor, k_new: torch.Tens
             and v_new.is_cuda and v_new.get_device() == index
             and (offset_dev is None or (offset_dev.dtype is torch.int64 and offset_dev.is_cuda
                                         and offset_dev.get_device() == index))
-            and not (_grad_enabled() and (k_new.requires_grad or v_new.requires_grad))):
+            and not (_grad_enabled() and (k_new.requires_grad or v_new.requires_grad))
+            and not (_forward_ad._current_level >= 0 and _tangents(k_new, v_new))):
         _refuse(what,
                 (all(x.is_cuda for x in (k_cache, v_cache, k_new, v_new)), "takes CUDA tensors (no CPU path)"),
                 (not _needs_grad(k_new, v_new), "inference-only (no gradient)"),
@@ -919,6 +927,7 @@ def tree_attention_q4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask_bi
             and mask_bits.is_cuda and mask_bits.get_device() == index and n and hq and hkv and hq % hkv == 0
             and mask_bits.dtype is torch.int32 and len(m_shape) == 2 and m_shape[0] >= n and m_shape[1] * 32 >= n
             and not (_grad_enabled() and q.requires_grad)
+            and not (_forward_ad._current_level >= 0 and _tangents(q))
             and (prefix_len_dev is None or (prefix_len_dev.dtype is torch.int64 and prefix_len_dev.is_cuda
                                             and prefix_len_dev.get_device() == index))):
         _refuse(what,

@@ -292,3 +292,23 @@ def test_calls_on_two_streams_at_once():
     torch.cuda.synchronize(dev)
     kernels.check_device_status(dev)
     assert all(torch.equal(got, want) for o in outs for got, want in o)
+
+
+def test_tangents_are_refused():
+    from torch.autograd import forward_ad
+    dev = cuda()
+    q, k, v = make(16, 20, 20, 8, 2, torch.bfloat16, dev)
+    slab = torch.zeros((2, 2, 32, 72), dtype=torch.uint8, device=dev)
+    bits = torch.ones((20, 1), dtype=torch.int32, device=dev)
+    with forward_ad.dual_level():
+        kernels.prompt_attention(q, k, v)  # (none of these has one)
+        for i in range(3):
+            args = [forward_ad.make_dual(x, torch.ones_like(x)) if j == i else x for j, x in enumerate((q, k, v))]
+            with pytest.raises(RuntimeError, match="gradient"):
+                kernels.prompt_attention(*args)
+            if i:
+                with pytest.raises(RuntimeError, match="gradient"):
+                    kernels.kv_append_q4(slab[0], slab[1], *args[1:])
+        with pytest.raises(RuntimeError, match="gradient"):
+            kernels.tree_attention_q4(forward_ad.make_dual(q, torch.ones_like(q)), slab[0], slab[1], bits, 4)
+    kernels.check_device_status(dev)

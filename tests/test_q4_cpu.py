@@ -130,3 +130,14 @@ def test_a_scale_covers_its_range_to_the_last_bit():
                 assert 15 * s >= span, (m, k)
                 step = Fraction(1, 4) if s > 2 else Fraction(1, 8)
                 assert 15 * (s - step if s > 1 else Fraction(15, 16)) < span, (m, k)
+
+
+def test_tangents_count_as_gradients():
+    from torch.autograd import forward_ad
+    x = torch.zeros(3)
+    assert not kernels._needs_grad(x)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones(3))
+        assert kernels._needs_grad(x, dual) and not kernels._needs_grad(x)
+        with torch.no_grad():  # (stops gradients of the backward pass only)
+            assert kernels._needs_grad(dual)
