@@ -821,7 +821,7 @@ def kv_append_q4(k_cache: torch.Tensor, v_cache: torch.Tensor, k_new: torch.Tens
             and new_shape == v_new.shape and heads == cache_heads and d == 128 and s2 == 1 and sv[2] == 1
             and v_cache.is_cuda and v_cache.get_device() == index and k_new.is_cuda and k_new.get_device() == index
             and v_new.is_cuda and v_new.get_device() == index
-            and (offset_dev is None or (offset_dev.dtype is torch.int64 and offset_dev.is_cuda
+            and (offset_dev is None or (offset_dev.dtype is torch.int64 and offset_dev.numel() and offset_dev.is_cuda
                                         and offset_dev.get_device() == index))
             and not (_grad_enabled() and (k_new.requires_grad or v_new.requires_grad))
             and not (_forward_ad._current_level >= 0 and _tangents(k_new, v_new))):
@@ -835,7 +835,8 @@ def kv_append_q4(k_cache: torch.Tensor, v_cache: torch.Tensor, k_new: torch.Tens
                 (k_new.dtype == _BF16 and v_new.dtype == _BF16, "takes bf16 rows"),
                 (k_new.shape == v_new.shape and heads == cache_heads and d == 128 and s2 == 1 and sv[2] == 1,
                  "new rows must be [cache heads, n, 128] with contiguous head_dim, the same for K and V"),
-                (offset_dev is None or offset_dev.dtype == torch.int64, "offset_dev must be int64"))
+                (offset_dev is None or (offset_dev.dtype == torch.int64 and offset_dev.numel() > 0),
+                 "offset_dev must be int64[1]"))
     if _current_device() != index:
         with torch.cuda.device(index):
             return kv_append_q4(k_cache, v_cache, k_new, v_new, offset, offset_dev)
@@ -928,7 +929,8 @@ def tree_attention_q4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask_bi
             and mask_bits.dtype is torch.int32 and len(m_shape) == 2 and m_shape[0] >= n and m_shape[1] * 32 >= n
             and not (_grad_enabled() and q.requires_grad)
             and not (_forward_ad._current_level >= 0 and _tangents(q))
-            and (prefix_len_dev is None or (prefix_len_dev.dtype is torch.int64 and prefix_len_dev.is_cuda
+            and (prefix_len_dev is None or (prefix_len_dev.dtype is torch.int64 and prefix_len_dev.numel()
+                                        and prefix_len_dev.is_cuda
                                             and prefix_len_dev.get_device() == index))):
         _refuse(what,
                 (q.is_cuda and k.is_cuda and v.is_cuda and mask_bits.is_cuda, "takes CUDA tensors (no CPU path)"),
@@ -943,7 +945,8 @@ def tree_attention_q4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask_bi
                  "at least one node, and key heads that divide the query heads"),
                 (mask_bits.dtype == torch.int32 and mask_bits.dim() == 2 and mask_bits.shape[0] >= n
                  and mask_bits.shape[1] * 32 >= n, "mask_bits must be int32 [n, at least ceil(n / 32)]"),
-                (prefix_len_dev is None or prefix_len_dev.dtype == torch.int64, "prefix_len_dev must be int64"))
+                (prefix_len_dev is None or (prefix_len_dev.dtype == torch.int64 and prefix_len_dev.numel() > 0),
+                 "prefix_len_dev must be int64[1]"))
     if _current_device() != index:
         with torch.cuda.device(index):
             return tree_attention_q4(q, k, v, mask_bits, prefix_len, scale, out, num_splits, prefix_len_dev)

@@ -424,3 +424,18 @@ def test_groups_read_as_zero_below_the_smallest_normal_scale():
     kernels.kv_append_q4(slab[0], slab[1], x, -x)
     kernels.check_device_status(dev)
     assert torch.equal(slab, q4.pack(torch.stack([x, -x])))
+
+
+def test_device_words_without_an_entry_are_refused():
+    """An empty tensor has no address, which would read as "no device word": the host's number."""
+    dev = cuda()
+    slab = torch.zeros((2, 2, 16, 72), dtype=torch.uint8, device=dev)
+    x = rows(1, dev, 2, 4)
+    none = torch.zeros(0, dtype=torch.int64, device=dev)
+    q = torch.zeros((1, 4, 128), dtype=torch.bfloat16, device=dev)
+    bits = torch.ones((1, 1), dtype=torch.int32, device=dev)
+    with pytest.raises(RuntimeError, match="offset_dev"):
+        kernels.kv_append_q4(slab[0], slab[1], x, x, offset_dev=none)
+    with pytest.raises(RuntimeError, match="prefix_len_dev"):
+        kernels.tree_attention_q4(q, slab[0], slab[1], bits, 8, prefix_len_dev=none)
+    assert int(slab.sum()) == 0
