@@ -718,8 +718,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     """Causal GQA attention over whole prompts, several sequences packed along the token axis.
 
     q: ``[T, Hq, 128]`` or HF's ``[1, Hq, T, 128]``; k, v: ``[Hkv, Tk, 128]`` or
-    ``[1, Hkv, Tk, 128]``, any token and head strides of 16 bytes; bf16 or
-    fp16.  ``cu_seqlens_q`` / ``cu_seqlens_k``: int32 CUDA offsets of the
+    ``[1, Hkv, Tk, 128]``, any token and head strides of 16 bytes (copied
+    where K and V differ in them); bf16 or fp16.  ``cu_seqlens_q`` / ``cu_seqlens_k``: int32 CUDA offsets of the
     sequences' queries and keys (``cu_seqlens_k=None``: the same offsets; both
     None: one sequence).  A sequence's queries are its last tokens: with lq
     queries and lk keys, query i sees keys ``j <= i + lk - lq``, so a chunk of a
@@ -770,8 +770,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         q, q0, q1 = _rows(q)
         k, k0, k1 = _rows(k)
         v, v0, v1 = _rows(v)
-        if (k0, k1) != (v0, v1):
-            raise RuntimeError(f"{what}: K and V must share strides")
+        if (k0, k1) != (v0, v1):  # (one set of strides for both)
+            k, v, k0, k1 = k.contiguous(), v.contiguous(), max(tk, 1) * 256, 256
     if out is None:
         out = q.new_empty((t, hq, 128))
         o0, o1 = hq * 256, 256
@@ -931,7 +931,7 @@ def tree_attention_q4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask_bi
             and not (_forward_ad._current_level >= 0 and _tangents(q))
             and (prefix_len_dev is None or (prefix_len_dev.dtype is torch.int64 and prefix_len_dev.numel()
                                         and prefix_len_dev.is_cuda
-                                            and prefix_len_dev.get_device() == index))):
+                                        and prefix_len_dev.get_device() == index))):
         _refuse(what,
                 (q.is_cuda and k.is_cuda and v.is_cuda and mask_bits.is_cuda, "takes CUDA tensors (no CPU path)"),
                 (not _needs_grad(q), "inference-only (no gradient)"),

@@ -312,3 +312,10 @@ def test_tangents_are_refused():
         with pytest.raises(RuntimeError, match="gradient"):
             kernels.tree_attention_q4(forward_ad.make_dual(q, torch.ones_like(q)), slab[0], slab[1], bits, 4)
     kernels.check_device_status(dev)
+
+
+def test_keys_and_values_of_different_strides():
+    dev = cuda()
+    q, k, v = make(17, 90, 90, 8, 2, torch.bfloat16, dev)         # rows of [tokens, heads, 128]
+    for k2, v2 in ((k.contiguous(), v), (k, v.contiguous()), (k[:1].expand(2, -1, -1), v)):
+        check(kernels.prompt_attention(q, k2, v2), q, k2, v2, [90], [90])
