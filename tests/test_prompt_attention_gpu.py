@@ -319,3 +319,83 @@ def test_keys_and_values_of_different_strides():
     q, k, v = make(17, 90, 90, 8, 2, torch.bfloat16, dev)         # rows of [tokens, heads, 128]
     for k2, v2 in ((k.contiguous(), v), (k, v.contiguous()), (k[:1].expand(2, -1, -1), v)):
         check(kernels.prompt_attention(q, k2, v2), q, k2, v2, [90], [90])
+
+
+@pytest.mark.parametrize("lens,past", [([300], [2500]), ([17], [9000]), ([1], [4000]), ([64, 200], [5000, 0])])
+def test_split_keys_fp16(lens, past):
+    dev = cuda()
+    both = [a + b for a, b in zip(lens, past)]
+    q, k, v = make(len(lens) + sum(past), sum(lens), sum(both), 8, 2, torch.float16, dev, "tokens")
+    assert kernels._prompt_workspace(0, sum(lens), sum(both), len(lens), 8, 2) > 0
+    out = kernels.prompt_attention(q, k, v, cu(lens, dev), cu(both, dev))
+    check(out, q, k, v, lens, both)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_split_keys_and_queries_without_keys(dtype):
+    """One sequence's keys are shared out, another has fewer keys than queries, a third none."""
+    dev = cuda()
+    lens, keys = [40, 60, 5, 300], [9000, 30, 0, 300]
+    q, k, v = make(21, sum(lens), sum(keys), 4, 2, dtype, dev)
+    assert kernels._prompt_workspace(0, sum(lens), sum(keys), len(lens), 4, 2) > 0
+    out = kernels.prompt_attention(q, k, v, cu(lens, dev), cu(keys, dev), out=torch.full_like(q, float("nan")))
+    check(out, q, k, v, lens, keys)
+    assert bool((out[40:70] == 0).all()) and bool((out[100:105] == 0).all())
+
+
+@pytest.mark.parametrize("what", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("where", ["k", "v"])
+@pytest.mark.parametrize("dtype,past", [(torch.bfloat16, 2500), (torch.float16, 2500), (torch.float16, 0)])
+def test_hidden_keys_do_not_reach_a_row_of_a_chunk(dtype, past, where, what):
+    """As above with the keys shared out (2500 earlier ones), and in fp16: what a row cannot see does not change it."""
+    dev = cuda()
+    n, keys = 300, 300 + past
+    q, k, v = make(22, n, keys, 8, 2, dtype, dev)
+    assert (kernels._prompt_workspace(0, n, keys, 1, 8, 2) > 0) == (past > 0)
+    offs = (cu([n], dev), cu([keys], dev))
+    clean = kernels.prompt_attention(q, k, v, *offs)
+    x = k if where == "k" else v
+    x[0, past + 250, 3] = what      # rows 250..299 of query heads 0-3 see it
+    x[1, keys - 1, :] = what        # the last row of heads 4-7 alone
+    out = kernels.prompt_attention(q, k, v, *offs)
+    kernels.check_device_status(dev)
+    touched = torch.zeros((n, 8), dtype=torch.bool, device=dev)
+    touched[250:, :4] = True
+    touched[-1, 4:] = True
+    assert torch.equal(out[~touched], clean[~touched])
+    if where == "v":
+        col = out[250:, :4, 3].float()
+        assert bool(col.isnan().all()) if what != what else bool((col == what).all())
+        rest = out[250:, :4].float()
+        rest[..., 3] = 0
+        assert bool(rest.isfinite().all())
+        last = out[-1, 4:].float()
+        assert bool(last.isnan().all()) if what != what else bool((last == what).all())
+    elif what != what:
+        assert bool(out[touched].isnan().all())
+
+
+def test_more_sequences_than_one_launch_takes():
+    dev = cuda()
+    g = torch.Generator().manual_seed(4)
+    lens = torch.randint(0, 4, (5000,), generator=g).tolist()
+    q, k, v = make(23, sum(lens), sum(lens), 4, 2, torch.bfloat16, dev)
+    out = kernels.prompt_attention(q, k, v, cu(lens, dev), out=torch.full_like(q, float("nan")))
+    kernels.check_device_status(dev)
+    # every sequence at once: [sequences, 3, ...] padded, the definition of `reference` in 64 bits
+    a = cu(lens, "cpu").long()[:-1].to(dev)
+    n = torch.tensor(lens, device=dev)
+    idx = a[:, None] + torch.arange(3, device=dev)
+    live = torch.arange(3, device=dev) < n[:, None]
+    idx = torch.where(live, idx, 0)
+    qq = q[idx].double()                                                        # [S, 3, 4, 128]
+    kk, vv = (x.transpose(0, 1)[idx].double().repeat_interleave(2, 2) for x in (k, v))
+    s = torch.einsum("sihd,sjhd->shij", qq, kk) * 128 ** -0.5
+    see = live[:, None, None, :] & torch.ones((3, 3), device=dev).tril().bool()
+    p = torch.softmax(s.masked_fill(~see, float("-inf")).nan_to_num(neginf=-1e30), -1) * see
+    ref, big = (torch.einsum("shij,sjhd->sihd", p, x) for x in (vv, vv.abs()))
+    err = (out[idx].double() - ref).abs()[live]
+    # weights and result rounded once each; the scores' part with the largest sum_d |q_d k_d| of the call
+    delta = 128 * 2.0 ** -23 * 128 ** -0.5 * float(torch.einsum("sihd,sjhd->shij", qq.abs(), kk.abs()).max())
+    bound = (2.0 ** -8 * ref.abs() + (2.0 ** -8 + 2.0 ** -20 + 3 * delta) * big)[live]
+    assert bool((err <= bound + 1e-30).all())

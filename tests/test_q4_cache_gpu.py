@@ -439,3 +439,14 @@ def test_device_words_without_an_entry_are_refused():
     with pytest.raises(RuntimeError, match="prefix_len_dev"):
         kernels.tree_attention_q4(q, slab[0], slab[1], bits, 8, prefix_len_dev=none)
     assert int(slab.sum()) == 0
+
+
+@pytest.mark.parametrize("hq,hkv", [(128, 1), (100, 1), (192, 2)])
+@pytest.mark.parametrize("n", [1, 2, 3])
+def test_groups_of_which_a_tile_holds_one_node(hq, hkv, n):
+    """More than 64 query heads a kv head: tiles of one node, with rows to spare."""
+    dev = cuda()
+    slab = caches(hq, dev, hkv, 400 + n)
+    q = rows(hq + 1, dev, n, hq)
+    parents, vis = random_tree(n, n - 1)
+    check(kernels.tree_attention_q4(q, slab[0], slab[1], bits_tensor(vis, dev), 400), q, slab, 400, vis)

@@ -273,3 +273,34 @@ def test_another_backend_over_a_4bit_cache_is_an_error():
             m(_ids(n, n, dev), past_key_values=cache, use_cache=True)
     with pytest.raises(RuntimeError, match="retree_tree"):
         TreeKVCacheQ4.for_model(m.config, capacity=64, device=dev)
+
+
+@torch.inference_mode()
+def test_a_target_split_by_kv_head_over_a_4bit_cache(model, monkeypatch):
+    """Each rank's heads over its own 4-bit cache (the gather left out) are the whole cache's heads."""
+    from retree_b200 import headsplit
+    dev = cuda()
+    monkeypatch.setattr(headsplit, "gather_heads", lambda out, group, world: out)
+    backend = headsplit.headsplit_backend(attention.tree_attention_forward)
+    L, n = 300, 17
+    k, v, q = (_rows(s, h, L + n, dev) for s, h in ((1, 2), (2, 2), (3, 8)))
+    _, vis = random_tree(7, n - 1)
+    bits = torch.from_numpy(ot.pack_bits(vis).view(np.int32)).to(dev)
+    mask = attention.attach(bits.view(1, 1, n, -1), bits)
+    outs = []
+    for heads, split in ((slice(0, 2), None), (slice(0, 1), (None, 2, 0)), (slice(1, 2), (None, 2, 1))):
+        c = make_cache(4, 1, heads.stop - heads.start, 128, 512, device=dev)
+        mod = _Module()
+        mod._rt_head_split = split
+        qh = q[:, 4 * heads.start:4 * heads.stop]
+        kh, vh = k[:, heads], v[:, heads]
+        rows = c.update(kh[:, :, :L], vh[:, :, :L], 0)
+        a, _ = backend(mod, qh[:, :, :L], *rows, None, scaling=128 ** -0.5)
+        rows = c.update(kh[:, :, L:], vh[:, :, L:], 0)
+        b, _ = backend(mod, qh[:, :, L:], *rows, mask, scaling=128 ** -0.5)
+        outs.append(torch.cat([a, b], 1))
+    kernels.check_device_status(dev)
+    split = torch.cat(outs[1:], 2)
+    # (the heads' work is shared out differently: two roundings of weights and of results, values of order one)
+    assert float((split.float() - outs[0].float()).abs().max()) < 4 * 2.0 ** -8 * float(v.abs().max())
+    assert _rel(split, outs[0]) < 2.0 ** -7
