@@ -1038,7 +1038,7 @@ extern "C" int rt_tree_attn_q4(const void* q, int64_t q_tok_stride, int64_t q_he
   if (!(scale >= 0.f) || scale > 3e38f) return RT_ERR_INVALID_ARGUMENT;
   if (head_dim != kHD) return RT_ERR_UNSUPPORTED;
   if (mask_words < (n + 31) / 32) return RT_ERR_INVALID_ARGUMENT;
-  if (prefix_len_dev == nullptr && prefix_len > kv_capacity - n) return RT_ERR_INVALID_ARGUMENT;
+  if (kv_capacity < n || (prefix_len_dev == nullptr && prefix_len > kv_capacity - n)) return RT_ERR_INVALID_ARGUMENT;
   const uint64_t align_bits = reinterpret_cast<uint64_t>(q) | reinterpret_cast<uint64_t>(k) |
                               reinterpret_cast<uint64_t>(v) | reinterpret_cast<uint64_t>(out) |
                               static_cast<uint64_t>(q_tok_stride) | static_cast<uint64_t>(q_head_stride) |

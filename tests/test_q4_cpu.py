@@ -141,3 +141,10 @@ def test_tangents_count_as_gradients():
         assert kernels._needs_grad(x, dual) and not kernels._needs_grad(x)
         with torch.no_grad():  # (stops gradients of the backward pass only)
             assert kernels._needs_grad(dual)
+
+
+def test_a_cache_too_small_for_the_tree_is_refused_with_a_device_length_too():
+    lib = _lib.load()
+    for cap, n in ((0, 1), (0, 40), (4, 6)):
+        assert lib.rt_tree_attn_q4(P, 8192, 256, P, P, 72 * 64, cap, P, 8192, 256, P, 2, n, 0, P, 32, 8, 128,
+                                   ctypes.c_float(1.0), 0, P, 1 << 30, None, None) == _lib.RT_ERR_INVALID_ARGUMENT
