@@ -275,10 +275,9 @@ __device__ __forceinline__ int warp_uniform2(int x) {
 }
 
 // Products issued by a whole converged warp, of which one lane (`me`, elect_one)
-// acts: the operands of tcgen05.mma are uniform registers, and without a branch
-// the compiler computes them there.  Eight products took 418 cycles to issue in a
-// branch of the elected lane, 187 in this form (descriptors by their low words,
-// `hi` the common high one); the tensor core runs them in 512.
+// acts, without a branch.  Eight products took 418 cycles to issue in a branch of the
+// elected lane, 187 in this form (descriptors by their low words, `hi` the common
+// high one); the tensor core runs them in 512.
 __device__ __forceinline__ void umma_f16_if(bool me, uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t hi,
                                             uint32_t idesc, bool accumulate) {
   asm volatile(

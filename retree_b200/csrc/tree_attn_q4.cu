@@ -21,8 +21,15 @@
 // The warps' results are merged in shared memory, the splits' in the cluster
 // (distributed shared memory) or through the workspace (attn_combine_kernel).
 // Measured (32 / 8 heads, in a graph): one token over 2048 rows 7.0 us (launch and
-// merges), over 131071 rows 42.7 us (3.5 TB/s): bound by instruction issue, 735 a
-// tile and warp, 64 % of the issue slots, the ALU pipe 54 % busy.
+// merges), over 131071 rows 42.7 us (3.5 TB/s).  735 instructions a tile and warp fill 64 % of
+// the issue slots, the ALU pipe is 54 % busy; of a warp's cycles an instruction it
+// spends 1.1 on a busy pipe, 1.0 on the latency of the instruction before, 0.6 at the
+// barriers and 0.4 each on memory and dispatch, and four warps a scheduler do not cover them.
+//
+// Up to 16 rows come here: over a short cache the other kernel is ahead at 9-16 rows
+// (32 / 8 heads, four nodes: 500 rows 10.5 us, 8.0 there; 2048 rows 11.5, 9.6), over a long
+// one this (32768 rows 24.4, 28.4; 131071 rows 59.1, 86.0), and so few rows are
+// single tokens of wide groups, or the smallest trees, for which the long cache counts.
 //
 // More query rows
 // ---------------------------------------------------------------------------

@@ -805,6 +805,7 @@ def kv_append_q4(k_cache: torch.Tensor, v_cache: torch.Tensor, k_new: torch.Tens
 
     ``offset_dev`` (int64[1] on the device) supplies the offset at run time;
     rows that do not fit are then left out and reported by the device status.
+    Any finite bf16 value can be held and read; ``tree_attention_q4`` needs values below 2^119.
     """
     what = "kv_append_q4"
     if k_new.dim() != 3 or v_new.dim() != 3:
@@ -908,7 +909,8 @@ def tree_attention_q4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask_bi
     """``tree_attention`` over a 4-bit cache.
 
     q: bf16 ``[n, Hq, 128]`` or HF's ``[1, Hq, n, 128]``; k, v: uint8 caches
-    ``[Hkv, capacity, 72]`` (an even capacity) of which rows ``[0, prefix_len + n)`` are used;
+    ``[Hkv, capacity, 72]`` (an even capacity; values below 2^119, whose scales times 192 stay
+    finite) of which rows ``[0, prefix_len + n)`` are used;
     mask_bits: int32 ``[n, W]`` ancestor bits of the tree block (one bit, set,
     for a single token).  ``prefix_len_dev`` (int64[1]) supplies the prefix
     length at run time; ``prefix_len`` is then its upper bound.  Returns ``out``
