@@ -169,7 +169,7 @@ def _check_key_offsets(cu_q, cu_k, keys: int) -> None:
     Callers without a cache pass the queries' offsets for both; over a cache those
     are in range, but name its first rows.  (One read of an offset, on this path only.)
     """
-    if cu_k is None or cu_k is cu_q or cu_k.data_ptr() == cu_q.data_ptr():
+    if cu_k is None or cu_k.numel() < 2 or cu_k is cu_q or cu_k.data_ptr() == cu_q.data_ptr():
         raise RuntimeError("packed queries over cached keys need the keys' own offsets")
     if cu_k.is_cuda and torch.cuda.is_current_stream_capturing():
         raise RuntimeError("packed queries over cached keys are not captured: their offsets are checked on the host")

@@ -19,7 +19,7 @@ def _call(n, keys, cu_q, cu_k):
                                             cu_seq_lens_k=cu_q if cu_k == "same" else off(cu_k))
 
 
-@pytest.mark.parametrize("cu_k", [None, "same", [0, 2, 6], [0, 4, 8]])
+@pytest.mark.parametrize("cu_k", [None, "same", [0, 2, 6], [0, 4, 8], [], [10]])
 def test_packed_queries_over_cached_keys_need_offsets_that_reach_the_last_key(cu_k):
     """Offsets of the queries, or of the first rows of a cache, would name other keys than the new ones."""
     with pytest.raises(RuntimeError, match="packed"):
