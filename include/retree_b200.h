@@ -515,7 +515,7 @@ int rt_prompt_attn(const void* q, int64_t q_tok_stride, int64_t q_head_stride, c
  *   rows of out (16-byte aligned).
  * rt_tree_attn_q4: rt_tree_attn on the values of such a cache (same masks,
  *   prefix, splits, output; see there).  k / v and kv_head_stride are multiples
- *   of 16 bytes, kv_capacity is even, scale >= 0 and finite, the cache's
+ *   of 16 bytes, kv_capacity is even and n at least, scale >= 0 and finite, the cache's
  *   scales s below 2^120 (values below 2^119); a node that sees no
  *   key gets a zero row; a prefix length outside the cache writes nothing
  *   (RT_DEV_BAD_INDEX).  workspace must hold
